@@ -69,6 +69,9 @@ _FWD_EXT_ARGS = [ctypes.c_void_p] * 5 + [ctypes.c_int] * 6 + [ctypes.c_float, ct
 _BWD_EXT_ARGS = [ctypes.c_void_p] * 9 + [ctypes.c_int] * 6 + [ctypes.c_float, ctypes.c_bool,
                                                               ctypes.c_void_p]
 
+_APPEND_PAGED_ARGS = ([ctypes.c_void_p] * 11 + [ctypes.c_int] * 13 +
+                      [ctypes.c_bool, ctypes.c_void_p])
+
 EXPORTED_SYMBOLS = (
     "cuflash_attention_forward_f32", "cuflash_attention_forward_f16",
     "cuflash_attention_forward_bf16", "cuflash_attention_backward_f32",
@@ -84,6 +87,10 @@ EXPORTED_SYMBOLS = (
     "cuflash_profile_enable", "cuflash_profile_report", "cuflash_attention_decode_noalloc_f16",
     "cuflash_release_workspaces",
 )
+
+# Declared in include/cuflash/paged_cache.h.
+PAGED_CACHE_SYMBOLS = tuple(f"cuflash_attention_{kind}_{sfx}" for kind in ("append_paged",)
+                            for sfx in ("f32", "f16", "bf16"))
 
 
 class CuFlashLibrary:
@@ -107,6 +114,8 @@ class CuFlashLibrary:
             fwd_ext.argtypes, fwd_ext.restype = _FWD_EXT_ARGS, ctypes.c_int
             bwd_ext = getattr(library, f"cuflash_attention_backward_ext_{sfx}")
             bwd_ext.argtypes, bwd_ext.restype = _BWD_EXT_ARGS, ctypes.c_int
+            append = getattr(library, f"cuflash_attention_append_paged_{sfx}")
+            append.argtypes, append.restype = _APPEND_PAGED_ARGS, ctypes.c_int
         noalloc = library.cuflash_attention_decode_noalloc_f16
         noalloc.argtypes, noalloc.restype = _DEC_ARGS, ctypes.c_int
         library.cuflash_error_string.argtypes = [ctypes.c_int]
@@ -369,11 +378,123 @@ def flash_attention_decode_paged(q, k_cache, v_cache, block_table, seq_lens,
     return out, lse
 
 
+def _check_paged(tensors, k_cache, v_cache, block_table, seq_lens, query_starts=None):
+    """What the calls on a paged cache have in common: one device, the current one; K and V cache
+    [P, page, Hkv, D] and contiguous; int32 tables. -> B, pages, page size, Hkv, D."""
+    torch = _torch()
+    dtype = k_cache.dtype
+    _suffix(k_cache)
+    ints = [t for t in (block_table, seq_lens, query_starts) if t is not None]
+    for t in (*tensors, k_cache, v_cache, *ints):
+        if not t.is_cuda:
+            raise ValueError("tensors must be on the GPU")
+    device = torch.cuda.current_device()
+    for t in (*tensors, k_cache, v_cache, *ints):
+        if t.device.index != device:
+            raise ValueError("tensors must be on the current device")
+    for t in (*tensors, v_cache):
+        if t.dtype != dtype:
+            raise ValueError("all tensors must share one dtype")
+    for t in ints:
+        if t.dtype != torch.int32:
+            raise TypeError("block_table, seq_lens and query_starts must be int32")
+    if not all(t.is_contiguous() for t in (k_cache, v_cache, *ints)):
+        raise ValueError("the caches and int32 tensors must be contiguous")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("expected k_cache, v_cache [P,page,Hkv,D]")
+    if block_table.dim() != 2 or tuple(seq_lens.shape) != block_table.shape[:1]:
+        raise ValueError("expected block_table [B,max_pages] and seq_lens [B]")
+    B = block_table.shape[0]
+    if query_starts is not None and tuple(query_starts.shape) != (B + 1,):
+        raise ValueError("expected query_starts [B+1]")
+    if any(t.data_ptr() % 16 for t in (*tensors, k_cache, v_cache)):
+        raise ValueError("tensors must start at a multiple of 16 bytes")
+    return (B, *k_cache.shape)
+
+
+def _output(given, like, shape, dtype, stream, name):
+    """The caller's output, checked, or a new one that belongs to the call's stream."""
+    if given is not None:
+        if (tuple(given.shape) != tuple(shape) or given.dtype != dtype
+                or given.device != like.device or not given.is_contiguous()
+                or given.data_ptr() % 16):
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on the "
+                             "inputs' device")
+        return given
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with _torch().cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _token_stride(x, name):
+    """Elements from token to token of x [T, heads, D], whose heads lie side by side."""
+    T, heads, D = x.shape
+    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != D):
+        raise ValueError(f"the heads of a token of {name} must be contiguous")
+    if T == 1:
+        return heads * D
+    if x.stride(0) < heads * D or x.stride(0) * x.element_size() % 16:
+        raise ValueError(f"the tokens of {name} must be a multiple of 16 bytes apart and not "
+                         "overlap")
+    return x.stride(0)
+
+
+def flash_attention_append_paged(k, v, k_cache, v_cache, block_table, seq_lens,
+                                 query_starts=None, q=None, cos=None, sin=None,
+                                 interleaved: bool = False, out=None, stream=None,
+                                 lib: Optional[CuFlashLibrary] = None):
+    """Writes new tokens' k, v [T, Hkv, D] to the pages of their positions in k_cache, v_cache
+    [P, page, Hkv, D] and rotates k, and q [T, H, D] if given, on the way (the tensors' tokens may
+    lie apart, as in a projection's joint output). Tokens query_starts[b] .. query_starts[b + 1] - 1
+    are the newest of sequence b, whose length with them is seq_lens[b]; without query_starts
+    there is one token per sequence. cos, sin float32 [positions, R / 2]: the first R elements of a
+    head are rotated, pairs (i, i + R / 2) or (2 i, 2 i + 1) if `interleaved`.
+    -> rotated q [T, H, D] or None (cuflash_attention_append_paged_*)."""
+    torch = _torch()
+    lib = lib or load_library()
+    given = (k, v) if q is None else (k, v, q)
+    B, pages, page_size, Hkv, D = _check_paged(given, k_cache, v_cache, block_table, seq_lens,
+                                               query_starts)
+    T = k.shape[0]
+    if any(x.dim() != 3 or x.shape[0] != T or x.shape[2] != D for x in given) \
+            or k.shape[1] != Hkv or v.shape[1] != Hkv:
+        raise ValueError("expected k, v [T,Hkv,D] and q [T,H,D] of the cache's Hkv and D")
+    R = positions = 0
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    if cos is not None:
+        if cos.dim() != 2 or sin.shape != cos.shape:
+            raise ValueError("expected cos, sin [positions, R / 2]")
+        for x in (cos, sin):
+            if x.dtype != torch.float32 or x.device != k.device or not x.is_contiguous() \
+                    or x.data_ptr() % 16:
+                raise ValueError("cos and sin must be contiguous float32 tensors on the inputs' "
+                                 "device")
+        positions, R = cos.shape[0], 2 * cos.shape[1]
+    strides = [_token_stride(x, n) for x, n in zip(given, ("k", "v", "q"))]
+    H = 0
+    if q is not None:
+        H = q.shape[1]
+        out = _output(out, q, (T, H, D), q.dtype, stream, "out")
+    elif out is not None:
+        raise ValueError("out is the rotated q: it needs q")
+    ptr = lambda x: None if x is None else x.data_ptr()  # noqa: E731
+    status = lib.fn("append_paged", _suffix(k))(
+        ptr(q), k.data_ptr(), v.data_ptr(), ptr(out), k_cache.data_ptr(), v_cache.data_ptr(),
+        block_table.data_ptr(), seq_lens.data_ptr(), ptr(query_starts), ptr(cos), ptr(sin), T, B,
+        H, Hkv, strides[2] if q is not None else 0, strides[0], strides[1], pages, page_size,
+        block_table.shape[1], D, R, positions, bool(interleaved), _stream_ptr(stream))
+    _raise(lib, status)
+    return out
+
+
 __all__ = [
     "CuFlashError", "CuFlashLibrary", "EXPORTED_SYMBOLS", "load_library",
     "candidate_library_paths", "flash_attention_forward", "flash_attention_backward",
     "flash_attention_forward_ext", "flash_attention_backward_ext", "flash_attention_decode",
-    "flash_attention_decode_paged", "SUCCESS", "INVALID_DIMENSION", "DIMENSION_MISMATCH",
+    "flash_attention_decode_paged", "flash_attention_append_paged", "PAGED_CACHE_SYMBOLS",
+    "SUCCESS", "INVALID_DIMENSION", "DIMENSION_MISMATCH",
     "NULL_POINTER", "CUDA_ERROR", "OUT_OF_MEMORY", "UNSUPPORTED_HEAD_DIM", "UNSUPPORTED_DTYPE",
 ]
 

@@ -1,0 +1,99 @@
+#pragma once
+
+// Serving from a paged key/value cache (additive; no counterpart in the reference, which has no
+// cache). Beside flash_attention_decode_paged (flash_attention.h), on the same cache:
+//   flash_attention_append_paged   writes new tokens' keys and values to their pages, rotating
+//                                  queries and keys by their positions on the way;
+//   flash_attention_forward_paged  several new tokens of every sequence attend to the cache;
+//   flash_attention_decode_shared  one query per sequence, for a batch whose first keys are the
+//                                  same pages: these are read once for the whole batch.
+//
+// Common to the three:
+//  * K_cache, V_cache [num_pages, page_size, num_kv_heads, head_dim]; block_table [batch_size,
+//    max_pages_per_seq] (int32): key j of sequence b is row j % page_size of page
+//    block_table[b][j / page_size].
+//  * Tokens are packed, [num_tokens, heads, head_dim]: those of sequence b are query_starts[b] ..
+//    query_starts[b + 1] - 1 (int32, batch_size + 1 values that do not decrease), the newest of
+//    the sequence. Sequences without tokens are allowed. Tokens from query_starts[batch_size] on
+//    are padding: their outputs are left as they were.
+//  * seq_lens [batch_size] (int32) counts a sequence's keys WITH its new tokens, so token t of
+//    sequence b stands at position seq_lens[b] - (query_starts[b + 1] - t), and the same array
+//    goes to the append and to the attention after it.
+//  * head_dim 32, 64 or 128; num_heads a multiple of num_kv_heads (query head h reads key/value
+//    head h / (num_heads / num_kv_heads)).
+//  * Pointers and token strides are multiples of 16 bytes. Every pointer is a device pointer.
+//    Calls are asynchronous on `stream` and can be captured into a HIP graph.
+// Validation, in this order: null pointers (NULL_POINTER), dimensions that are not positive
+// (INVALID_DIMENSION), head_dim (UNSUPPORTED_HEAD_DIM), scale (INVALID_DIMENSION), then the
+// relations between sizes (DIMENSION_MISMATCH), sizes whose products exceed 32 bits and alignment
+// (INVALID_DIMENSION).
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include "cuflash/export.h"
+#include "cuflash/flash_attention.h"
+
+namespace cuflash {
+
+// ---- Append ----
+// Writes K [num_tokens, num_kv_heads, head_dim] and V to the cache rows of their positions. Rows
+// of Q, K and V are q_stride, k_stride and v_stride elements apart from token to token (the heads of
+// a token are contiguous), so the three may be parts of one projection's output.
+// rope_cos, rope_sin: float [max_positions, rotary_dim / 2], or both null (no rotation; rotary_dim
+// 0). The first rotary_dim elements of every query and key head (a multiple of 16, at most head_dim)
+// are rotated by row p = position: the pair (x1, x2) = elements (i, i + rotary_dim / 2), or (2 i,
+// 2 i + 1) if `interleaved`, becomes (x1 cos - x2 sin, x2 cos + x1 sin), computed in float and
+// rounded once. Rotated queries go to Q_out [num_tokens, num_heads, head_dim], which may be Q itself
+// where Q is packed (q_stride = num_heads * head_dim). Q and Q_out may both be null.
+// query_starts may be null: then token t is the one new token of sequence t (num_tokens ==
+// batch_size).
+// What the host cannot see is not an error but left out: a token whose position is negative or past
+// the block table, and one whose page is not in [0, num_pages) (so -1 marks rows that have none), is
+// not written; a query whose position is outside the rotation's tables becomes NaN, and its token is
+// not written. Two tokens for one cache row: one of them is kept.
+CUFLASH_EXPORT FlashAttentionError flash_attention_append_paged(
+    const float* Q, const float* K, const float* V, float* Q_out, float* K_cache, float* V_cache,
+    const int* block_table, const int* seq_lens, const int* query_starts, const float* rope_cos,
+    const float* rope_sin, int num_tokens, int batch_size, int num_heads, int num_kv_heads,
+    int q_stride, int k_stride, int v_stride, int num_pages, int page_size, int max_pages_per_seq,
+    int head_dim, int rotary_dim, int max_positions, bool interleaved, hipStream_t stream = 0);
+CUFLASH_EXPORT FlashAttentionError flash_attention_append_paged(
+    const __half* Q, const __half* K, const __half* V, __half* Q_out, __half* K_cache,
+    __half* V_cache, const int* block_table, const int* seq_lens, const int* query_starts,
+    const float* rope_cos, const float* rope_sin, int num_tokens, int batch_size, int num_heads,
+    int num_kv_heads, int q_stride, int k_stride, int v_stride, int num_pages, int page_size,
+    int max_pages_per_seq, int head_dim, int rotary_dim, int max_positions, bool interleaved,
+    hipStream_t stream = 0);
+CUFLASH_EXPORT FlashAttentionError flash_attention_append_paged(
+    const __hip_bfloat16* Q, const __hip_bfloat16* K, const __hip_bfloat16* V,
+    __hip_bfloat16* Q_out, __hip_bfloat16* K_cache, __hip_bfloat16* V_cache,
+    const int* block_table, const int* seq_lens, const int* query_starts, const float* rope_cos,
+    const float* rope_sin, int num_tokens, int batch_size, int num_heads, int num_kv_heads,
+    int q_stride, int k_stride, int v_stride, int num_pages, int page_size, int max_pages_per_seq,
+    int head_dim, int rotary_dim, int max_positions, bool interleaved, hipStream_t stream = 0);
+
+}  // namespace cuflash
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+// C ABI of the functions above; the integer value of cuflash::FlashAttentionError.
+#define CUFLASH_DECLARE_PAGED_CACHE(SFX, T)                                                       \
+    CUFLASH_EXPORT int cuflash_attention_append_paged_##SFX(                                      \
+        const T* Q, const T* K, const T* V, T* Q_out, T* K_cache, T* V_cache,                     \
+        const int* block_table, const int* seq_lens, const int* query_starts,                     \
+        const float* rope_cos, const float* rope_sin, int num_tokens, int batch_size,             \
+        int num_heads, int num_kv_heads, int q_stride, int k_stride, int v_stride, int num_pages, \
+        int page_size, int max_pages_per_seq, int head_dim, int rotary_dim, int max_positions,    \
+        bool interleaved, hipStream_t stream);
+CUFLASH_DECLARE_PAGED_CACHE(f32, float)
+CUFLASH_DECLARE_PAGED_CACHE(f16, __half)
+CUFLASH_DECLARE_PAGED_CACHE(bf16, __hip_bfloat16)
+#undef CUFLASH_DECLARE_PAGED_CACHE
+
+#ifdef __cplusplus
+}
+#endif
