@@ -34,7 +34,8 @@ LIB_PATH = os.path.join(BUILD_DIR, LIB_NAME)
 RELEASE_LINK = os.path.join(BUILD_DIR, "release", LIB_NAME)
 
 SOURCES = ["api.cpp", "paged_api.cpp", "profile.cpp", "workspace.cpp", "forward.hip",
-           "backward.hip", "decode.hip", "append.hip", "primitives.hip"]
+           "backward.hip", "decode.hip", "append.hip", "paged.hip",
+           "primitives.hip"]
 # C++ test programs linked against the library (sources under tests/cpp, binaries in build/).
 TEST_PROGRAMS = {"test_primitives": "test_primitives.cpp"}
 TEST_SRC = os.path.join(REPO_ROOT, "tests", "cpp")

@@ -15,6 +15,7 @@
 #include "launch.hpp"
 #include "paged_launch.hpp"
 #include "profile.hpp"
+#include "wave.hpp"
 
 namespace cuflash {
 namespace dev {
@@ -30,19 +31,6 @@ struct AppendArgs {
     int num_pages, page_size, max_pages;
     int rotary, max_positions;
 };
-
-// Sequence of packed token t: the number of sequences that end at or before it (starts do not
-// decrease). The whole wave looks, 64 sequences at a time.
-__device__ __forceinline__ int sequence_of(const int* starts, int B, int t) {
-    const int lane = threadIdx.x & 63;
-    int b = 0;
-    for (int b0 = 0; b0 < B; b0 += 64) {
-        const int n = __popcll(__ballot(b0 + lane < B && starts[min(b0 + lane, B - 1) + 1] <= t));
-        b += n;
-        if (n < 64) break;
-    }
-    return b;
-}
 
 template <typename T, int D, bool kInterleaved>
 __global__ void __launch_bounds__(1024)
@@ -84,7 +72,7 @@ __global__ void __launch_bounds__(1024)
     int last = t + 1;  // end of the sequence's tokens
     if (a.query_starts) {
         b = sequence_of(a.query_starts, a.B, t);
-        if (b >= a.B || t < a.query_starts[b]) return;  // padding
+        if (b == a.B) return;  // padding
         last = a.query_starts[b + 1];
     }
     // -1: no position, or one outside the rotation's tables.

@@ -24,6 +24,7 @@
 #include "profile.hpp"
 #include "softmax.hpp"
 #include "tile_groups.hpp"
+#include "wave.hpp"
 
 namespace cuflash {
 namespace dev {
@@ -39,21 +40,6 @@ struct DecCfg {
     static constexpr int kThreads = 64 * kWaves;
     static constexpr int ROWS_PER_ITER = RPW * UNROLL * kWaves;
 };
-
-// DPP lane permutations (row = 16 lanes).
-constexpr int kDppXor1 = 0xB1;        // quad_perm [1,0,3,2]
-constexpr int kDppXor2 = 0x4E;        // quad_perm [2,3,0,1]
-constexpr int kDppHalfMirror = 0x141;  // lane i <-> 7 - i within each 8 lanes
-constexpr int kDppMirror = 0x140;      // lane i <-> 15 - i within each row
-constexpr int kDppRowShr = 0x110;      // + n: lane i takes lane i - n of its row
-constexpr int kDppRowBcast15 = 0x142;  // the last lane of a row to the next row
-constexpr int kDppRowBcast31 = 0x143;  // lane 31 to rows 2 and 3
-
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-    return __builtin_bit_cast(
-        float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
-}
 
 // Sum over aligned groups of G lanes (G = 2 .. 32); every lane of the group gets the total.
 template <int G>
@@ -91,36 +77,6 @@ __device__ __forceinline__ void to_floats(u32x4 v, float (&out)[VEC]) {
 __device__ __forceinline__ float exp2_rel(float x, float m) {
     return x == -INFINITY ? 0.0f : fast_exp2(x - m);
 }
-
-// The 64 lanes of a wave for paged_segment (paged_split.hpp); results are wave-uniform.
-struct GpuWave {
-    using Int = int;
-    template <class F>
-    __device__ static Int each(F f) {
-        return f(static_cast<int>(threadIdx.x & 63));
-    }
-    template <class F>
-    __device__ static Int map(Int v, F f) {
-        return f(v);
-    }
-    __device__ static Int add(Int a, Int b) { return a + b; }
-    // Inclusive sum over the lanes.
-    __device__ static Int scan(Int v) {
-        v += __builtin_amdgcn_update_dpp(0, v, kDppRowShr + 1, 0xF, 0xF, false);
-        v += __builtin_amdgcn_update_dpp(0, v, kDppRowShr + 2, 0xF, 0xF, false);
-        v += __builtin_amdgcn_update_dpp(0, v, kDppRowShr + 4, 0xF, 0xF, false);
-        v += __builtin_amdgcn_update_dpp(0, v, kDppRowShr + 8, 0xF, 0xF, false);
-        v += __builtin_amdgcn_update_dpp(0, v, kDppRowBcast15, 0xA, 0xF, false);
-        v += __builtin_amdgcn_update_dpp(0, v, kDppRowBcast31, 0xC, 0xF, false);
-        return v;
-    }
-    __device__ static int lane(Int v, int i) { return __builtin_amdgcn_readlane(v, i); }
-    // The first lane where f is not 0, or -1.
-    template <class F>
-    __device__ static int first(Int v, F f) {
-        return __ffsll(static_cast<unsigned long long>(__ballot(f(v)))) - 1;
-    }
-};
 
 template <typename T, int D, int G, bool PAGED>
 __global__ void __launch_bounds__(256)

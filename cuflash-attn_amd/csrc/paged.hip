@@ -1,0 +1,811 @@
+// Attention of packed tokens over a paged cache for gfx950 (MI355X): flash_attention_forward_paged
+// and flash_attention_decode_shared (cuflash/paged_cache.h). One launch of paged_kernel, cut by
+// paged_plan.hpp, and where keys are cut into chunks a launch of paged_combine_kernel.
+//
+// The query heads of one key/value head are packed into the rows of a tile (row r of a unit is token
+// r / group, head r % group), so its keys are read once for all of them. A wave holds 32 rows in the
+// forward kernels' transposed tiles: S^T = K Q^T, a lane pair per row, the online softmax in the
+// score registers, O^T += V^T P^T (kv_block32). The two kinds of items:
+//  * many rows: each wave has 32 rows of its own, and all of them share the key tiles;
+//  * few rows: 32 rows in all, each wave takes other 32-key blocks through tiles of its own, and the
+//    waves' (O, m, l) are merged through LDS at the end. This is what keeps enough bytes in flight
+//    where a sequence's keys are read for a handful of rows.
+// Tiles are filled by LDS-DMA loads, one kilobyte of whole key rows each: where the rows of a load
+// cannot cross a page, from a scalar base (the page index by a scalar load) and a fixed lane offset;
+// otherwise, and in a sequence's last tile, from an address per lane. Rows past the end are the last
+// key again, and masked.
+
+#include <algorithm>
+#include <type_traits>
+
+#include "common.hpp"
+#include "kv_block.hpp"
+#include "launch.hpp"
+#include "paged_launch.hpp"
+#include "paged_plan.hpp"
+#include "profile.hpp"
+#include "softmax.hpp"
+#include "tile_groups.hpp"
+#include "wave.hpp"
+
+namespace cuflash {
+namespace dev {
+
+// What differs between the types: tiles of 32 keys in LDS and the block over one of them.
+template <typename T, int D>
+struct PagedEngine {
+    using Lay = TileGroups<D>;
+    using Frag = typename Elem<T>::frag;
+    static constexpr int kWaves = 8;
+    static constexpr int kStepBlocks = 2;              // 32-key blocks of a step (many rows)
+    static constexpr int kGroupRows = Lay::kRows;      // key rows of one load
+    static constexpr int kGroups = 32 / kGroupRows;    // loads of a tile
+    static constexpr int kGroupBytes = Lay::kBytes;
+    static constexpr int kTile = kGroups * kGroupBytes;
+    struct Query {
+        Frag f[D / 16];
+    };
+    __device__ __forceinline__ static void load(Query& q, const uint16_t* row, bool on, int g2) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if (on) v = ld16(row + 16 * ks + 8 * g2);
+            q.f[ks] = as_frag<T>(v);
+        }
+    }
+    __device__ __forceinline__ static int ld_row(int lane) { return Lay::ld_row(lane); }
+    __device__ __forceinline__ static int ld_col(int lane, int) { return Lay::ld_col(lane); }
+    struct Offsets {
+        int k[2], v;
+    };
+    __device__ __forceinline__ static Offsets offsets(int lane) {
+        return {{Lay::row_base(lane, 0), Lay::row_base(lane, 1)}, Lay::tr_off(lane)};
+    }
+    template <class F>
+    __device__ __forceinline__ static void block(const unsigned char* kt, const unsigned char* vt,
+                                                 const Offsets& at, int key0, int mask_from,
+                                                 int kend, int g2, float cs, const Query& q,
+                                                 f32x16 (&o)[D / 32], float& m, float& l,
+                                                 F&& before_pv) {
+        kv_block32<T, D, Lay>(kt, vt, at.k, at.v, key0, mask_from, kend, g2, cs, q.f, o, m, l,
+                              before_pv);
+    }
+};
+
+// fp32 on v_mfma_f32_32x32x2f32. Key row r of a tile starts at 4 D r, its 16-byte chunk c at slot
+// c ^ (r & kSwizzle): 16 rows read at one chunk fall into 16 bank slots (8 at head_dim 32). Lane
+// half h supplies chunk 2 j + h of both K and Q to the four products of step j: any assignment of
+// the k index does, as long as both agree. The scores and P stay in fp32.
+template <int D>
+struct PagedEngine<float, D> {
+    static constexpr int kWaves = 4;
+    static constexpr int kStepBlocks = 1;
+    static constexpr int kGroupRows = 256 / D;
+    static constexpr int kGroups = 32 / kGroupRows;
+    static constexpr int kGroupBytes = 1024;
+    static constexpr int kTile = kGroups * kGroupBytes;
+    static constexpr int kSwizzle = D >= 64 ? 15 : 7;
+    struct Query {
+        f32x4 f[D / 8];
+    };
+    __device__ __forceinline__ static void load(Query& q, const float* row, bool on, int g2) {
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if (on) v = ld16(row + 8 * j + 4 * g2);
+            q.f[j] = __builtin_bit_cast(f32x4, v);
+        }
+    }
+    __device__ __forceinline__ static int ld_row(int lane) { return lane / (D / 4); }
+    __device__ __forceinline__ static int ld_col(int lane, int g) {
+        const int r = kGroupRows * g + ld_row(lane);
+        return ((lane % (D / 4)) ^ (r & kSwizzle)) * 4;
+    }
+    struct Offsets {
+        int k;     // K row l32
+        int k_x;   // its swizzle
+        int v[4];  // V row 4 g2 + i, this lane's column of dims 0 .. 31
+    };
+    __device__ __forceinline__ static Offsets offsets(int lane) {
+        const int l32 = lane & 31, g2 = lane >> 5;
+        Offsets o;
+        o.k = l32 * 4 * D;
+        o.k_x = l32 & kSwizzle;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            o.v[i] = (4 * g2 + i) * 4 * D + (((l32 >> 2) ^ (4 * g2 + i)) * 16) + (l32 & 3) * 4;
+        return o;
+    }
+    template <class F>
+    __device__ __forceinline__ static void block(const unsigned char* kt, const unsigned char* vt,
+                                                 const Offsets& at, int key0, int mask_from,
+                                                 int kend, int g2, float cs, const Query& q,
+                                                 f32x16 (&o)[D / 32], float& m, float& l,
+                                                 F&& before_pv) {
+        f32x16 s = f32x16{};
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+            const f32x4 k = __builtin_bit_cast(
+                f32x4, ld16(kt + at.k + (((2 * j + g2) ^ at.k_x) * 16)));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s = mma_f32(k[i], q.f[j][i], s);
+        }
+        if (key0 + 32 > mask_from) {
+            const int lim = kend - key0 - 4 * g2;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = (8 * (r >> 2) + (r & 3) < lim) ? s[r] : -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = __builtin_elementwise_maximum(mx, s[r]);
+        const float m_new = fmaxf(m, pair_max(mx) * cs);
+        const bool grow = m_new > m + kLazyRescale;
+        const float alpha = grow ? fast_exp2(m_new == -INFINITY ? 0.0f : m - m_new) : 1.0f;
+        m = grow ? m_new : m;
+        l *= alpha;
+        if (__ballot(grow) != 0) {
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt) o[dt] *= alpha;
+        }
+        const float m_use = (m == -INFINITY) ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = fast_exp2(fmaf(s[r], cs, -m_use));
+            sum += s[r];
+        }
+        l += sum;
+        before_pv();
+        // Score register r holds key 8 (r / 4) + 4 g2 + r % 4: bit 3 of its swizzle swaps
+        // neighbouring 32-column tiles (head_dim 64 and 128).
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt) {
+                const int tile = D >= 64 ? dt ^ ((r >> 2) & 1) : dt;
+                const float v = *reinterpret_cast<const float*>(
+                    vt + at.v[r & 3] + (r >> 2) * 8 * 4 * D + tile * 128);
+                o[dt] = mma_f32(v, s[r], o[dt]);
+            }
+        }
+    }
+};
+
+template <typename T, int D>
+using PagedShapeOf = PagedShape<32 * PagedEngine<T, D>::kWaves, 32 * PagedEngine<T, D>::kStepBlocks,
+                                32 * PagedEngine<T, D>::kWaves>;
+
+// The rows of one key/value head in the cache, from their position in a sequence.
+template <typename E>
+struct CacheRows {
+    // Uniform reads go through the scalar cache: the table does not change during the launch.
+    typedef const __attribute__((address_space(4))) int* ConstInts;
+    const int* table;
+    FastDiv page_div;
+    int page_size;
+    size_t pitch;  // elements from key to key
+    __device__ __forceinline__ size_t at(int t, int j, int page) const {
+        return (static_cast<size_t>(page) * page_size + (t - j * page_size)) * pitch;
+    }
+    __device__ __forceinline__ size_t uniform(int t) const {
+        const int j = page_div(t);
+        return at(t, j, ((ConstInts)table)[j]);
+    }
+    __device__ __forceinline__ size_t lane(int t) const {
+        const int j = page_div(t);
+        return at(t, j, table[j]);
+    }
+};
+
+template <typename T, int D>
+struct PagedWork {
+    using Eng = PagedEngine<T, D>;
+    using E = typename Mma<T>::elem;
+    const E* Q;
+    const E* K;  // of the item's key/value head
+    const E* V;
+    E* O;
+    float* L;
+    const PagedArgs& a;
+    const PagedItem& it;
+    int hk;
+    CacheRows<E> rows;
+    bool whole;  // a load's rows lie on one page
+
+    // Row r of the unit in Q, O and L.
+    __device__ __forceinline__ int out_row(int r) const {
+        const int i = a.group_div(r);
+        return (it.unit.t0 + i) * a.H + hk * a.group + (r - i * a.group);
+    }
+    // Keys below this are seen by row r of the unit, within the item.
+    __device__ __forceinline__ int row_end(int r) const {
+        return min(it.kend, paged_limit(a, it.u, it.unit, a.group_div(r)));
+    }
+    // Group g of the tile that begins at key0, from K and V alike.
+    template <int N>
+    __device__ __forceinline__ void load_groups(const E* src, int key0, int tile_end, int g0,
+                                                int step, unsigned char* dst) const {
+        const int lane = threadIdx.x & 63;
+        const int ld_row = Eng::ld_row(lane);
+        if (whole && tile_end <= it.kend) {
+            const int row = ld_row * static_cast<int>(rows.pitch);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int g = g0 + step * i;
+                const E* base = src + rows.uniform(key0 + Eng::kGroupRows * g);
+                lds_dma16_async_s(base,
+                                  static_cast<unsigned>((row + Eng::ld_col(lane, g)) * sizeof(E)),
+                                  dst + g * Eng::kGroupBytes);
+            }
+        } else {
+            size_t off[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int t = key0 + Eng::kGroupRows * (g0 + step * i) + ld_row;
+                off[i] = rows.lane(min(t, it.kend - 1));
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int g = g0 + step * i;
+                lds_dma16_async(src + off[i] + Eng::ld_col(lane, g), dst + g * Eng::kGroupBytes);
+            }
+        }
+    }
+    // One row's result: its 16-byte piece cc of D, from the unnormalized sums.
+    __device__ __forceinline__ static u32x4 finish(const float* x, float inv) {
+        u32x4 w;
+        if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(x[i] * inv);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = Elem<T>::pack2(x[2 * i] * inv, x[2 * i + 1] * inv);
+        }
+        return w;
+    }
+
+    __device__ __forceinline__ void many_rows(unsigned char* smem) const;
+    __device__ __forceinline__ void few_rows(unsigned char* smem, float (*s_m)[32],
+                                             float (*s_l)[32]) const;
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void PagedWork<T, D>::many_rows(unsigned char* smem) const {
+    constexpr int kBlocks = Eng::kStepBlocks;
+    constexpr int kStep = 32 * kBlocks;
+    constexpr int kBytes = kBlocks * Eng::kTile;  // of a step's K or V
+    constexpr int kParts = kBlocks * Eng::kGroups / Eng::kWaves;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31;
+    const int g2 = lane >> 5;
+    const int row = it.r0 + wave * 32 + l32;
+    const bool on = row < it.rows;
+    const int orow = on ? out_row(row) : -1;
+
+    typename Eng::Query q;
+    Eng::load(q, Q + static_cast<size_t>(on ? orow : 0) * D, on, g2);
+    // This lane's keys, and the least and the greatest end of the wave's rows.
+    const int kend = on ? row_end(row) : it.kend;
+    int least = kend, most = on ? kend : 0;
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1) {
+        least = min(least, __shfl_xor(least, w, 64));
+        most = max(most, __shfl_xor(most, w, 64));
+    }
+    const int mask_from = __builtin_amdgcn_readfirstlane(least);
+    const int wave_end = __builtin_amdgcn_readfirstlane(most);
+    const int nsteps = it.kend > it.kbeg ? (it.kend - it.kbeg + kStep - 1) / kStep : 0;
+
+    unsigned char* const k0 = smem;
+    unsigned char* const v0 = smem + kBytes;
+    unsigned char* const k1 = smem + 2 * kBytes;
+    unsigned char* const v1 = smem + 3 * kBytes;
+    auto load = [&](int j, unsigned char* kt, unsigned char* vt) {
+        const int key0 = it.kbeg + j * kStep;
+        load_groups<kParts>(K, key0, key0 + kStep, wave, Eng::kWaves, kt);
+        load_groups<kParts>(V, key0, key0 + kStep, wave, Eng::kWaves, vt);
+    };
+    const auto at = Eng::offsets(lane);
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) o[dt] = f32x16{};
+    float m = -INFINITY, l = 0.0f;
+    const float cs = fmaxf(a.c, kFltMin);  // scale 0: -inf * 0 would make the masked scores NaN
+    auto step = [&](int j, const unsigned char* kt, const unsigned char* vt) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            const int key0 = it.kbeg + j * kStep + 32 * b;
+            if (key0 < wave_end)
+                Eng::block(kt + b * Eng::kTile, vt + b * Eng::kTile, at, key0, mask_from, kend, g2,
+                           cs, q, o, m, l, [] {});
+        }
+    };
+    // Step j in buffers j & 1: the loads of step j + 1 are issued behind the barrier that ends every
+    // wave's reads of step j - 1.
+    if (nsteps > 0) load(0, k0, v0);
+    for (int j = 0; j < nsteps; j += 2) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (j + 1 < nsteps) load(j + 1, k1, v1);
+        step(j, k0, v0);
+        if (j + 1 >= nsteps) break;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (j + 2 < nsteps) load(j + 2, k0, v0);
+        step(j + 1, k1, v1);
+    }
+
+    l = pair_sum(l);
+    if (!it.direct) {
+        if (!on) return;
+        const size_t slot =
+            paged_slot_row<PagedShapeOf<T, D>>(a, hk, true, it.index, wave * 32 + l32);
+        float* dst = a.acc + slot * D + 4 * g2;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f32x4 w;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) w[u] = o[dt][4 * i + u];
+                st16(dst + 32 * dt + 8 * i, __builtin_bit_cast(u32x4, w));
+            }
+        }
+        if (g2 == 0) a.ml[slot] = make_float2(m, l);
+        return;
+    }
+    // O rows through LDS, so that a store writes whole rows: 16 bytes a lane.
+    constexpr int P = D * static_cast<int>(sizeof(E)) + 16;
+    constexpr int kChunks = D * static_cast<int>(sizeof(E)) / 16;  // per row
+    static_assert(32 * P <= 2 * Eng::kTile, "the O rows fit the tiles");
+    __syncthreads();  // every wave is past its last tile
+    unsigned char* stage = smem + wave * 32 * P;
+    const bool none = l == 0.0f;  // no key, or every score -inf: O = 0, L = -inf
+    const float inv = none ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = none ? 0.0f : o[dt][4 * i + u] * inv;
+            unsigned char* dst = stage + l32 * P + (32 * dt + 8 * i + 4 * g2) * sizeof(E);
+            if constexpr (std::is_same<T, float>::value) {
+                st16(dst, u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]),
+                                __float_as_uint(x[2]), __float_as_uint(x[3])});
+            } else {
+                st8(dst, u32x2{Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3])});
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 32 * kChunks / 64; ++i) {
+        const int r = (64 * i + lane) / kChunks;
+        const int cc = (64 * i + lane) % kChunks;
+        const int to = __shfl(orow, r, 64);
+        const u32x4 v = ld16(stage + r * P + cc * 16);
+        if (to >= 0)
+            st16(reinterpret_cast<unsigned char*>(O) + static_cast<size_t>(to) * (D * sizeof(E)) +
+                     cc * 16,
+                 v);
+    }
+    if (g2 == 0 && on) L[orow] = none ? -INFINITY : (m + fast_log2(l)) * kLn2;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void PagedWork<T, D>::few_rows(unsigned char* smem, float (*s_m)[32],
+                                                          float (*s_l)[32]) const {
+    constexpr int NW = Eng::kWaves;
+    constexpr int kLoads = Eng::kGroups;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31;
+    const int g2 = lane >> 5;
+    const int row = it.r0 + l32;
+    const bool on = row < it.rows;
+
+    typename Eng::Query q;
+    Eng::load(q, Q + static_cast<size_t>(on ? out_row(row) : 0) * D, on, g2);
+    const int kend = on ? row_end(row) : it.kend;
+    int least = kend;
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1) least = min(least, __shfl_xor(least, w, 64));
+    const int mask_from = __builtin_amdgcn_readfirstlane(least);
+    const int nblk = it.kend > it.kbeg ? (it.kend - it.kbeg + 31) / 32 : 0;
+
+    unsigned char* kt = smem + wave * 2 * Eng::kTile;
+    unsigned char* vt = kt + Eng::kTile;
+    auto load = [&](const E* src, int b, unsigned char* dst) {
+        const int key0 = it.kbeg + 32 * b;
+        load_groups<kLoads>(src, key0, key0 + 32, 0, 1, dst);
+    };
+    // After the Q loads (see the waits of the loop below).
+    asm volatile("" ::: "memory");
+    if (wave < nblk) {
+        load(K, wave, kt);
+        load(V, wave, vt);
+    }
+    const auto at = Eng::offsets(lane);
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) o[dt] = f32x16{};
+    float m = -INFINITY, l = 0.0f;
+    const float cs = fmaxf(a.c, kFltMin);
+    // K and V are waited for separately (vmcnt counts a wave's loads in order, kLoads per tile): K
+    // before the scores, V before P V; the next K is issued once the scores have read this one, the
+    // next V once P V has.
+    for (int b = wave; b < nblk; b += NW) {
+        const bool next = b + NW < nblk;
+        wait_loads<kLoads>();
+        Eng::block(kt, vt, at, it.kbeg + 32 * b, mask_from, kend, g2, cs, q, o, m, l, [&] {
+            if (next) {
+                wait_lds();
+                load(K, b + NW, kt);
+                wait_loads<kLoads>();
+            } else {
+                wait_loads<0>();
+            }
+        });
+        if (next) {
+            wait_lds();
+            load(V, b + NW, vt);
+        }
+    }
+
+    // Merge: every wave scales its rows to the common max and leaves them in LDS, then the
+    // workgroup sums them wave after wave.
+    constexpr int P = D + 4;  // pitch of the merge rows (floats)
+    static_assert(NW * 32 * P * 4 <= NW * 2 * Eng::kTile, "the merge rows fit the tiles");
+    l = pair_sum(l);
+    if (g2 == 0) {
+        s_m[wave][l32] = m;
+        s_l[wave][l32] = l;
+    }
+    __syncthreads();  // also ends every wave's use of its tiles
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, s_m[w][l32]);
+    const float f = m == -INFINITY ? 0.0f : fast_exp2(m - M);
+    float* mrg = reinterpret_cast<float*>(smem);
+    {
+        float* dst = mrg + (wave * 32 + l32) * P + 4 * g2;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f32x4 w;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) w[u] = o[dt][4 * i + u] * f;
+                st16(dst + 32 * dt + 8 * i, __builtin_bit_cast(u32x4, w));
+            }
+        }
+    }
+    __syncthreads();
+    constexpr int kPiece = 16 / static_cast<int>(sizeof(E));  // columns of an output's 16 bytes
+    constexpr int kPieces = D / kPiece;
+#pragma unroll
+    for (int i0 = 0; i0 < 32 * kPieces; i0 += 64 * NW) {
+        const int i = i0 + threadIdx.x;
+        const int r = i / kPieces;
+        const int cc = (i % kPieces) * kPiece;
+        if (r >= 32 || it.r0 + r >= it.rows) break;
+        float ms[NW], MM = -INFINITY, lt = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            ms[w] = s_m[w][r];
+            MM = fmaxf(MM, ms[w]);
+        }
+        float x[kPiece];
+#pragma unroll
+        for (int u = 0; u < kPiece; ++u) x[u] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            lt = fmaf(s_l[w][r], ms[w] == -INFINITY ? 0.0f : fast_exp2(ms[w] - MM), lt);
+#pragma unroll
+            for (int u = 0; u < kPiece; u += 4) {
+                const f32x4 y =
+                    __builtin_bit_cast(f32x4, ld16(mrg + (w * 32 + r) * P + cc + u));
+#pragma unroll
+                for (int v = 0; v < 4; ++v) x[u + v] += y[v];
+            }
+        }
+        if (!it.direct) {
+            const size_t slot = paged_slot_row<PagedShapeOf<T, D>>(a, hk, false, it.index, r);
+#pragma unroll
+            for (int u = 0; u < kPiece; u += 4)
+                st16(a.acc + slot * D + cc + u,
+                     __builtin_bit_cast(u32x4, f32x4{x[u], x[u + 1], x[u + 2], x[u + 3]}));
+            if (cc == 0) a.ml[slot] = make_float2(MM, lt);
+            continue;
+        }
+        const bool none = lt == 0.0f;
+        if (none) {
+#pragma unroll
+            for (int u = 0; u < kPiece; ++u) x[u] = 0.0f;
+        }
+        const int to = out_row(it.r0 + r);
+        st16(O + static_cast<size_t>(to) * D + cc, finish(x, none ? 0.0f : 1.0f / lt));
+        if (cc == 0) L[to] = none ? -INFINITY : (MM + fast_log2(lt)) * kLn2;
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__((64 * PagedEngine<T, D>::kWaves), (D <= 64 ? 2 : 1))
+    paged_kernel(const typename Mma<T>::elem* __restrict__ Q,
+                 const typename Mma<T>::elem* __restrict__ K,
+                 const typename Mma<T>::elem* __restrict__ V,
+                 typename Mma<T>::elem* __restrict__ O, float* __restrict__ L, PagedArgs a) {
+    using Eng = PagedEngine<T, D>;
+    constexpr int kBytes = Eng::kWaves * 2 * Eng::kTile;
+    static_assert(kBytes >= 4 * Eng::kStepBlocks * Eng::kTile, "either kind's tiles");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kBytes];
+    __shared__ float s_m[Eng::kWaves][32];
+    __shared__ float s_l[Eng::kWaves][32];
+    // The items of a key/value head stay on one XCD where the heads can be dealt out evenly.
+    int hk, x;
+    head_rank_order(blockIdx.x, a.Hkv, hk, x);
+    const PagedItem it = paged_item<PagedShapeOf<T, D>, GpuWave>(a, x);
+    if (!it.found) return;
+    const int* table = !a.shared    ? a.block_table + static_cast<size_t>(it.u) * a.max_pages
+                       : it.u == 0 ? a.prefix_table
+                                   : a.block_table + static_cast<size_t>(it.u - 1) * a.max_pages;
+    const PagedWork<T, D> work{Q,
+                               K + static_cast<size_t>(hk) * D,
+                               V + static_cast<size_t>(hk) * D,
+                               O,
+                               L,
+                               a,
+                               it,
+                               hk,
+                               {table, a.page_div, a.page_size,
+                                static_cast<size_t>(a.Hkv) * D},
+                               // Tiles begin at the unit's first key: behind a prefix, anywhere.
+                               a.whole_groups && it.unit.kbeg % Eng::kGroupRows == 0};
+    if (it.many)
+        work.many_rows(smem);
+    else
+        work.few_rows(smem, s_m, s_l);
+}
+
+// Merges the parts of each row: O = sum O_i 2^(m_i - M) / l with M = max m_i and l = sum l_i
+// 2^(m_i - M), L = (M + log2 l) ln 2. One workgroup per token and 256 / (D / 4) query heads, D / 4
+// lanes a row, four columns each; kBatch parts of a row in flight.
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+    paged_combine_kernel(typename Mma<T>::elem* __restrict__ O, float* __restrict__ L,
+                         PagedArgs a) {
+    using E = typename Mma<T>::elem;
+    using Shape = PagedShapeOf<T, D>;
+    constexpr int LPR = D / 4;
+    constexpr int kRows = 256 / LPR;
+    constexpr int kBatch = 8;
+    const int t = blockIdx.x;
+    const int h = blockIdx.y * kRows + threadIdx.x / LPR;
+    const int part = threadIdx.x % LPR;
+    int u = t + 1;
+    if (!a.shared) {
+        u = sequence_of(a.starts, a.B, t);
+        if (u == a.B) return;  // padding
+    }
+    const auto first = PagedPlan<Shape, GpuWave>::batch(a, 0);
+    const PagedCut cut = PagedPlan<Shape, GpuWave>::cut(a, first);
+    const PagedUnitItems own = paged_unit_items<Shape, GpuWave>(a, cut, first, u);
+    if (!a.shared && own.chunks == 1) return;  // written already
+    PagedUnitItems pre{};
+    if (a.shared) pre = paged_unit_items<Shape, GpuWave>(a, cut, first, 0);
+    if (h >= a.H) return;
+    const int hk = a.group_div(h);
+    const int g = h - hk * a.group;
+    // Slot of part p of a unit's row r.
+    auto slot = [&](const PagedUnitItems& ui, int p, int r) {
+        const int tile = ui.many ? r / Shape::kTile : r / 32;
+        const int in = ui.many ? r % Shape::kTile : r % 32;
+        return paged_slot_row<Shape>(
+            a, hk, ui.many,
+            ui.first + p * ui.tiles + (a.causal ? ui.tiles - 1 - tile : tile), in);
+    };
+    const int own_row = a.shared ? g : (t - a.starts[u]) * a.group + g;
+    const int pre_row = t * a.group + g;
+    const int parts = pre.chunks + own.chunks;
+    float M = -INFINITY, l = 0.0f;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p0 = 0; p0 < parts; p0 += kBatch) {
+        float2 v[kBatch];
+        f32x4 x[kBatch];
+        float M2 = M;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int p = p0 + i;
+            v[i] = make_float2(-INFINITY, 0.0f);
+            x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (p < parts) {
+                const size_t s = p < pre.chunks ? slot(pre, p, pre_row)
+                                                : slot(own, p - pre.chunks, own_row);
+                v[i] = a.ml[s];
+                x[i] = __builtin_bit_cast(f32x4, ld16(a.acc + s * D + 4 * part));
+                // No key of this row, or every score -inf: such a part has no say, also where
+                // 0 times a value made it NaN.
+                if (v[i].x == -INFINITY) x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) M2 = fmaxf(M2, v[i].x);
+        auto weight = [&](float mi) { return mi == -INFINITY ? 0.0f : fast_exp2(mi - M2); };
+        const float f0 = weight(M);
+        l *= f0;
+        acc *= f0;
+        M = M2;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const float f = weight(v[i].x);
+            l = fmaf(v[i].y, f, l);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = fmaf(x[i][c], f, acc[c]);
+        }
+    }
+    const bool none = l == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / l;
+    float y[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) y[c] = none ? 0.0f : acc[c] * inv;
+    const size_t row = static_cast<size_t>(t) * a.H + h;
+    E* dst = O + row * D + 4 * part;
+    if constexpr (std::is_same<T, float>::value)
+        st16(dst, u32x4{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]),
+                        __float_as_uint(y[3])});
+    else
+        st8(dst, u32x2{Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3])});
+    if (part == 0) L[row] = none ? -INFINITY : (M + fast_log2(l)) * kLn2;
+}
+
+}  // namespace dev
+
+namespace detail {
+namespace {
+
+// The sizes of one launch: grid and slots.
+template <typename T, int D>
+struct PagedGrid {
+    using Shape = dev::PagedShapeOf<T, D>;
+    int per_head;         // 0: keys are not cut into chunks
+    long long many, few;  // items per key/value head at most, of either kind
+    int kv_heads;
+
+    PagedGrid(const PagedCall& call, bool shared, bool chunks_allowed) {
+        kv_heads = call.num_kv_heads;
+        const long long tokens = call.num_tokens;
+        const int group = call.num_heads / kv_heads;
+        dev::PagedTiles tiles =
+            dev::paged_tiles<Shape>(tokens, shared ? 1 : call.batch_size, group);
+        if (shared) {
+            const dev::PagedTiles own = dev::paged_tiles<Shape>(1, 1, group);
+            tiles.many += tokens * own.many;
+            tiles.few += tokens * own.few;
+        }
+        // Workgroups that run at once.
+        const long long at_once = (D <= 64 ? 2LL : 1LL) * compute_units();
+        const bool chunks =
+            chunks_allowed &&
+            (shared || tokens * group / Shape::kTile * kv_heads < 2 * at_once);
+        per_head = chunks ? static_cast<int>((at_once + kv_heads - 1) / kv_heads) : 0;
+        many = tiles.many ? tiles.many + per_head : 0;
+        few = tiles.few + per_head;
+    }
+    long long blocks() const { return (many + few) * kv_heads; }
+    size_t slots() const {  // rows of partial results
+        return static_cast<size_t>(kv_heads) * (many * Shape::kTile + few * 32);
+    }
+    size_t bytes() const {
+        return per_head ? slots() * (D * sizeof(float) + sizeof(float2)) : 0;
+    }
+};
+
+template <typename T, int D>
+FlashAttentionError run_paged(const PagedCall& call, hipStream_t stream) {
+    using E = typename dev::Mma<T>::elem;
+    using Eng = dev::PagedEngine<T, D>;
+    const bool shared = call.query_starts == nullptr;
+    dev::PagedArgs a{};
+    a.block_table = call.block_table;
+    a.prefix_table = call.prefix_table;
+    a.seq_lens = call.seq_lens;
+    a.starts = call.query_starts;
+    a.B = call.batch_size;
+    a.T = call.num_tokens;
+    a.H = call.num_heads;
+    a.Hkv = call.num_kv_heads;
+    a.group = a.H / a.Hkv;
+    a.page_size = call.page_size;
+    a.max_pages = call.max_pages;
+    a.cap = a.page_size * a.max_pages;
+    a.page_div = dev::fast_div(a.page_size);
+    a.group_div = dev::fast_div(a.group);
+    a.shared = shared;
+    a.causal = call.causal;
+    a.prefix = call.prefix_len;
+    // Loads from a multiple of their rows stay on one page, and their lane offsets fit 32 bits.
+    a.whole_groups = a.page_size % Eng::kGroupRows == 0 &&
+                     static_cast<long long>(a.Hkv) * D * Eng::kGroupRows * 4 < (1LL << 31);
+    a.c = call.scale * dev::kLog2e;
+    a.min_steps = 8;
+    a.min_rounds = 1;
+
+    // A graph's replays need memory that is theirs: the caller's. (Memory that the graph itself
+    // allocates, a recorded hipMallocAsync, was not there in the replay of two graphs in a row.)
+    const bool own = call.workspace == nullptr;
+    PagedGrid<T, D> grid(call, shared, true);
+    if (grid.per_head && own && stream_capturing(stream)) {
+        if (shared) return FlashAttentionError::OUT_OF_MEMORY;
+        grid = PagedGrid<T, D>(call, shared, false);
+    }
+    if (grid.blocks() > 0x7fffffffLL) return FlashAttentionError::INVALID_DIMENSION;
+    a.per_head = grid.per_head;
+    a.max_many = static_cast<int>(grid.many);
+    a.max_few = static_cast<int>(grid.few);
+    StreamWorkspace ws(stream, true);
+    if (grid.per_head) {
+        void* base = call.workspace;
+        if (own) {
+            FlashAttentionError err = ws.alloc(grid.bytes());
+            if (err != FlashAttentionError::SUCCESS) return err;
+            base = ws.get();
+        } else if (call.workspace_bytes < grid.bytes()) {
+            return FlashAttentionError::OUT_OF_MEMORY;
+        }
+        a.acc = static_cast<float*>(base);
+        a.ml = reinterpret_cast<float2*>(a.acc + grid.slots() * D);
+    }
+    ProfileEvents tok = profile_kernel<T, D>(shared ? "decode_shared" : "forward_paged");
+    launch_kernel(tok, (dev::paged_kernel<T, D>), dim3(static_cast<unsigned>(grid.blocks())),
+                  dim3(64 * Eng::kWaves), 0, stream, static_cast<const E*>(call.Q),
+                  static_cast<const E*>(call.K_cache), static_cast<const E*>(call.V_cache),
+                  static_cast<E*>(call.O), call.L, a);
+    FlashAttentionError err = from_hip(hipGetLastError());
+    if (err != FlashAttentionError::SUCCESS || !grid.per_head) return err;
+    constexpr int kRows = 256 / (D / 4);
+    tok = profile_kernel<T, D>("paged_combine");
+    launch_kernel(tok, (dev::paged_combine_kernel<T, D>),
+                  dim3(static_cast<unsigned>(a.T),
+                       static_cast<unsigned>((a.H + kRows - 1) / kRows)),
+                  dim3(256), 0, stream, static_cast<E*>(call.O), call.L, a);
+    return from_hip(hipGetLastError());
+}
+
+template <typename T, int D>
+long long workspace_of(const PagedCall& call) {
+    const PagedGrid<T, D> grid(call, call.prefix_len > 0, true);
+    return grid.blocks() > 0x7fffffffLL ? -1 : static_cast<long long>(grid.bytes());
+}
+
+}  // namespace
+
+template <typename T>
+long long paged_workspace(const PagedCall& c) {
+    return c.head_dim == 32   ? workspace_of<T, 32>(c)
+           : c.head_dim == 64 ? workspace_of<T, 64>(c)
+                              : workspace_of<T, 128>(c);
+}
+
+template <typename T>
+FlashAttentionError launch_paged(const PagedCall& c, hipStream_t stream) {
+    switch (c.head_dim) {
+        case 32:
+            return run_paged<T, 32>(c, stream);
+        case 64:
+            return run_paged<T, 64>(c, stream);
+        case 128:
+            return run_paged<T, 128>(c, stream);
+    }
+    return FlashAttentionError::UNSUPPORTED_HEAD_DIM;
+}
+#define CUFLASH_PAGED_TYPE(T)                              \
+    template long long paged_workspace<T>(const PagedCall&); \
+    template FlashAttentionError launch_paged<T>(const PagedCall&, hipStream_t);
+CUFLASH_PAGED_TYPE(float)
+CUFLASH_PAGED_TYPE(__half)
+CUFLASH_PAGED_TYPE(__hip_bfloat16)
+#undef CUFLASH_PAGED_TYPE
+
+}  // namespace detail
+}  // namespace cuflash

@@ -71,6 +71,10 @@ _BWD_EXT_ARGS = [ctypes.c_void_p] * 9 + [ctypes.c_int] * 6 + [ctypes.c_float, ct
 
 _APPEND_PAGED_ARGS = ([ctypes.c_void_p] * 11 + [ctypes.c_int] * 13 +
                       [ctypes.c_bool, ctypes.c_void_p])
+_FWD_PAGED_ARGS = ([ctypes.c_void_p] * 8 + [ctypes.c_int] * 7 +
+                   [ctypes.c_float, ctypes.c_bool, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p])
+_DEC_SHARED_ARGS = ([ctypes.c_void_p] * 8 + [ctypes.c_int] * 7 +
+                    [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p])
 
 EXPORTED_SYMBOLS = (
     "cuflash_attention_forward_f32", "cuflash_attention_forward_f16",
@@ -89,7 +93,9 @@ EXPORTED_SYMBOLS = (
 )
 
 # Declared in include/cuflash/paged_cache.h.
-PAGED_CACHE_SYMBOLS = tuple(f"cuflash_attention_{kind}_{sfx}" for kind in ("append_paged",)
+PAGED_CACHE_SYMBOLS = tuple(f"cuflash_attention_{kind}_{sfx}"
+                            for kind in ("append_paged", "forward_paged", "decode_shared",
+                                         "forward_paged_workspace", "decode_shared_workspace")
                             for sfx in ("f32", "f16", "bf16"))
 
 
@@ -116,6 +122,13 @@ class CuFlashLibrary:
             bwd_ext.argtypes, bwd_ext.restype = _BWD_EXT_ARGS, ctypes.c_int
             append = getattr(library, f"cuflash_attention_append_paged_{sfx}")
             append.argtypes, append.restype = _APPEND_PAGED_ARGS, ctypes.c_int
+            fwd_paged = getattr(library, f"cuflash_attention_forward_paged_{sfx}")
+            fwd_paged.argtypes, fwd_paged.restype = _FWD_PAGED_ARGS, ctypes.c_int
+            shared = getattr(library, f"cuflash_attention_decode_shared_{sfx}")
+            shared.argtypes, shared.restype = _DEC_SHARED_ARGS, ctypes.c_int
+            for kind, n in (("forward_paged", 5), ("decode_shared", 4)):
+                size = getattr(library, f"cuflash_attention_{kind}_workspace_{sfx}")
+                size.argtypes, size.restype = [ctypes.c_int] * n, ctypes.c_longlong
         noalloc = library.cuflash_attention_decode_noalloc_f16
         noalloc.argtypes, noalloc.restype = _DEC_ARGS, ctypes.c_int
         library.cuflash_error_string.argtypes = [ctypes.c_int]
@@ -427,6 +440,19 @@ def _output(given, like, shape, dtype, stream, name):
         return like.new_empty(shape, dtype=dtype)
 
 
+def _captured_workspace(lib, kind, like, stream, *sizes):
+    """Pointer and bytes of the workspace of a call that is being captured: torch's allocator gives it
+    from the graph's own pool. Eager calls use the library's: None, 0. The third value keeps it."""
+    torch = _torch()
+    if not torch.cuda.is_current_stream_capturing():
+        return None, 0, None
+    need = lib.fn(f"{kind}_workspace", _suffix(like))(*sizes)
+    if need <= 0:
+        return None, 0, None
+    ws = _output(None, like, (need,), torch.uint8, stream, "workspace")
+    return ws.data_ptr(), need, ws
+
+
 def _token_stride(x, name):
     """Elements from token to token of x [T, heads, D], whose heads lie side by side."""
     T, heads, D = x.shape
@@ -489,11 +515,73 @@ def flash_attention_append_paged(k, v, k_cache, v_cache, block_table, seq_lens,
     return out
 
 
+def flash_attention_forward_paged(q, k_cache, v_cache, block_table, seq_lens, query_starts,
+                                  scale: Optional[float] = None, causal: bool = False, out=None,
+                                  lse=None, stream=None, lib: Optional[CuFlashLibrary] = None):
+    """Attention of new tokens over a paged cache: q [T, H, D], tokens query_starts[b] ..
+    query_starts[b + 1] - 1 being the newest of sequence b, whose keys, theirs among them, number
+    seq_lens[b] (flash_attention_append_paged writes them). With `causal` a token sees the keys up
+    to its own. Cache and block table as in flash_attention_decode_paged.
+    -> O [T, H, D], L float32 [T, H] (cuflash_attention_forward_paged_*)."""
+    torch = _torch()
+    lib = lib or load_library()
+    B, _, page_size, Hkv, D = _check_paged((q,), k_cache, v_cache, block_table, seq_lens,
+                                           query_starts)
+    if q.dim() != 3 or q.shape[2] != D or not q.is_contiguous():
+        raise ValueError("expected contiguous q [T,H,D] of the cache's D")
+    T, H = q.shape[:2]
+    scale = float(D ** -0.5) if scale is None else float(scale)
+    out = _output(out, q, (T, H, D), q.dtype, stream, "out")
+    lse = _output(lse, q, (T, H), torch.float32, stream, "lse")
+    ws, ws_bytes, _keep = _captured_workspace(lib, "forward_paged", q, stream, T, B, H, Hkv, D)
+    status = lib.fn("forward_paged", _suffix(q))(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(),
+        block_table.data_ptr(), seq_lens.data_ptr(), query_starts.data_ptr(), T, B, H, Hkv,
+        page_size, block_table.shape[1], D, scale, bool(causal), ws, ws_bytes,
+        _stream_ptr(stream))
+    _raise(lib, status)
+    return out, lse
+
+
+def flash_attention_decode_shared(q, k_cache, v_cache, prefix_table, prefix_len: int, block_table,
+                                  seq_lens, scale: Optional[float] = None, out=None, lse=None,
+                                  stream=None, lib: Optional[CuFlashLibrary] = None):
+    """flash_attention_decode_paged for a batch whose first prefix_len keys are the same: they come
+    from the pages of prefix_table [pages] int32 and are read once for the batch, the keys from
+    prefix_len on from block_table (whose earlier entries are not used). seq_lens counts both.
+    -> O [B, H, 1, D], L [B, H, 1] (cuflash_attention_decode_shared_*)."""
+    torch = _torch()
+    lib = lib or load_library()
+    B, _, page_size, Hkv, D = _check_paged((q,), k_cache, v_cache, block_table, seq_lens)
+    if q.dim() != 4 or q.shape[0] != B or q.shape[2] != 1 or q.shape[3] != D \
+            or not q.is_contiguous():
+        raise ValueError("expected contiguous q [B,H,1,D] of the cache's D")
+    if prefix_table.dtype != torch.int32:
+        raise TypeError("prefix_table must be int32")
+    if prefix_table.device != q.device or prefix_table.dim() != 1 \
+            or not prefix_table.is_contiguous() \
+            or prefix_table.shape[0] * page_size < prefix_len:
+        raise ValueError("prefix_table must name the pages of prefix_len keys, on q's device")
+    H = q.shape[1]
+    scale = float(D ** -0.5) if scale is None else float(scale)
+    out = _output(out, q, (B, H, 1, D), q.dtype, stream, "out")
+    lse = _output(lse, q, (B, H, 1), torch.float32, stream, "lse")
+    ws, ws_bytes, _keep = _captured_workspace(lib, "decode_shared", q, stream, B, H, Hkv, D)
+    status = lib.fn("decode_shared", _suffix(q))(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(),
+        prefix_table.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), B, H, Hkv,
+        int(prefix_len), page_size, block_table.shape[1], D, scale, ws, ws_bytes,
+        _stream_ptr(stream))
+    _raise(lib, status)
+    return out, lse
+
+
 __all__ = [
     "CuFlashError", "CuFlashLibrary", "EXPORTED_SYMBOLS", "load_library",
     "candidate_library_paths", "flash_attention_forward", "flash_attention_backward",
     "flash_attention_forward_ext", "flash_attention_backward_ext", "flash_attention_decode",
-    "flash_attention_decode_paged", "flash_attention_append_paged", "PAGED_CACHE_SYMBOLS",
+    "flash_attention_decode_paged", "flash_attention_append_paged",
+    "flash_attention_forward_paged", "flash_attention_decode_shared", "PAGED_CACHE_SYMBOLS",
     "SUCCESS", "INVALID_DIMENSION", "DIMENSION_MISMATCH",
     "NULL_POINTER", "CUDA_ERROR", "OUT_OF_MEMORY", "UNSUPPORTED_HEAD_DIM", "UNSUPPORTED_DTYPE",
 ]

@@ -22,7 +22,7 @@
 //  * head_dim 32, 64 or 128; num_heads a multiple of num_kv_heads (query head h reads key/value
 //    head h / (num_heads / num_kv_heads)).
 //  * Pointers and token strides are multiples of 16 bytes. Every pointer is a device pointer.
-//    Calls are asynchronous on `stream` and can be captured into a HIP graph.
+//    Calls are asynchronous on `stream` and can be captured into a HIP graph (see Workspaces).
 // Validation, in this order: null pointers (NULL_POINTER), dimensions that are not positive
 // (INVALID_DIMENSION), head_dim (UNSUPPORTED_HEAD_DIM), scale (INVALID_DIMENSION), then the
 // relations between sizes (DIMENSION_MISMATCH), sizes whose products exceed 32 bits and alignment
@@ -74,13 +74,77 @@ CUFLASH_EXPORT FlashAttentionError flash_attention_append_paged(
     int q_stride, int k_stride, int v_stride, int num_pages, int page_size, int max_pages_per_seq,
     int head_dim, int rotary_dim, int max_positions, bool interleaved, hipStream_t stream = 0);
 
+// ---- Workspaces of the two attentions ----
+// Keys that are cut into chunks leave partial results in a workspace. With workspace null the library
+// uses its own per-stream buffer, as every call with a workspace does (see
+// cuflash_release_workspaces). A call that is captured into a graph gets its workspace from the
+// caller: a device buffer of the size that cuflash_attention_forward_paged_workspace_* and
+// cuflash_attention_decode_shared_workspace_* return for its sizes, 256-byte aligned, that stays
+// allocated as long as the graph and is not used by other work while a replay runs (graphs that are
+// replayed one after the other may share it). Captured without one, the forward runs in one chunk,
+// slower where few tokens meet long caches and with sums in another order, and the shared decode is
+// refused: OUT_OF_MEMORY. A workspace that is given is used by eager calls too; one that is too small
+// is OUT_OF_MEMORY, one that is not aligned INVALID_DIMENSION.
+// ---- Several new tokens of every sequence ----
+// O = softmax(scale Q K^T) V over the cache, L the logsumexp: Q, O [num_tokens, num_heads,
+// head_dim], L [num_tokens, num_heads] float. Token t of sequence b sees all seq_lens[b] keys (fewer
+// where the block table ends before), with `causal` those up to its own position. A query that sees
+// no key, or whose scores are all -inf, has O = 0 and L = -inf. Cache rows from seq_lens[b] on and
+// table entries past a sequence's pages are not read. A sequence whose pages are wanted must name
+// pages of the cache (they are not range-checked).
+CUFLASH_EXPORT FlashAttentionError flash_attention_forward_paged(
+    const float* Q, const float* K_cache, const float* V_cache, float* O, float* L,
+    const int* block_table, const int* seq_lens, const int* query_starts, int num_tokens,
+    int batch_size, int num_heads, int num_kv_heads, int page_size, int max_pages_per_seq,
+    int head_dim, float scale, bool causal, void* workspace,
+    size_t workspace_bytes, hipStream_t stream = 0);
+CUFLASH_EXPORT FlashAttentionError flash_attention_forward_paged(
+    const __half* Q, const __half* K_cache, const __half* V_cache, __half* O, float* L,
+    const int* block_table, const int* seq_lens, const int* query_starts, int num_tokens,
+    int batch_size, int num_heads, int num_kv_heads, int page_size, int max_pages_per_seq,
+    int head_dim, float scale, bool causal, void* workspace,
+    size_t workspace_bytes, hipStream_t stream = 0);
+CUFLASH_EXPORT FlashAttentionError flash_attention_forward_paged(
+    const __hip_bfloat16* Q, const __hip_bfloat16* K_cache, const __hip_bfloat16* V_cache,
+    __hip_bfloat16* O, float* L, const int* block_table, const int* seq_lens,
+    const int* query_starts, int num_tokens, int batch_size, int num_heads, int num_kv_heads,
+    int page_size, int max_pages_per_seq, int head_dim, float scale, bool causal, void* workspace,
+    size_t workspace_bytes, hipStream_t stream = 0);
+
+// ---- Decode of a batch that shares its first keys ----
+// flash_attention_decode_paged for sequences whose first prefix_len keys are the same: these are read
+// from the pages that prefix_table (int32, ceil(prefix_len / page_size) of them) names, once for the
+// batch, the others from block_table. Q, O [batch_size, num_heads, 1, head_dim], L [batch_size,
+// num_heads] float. seq_lens counts all keys of a sequence, the shared ones among them; positions stay
+// what they are, so block_table[b][j / page_size] is read for the keys j >= prefix_len only (where the
+// prefix ends inside a page, that entry is the sequence's own page, whose first rows are not read). A
+// sequence shorter than the prefix sees its first seq_lens[b] keys. prefix_len 0 is
+// flash_attention_decode_paged; prefix_len past the block table's capacity is DIMENSION_MISMATCH.
+CUFLASH_EXPORT FlashAttentionError flash_attention_decode_shared(
+    const float* Q, const float* K_cache, const float* V_cache, float* O, float* L,
+    const int* prefix_table, const int* block_table, const int* seq_lens, int batch_size,
+    int num_heads, int num_kv_heads, int prefix_len, int page_size, int max_pages_per_seq,
+    int head_dim, float scale, void* workspace, size_t workspace_bytes, hipStream_t stream = 0);
+CUFLASH_EXPORT FlashAttentionError flash_attention_decode_shared(
+    const __half* Q, const __half* K_cache, const __half* V_cache, __half* O, float* L,
+    const int* prefix_table, const int* block_table, const int* seq_lens, int batch_size,
+    int num_heads, int num_kv_heads, int prefix_len, int page_size, int max_pages_per_seq,
+    int head_dim, float scale, void* workspace, size_t workspace_bytes, hipStream_t stream = 0);
+CUFLASH_EXPORT FlashAttentionError flash_attention_decode_shared(
+    const __hip_bfloat16* Q, const __hip_bfloat16* K_cache, const __hip_bfloat16* V_cache,
+    __hip_bfloat16* O, float* L, const int* prefix_table, const int* block_table,
+    const int* seq_lens, int batch_size, int num_heads, int num_kv_heads, int prefix_len,
+    int page_size, int max_pages_per_seq, int head_dim, float scale, void* workspace,
+    size_t workspace_bytes, hipStream_t stream = 0);
+
 }  // namespace cuflash
 
 #ifdef __cplusplus
 extern "C" {
 #endif
 
-// C ABI of the functions above; the integer value of cuflash::FlashAttentionError.
+// C ABI of the functions above; the integer value of cuflash::FlashAttentionError. The workspace
+// sizes: bytes for a call of these sizes, 0 where none is needed, -1 where it would be refused.
 #define CUFLASH_DECLARE_PAGED_CACHE(SFX, T)                                                       \
     CUFLASH_EXPORT int cuflash_attention_append_paged_##SFX(                                      \
         const T* Q, const T* K, const T* V, T* Q_out, T* K_cache, T* V_cache,                     \
@@ -88,7 +152,21 @@ extern "C" {
         const float* rope_cos, const float* rope_sin, int num_tokens, int batch_size,             \
         int num_heads, int num_kv_heads, int q_stride, int k_stride, int v_stride, int num_pages, \
         int page_size, int max_pages_per_seq, int head_dim, int rotary_dim, int max_positions,    \
-        bool interleaved, hipStream_t stream);
+        bool interleaved, hipStream_t stream);                                                    \
+    CUFLASH_EXPORT int cuflash_attention_forward_paged_##SFX(                                     \
+        const T* Q, const T* K_cache, const T* V_cache, T* O, float* L, const int* block_table,   \
+        const int* seq_lens, const int* query_starts, int num_tokens, int batch_size,             \
+        int num_heads, int num_kv_heads, int page_size, int max_pages_per_seq, int head_dim,      \
+        float scale, bool causal, void* workspace, size_t workspace_bytes, hipStream_t stream);   \
+    CUFLASH_EXPORT long long cuflash_attention_forward_paged_workspace_##SFX(                     \
+        int num_tokens, int batch_size, int num_heads, int num_kv_heads, int head_dim);           \
+    CUFLASH_EXPORT int cuflash_attention_decode_shared_##SFX(                                     \
+        const T* Q, const T* K_cache, const T* V_cache, T* O, float* L, const int* prefix_table,  \
+        const int* block_table, const int* seq_lens, int batch_size, int num_heads,               \
+        int num_kv_heads, int prefix_len, int page_size, int max_pages_per_seq, int head_dim,     \
+        float scale, void* workspace, size_t workspace_bytes, hipStream_t stream);                \
+    CUFLASH_EXPORT long long cuflash_attention_decode_shared_workspace_##SFX(                     \
+        int batch_size, int num_heads, int num_kv_heads, int head_dim);
 CUFLASH_DECLARE_PAGED_CACHE(f32, float)
 CUFLASH_DECLARE_PAGED_CACHE(f16, __half)
 CUFLASH_DECLARE_PAGED_CACHE(bf16, __hip_bfloat16)

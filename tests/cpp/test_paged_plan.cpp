@@ -1,0 +1,200 @@
+// The cut of a paged attention into workgroups (cuflash-attn_amd/csrc/paged_plan.hpp) on the host: the
+// code that the kernels run, over random launches, tokens and lengths, with every index that becomes an
+// address checked against the array it goes to. No GPU call is made.
+//
+// Checked for each launch: every row of every unit meets every key it sees in exactly one item; items
+// are numbered below the grid and partial results below the slots; direct items are the only ones of
+// their rows; the combine finds the slot that an item wrote; items of causal tiles end where their last
+// row's keys do; fast_div divides.
+//
+// Arguments: the number of launches, the seed.
+
+#include <algorithm>
+#include <array>
+#include <cmath>
+#include <cstdio>
+#include <cstdlib>
+#include <map>
+#include <random>
+#include <vector>
+
+#include "paged_plan.hpp"
+
+namespace {
+
+using namespace cuflash::dev;
+
+struct HostWave {
+    using Int = std::array<int, 64>;
+    template <class F>
+    static Int each(F f) {
+        Int v;
+        for (int i = 0; i < 64; ++i) v[i] = f(i);
+        return v;
+    }
+    template <class F>
+    static Int map2(const Int& x, const Int& y, F f) {
+        return each([&](int i) { return f(x[i], y[i]); });
+    }
+    static Int scan(Int v) {
+        for (int i = 1; i < 64; ++i) {
+            if (v[i] < 0 || __builtin_add_overflow(v[i], v[i - 1], &v[i])) std::abort();
+        }
+        return v;
+    }
+    static int lane(const Int& v, int i) {
+        if (i < 0 || i >= 64) std::abort();
+        return v[i];
+    }
+    template <class F>
+    static int first(const Int& v, F f) {
+        for (int i = 0; i < 64; ++i)
+            if (f(v[i])) return i;
+        return -1;
+    }
+};
+
+int g_case = 0;
+#define CHECK(cond)                                                            \
+    do {                                                                       \
+        if (!(cond)) {                                                         \
+            std::printf("launch %d, line %d: %s\n", g_case, __LINE__, #cond); \
+            std::exit(1);                                                      \
+        }                                                                      \
+    } while (0)
+
+int spread(std::mt19937& rng, int lo, int hi) {  // over the logarithm
+    std::uniform_real_distribution<double> u(std::log(double(lo)), std::log(double(hi) + 1.0));
+    return std::min(hi, std::max(lo, int(std::exp(u(rng)))));
+}
+
+template <class Shape>
+bool launch(std::mt19937& rng) {  // whether something was cut into chunks
+    auto pick = [&](int n) { return int(rng() % unsigned(n)); };
+    PagedArgs a{};
+    a.Hkv = std::array<int, 4>{1, 2, 8, 12}[pick(4)];
+    a.group = std::array<int, 6>{1, 2, 3, 4, 8, 40}[pick(6)];
+    a.H = a.Hkv * a.group;
+    a.group_div = fast_div(a.group);
+    a.page_size = std::array<int, 6>{1, 6, 16, 24, 64, 256}[pick(6)];
+    a.page_div = fast_div(a.page_size);
+    a.B = spread(rng, 1, 200);
+    a.max_pages = spread(rng, 1, std::max(1, 40000 / a.page_size));
+    a.cap = a.page_size * a.max_pages;
+    a.shared = pick(3) == 0;
+    a.causal = !a.shared && pick(3) > 0;
+    a.min_steps = 1 + pick(8);
+    a.min_rounds = 1 + pick(2);
+    std::vector<int> lens(a.B), starts(a.B + 1);
+    const int most = spread(rng, 1, a.shared ? 1 : 3000);
+    const int kind = pick(4);
+    for (int b = 0; b < a.B; ++b) {
+        const int n = a.shared ? 1 : kind == 0 ? pick(2) : kind == 1 ? (b == 0 ? most : 1)
+                                                         : pick(most + 1);
+        starts[b + 1] = starts[b] + n;
+        lens[b] = pick(5) == 0 ? pick(40) : spread(rng, 1, a.cap);
+        if (pick(3) > 0) lens[b] = std::max(lens[b], n);
+        if (pick(20) == 0) lens[b] = -pick(9);
+        if (pick(20) == 0) lens[b] = a.cap + pick(1000);
+    }
+    a.T = starts[a.B];
+    if (a.T == 0) return false;
+    if (!a.shared && pick(4) == 0) a.T += pick(50);        // padding
+    if (!a.shared && pick(8) == 0) a.T = std::max(1, a.T - pick(50));  // starts past the tokens
+    a.seq_lens = lens.data();
+    a.starts = starts.data();
+    a.prefix = a.shared ? spread(rng, 1, a.cap) : 0;
+
+    PagedTiles t = a.shared ? paged_tiles<Shape>(a.B, 1, a.group)
+                            : paged_tiles<Shape>(a.T, a.B, a.group);
+    if (a.shared) t.few += static_cast<long long>(a.B) * ((a.group + 31) / 32);
+    if (a.shared && a.group > kManyRows) return false;
+    a.per_head = pick(4) == 0 ? 0 : spread(rng, 1, 300);
+    a.max_many = t.many > 0 ? int(t.many) + a.per_head : 0;
+    a.max_few = int(t.few) + a.per_head;
+
+    using Plan = PagedPlan<Shape, HostWave>;
+    const auto first = Plan::batch(a, 0);
+    const PagedCut cut = Plan::cut(a, first);
+    CHECK(cut.many <= a.max_many && cut.few <= a.max_few);
+    bool chunked = false;
+    // (unit, tile row) -> the key ranges of its items; slots taken.
+    std::map<std::pair<int, int>, std::vector<std::array<int, 2>>> met;
+    std::map<std::pair<bool, int>, int> slots;
+    const int grid = a.max_many + a.max_few;
+    for (int x = 0; x < grid + 3; ++x) {
+        const PagedItem it = paged_item<Shape, HostWave>(a, x);
+        CHECK(it.found == (x < cut.many + cut.few));
+        if (!it.found) continue;
+        CHECK(x < grid);
+        CHECK(it.u >= 0 && it.u < paged_units(a));
+        const PagedUnit u = paged_unit(a, it.u);
+        CHECK(u.t0 >= 0 && u.n > 0 && u.t0 + u.n <= a.T && it.rows == u.n * a.group);
+        CHECK(it.many == (it.rows > kManyRows));
+        const int tile = it.many ? Shape::kTile : 32;
+        CHECK(it.r0 >= 0 && it.r0 % tile == 0 && it.r0 < it.rows);
+        CHECK(it.kbeg >= u.kbeg && it.kend <= u.kend);
+        CHECK(it.index >= 0 && it.index < (it.many ? a.max_many : a.max_few));
+        const int taken = ++slots[{it.many, it.index}];
+        CHECK(taken == 1);
+        const int last = a.group_div(std::min(it.rows, it.r0 + tile) - 1);
+        if (a.causal) CHECK(it.kend <= paged_limit(a, it.u, u, last));
+        auto& ranges = met[{it.u, it.r0}];
+        CHECK(!it.direct || ranges.empty());
+        ranges.push_back({it.kbeg, it.kend});
+        const PagedUnitItems ui = paged_unit_items<Shape, HostWave>(a, cut, first, it.u);
+        CHECK(ui.many == it.many);
+        CHECK(it.direct == (ui.chunks == 1 && !a.shared));
+        chunked |= ui.chunks > 1;
+        const int i = it.r0 / tile;
+        const int at = it.index - ui.first;
+        CHECK(at >= 0 && at < ui.tiles * ui.chunks);
+        CHECK(at % ui.tiles == (a.causal ? ui.tiles - 1 - i : i));
+        const size_t row = paged_slot_row<Shape>(a, a.Hkv - 1, it.many, it.index, tile - 1);
+        CHECK(row < static_cast<size_t>(a.Hkv) * a.max_many * Shape::kTile +
+                        static_cast<size_t>(a.Hkv) * a.max_few * 32);
+    }
+    for (int u = 0; u < paged_units(a); ++u) {
+        const PagedUnit pu = paged_unit(a, u);
+        const int rows = pu.n * a.group;
+        const int tile = rows > kManyRows ? Shape::kTile : 32;
+        const PagedUnitItems ui = paged_unit_items<Shape, HostWave>(a, cut, first, u);
+        if (pu.n > 0) CHECK(ui.chunks == 0 || ui.tiles == (rows + tile - 1) / tile);
+        for (int r0 = 0; r0 < rows; r0 += tile) {
+            auto ranges = met[{u, r0}];
+            CHECK(int(ranges.size()) == ui.chunks);
+            std::sort(ranges.begin(), ranges.end());
+            int at = pu.kbeg;  // keys below `at` are met
+            for (auto& k : ranges) {
+                if (k[1] <= k[0]) continue;
+                CHECK(k[0] == at);
+                at = k[1];
+            }
+            for (int r : {r0, std::min(rows, r0 + tile) - 1}) {
+                const int lim = paged_limit(a, u, pu, a.group_div(r));
+                CHECK(lim <= at || lim <= pu.kbeg);
+                CHECK(lim <= pu.kend && lim >= 0);
+            }
+        }
+    }
+    return chunked;
+}
+
+}  // namespace
+
+int main(int argc, char** argv) {
+    const int n = argc > 1 ? std::atoi(argv[1]) : 1000;
+    std::mt19937 rng(argc > 2 ? std::atoi(argv[2]) : 1);
+    for (int i = 0; i < 200000; ++i) {
+        const int d = 1 + int(rng() >> (1 + rng() % 31)), v = int(rng() >> 1);
+        const FastDiv f = fast_div(std::max(1, d));
+        for (int x : {v, 0x7fffffff, 0, v / d * d, std::max(0, v / d * d - 1)}) CHECK(f(x) == x / d);
+    }
+    int chunked = 0;
+    for (g_case = 0; g_case < n; ++g_case) {
+        chunked += g_case % 2 ? launch<PagedShape<256, 64, 256>>(rng)
+                              : launch<PagedShape<128, 32, 128>>(rng);
+    }
+    std::printf("%d launches, %d of them with chunks\n", n, chunked);
+    return chunked > n / 10 ? 0 : 1;
+}

@@ -13,7 +13,7 @@ import pytest
 import cuflash_attn
 from conftest import REPO
 from cuflash_attn import (DIMENSION_MISMATCH, INVALID_DIMENSION, NULL_POINTER,
-                          UNSUPPORTED_HEAD_DIM)
+                          OUT_OF_MEMORY, UNSUPPORTED_HEAD_DIM)
 
 HEADER = os.path.join(REPO, "include", "cuflash", "paged_cache.h")
 
@@ -34,7 +34,7 @@ def _call(lib, kind, sfx, ok, **kw):
 
 def test_every_declared_symbol_is_bound_and_exported(lib):
     text = open(HEADER).read()
-    declared = {m.replace("##SFX", s) for m in re.findall(r"int (cuflash_\w+##SFX)\(", text)
+    declared = {m.replace("##SFX", s) for m in re.findall(r"(cuflash_\w+##SFX)\(", text)
                 for s in ("f32", "f16", "bf16")}
     assert declared == set(cuflash_attn.PAGED_CACHE_SYMBOLS)
     out = subprocess.run(["nm", "-D", "--defined-only", lib.path], capture_output=True, text=True,
@@ -76,6 +76,68 @@ def test_append_refusals(lib, sfx):
     assert call(k=None, d=48, tokens=0) == NULL_POINTER
     assert call(tokens=0, d=48) == INVALID_DIMENSION
     assert call(d=48, kv_heads=3) == UNSUPPORTED_HEAD_DIM
+
+FORWARD = dict(q=P, k_cache=P, v_cache=P, o=P, l=P, table=P, lens=P, starts=P, tokens=8, batch=2,
+               heads=8, kv_heads=2, page=16, max_pages=3, d=64, scale=0.125, causal=True,
+               ws=None, ws_bytes=0, stream=None)
+SHARED = dict(q=P, k_cache=P, v_cache=P, o=P, l=P, prefix_table=P, table=P, lens=P, batch=2,
+              heads=8, kv_heads=2, prefix=20, page=16, max_pages=3, d=64, scale=0.125,
+              ws=None, ws_bytes=0, stream=None)
+
+
+@pytest.mark.parametrize("sfx", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kind,ok", [("forward_paged", FORWARD), ("decode_shared", SHARED)])
+def test_attention_refusals(lib, sfx, kind, ok):
+    def call(**kw):
+        return _call(lib, kind, sfx, ok, **kw)
+
+    for name in (n for n in ok if ok[n] == P):
+        assert call(**{name: None}) == NULL_POINTER, name
+    for name in ("tokens", "batch", "heads", "kv_heads", "page", "max_pages", "d"):
+        for bad in (0, -1):
+            if name in ok:
+                assert call(**{name: bad}) == INVALID_DIMENSION, name
+    for d in (16, 48, 96, 256):
+        assert call(d=d) == UNSUPPORTED_HEAD_DIM
+    for scale in (float("nan"), float("inf"), -1.0):
+        assert call(scale=scale) == INVALID_DIMENSION
+    assert call(kv_heads=3) == DIMENSION_MISMATCH
+    assert call(page=1 << 16, max_pages=1 << 16) == INVALID_DIMENSION
+    many = {"tokens": 1 << 28} if "tokens" in ok else {"batch": 1 << 28}
+    assert call(**many) == INVALID_DIMENSION  # tokens times heads beyond 32 bits
+    for name in ("q", "k_cache", "v_cache", "o"):
+        assert call(**{name: P + 8}) == INVALID_DIMENSION, name
+    assert call(ws=(P + 255) // 256 * 256 + 16, ws_bytes=1 << 30) == INVALID_DIMENSION
+    assert call(ws=(P + 255) // 256 * 256, ws_bytes=16) == OUT_OF_MEMORY
+    if kind == "decode_shared":
+        assert call(prefix=-1) == INVALID_DIMENSION
+        assert call(prefix=49) == DIMENSION_MISMATCH  # past the block table
+    assert call(q=None, d=48) == NULL_POINTER
+    assert call(heads=0, d=48) == INVALID_DIMENSION
+    assert call(d=48, scale=-1.0) == UNSUPPORTED_HEAD_DIM
+    assert call(scale=-1.0, kv_heads=3) == INVALID_DIMENSION
+
+
+@pytest.mark.parametrize("sfx", ["f32", "f16", "bf16"])
+def test_grids_beyond_32_bits_are_refused(lib, sfx):
+    """One token each of many sequences, one key/value head for every query head: valid sizes whose
+    workgroups are too many."""
+    n = 1 << 22
+    assert _call(lib, "forward_paged", sfx, FORWARD, tokens=n, batch=n, heads=500, kv_heads=500,
+                 d=32) == INVALID_DIMENSION
+
+
+@pytest.mark.parametrize("sfx", ["f32", "f16", "bf16"])
+def test_workspace_sizes(lib, sfx):
+    forward, shared = (lib.fn(f"{kind}_workspace", sfx) for kind in ("forward_paged",
+                                                                     "decode_shared"))
+    assert forward(4, 2, 8, 2, 64) > 0 and shared(4, 8, 2, 64) > 0
+    assert forward(1 << 20, 2, 8, 2, 64) == 0  # enough rows without chunks
+    for bad in ((0, 2, 8, 2, 64), (4, -1, 8, 2, 64), (4, 2, 8, 3, 64), (4, 2, 8, 2, 48),
+                (1 << 28, 2, 8, 2, 64)):
+        assert forward(*bad) == -1
+    for bad in ((0, 8, 2, 64), (4, 8, 3, 64), (4, 8, 2, 256)):
+        assert shared(*bad) == -1
 
 
 class _Fake:
@@ -129,3 +191,40 @@ def test_append_helper_refusals(monkeypatch):
     refused("needs q", out=f(4, 2, 64))
     with pytest.raises(cuflash_attn.CuFlashError):
         append(**dict(good, k_cache=f(3, 16, 2, 64, dtype=torch.float64)), lib=object())
+
+
+def test_attention_helper_refusals(monkeypatch):
+    import torch
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    f = lambda *s, **k: _Fake(torch.zeros(s, **k))  # noqa: E731
+    i = dict(dtype=torch.int32)
+    good = _fakes(torch)
+    del good["k"], good["v"]
+    forward = dict(good, q=f(4, 4, 64))
+    shared = dict(good, q=f(2, 4, 1, 64), prefix_table=f(2, **i), prefix_len=20)
+    del shared["query_starts"]
+
+    def refused(fn, args, match, error=ValueError, **kw):
+        with pytest.raises(error, match=match):
+            fn(**dict(args, **kw), lib=object())
+
+    fwd, dec = cuflash_attn.flash_attention_forward_paged, cuflash_attn.flash_attention_decode_shared
+    refused(fwd, forward, r"q \[T,H,D\]", q=f(4, 4, 32))
+    refused(fwd, forward, r"q \[T,H,D\]", q=_Fake(torch.zeros(4, 64, 4).transpose(1, 2)))
+    refused(fwd, forward, "one dtype", q=f(4, 4, 64, dtype=torch.float16))
+    refused(fwd, forward, "query_starts", query_starts=f(4, **i))
+    refused(fwd, forward, "16 bytes", q=_Fake(torch.zeros(4 * 4 * 64 + 1)[1:].view(4, 4, 64)))
+    refused(dec, shared, r"q \[B,H,1,D\]", q=f(3, 4, 1, 64))
+    refused(dec, shared, r"q \[B,H,1,D\]", q=f(2, 4, 2, 64))
+    refused(dec, shared, "int32", TypeError, prefix_table=f(2))
+    for fn, args in ((fwd, forward), (dec, shared)):
+        with pytest.raises(ValueError, match="on the GPU"):
+            fn(**dict(args, q=torch.zeros(4, 4, 64)), lib=object())
+
+
+def test_cut_into_workgroups_stays_in_bounds(tmp_path):
+    """The host run of the kernels' plan (tests/cpp/test_paged_plan.cpp)."""
+    from test_host_rules import run_program
+
+    run_program("test_paged_plan", tmp_path, 6000, 1)
