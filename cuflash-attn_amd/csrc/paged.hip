@@ -32,11 +32,15 @@ namespace cuflash {
 namespace dev {
 
 // What differs between the types: tiles of 32 keys in LDS and the block over one of them.
-template <typename T, int D>
+template <typename T_, int D_, int NW>
 struct PagedEngine {
+    using T = T_;
+    static constexpr int D = D_;
     using Lay = TileGroups<D>;
     using Frag = typename Elem<T>::frag;
-    static constexpr int kWaves = 8;
+    static constexpr int kWaves = NW;
+    static constexpr int kPerCu = D <= 64 || NW <= 4 ? 2 : 1;  // workgroups (LDS)
+    static constexpr int kRoundCost = 2;
     static constexpr int kStepBlocks = 2;              // 32-key blocks of a step (many rows)
     static constexpr int kGroupRows = Lay::kRows;      // key rows of one load
     static constexpr int kGroups = 32 / kGroupRows;    // loads of a tile
@@ -76,9 +80,13 @@ struct PagedEngine {
 // c ^ (r & kSwizzle): 16 rows read at one chunk fall into 16 bank slots (8 at head_dim 32). Lane
 // half h supplies chunk 2 j + h of both K and Q to the four products of step j: any assignment of
 // the k index does, as long as both agree. The scores and P stay in fp32.
-template <int D>
-struct PagedEngine<float, D> {
-    static constexpr int kWaves = 4;
+template <int D_, int NW>
+struct PagedEngine<float, D_, NW> {
+    using T = float;
+    static constexpr int D = D_;
+    static constexpr int kWaves = NW;
+    static constexpr int kPerCu = D <= 64 ? 2 : 1;
+    static constexpr int kRoundCost = 1;
     static constexpr int kStepBlocks = 1;
     static constexpr int kGroupRows = 256 / D;
     static constexpr int kGroups = 32 / kGroupRows;
@@ -171,9 +179,9 @@ struct PagedEngine<float, D> {
     }
 };
 
-template <typename T, int D>
-using PagedShapeOf = PagedShape<32 * PagedEngine<T, D>::kWaves, 32 * PagedEngine<T, D>::kStepBlocks,
-                                32 * PagedEngine<T, D>::kWaves>;
+template <class Eng>
+using PagedShapeOf =
+    PagedShape<32 * Eng::kWaves, 32 * Eng::kStepBlocks, 32 * Eng::kWaves, Eng::kRoundCost>;
 
 // The rows of one key/value head in the cache, from their position in a sequence.
 template <typename E>
@@ -197,9 +205,10 @@ struct CacheRows {
     }
 };
 
-template <typename T, int D>
+template <class Eng>
 struct PagedWork {
-    using Eng = PagedEngine<T, D>;
+    using T = typename Eng::T;
+    static constexpr int D = Eng::D;
     using E = typename Mma<T>::elem;
     const E* Q;
     const E* K;  // of the item's key/value head
@@ -269,8 +278,8 @@ struct PagedWork {
                                              float (*s_l)[32]) const;
 };
 
-template <typename T, int D>
-__device__ __forceinline__ void PagedWork<T, D>::many_rows(unsigned char* smem) const {
+template <class Eng>
+__device__ __forceinline__ void PagedWork<Eng>::many_rows(unsigned char* smem) const {
     constexpr int kBlocks = Eng::kStepBlocks;
     constexpr int kStep = 32 * kBlocks;
     constexpr int kBytes = kBlocks * Eng::kTile;  // of a step's K or V
@@ -340,7 +349,7 @@ __device__ __forceinline__ void PagedWork<T, D>::many_rows(unsigned char* smem) 
     if (!it.direct) {
         if (!on) return;
         const size_t slot =
-            paged_slot_row<PagedShapeOf<T, D>>(a, hk, true, it.index, wave * 32 + l32);
+            paged_slot_row<PagedShapeOf<Eng>>(a, hk, true, it.index, wave * 32 + l32);
         float* dst = a.acc + slot * D + 4 * g2;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) {
@@ -393,8 +402,8 @@ __device__ __forceinline__ void PagedWork<T, D>::many_rows(unsigned char* smem) 
     if (g2 == 0 && on) L[orow] = none ? -INFINITY : (m + fast_log2(l)) * kLn2;
 }
 
-template <typename T, int D>
-__device__ __forceinline__ void PagedWork<T, D>::few_rows(unsigned char* smem, float (*s_m)[32],
+template <class Eng>
+__device__ __forceinline__ void PagedWork<Eng>::few_rows(unsigned char* smem, float (*s_m)[32],
                                                           float (*s_l)[32]) const {
     constexpr int NW = Eng::kWaves;
     constexpr int kLoads = Eng::kGroups;
@@ -511,7 +520,7 @@ __device__ __forceinline__ void PagedWork<T, D>::few_rows(unsigned char* smem, f
             }
         }
         if (!it.direct) {
-            const size_t slot = paged_slot_row<PagedShapeOf<T, D>>(a, hk, false, it.index, r);
+            const size_t slot = paged_slot_row<PagedShapeOf<Eng>>(a, hk, false, it.index, r);
 #pragma unroll
             for (int u = 0; u < kPiece; u += 4)
                 st16(a.acc + slot * D + cc + u,
@@ -530,13 +539,15 @@ __device__ __forceinline__ void PagedWork<T, D>::few_rows(unsigned char* smem, f
     }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__((64 * PagedEngine<T, D>::kWaves), (D <= 64 ? 2 : 1))
-    paged_kernel(const typename Mma<T>::elem* __restrict__ Q,
-                 const typename Mma<T>::elem* __restrict__ K,
-                 const typename Mma<T>::elem* __restrict__ V,
-                 typename Mma<T>::elem* __restrict__ O, float* __restrict__ L, PagedArgs a) {
-    using Eng = PagedEngine<T, D>;
+// Second launch bound: waves per SIMD of the workgroups that share a CU.
+template <class Eng>
+__global__ void __launch_bounds__((64 * Eng::kWaves), (Eng::kPerCu * Eng::kWaves / 4))
+    paged_kernel(const typename Mma<typename Eng::T>::elem* __restrict__ Q,
+                 const typename Mma<typename Eng::T>::elem* __restrict__ K,
+                 const typename Mma<typename Eng::T>::elem* __restrict__ V,
+                 typename Mma<typename Eng::T>::elem* __restrict__ O, float* __restrict__ L,
+                 PagedArgs a) {
+    constexpr int D = Eng::D;
     constexpr int kBytes = Eng::kWaves * 2 * Eng::kTile;
     static_assert(kBytes >= 4 * Eng::kStepBlocks * Eng::kTile, "either kind's tiles");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[kBytes];
@@ -545,12 +556,22 @@ __global__ void __launch_bounds__((64 * PagedEngine<T, D>::kWaves), (D <= 64 ? 2
     // The items of a key/value head stay on one XCD where the heads can be dealt out evenly.
     int hk, x;
     head_rank_order(blockIdx.x, a.Hkv, hk, x);
-    const PagedItem it = paged_item<PagedShapeOf<T, D>, GpuWave>(a, x);
+    const PagedItem it = paged_item<PagedShapeOf<Eng>, GpuWave>(a, x);
     if (!it.found) return;
+    if (a.wgs > 0 && it.first && hk == 0 && threadIdx.x == 0)
+        a.units[it.u] = make_int4(it.of.first, it.of.tiles, it.of.chunks, it.many);
+    if (!it.direct && it.kend <= it.kbeg) {
+        // No keys of this chunk for these rows (a causal mask): nothing but the mark of an empty part.
+        const int n = min(it.rows - it.r0, it.many ? PagedShapeOf<Eng>::kTile : 32);
+        for (int r = threadIdx.x; r < n; r += 64 * Eng::kWaves)
+            a.ml[paged_slot_row<PagedShapeOf<Eng>>(a, hk, it.many, it.index, r)] =
+                make_float2(-INFINITY, 0.0f);
+        return;
+    }
     const int* table = !a.shared    ? a.block_table + static_cast<size_t>(it.u) * a.max_pages
                        : it.u == 0 ? a.prefix_table
                                    : a.block_table + static_cast<size_t>(it.u - 1) * a.max_pages;
-    const PagedWork<T, D> work{Q,
+    const PagedWork<Eng> work{Q,
                                K + static_cast<size_t>(hk) * D,
                                V + static_cast<size_t>(hk) * D,
                                O,
@@ -571,15 +592,17 @@ __global__ void __launch_bounds__((64 * PagedEngine<T, D>::kWaves), (D <= 64 ? 2
 // Merges the parts of each row: O = sum O_i 2^(m_i - M) / l with M = max m_i and l = sum l_i
 // 2^(m_i - M), L = (M + log2 l) ln 2. One workgroup per token and 256 / (D / 4) query heads, D / 4
 // lanes a row, four columns each; kBatch parts of a row in flight.
-template <typename T, int D>
+template <class Eng>
 __global__ void __launch_bounds__(256)
-    paged_combine_kernel(typename Mma<T>::elem* __restrict__ O, float* __restrict__ L,
-                         PagedArgs a) {
+    paged_combine_kernel(typename Mma<typename Eng::T>::elem* __restrict__ O,
+                         float* __restrict__ L, PagedArgs a) {
+    using T = typename Eng::T;
     using E = typename Mma<T>::elem;
-    using Shape = PagedShapeOf<T, D>;
+    using Shape = PagedShapeOf<Eng>;
+    constexpr int D = Eng::D;
     constexpr int LPR = D / 4;
     constexpr int kRows = 256 / LPR;
-    constexpr int kBatch = 8;
+    constexpr int kBatch = 16;
     const int t = blockIdx.x;
     const int h = blockIdx.y * kRows + threadIdx.x / LPR;
     const int part = threadIdx.x % LPR;
@@ -588,26 +611,35 @@ __global__ void __launch_bounds__(256)
         u = sequence_of(a.starts, a.B, t);
         if (u == a.B) return;  // padding
     }
-    const auto first = PagedPlan<Shape, GpuWave>::batch(a, 0);
-    const PagedCut cut = PagedPlan<Shape, GpuWave>::cut(a, first);
-    const PagedUnitItems own = paged_unit_items<Shape, GpuWave>(a, cut, first, u);
-    if (!a.shared && own.chunks == 1) return;  // written already
-    PagedUnitItems pre{};
-    if (a.shared) pre = paged_unit_items<Shape, GpuWave>(a, cut, first, 0);
     if (h >= a.H) return;
     const int hk = a.group_div(h);
     const int g = h - hk * a.group;
-    // Slot of part p of a unit's row r.
-    auto slot = [&](const PagedUnitItems& ui, int p, int r) {
-        const int tile = ui.many ? r / Shape::kTile : r / 32;
-        const int in = ui.many ? r % Shape::kTile : r % 32;
-        return paged_slot_row<Shape>(
-            a, hk, ui.many,
-            ui.first + p * ui.tiles + (a.causal ? ui.tiles - 1 - tile : tile), in);
+    // The parts of unit v's row r: `n` of them, from row `at` of acc and ml on, `step` rows apart.
+    struct Parts {
+        int n;
+        size_t at, step;
     };
-    const int own_row = a.shared ? g : (t - a.starts[u]) * a.group + g;
-    const int pre_row = t * a.group + g;
-    const int parts = pre.chunks + own.chunks;
+    auto parts_of = [&](int v, int r) {
+        const int4 d = a.units[v];
+        const bool many = d.w != 0;
+        const int tile = many ? r / Shape::kTile : r / 32;
+        const int in = many ? r % Shape::kTile : r % 32;
+        const int first = d.x + (a.causal ? d.y - 1 - tile : tile);
+        // Where starts that decrease left a unit without items the note is not this call's.
+        const bool ok = d.x >= 0 && d.z >= 0 && tile < d.y &&
+                        d.x + static_cast<long long>(d.y) * d.z <= (many ? a.max_many : a.max_few);
+        return Parts{ok ? d.z : 0, ok ? paged_slot_row<Shape>(a, hk, many, first, in) : 0,
+                     static_cast<size_t>(d.y) * (many ? Shape::kTile : 32)};
+    };
+    Parts pre{0, 0, 0}, own{0, 0, 0};
+    if (a.shared) {
+        pre = parts_of(0, t * a.group + g);
+        if (paged_seq_len(a, t) > a.prefix) own = parts_of(u, g);
+    } else {
+        own = parts_of(u, (t - a.starts[u]) * a.group + g);
+        if (own.n == 1) return;  // written already
+    }
+    const int parts = pre.n + own.n;
     float M = -INFINITY, l = 0.0f;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int p0 = 0; p0 < parts; p0 += kBatch) {
@@ -620,8 +652,8 @@ __global__ void __launch_bounds__(256)
             v[i] = make_float2(-INFINITY, 0.0f);
             x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             if (p < parts) {
-                const size_t s = p < pre.chunks ? slot(pre, p, pre_row)
-                                                : slot(own, p - pre.chunks, own_row);
+                const size_t s = p < pre.n ? pre.at + p * pre.step
+                                           : own.at + (p - pre.n) * own.step;
                 v[i] = a.ml[s];
                 x[i] = __builtin_bit_cast(f32x4, ld16(a.acc + s * D + 4 * part));
                 // No key of this row, or every score -inf: such a part has no say, also where
@@ -665,15 +697,18 @@ namespace detail {
 namespace {
 
 // The sizes of one launch: grid and slots.
-template <typename T, int D>
+template <class Eng>
 struct PagedGrid {
-    using Shape = dev::PagedShapeOf<T, D>;
-    int per_head;         // 0: keys are not cut into chunks
-    long long many, few;  // items per key/value head at most, of either kind
+    using Shape = dev::PagedShapeOf<Eng>;
+    static constexpr int D = Eng::D;
+    int wgs;                     // 0: keys are not cut into chunks
+    long long items, many, few;  // per key/value head: items, and slots of either kind
+    long long units;
     int kv_heads;
 
-    PagedGrid(const PagedCall& call, bool shared, bool chunks_allowed) {
+    PagedGrid(const PagedCall& call, bool shared, bool chunks) {
         kv_heads = call.num_kv_heads;
+        units = call.batch_size + (shared ? 1LL : 0LL);
         const long long tokens = call.num_tokens;
         const int group = call.num_heads / kv_heads;
         dev::PagedTiles tiles =
@@ -683,28 +718,39 @@ struct PagedGrid {
             tiles.many += tokens * own.many;
             tiles.few += tokens * own.few;
         }
-        // Workgroups that run at once.
-        const long long at_once = (D <= 64 ? 2LL : 1LL) * compute_units();
-        const bool chunks =
-            chunks_allowed &&
-            (shared || tokens * group / Shape::kTile * kv_heads < 2 * at_once);
-        per_head = chunks ? static_cast<int>((at_once + kv_heads - 1) / kv_heads) : 0;
-        many = tiles.many ? tiles.many + per_head : 0;
-        few = tiles.few + per_head;
+        wgs = chunks ? (Eng::kPerCu * compute_units() + kv_heads - 1) / kv_heads : 0;
+        items = tiles.many + tiles.few;
+        many = few = 0;
+        if (chunks) {
+            const long long total = items;
+            items = (total + wgs / 2 + wgs) / wgs * wgs;  // paged_room, in 64 bits
+            many = tiles.many ? items : 0;
+            few = items;
+        }
     }
-    long long blocks() const { return (many + few) * kv_heads; }
+    bool too_large() const { return items * kv_heads > 0x7fffffffLL; }
     size_t slots() const {  // rows of partial results
         return static_cast<size_t>(kv_heads) * (many * Shape::kTile + few * 32);
     }
     size_t bytes() const {
-        return per_head ? slots() * (D * sizeof(float) + sizeof(float2)) : 0;
+        return wgs ? slots() * (D * sizeof(float) + sizeof(float2)) + units * sizeof(int4) : 0;
     }
 };
 
-template <typename T, int D>
-FlashAttentionError run_paged(const PagedCall& call, hipStream_t stream) {
+// Whether the tiles alone, at least so many, leave no workgroup place free.
+template <class Eng>
+bool fills_chip(const PagedCall& call) {
+    const long long rows =
+        static_cast<long long>(call.num_tokens) * (call.num_heads / call.num_kv_heads);
+    return rows / dev::PagedShapeOf<Eng>::kTile * call.num_kv_heads >=
+           static_cast<long long>(Eng::kPerCu) * compute_units();
+}
+
+template <class Eng>
+FlashAttentionError run_paged(const PagedCall& call, bool chunks, hipStream_t stream) {
+    using T = typename Eng::T;
     using E = typename dev::Mma<T>::elem;
-    using Eng = dev::PagedEngine<T, D>;
+    constexpr int D = Eng::D;
     const bool shared = call.query_starts == nullptr;
     dev::PagedArgs a{};
     a.block_table = call.block_table;
@@ -731,22 +777,15 @@ FlashAttentionError run_paged(const PagedCall& call, hipStream_t stream) {
     a.min_steps = 8;
     a.min_rounds = 1;
 
-    // A graph's replays need memory that is theirs: the caller's. (Memory that the graph itself
-    // allocates, a recorded hipMallocAsync, was not there in the replay of two graphs in a row.)
-    const bool own = call.workspace == nullptr;
-    PagedGrid<T, D> grid(call, shared, true);
-    if (grid.per_head && own && stream_capturing(stream)) {
-        if (shared) return FlashAttentionError::OUT_OF_MEMORY;
-        grid = PagedGrid<T, D>(call, shared, false);
-    }
-    if (grid.blocks() > 0x7fffffffLL) return FlashAttentionError::INVALID_DIMENSION;
-    a.per_head = grid.per_head;
+    const PagedGrid<Eng> grid(call, shared, chunks);
+    if (grid.too_large()) return FlashAttentionError::INVALID_DIMENSION;
+    a.wgs = grid.wgs;
     a.max_many = static_cast<int>(grid.many);
     a.max_few = static_cast<int>(grid.few);
     StreamWorkspace ws(stream, true);
-    if (grid.per_head) {
+    if (chunks) {
         void* base = call.workspace;
-        if (own) {
+        if (base == nullptr) {
             FlashAttentionError err = ws.alloc(grid.bytes());
             if (err != FlashAttentionError::SUCCESS) return err;
             base = ws.get();
@@ -755,27 +794,54 @@ FlashAttentionError run_paged(const PagedCall& call, hipStream_t stream) {
         }
         a.acc = static_cast<float*>(base);
         a.ml = reinterpret_cast<float2*>(a.acc + grid.slots() * D);
+        a.units = reinterpret_cast<int4*>(a.ml + grid.slots());
     }
     ProfileEvents tok = profile_kernel<T, D>(shared ? "decode_shared" : "forward_paged");
-    launch_kernel(tok, (dev::paged_kernel<T, D>), dim3(static_cast<unsigned>(grid.blocks())),
-                  dim3(64 * Eng::kWaves), 0, stream, static_cast<const E*>(call.Q),
-                  static_cast<const E*>(call.K_cache), static_cast<const E*>(call.V_cache),
-                  static_cast<E*>(call.O), call.L, a);
+    launch_kernel(tok, (dev::paged_kernel<Eng>),
+                  dim3(static_cast<unsigned>(grid.items * a.Hkv)), dim3(64 * Eng::kWaves), 0,
+                  stream, static_cast<const E*>(call.Q), static_cast<const E*>(call.K_cache),
+                  static_cast<const E*>(call.V_cache), static_cast<E*>(call.O), call.L, a);
     FlashAttentionError err = from_hip(hipGetLastError());
-    if (err != FlashAttentionError::SUCCESS || !grid.per_head) return err;
+    if (err != FlashAttentionError::SUCCESS || !chunks) return err;
     constexpr int kRows = 256 / (D / 4);
     tok = profile_kernel<T, D>("paged_combine");
-    launch_kernel(tok, (dev::paged_combine_kernel<T, D>),
+    launch_kernel(tok, (dev::paged_combine_kernel<Eng>),
                   dim3(static_cast<unsigned>(a.T),
                        static_cast<unsigned>((a.H + kRows - 1) / kRows)),
                   dim3(256), 0, stream, static_cast<E*>(call.O), call.L, a);
     return from_hip(hipGetLastError());
 }
 
+// Workgroups of a launch with chunks and of one without.
+template <typename T, int D>
+struct PagedEngines {
+    static constexpr int kWaves = std::is_same<T, float>::value ? 4 : 8;
+    using Chunked = dev::PagedEngine<T, D, D == 128 ? 4 : kWaves>;
+    using Whole = dev::PagedEngine<T, D, kWaves>;
+};
+
+template <typename T, int D>
+FlashAttentionError run_paged_dim(const PagedCall& call, hipStream_t stream) {
+    using Engines = PagedEngines<T, D>;
+    const bool shared = call.query_starts == nullptr;
+    if (shared || !fills_chip<typename Engines::Whole>(call)) {
+        // A graph's replays need memory that is theirs: the caller's. (Memory that the graph itself
+        // allocates, a recorded hipMallocAsync, was not there in the replay of two graphs in a row.)
+        if (call.workspace != nullptr || !stream_capturing(stream))
+            return run_paged<typename Engines::Chunked>(call, true, stream);
+        if (shared) return FlashAttentionError::OUT_OF_MEMORY;
+    }
+    return run_paged<typename Engines::Whole>(call, false, stream);
+}
+
 template <typename T, int D>
 long long workspace_of(const PagedCall& call) {
-    const PagedGrid<T, D> grid(call, call.prefix_len > 0, true);
-    return grid.blocks() > 0x7fffffffLL ? -1 : static_cast<long long>(grid.bytes());
+    using Engines = PagedEngines<T, D>;
+    const bool shared = call.prefix_len > 0;
+    if (!shared && fills_chip<typename Engines::Whole>(call))
+        return PagedGrid<typename Engines::Whole>(call, false, false).too_large() ? -1 : 0;
+    const PagedGrid<typename Engines::Chunked> grid(call, shared, true);
+    return grid.too_large() ? -1 : static_cast<long long>(grid.bytes());
 }
 
 }  // namespace
@@ -791,11 +857,11 @@ template <typename T>
 FlashAttentionError launch_paged(const PagedCall& c, hipStream_t stream) {
     switch (c.head_dim) {
         case 32:
-            return run_paged<T, 32>(c, stream);
+            return run_paged_dim<T, 32>(c, stream);
         case 64:
-            return run_paged<T, 64>(c, stream);
+            return run_paged_dim<T, 64>(c, stream);
         case 128:
-            return run_paged<T, 128>(c, stream);
+            return run_paged_dim<T, 128>(c, stream);
     }
     return FlashAttentionError::UNSUPPORTED_HEAD_DIM;
 }

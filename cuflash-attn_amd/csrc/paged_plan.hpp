@@ -33,19 +33,21 @@ inline FastDiv fast_div(int d) {
 // tokens times the query heads of one key/value head (row r: token r / group, head r % group).
 //  * More than kManyRows rows: tiles of kTile rows, one 32-row strip per wave, whose waves share the
 //    keys, kStep at a time.
-//  * Fewer: tiles of 32 rows whose keys are spread over the waves, kRound keys in each round.
-// Where the tiles alone do not fill the chip (per_head > 0), the keys of every unit are cut into
-// chunks of whole steps or rounds, at most `s` of them, the least s with which the items of one
-// key/value head number about per_head: the work of a head is W = sum of tiles times steps, and s =
-// W / per_head rounded up gives at most per_head items and one more per tile. Chunks leave partial
-// results in slots of their own, numbered like the items.
+//  * Fewer: tiles of 32 rows whose keys are spread over the waves, kRound keys in each round. A round
+//    brings as many bytes as kRoundCost steps take time for.
+// Where the tiles alone do not fill the chip (`wgs` > 0), the keys of every unit are cut into chunks
+// that cost at most `s`, with the least s that leaves the items of one key/value head at whole rounds
+// of the workgroups that run at once: the next multiple of wgs beyond tiles + wgs / 2. Chunks leave
+// partial results in slots of their own, numbered like the items, and the first item of a unit notes
+// where they are.
 constexpr int kManyRows = 96;
 
-template <int TILE, int STEP, int ROUND>
+template <int TILE, int STEP, int ROUND, int COST>
 struct PagedShape {
     static constexpr int kTile = TILE;
     static constexpr int kStep = STEP;
     static constexpr int kRound = ROUND;
+    static constexpr int kRoundCost = COST;
 };
 
 struct PagedArgs {
@@ -59,12 +61,13 @@ struct PagedArgs {
     bool shared, causal;
     bool whole_groups;  // the rows of one load are a divisor of the page's
     int prefix;         // shared keys
-    int per_head;       // items per key/value head that the chunks aim at; 0: no chunks
-    int min_steps, min_rounds;   // least per chunk
-    int max_many, max_few;       // slots per key/value head for the items of either kind
-    float c;                     // scale * log2(e)
-    float* acc;  // [Hkv, max_many, kTile, D], then [Hkv, max_few, 32, D]
-    float2* ml;  // the same without D: m in log2 units, l
+    int wgs;            // workgroups per key/value head that run at once; 0: no chunks
+    int min_steps, min_rounds;  // least per chunk
+    int max_many, max_few;      // slots per key/value head for the items of either kind
+    float c;                    // scale * log2(e)
+    float* acc;   // [Hkv, max_many, kTile, D], then [Hkv, max_few, 32, D]
+    float2* ml;   // the same without D: m in log2 units, l
+    int4* units;  // [units]: see PagedUnitItems
 };
 
 struct PagedUnit {
@@ -103,13 +106,11 @@ __host__ __device__ __forceinline__ int paged_limit(const PagedArgs& a, int u, c
     return lim > 0 ? lim : 0;
 }
 
-// The cut of one launch: chunks of at most s steps, and the items of either kind.
-struct PagedCut {
-    int s;
-    int many, few;
-};
+__host__ __device__ __forceinline__ int paged_room(int tiles, int wgs) {
+    return (tiles + wgs / 2 + wgs) / wgs * wgs;
+}
 
-// The sums over the units. W: the 64 lanes of a wave, one int each in W::Int.
+// The cut of one launch. W: the 64 lanes of a wave, one int each in W::Int.
 template <class Shape, class W>
 struct PagedPlan {
     using Int = typename W::Int;
@@ -122,14 +123,17 @@ struct PagedPlan {
         return rows > kManyRows ? keys / Shape::kStep + (keys % Shape::kStep > 0)
                                 : keys / Shape::kRound + (keys % Shape::kRound > 0);
     }
-    // Chunks of a unit. One without keys still has outputs, but for a shared decode, where the
-    // combine writes them.
-    __host__ __device__ static int chunks(const PagedArgs& a, int rows, int keys, int s) {
-        const int n = steps(rows, keys);
+    // Steps or rounds of a chunk that costs at most s.
+    __host__ __device__ static int longest(const PagedArgs& a, bool many, int s) {
+        if (many) return s > a.min_steps ? s : a.min_steps;
+        s /= Shape::kRoundCost;
+        return s > a.min_rounds ? s : a.min_rounds;
+    }
+    // Chunks of a unit of n steps. One without keys still has outputs, but for a shared decode,
+    // where the combine writes them.
+    __host__ __device__ static int chunks(const PagedArgs& a, int n, int most) {
         if (n == 0) return a.shared ? 0 : 1;
-        const int least = rows > kManyRows ? a.min_steps : a.min_rounds;
-        if (s < least) s = least;
-        return s >= n ? 1 : (n + s - 1) / s;
+        return most >= n ? 1 : (n + most - 1) / most;
     }
     struct Batch {  // 64 units
         Int rows, keys;
@@ -147,60 +151,85 @@ struct PagedPlan {
         });
         return b;
     }
-    __host__ __device__ static Int items(const PagedArgs& a, const Batch& b, int s, bool many) {
+    // Items of every unit.
+    __host__ __device__ static Int items(const PagedArgs& a, const Batch& b, int s) {
+        const int many = longest(a, true, s), few = longest(a, false, s);
         return W::map2(b.rows, b.keys, [&](int rows, int keys) {
-            return (rows > kManyRows) == many ? tiles(rows) * chunks(a, rows, keys, s) : 0;
+            return tiles(rows) * chunks(a, steps(rows, keys), rows > kManyRows ? many : few);
         });
     }
-    __host__ __device__ static void count(const PagedArgs& a, const Batch& first, PagedCut& cut) {
-        cut.many = cut.few = 0;
+    __host__ __device__ static Int of_kind(const Batch& b, const Int& items, bool many) {
+        return W::map2(b.rows, items,
+                       [&](int rows, int n) { return (rows > kManyRows) == many ? n : 0; });
+    }
+    // f summed over the units.
+    template <class F>
+    __host__ __device__ static int sum(const PagedArgs& a, const Batch& first, F f) {
+        int total = 0;
+        for (int u0 = 0; u0 < paged_units(a); u0 += 64)
+            total += W::lane(W::scan(f(u0 == 0 ? first : batch(a, u0))), 63);
+        return total;
+    }
+    // The greatest cost of a chunk: integers only, every workgroup comes to the same.
+    __host__ __device__ static int cut(const PagedArgs& a, const Batch& first) {
+        if (a.wgs == 0) return kNoChunks;
+        const int total = sum(a, first, [&](const Batch& b) {
+            return W::map2(b.rows, b.keys, [&](int rows, int) { return tiles(rows); });
+        });
+        int work = 0;
         for (int u0 = 0; u0 < paged_units(a); u0 += 64) {
             const Batch b = u0 == 0 ? first : batch(a, u0);
-            cut.many += W::lane(W::scan(items(a, b, cut.s, true)), 63);
-            cut.few += W::lane(W::scan(items(a, b, cut.s, false)), 63);
+            const Int w = W::map2(b.rows, b.keys, [&](int rows, int keys) {
+                const float x = static_cast<float>(tiles(rows)) *
+                                static_cast<float>(steps(rows, keys)) *
+                                (rows > kManyRows ? 1 : Shape::kRoundCost);
+                return x > 16777216.0f ? 1 << 24 : static_cast<int>(x);  // exact below
+            });
+            work += W::lane(W::scan(w), 63);  // at most 2^30
+            if (work > 1 << 30) work = 1 << 30;
         }
-    }
-    // Every workgroup and the combine come to the same cut: integers only.
-    __host__ __device__ static PagedCut cut(const PagedArgs& a, const Batch& first) {
-        PagedCut c{kNoChunks, 0, 0};
-        if (a.per_head > 0) {
-            int work = 0;
-            for (int u0 = 0; u0 < paged_units(a); u0 += 64) {
-                const Batch b = u0 == 0 ? first : batch(a, u0);
-                const Int w = W::map2(b.rows, b.keys, [&](int rows, int keys) {
-                    const int64_t x = static_cast<int64_t>(tiles(rows)) * steps(rows, keys);
-                    return x > (1 << 24) ? 1 << 24 : static_cast<int>(x);
-                });
-                work += W::lane(W::scan(w), 63);  // at most 2^30
-                if (work > 1 << 30) work = 1 << 30;
-            }
-            c.s = work / a.per_head + 1;
-            count(a, first, c);
-            // More items than slots (a sum of work above that was cut off): no chunks.
-            if (c.many <= a.max_many && c.few <= a.max_few) return c;
-            c.s = kNoChunks;
+        // Chunks of at most s: at most work / s + tiles items, so the least s that keeps them within
+        // the room lies in [work / room, work / (room - tiles)], rounded up. (A round of a few-rows
+        // unit cannot be cut, and counts as one chunk of its own: the bound holds for s >= kRoundCost.)
+        const int room = paged_room(total, a.wgs);
+        int lo = (work + room - 1) / room;
+        if (lo < Shape::kRoundCost) lo = Shape::kRoundCost;
+        int hi = (work + room - total - 1) / (room - total) + Shape::kRoundCost - 1;
+        if (hi < lo) hi = lo;
+        auto fits = [&](int s) {
+            return sum(a, first, [&](const Batch& b) { return items(a, b, s); }) <= room;
+        };
+        // With several batches of units every trial reads them all again: the upper end then.
+        if (paged_units(a) > 64) lo = hi;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (fits(mid))
+                hi = mid;
+            else
+                lo = mid + 1;
         }
-        count(a, first, c);
-        return c;
+        return lo;
     }
 };
 
 // A unit's items in one launch: `first` is the index of its first one among those of its kind; item
 // first + chunk * tiles + i is chunk `chunk` of tile i (of tile tiles - 1 - i with a causal mask:
-// the longest tiles start first).
+// the longest tiles start first). As noted in PagedArgs::units: {first, tiles, chunks, many}.
 struct PagedUnitItems {
-    bool many;
     int first, tiles, chunks;
+    bool many;
 };
 
 // One workgroup's part: rows [r0, r0 + kTile or 32) of unit u's `rows`, keys [kbeg, kend).
 struct PagedItem {
     bool found, many;
     bool direct;  // the only part of its rows: outputs, no partial results
+    bool first;   // the first item of its unit
     int u, rows, r0;
     int kbeg, kend;
     int index;  // among the items of its kind: the slot
     PagedUnit unit;
+    PagedUnitItems of;  // the unit's items
 };
 
 template <class Shape, class W>
@@ -208,74 +237,57 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
     using Plan = PagedPlan<Shape, W>;
     PagedItem r{};
     const auto first = Plan::batch(a, 0);
-    const PagedCut cut = Plan::cut(a, first);
-    if (x >= cut.many + cut.few) return r;
-    r.many = x < cut.many;
-    r.index = r.many ? x : x - cut.many;
-    int before = 0;
-    for (int u0 = 0; u0 < paged_units(a); u0 += 64) {
-        const auto b = u0 == 0 ? first : Plan::batch(a, u0);
-        const auto own = Plan::items(a, b, cut.s, r.many);
-        const auto incl = W::scan(own);
-        const int i = W::first(incl, [&](int n) { return before + n > r.index; });
-        if (i < 0) {
-            before += W::lane(incl, 63);
-            continue;
-        }
-        r.found = true;
-        r.u = u0 + i;
-        r.rows = W::lane(b.rows, i);
-        const int keys = W::lane(b.keys, i);
-        const int at = r.index - before - (W::lane(incl, i) - W::lane(own, i));
-        const int tiles = Plan::tiles(r.rows);
-        const int chunks = Plan::chunks(a, r.rows, keys, cut.s);
-        const int chunk = at / tiles;
-        const int tile = a.causal ? tiles - 1 - (at - chunk * tiles) : at - chunk * tiles;
-        r.r0 = tile * (r.many ? Shape::kTile : 32);
-        r.direct = chunks == 1 && !a.shared;
-        r.unit = paged_unit(a, r.u);
-        // (chunks - 1) each <= (chunks - 1) s < steps: the last chunk has keys as well.
-        const int each = (Plan::steps(r.rows, keys) + chunks - 1) / chunks;
-        const int64_t len = static_cast<int64_t>(each) * (r.many ? Shape::kStep : Shape::kRound);
-        const int64_t beg = r.unit.kbeg + chunk * len;
-        r.kbeg = static_cast<int>(beg);
-        r.kend = beg + len < r.unit.kend ? static_cast<int>(beg + len) : r.unit.kend;
-        // With a causal mask, no further than the last row of the tile sees.
-        if (a.causal && !a.shared) {
-            const int last = (r.many ? Shape::kTile : 32) + r.r0;
-            const int lim =
-                paged_limit(a, r.u, r.unit, a.group_div((last < r.rows ? last : r.rows) - 1));
-            if (lim < r.kend) r.kend = lim;
-        }
-        return r;
-    }
-    return r;
-}
-
-template <class Shape, class W>
-__host__ __device__ __forceinline__ PagedUnitItems
-paged_unit_items(const PagedArgs& a, const PagedCut& cut,
-                 const typename PagedPlan<Shape, W>::Batch& first, int u) {
-    using Plan = PagedPlan<Shape, W>;
-    int before_many = 0, before_few = 0;
-    for (int u0 = 0;; u0 += 64) {
-        const auto b = u0 == 0 ? first : Plan::batch(a, u0);
-        const auto many = W::scan(Plan::items(a, b, cut.s, true));
-        const auto few = W::scan(Plan::items(a, b, cut.s, false));
-        if (u < u0 + 64) {
-            const int i = u - u0;
-            const int rows = W::lane(b.rows, i);
-            PagedUnitItems r;
-            r.many = rows > kManyRows;
-            r.tiles = Plan::tiles(rows);
-            r.chunks = Plan::chunks(a, rows, W::lane(b.keys, i), cut.s);
-            r.first = (r.many ? before_many + W::lane(many, i) : before_few + W::lane(few, i)) -
-                      r.tiles * r.chunks;
+    const int s = Plan::cut(a, first);
+    // Items of many rows come first: they take longest.
+    const int units = paged_units(a);
+    for (int kind = 0; kind < 2; ++kind) {
+        r.many = kind == 0;
+        int before = 0;
+        for (int u0 = 0; u0 < units; u0 += 64) {
+            const auto b = u0 == 0 ? first : Plan::batch(a, u0);
+            const auto own = Plan::of_kind(b, Plan::items(a, b, s), r.many);
+            const auto incl = W::scan(own);
+            const int i = W::first(incl, [&](int n) { return before + n > x; });
+            if (i < 0) {
+                before += W::lane(incl, 63);
+                continue;
+            }
+            r.u = u0 + i;
+            r.rows = W::lane(b.rows, i);
+            r.index = x;
+            const int slots = r.many ? a.max_many : a.max_few;
+            r.found = a.wgs == 0 || before + W::lane(incl, i) <= slots;
+            const int keys = W::lane(b.keys, i);
+            const int at = x - before - (W::lane(incl, i) - W::lane(own, i));
+            r.of.first = x - at;
+            r.of.tiles = Plan::tiles(r.rows);
+            r.of.many = r.many;
+            const int n = Plan::steps(r.rows, keys);
+            r.of.chunks = Plan::chunks(a, n, Plan::longest(a, r.many, s));
+            const int chunk = at / r.of.tiles;
+            const int in = at - chunk * r.of.tiles;
+            r.first = at == 0;
+            r.r0 = (a.causal ? r.of.tiles - 1 - in : in) * (r.many ? Shape::kTile : 32);
+            r.direct = r.of.chunks == 1 && !a.shared;
+            r.unit = paged_unit(a, r.u);
+            // (chunks - 1) each <= (chunks - 1) most < n: the last chunk has keys as well.
+            const int each = (n + r.of.chunks - 1) / r.of.chunks;
+            const int64_t len = static_cast<int64_t>(each) * (r.many ? Shape::kStep : Shape::kRound);
+            const int64_t beg = r.unit.kbeg + chunk * len;
+            r.kbeg = static_cast<int>(beg);
+            r.kend = beg + len < r.unit.kend ? static_cast<int>(beg + len) : r.unit.kend;
+            // With a causal mask, no further than the last row of the tile sees.
+            if (a.causal && !a.shared) {
+                const int last = (r.many ? Shape::kTile : 32) + r.r0;
+                const int lim =
+                    paged_limit(a, r.u, r.unit, a.group_div((last < r.rows ? last : r.rows) - 1));
+                if (lim < r.kend) r.kend = lim;
+            }
             return r;
         }
-        before_many += W::lane(many, 63);
-        before_few += W::lane(few, 63);
+        x -= before;
     }
+    return r;
 }
 
 // Row of `acc` and `ml` that item `index`'s row r has.

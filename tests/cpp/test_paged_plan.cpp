@@ -107,24 +107,32 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
 
     PagedTiles t = a.shared ? paged_tiles<Shape>(a.B, 1, a.group)
                             : paged_tiles<Shape>(a.T, a.B, a.group);
-    if (a.shared) t.few += static_cast<long long>(a.B) * ((a.group + 31) / 32);
-    if (a.shared && a.group > kManyRows) return false;
-    a.per_head = pick(4) == 0 ? 0 : spread(rng, 1, 300);
-    a.max_many = t.many > 0 ? int(t.many) + a.per_head : 0;
-    a.max_few = int(t.few) + a.per_head;
+    if (a.shared) {
+        const PagedTiles own = paged_tiles<Shape>(1, 1, a.group);
+        t.many += a.B * own.many;
+        t.few += a.B * own.few;
+    }
+    a.wgs = pick(4) == 0 ? 0 : spread(rng, 1, 300);
+    const int room = a.wgs ? paged_room(int(t.many + t.few), a.wgs) : int(t.many + t.few);
+    a.max_many = t.many > 0 ? (a.wgs ? room : int(t.many)) : 0;
+    a.max_few = a.wgs ? room : int(t.few);
 
     using Plan = PagedPlan<Shape, HostWave>;
     const auto first = Plan::batch(a, 0);
-    const PagedCut cut = Plan::cut(a, first);
-    CHECK(cut.many <= a.max_many && cut.few <= a.max_few);
+    const int cut = Plan::cut(a, first);
+    int items = 0;
+    for (int u0 = 0; u0 < paged_units(a); u0 += 64)
+        items += HostWave::lane(HostWave::scan(Plan::items(a, Plan::batch(a, u0), cut)), 63);
+    CHECK(items <= room);
+    std::vector<int4> noted(paged_units(a), make_int4(-1, -1, -1, -1));
     bool chunked = false;
     // (unit, tile row) -> the key ranges of its items; slots taken.
     std::map<std::pair<int, int>, std::vector<std::array<int, 2>>> met;
     std::map<std::pair<bool, int>, int> slots;
-    const int grid = a.max_many + a.max_few;
+    const int grid = room;
     for (int x = 0; x < grid + 3; ++x) {
         const PagedItem it = paged_item<Shape, HostWave>(a, x);
-        CHECK(it.found == (x < cut.many + cut.few));
+        CHECK(it.found == (x < items));
         if (!it.found) continue;
         CHECK(x < grid);
         CHECK(it.u >= 0 && it.u < paged_units(a));
@@ -142,8 +150,12 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         auto& ranges = met[{it.u, it.r0}];
         CHECK(!it.direct || ranges.empty());
         ranges.push_back({it.kbeg, it.kend});
-        const PagedUnitItems ui = paged_unit_items<Shape, HostWave>(a, cut, first, it.u);
-        CHECK(ui.many == it.many);
+        const PagedUnitItems ui = it.of;
+        if (it.first) {
+            CHECK(noted[it.u].x == -1);
+            noted[it.u] = make_int4(ui.first, ui.tiles, ui.chunks, ui.many);
+        }
+        CHECK(ui.many == it.many && ui.first >= 0);
         CHECK(it.direct == (ui.chunks == 1 && !a.shared));
         chunked |= ui.chunks > 1;
         const int i = it.r0 / tile;
@@ -158,8 +170,15 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         const PagedUnit pu = paged_unit(a, u);
         const int rows = pu.n * a.group;
         const int tile = rows > kManyRows ? Shape::kTile : 32;
-        const PagedUnitItems ui = paged_unit_items<Shape, HostWave>(a, cut, first, u);
-        if (pu.n > 0) CHECK(ui.chunks == 0 || ui.tiles == (rows + tile - 1) / tile);
+        // What the combine finds: noted by the unit's first item, but where there is none.
+        const int4 n = noted[u];
+        const PagedUnitItems ui = n.x >= 0 ? PagedUnitItems{n.x, n.y, n.z, n.w != 0}
+                                           : PagedUnitItems{0, 0, 0, false};
+        if (n.x < 0) CHECK(pu.n == 0 || (a.shared && pu.kend == pu.kbeg));
+        if (n.x >= 0) {
+            CHECK(ui.tiles == (rows + tile - 1) / tile && ui.many == (rows > kManyRows));
+            CHECK(ui.first + ui.tiles * ui.chunks <= (ui.many ? a.max_many : a.max_few));
+        }
         for (int r0 = 0; r0 < rows; r0 += tile) {
             auto ranges = met[{u, r0}];
             CHECK(int(ranges.size()) == ui.chunks);
@@ -192,8 +211,8 @@ int main(int argc, char** argv) {
     }
     int chunked = 0;
     for (g_case = 0; g_case < n; ++g_case) {
-        chunked += g_case % 2 ? launch<PagedShape<256, 64, 256>>(rng)
-                              : launch<PagedShape<128, 32, 128>>(rng);
+        chunked += g_case % 2 ? launch<PagedShape<256, 64, 256, 2>>(rng)
+                              : launch<PagedShape<128, 32, 128, 1>>(rng);
     }
     std::printf("%d launches, %d of them with chunks\n", n, chunked);
     return chunked > n / 10 ? 0 : 1;
