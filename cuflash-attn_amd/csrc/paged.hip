@@ -540,7 +540,7 @@ __device__ __forceinline__ void PagedWork<Eng>::few_rows(unsigned char* smem, fl
 }
 
 // Second launch bound: waves per SIMD of the workgroups that share a CU.
-template <class Eng>
+template <class Eng, bool kShared>
 __global__ void __launch_bounds__((64 * Eng::kWaves), (Eng::kPerCu * Eng::kWaves / 4))
     paged_kernel(const typename Mma<typename Eng::T>::elem* __restrict__ Q,
                  const typename Mma<typename Eng::T>::elem* __restrict__ K,
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__((64 * Eng::kWaves), (Eng::kPerCu * Eng::kWaves
     // The items of a key/value head stay on one XCD where the heads can be dealt out evenly.
     int hk, x;
     head_rank_order(blockIdx.x, a.Hkv, hk, x);
-    const PagedItem it = paged_item<PagedShapeOf<Eng>, GpuWave>(a, x);
+    const PagedItem it = paged_item<PagedShapeOf<Eng>, kShared, GpuWave>(a, x);
     if (!it.found) return;
     if (a.wgs > 0 && it.first && hk == 0 && threadIdx.x == 0)
         a.units[it.u] = make_int4(it.of.first, it.of.tiles, it.of.chunks, it.many);
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__((64 * Eng::kWaves), (Eng::kPerCu * Eng::kWaves
                 make_float2(-INFINITY, 0.0f);
         return;
     }
-    const int* table = !a.shared    ? a.block_table + static_cast<size_t>(it.u) * a.max_pages
+    const int* table = !kShared     ? a.block_table + static_cast<size_t>(it.u) * a.max_pages
                        : it.u == 0 ? a.prefix_table
                                    : a.block_table + static_cast<size_t>(it.u - 1) * a.max_pages;
     const PagedWork<Eng> work{Q,
@@ -746,12 +746,12 @@ bool fills_chip(const PagedCall& call) {
            static_cast<long long>(Eng::kPerCu) * compute_units();
 }
 
-template <class Eng>
+template <class Eng, bool kShared>
 FlashAttentionError run_paged(const PagedCall& call, bool chunks, hipStream_t stream) {
     using T = typename Eng::T;
     using E = typename dev::Mma<T>::elem;
     constexpr int D = Eng::D;
-    const bool shared = call.query_starts == nullptr;
+    constexpr bool shared = kShared;
     dev::PagedArgs a{};
     a.block_table = call.block_table;
     a.prefix_table = call.prefix_table;
@@ -797,10 +797,16 @@ FlashAttentionError run_paged(const PagedCall& call, bool chunks, hipStream_t st
         a.units = reinterpret_cast<int4*>(a.ml + grid.slots());
     }
     ProfileEvents tok = profile_kernel<T, D>(shared ? "decode_shared" : "forward_paged");
-    launch_kernel(tok, (dev::paged_kernel<Eng>),
-                  dim3(static_cast<unsigned>(grid.items * a.Hkv)), dim3(64 * Eng::kWaves), 0,
-                  stream, static_cast<const E*>(call.Q), static_cast<const E*>(call.K_cache),
-                  static_cast<const E*>(call.V_cache), static_cast<E*>(call.O), call.L, a);
+    auto go = [&](auto kernel) {
+        launch_kernel(tok, kernel, dim3(static_cast<unsigned>(grid.items * a.Hkv)),
+                      dim3(64 * Eng::kWaves), 0, stream, static_cast<const E*>(call.Q),
+                      static_cast<const E*>(call.K_cache), static_cast<const E*>(call.V_cache),
+                      static_cast<E*>(call.O), call.L, a);
+    };
+    if constexpr (kShared)
+        go(dev::paged_kernel<Eng, true>);
+    else
+        go(dev::paged_kernel<Eng, false>);
     FlashAttentionError err = from_hip(hipGetLastError());
     if (err != FlashAttentionError::SUCCESS || !chunks) return err;
     constexpr int kRows = 256 / (D / 4);
@@ -828,10 +834,11 @@ FlashAttentionError run_paged_dim(const PagedCall& call, hipStream_t stream) {
         // A graph's replays need memory that is theirs: the caller's. (Memory that the graph itself
         // allocates, a recorded hipMallocAsync, was not there in the replay of two graphs in a row.)
         if (call.workspace != nullptr || !stream_capturing(stream))
-            return run_paged<typename Engines::Chunked>(call, true, stream);
+            return shared ? run_paged<typename Engines::Chunked, true>(call, true, stream)
+                          : run_paged<typename Engines::Chunked, false>(call, true, stream);
         if (shared) return FlashAttentionError::OUT_OF_MEMORY;
     }
-    return run_paged<typename Engines::Whole>(call, false, stream);
+    return run_paged<typename Engines::Whole, false>(call, false, stream);
 }
 
 template <typename T, int D>

@@ -110,105 +110,165 @@ __host__ __device__ __forceinline__ int paged_room(int tiles, int wgs) {
     return (tiles + wgs / 2 + wgs) / wgs * wgs;
 }
 
-// The cut of one launch. W: the 64 lanes of a wave, one int each in W::Int.
-template <class Shape, class W>
+// Division by a number that is the same for the whole launch, by its reciprocal: n < 2^31. The first
+// quotient is off by a few, what remains of n is small, and the second by at most one.
+struct UniformDiv {
+    int d;
+    float r;
+    __host__ __device__ __forceinline__ explicit UniformDiv(int by) : d(by) {
+#ifdef __HIP_DEVICE_COMPILE__
+        r = __builtin_amdgcn_rcpf(static_cast<float>(by));
+#else
+        r = 1.0f / static_cast<float>(by);
+#endif
+    }
+    __host__ __device__ __forceinline__ int operator()(int n) const {
+        int q = static_cast<int>(static_cast<float>(n) * r);
+        // In 64 bits where q d may pass 2^31 by the error of q.
+        int rest = static_cast<int>(n - static_cast<int64_t>(q) * d);
+        const int more = static_cast<int>(static_cast<float>(rest) * r);
+        q += more;
+        rest -= more * d;
+        if (rest < 0) {
+            --q;
+            rest += d;
+        }
+        return rest >= d ? q + 1 : q;
+    }
+};
+
+// The cut of one launch, found by every wave for itself: a few hundred instructions and two loads that
+// need each other, which every workgroup waits for. W: the 64 lanes of a wave, one int each in W::Int.
+// Lane i has the `per` sequences from i per on, the first of them in registers. A shared decode's unit 0
+// stands apart.
+template <class Shape, bool kShared, class W>
 struct PagedPlan {
     using Int = typename W::Int;
-    static constexpr int kNoChunks = 0x7fffffff;
 
-    __host__ __device__ static int tiles(int rows) {
-        return rows > kManyRows ? (rows + Shape::kTile - 1) / Shape::kTile : (rows + 31) / 32;
+    const PagedArgs& a;
+    int per;
+    Int rows0, keys0;
+    int pre_tiles, pre_steps;  // unit 0 of a shared decode
+    bool pre_many;
+    UniformDiv most_many, most_few;  // steps, rounds of a chunk
+    Int many, few;                   // items of either kind up to and with the lane's
+    int pre_items;
+
+    __host__ __device__ __forceinline__ static int up(int x, int by) {
+        return static_cast<int>((static_cast<uint32_t>(x) + (by - 1)) / by);
     }
-    __host__ __device__ static int steps(int rows, int keys) {
-        return rows > kManyRows ? keys / Shape::kStep + (keys % Shape::kStep > 0)
-                                : keys / Shape::kRound + (keys % Shape::kRound > 0);
+    __host__ __device__ __forceinline__ static int tiles(int rows) {
+        return rows > kManyRows ? up(rows, Shape::kTile) : up(rows, 32);
     }
-    // Steps or rounds of a chunk that costs at most s.
-    __host__ __device__ static int longest(const PagedArgs& a, bool many, int s) {
-        if (many) return s > a.min_steps ? s : a.min_steps;
-        s /= Shape::kRoundCost;
-        return s > a.min_rounds ? s : a.min_rounds;
+    __host__ __device__ __forceinline__ static int steps(int rows, int keys) {
+        return rows > kManyRows ? up(keys, Shape::kStep) : up(keys, Shape::kRound);
     }
-    // Chunks of a unit of n steps. One without keys still has outputs, but for a shared decode,
-    // where the combine writes them.
-    __host__ __device__ static int chunks(const PagedArgs& a, int n, int most) {
-        if (n == 0) return a.shared ? 0 : 1;
-        return most >= n ? 1 : (n + most - 1) / most;
+    // Rows and keys of sequence b's unit; no rows: it has no items.
+    __host__ __device__ __forceinline__ int keys_of(int b) const {
+        const int len = paged_seq_len(a, b);
+        return !kShared ? len : len > a.prefix ? len - a.prefix : 0;
     }
-    struct Batch {  // 64 units
-        Int rows, keys;
-    };
-    __host__ __device__ static Batch batch(const PagedArgs& a, int u0) {
-        const int units = paged_units(a);
-        Batch b;
-        b.rows = W::each([&](int lane) {
-            return u0 + lane < units ? paged_unit(a, u0 + lane).n * a.group : 0;
-        });
-        b.keys = W::each([&](int lane) {
-            if (u0 + lane >= units) return 0;
-            const PagedUnit u = paged_unit(a, u0 + lane);
-            return u.kend - u.kbeg;
-        });
-        return b;
+    __host__ __device__ __forceinline__ int rows_of(int b, int keys) const {
+        if (kShared) return keys > 0 ? a.group : 0;
+        const int t0 = paged_clamp(a.starts[b], 0, a.T);
+        return (paged_clamp(a.starts[b + 1], t0, a.T) - t0) * a.group;
     }
-    // Items of every unit.
-    __host__ __device__ static Int items(const PagedArgs& a, const Batch& b, int s) {
-        const int many = longest(a, true, s), few = longest(a, false, s);
-        return W::map2(b.rows, b.keys, [&](int rows, int keys) {
-            return tiles(rows) * chunks(a, steps(rows, keys), rows > kManyRows ? many : few);
-        });
+    // Chunks of n steps, items of a unit. A unit with rows but no keys has outputs all the same.
+    __host__ __device__ __forceinline__ int chunks(bool is_many, int n) const {
+        return n == 0 ? 1 : (is_many ? most_many : most_few)(n - 1) + 1;
     }
-    __host__ __device__ static Int of_kind(const Batch& b, const Int& items, bool many) {
-        return W::map2(b.rows, items,
-                       [&](int rows, int n) { return (rows > kManyRows) == many ? n : 0; });
+    __host__ __device__ __forceinline__ int items(int rows, int keys) const {
+        return tiles(rows) * chunks(rows > kManyRows, steps(rows, keys));
     }
-    // f summed over the units.
+    // f(rows, keys) summed over the sequences of each lane, f(0, 0) = 0.
     template <class F>
-    __host__ __device__ static int sum(const PagedArgs& a, const Batch& first, F f) {
-        int total = 0;
-        for (int u0 = 0; u0 < paged_units(a); u0 += 64)
-            total += W::lane(W::scan(f(u0 == 0 ? first : batch(a, u0))), 63);
-        return total;
+    __host__ __device__ __forceinline__ Int per_lane(F f) const {
+        Int sum = W::map2(rows0, keys0, f);
+        if (per > 1)
+            sum = W::add(sum, W::each([&](int lane) {
+                             int x = 0;
+                             for (int j = 1; j < per && lane * per + j < a.B; ++j) {
+                                 const int keys = keys_of(lane * per + j);
+                                 x += f(rows_of(lane * per + j, keys), keys);
+                             }
+                             return x;
+                         }));
+        return sum;
     }
-    // The greatest cost of a chunk: integers only, every workgroup comes to the same.
-    __host__ __device__ static int cut(const PagedArgs& a, const Batch& first) {
-        if (a.wgs == 0) return kNoChunks;
-        const int total = sum(a, first, [&](const Batch& b) {
-            return W::map2(b.rows, b.keys, [&](int rows, int) { return tiles(rows); });
+    // Chunks that cost at most s.
+    __host__ __device__ __forceinline__ void set(int s) {
+        const int few_s = s / Shape::kRoundCost;
+        most_many = UniformDiv(s > a.min_steps ? s : a.min_steps);
+        most_few = UniformDiv(few_s > a.min_rounds ? few_s : a.min_rounds);
+        pre_items = kShared ? pre_tiles * chunks(pre_many, pre_steps) : 0;
+    }
+
+    __host__ __device__ __forceinline__ explicit PagedPlan(const PagedArgs& args)
+        : a(args), most_many(1), most_few(1) {
+        per = (a.B + 63) / 64;
+        keys0 = W::each([&](int lane) { return lane * per < a.B ? keys_of(lane * per) : 0; });
+        rows0 = W::map1(keys0, [&](int lane, int keys) {
+            return lane * per < a.B ? rows_of(lane * per, keys) : 0;
         });
-        int work = 0;
-        for (int u0 = 0; u0 < paged_units(a); u0 += 64) {
-            const Batch b = u0 == 0 ? first : batch(a, u0);
-            const Int w = W::map2(b.rows, b.keys, [&](int rows, int keys) {
-                const float x = static_cast<float>(tiles(rows)) *
-                                static_cast<float>(steps(rows, keys)) *
-                                (rows > kManyRows ? 1 : Shape::kRoundCost);
-                return x > 16777216.0f ? 1 << 24 : static_cast<int>(x);  // exact below
-            });
-            work += W::lane(W::scan(w), 63);  // at most 2^30
-            if (work > 1 << 30) work = 1 << 30;
+        const int pre_rows = kShared ? a.B * a.group : 0;
+        pre_many = pre_rows > kManyRows;
+        pre_tiles = tiles(pre_rows);
+        pre_steps = steps(pre_rows, a.prefix);
+        const int room = choose();
+        for (int s = 0;; s = s ? 2 * s : most_many.d) {
+            if (s) set(s);
+            many = W::scan(per_lane(
+                [&](int rows, int keys) { return rows > kManyRows ? items(rows, keys) : 0; }));
+            few = W::scan(per_lane(
+                [&](int rows, int keys) { return rows > kManyRows ? 0 : items(rows, keys); }));
+            // Only units whose work was cut off (choose) can leave more than there is room for.
+            if (a.wgs == 0 || W::lane(many, 63) + W::lane(few, 63) + pre_items <= room ||
+                s > 1 << 28)
+                return;
         }
-        // Chunks of at most s: at most work / s + tiles items, so the least s that keeps them within
-        // the room lies in [work / room, work / (room - tiles)], rounded up. (A round of a few-rows
-        // unit cannot be cut, and counts as one chunk of its own: the bound holds for s >= kRoundCost.)
+    }
+
+    // Sets the chunks; the room for items.
+    __host__ __device__ __forceinline__ int choose() {
+        if (a.wgs == 0) {
+            set(0x7fffffff);
+            return 0;
+        }
+        const Int n_tiles = per_lane([](int rows, int) { return tiles(rows); });
+        // A lane's work, cut off where the sum would pass 2^30.
+        const int cap = per > 64 ? (1 << 24) / per : 1 << 18;
+        const Int cost = per_lane([&](int rows, int keys) {
+            const float x = static_cast<float>(tiles(rows)) *
+                            static_cast<float>(steps(rows, keys)) *
+                            (rows > kManyRows ? 1 : Shape::kRoundCost);
+            return x > static_cast<float>(cap) ? cap : static_cast<int>(x);
+        });
+        const int total = W::lane(W::scan(n_tiles), 63) + pre_tiles;
+        const float work = static_cast<float>(W::lane(W::scan(cost), 63)) +
+                           static_cast<float>(pre_tiles) * static_cast<float>(pre_steps) *
+                               (pre_many ? 1 : Shape::kRoundCost);
+        // Chunks of at most s: at most work / s + total items, on average work / s + total / 2. So
+        // the least s that leaves no more than there is room for lies between work / room and
+        // work / (room - total), rounded up (a round is not divided: the bound holds for multiples of
+        // its cost). The least of four in between that does is taken.
         const int room = paged_room(total, a.wgs);
-        int lo = (work + room - 1) / room;
-        if (lo < Shape::kRoundCost) lo = Shape::kRoundCost;
-        int hi = (work + room - total - 1) / (room - total) + Shape::kRoundCost - 1;
-        if (hi < lo) hi = lo;
-        auto fits = [&](int s) {
-            return sum(a, first, [&](const Batch& b) { return items(a, b, s); }) <= room;
+        auto over = [&](int items) {
+            const float x = work / static_cast<float>(items);
+            const int s = x < 1e9f ? static_cast<int>(x) + 1 : 1000000000;
+            return s < Shape::kRoundCost ? Shape::kRoundCost : s;
         };
-        // With several batches of units every trial reads them all again: the upper end then.
-        if (paged_units(a) > 64) lo = hi;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (fits(mid))
-                hi = mid;
-            else
-                lo = mid + 1;
-        }
-        return lo;
+        const int lo = over(room), hi = over(room - total) + Shape::kRoundCost;
+        const int s1 = lo + (hi - lo) / 4, s2 = lo + (hi - lo) / 2, s3 = hi - (hi - lo) / 4;
+        auto count = [&](int s) {
+            set(s);
+            return W::lane(
+                       W::scan(per_lane([&](int rows, int keys) { return items(rows, keys); })),
+                       63) +
+                   pre_items;
+        };
+        const int n1 = count(s1), n2 = count(s2), n3 = count(s3);
+        set(n1 <= room ? s1 : n2 <= room ? s2 : n3 <= room ? s3 : hi);
+        return room;
     }
 };
 
@@ -232,60 +292,72 @@ struct PagedItem {
     PagedUnitItems of;  // the unit's items
 };
 
-template <class Shape, class W>
+template <class Shape, bool kShared, class W>
 __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int x) {
-    using Plan = PagedPlan<Shape, W>;
     PagedItem r{};
-    const auto first = Plan::batch(a, 0);
-    const int s = Plan::cut(a, first);
-    // Items of many rows come first: they take longest.
-    const int units = paged_units(a);
-    for (int kind = 0; kind < 2; ++kind) {
-        r.many = kind == 0;
-        int before = 0;
-        for (int u0 = 0; u0 < units; u0 += 64) {
-            const auto b = u0 == 0 ? first : Plan::batch(a, u0);
-            const auto own = Plan::of_kind(b, Plan::items(a, b, s), r.many);
-            const auto incl = W::scan(own);
-            const int i = W::first(incl, [&](int n) { return before + n > x; });
-            if (i < 0) {
-                before += W::lane(incl, 63);
-                continue;
-            }
-            r.u = u0 + i;
-            r.rows = W::lane(b.rows, i);
-            r.index = x;
-            const int slots = r.many ? a.max_many : a.max_few;
-            r.found = a.wgs == 0 || before + W::lane(incl, i) <= slots;
-            const int keys = W::lane(b.keys, i);
-            const int at = x - before - (W::lane(incl, i) - W::lane(own, i));
-            r.of.first = x - at;
-            r.of.tiles = Plan::tiles(r.rows);
-            r.of.many = r.many;
-            const int n = Plan::steps(r.rows, keys);
-            r.of.chunks = Plan::chunks(a, n, Plan::longest(a, r.many, s));
-            const int chunk = at / r.of.tiles;
-            const int in = at - chunk * r.of.tiles;
-            r.first = at == 0;
-            r.r0 = (a.causal ? r.of.tiles - 1 - in : in) * (r.many ? Shape::kTile : 32);
-            r.direct = r.of.chunks == 1 && !a.shared;
-            r.unit = paged_unit(a, r.u);
-            // (chunks - 1) each <= (chunks - 1) most < n: the last chunk has keys as well.
-            const int each = (n + r.of.chunks - 1) / r.of.chunks;
-            const int64_t len = static_cast<int64_t>(each) * (r.many ? Shape::kStep : Shape::kRound);
-            const int64_t beg = r.unit.kbeg + chunk * len;
-            r.kbeg = static_cast<int>(beg);
-            r.kend = beg + len < r.unit.kend ? static_cast<int>(beg + len) : r.unit.kend;
-            // With a causal mask, no further than the last row of the tile sees.
-            if (a.causal && !a.shared) {
-                const int last = (r.many ? Shape::kTile : 32) + r.r0;
-                const int lim =
-                    paged_limit(a, r.u, r.unit, a.group_div((last < r.rows ? last : r.rows) - 1));
-                if (lim < r.kend) r.kend = lim;
-            }
-            return r;
+    const PagedPlan<Shape, kShared, W> plan(a);
+    using Plan = PagedPlan<Shape, kShared, W>;
+    // Items of many rows come first: they take longest. Those of unit 0 come before its kind's others.
+    const int pre_many = plan.pre_many ? plan.pre_items : 0;
+    const int pre_few = plan.pre_items - pre_many;
+    const int total_many = W::lane(plan.many, 63) + pre_many;
+    if (x >= total_many + W::lane(plan.few, 63) + pre_few) return r;
+    r.many = x < total_many;
+    if (!r.many) x -= total_many;
+    r.index = x;
+    const int pre = r.many ? pre_many : pre_few;
+    int at = x, keys = 0;
+    if (kShared && x < pre) {
+        r.u = 0;
+        r.rows = a.B * a.group;
+        keys = a.prefix;
+        r.unit = PagedUnit{0, a.B, 0, a.prefix};
+    } else {
+        const auto& incl = r.many ? plan.many : plan.few;
+        const int i = W::first(incl, [&](int n) { return pre + n > x; });
+        at -= pre + (i > 0 ? W::lane(incl, i > 0 ? i - 1 : 0) : 0);
+        // The sequence among the lane's.
+        r.rows = W::lane(plan.rows0, i);
+        keys = W::lane(plan.keys0, i);
+        int b = i * plan.per;
+        for (;;) {
+            const int own = (r.rows > kManyRows) == r.many ? plan.items(r.rows, keys) : 0;
+            if (at < own) break;
+            at -= own;
+            if (++b >= a.B) return r;  // not reached
+            keys = plan.keys_of(b);
+            r.rows = plan.rows_of(b, keys);
         }
-        x -= before;
+        r.u = kShared ? b + 1 : b;
+        r.unit.n = kShared ? 1 : a.group_div(r.rows);
+        r.unit.t0 = kShared ? b : paged_clamp(a.starts[b], 0, a.T);
+        r.unit.kbeg = kShared ? a.prefix : 0;
+        r.unit.kend = r.unit.kbeg + keys;
+    }
+    r.of.first = x - at;
+    r.of.many = r.many;
+    r.of.tiles = Plan::tiles(r.rows);
+    int each = Plan::steps(r.rows, keys);
+    r.of.chunks = plan.chunks(r.many, each);
+    r.found = a.wgs == 0 ||
+              r.of.first + r.of.tiles * r.of.chunks <= (r.many ? a.max_many : a.max_few);
+    const int chunk = r.of.chunks == 1 ? 0 : at / r.of.tiles;
+    const int in = at - chunk * r.of.tiles;
+    r.first = at == 0;
+    r.r0 = (a.causal ? r.of.tiles - 1 - in : in) * (r.many ? Shape::kTile : 32);
+    r.direct = r.of.chunks == 1 && !kShared;
+    // (chunks - 1) each <= (chunks - 1) most < steps: the last chunk has keys as well.
+    if (r.of.chunks > 1) each = (each + r.of.chunks - 1) / r.of.chunks;
+    const int64_t len = static_cast<int64_t>(each) * (r.many ? Shape::kStep : Shape::kRound);
+    const int64_t beg = r.unit.kbeg + chunk * len;
+    r.kbeg = static_cast<int>(beg);
+    r.kend = beg + len < r.unit.kend ? static_cast<int>(beg + len) : r.unit.kend;
+    // With a causal mask, no further than the last row of the tile sees.
+    if (!kShared && a.causal) {
+        const int last = (r.many ? Shape::kTile : 32) + r.r0;
+        const int lim =
+            paged_limit(a, r.u, r.unit, a.group_div((last < r.rows ? last : r.rows) - 1));
+        if (lim < r.kend) r.kend = lim;
     }
     return r;
 }

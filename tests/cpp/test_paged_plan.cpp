@@ -32,6 +32,13 @@ struct HostWave {
         for (int i = 0; i < 64; ++i) v[i] = f(i);
         return v;
     }
+    static Int add(const Int& x, const Int& y) {
+        return each([&](int i) { return x[i] + y[i]; });
+    }
+    template <class F>
+    static Int map1(const Int& x, F f) {
+        return each([&](int i) { return f(i, x[i]); });
+    }
     template <class F>
     static Int map2(const Int& x, const Int& y, F f) {
         return each([&](int i) { return f(x[i], y[i]); });
@@ -68,7 +75,7 @@ int spread(std::mt19937& rng, int lo, int hi) {  // over the logarithm
     return std::min(hi, std::max(lo, int(std::exp(u(rng)))));
 }
 
-template <class Shape>
+template <class Shape, bool kShared>
 bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     auto pick = [&](int n) { return int(rng() % unsigned(n)); };
     PagedArgs a{};
@@ -78,10 +85,10 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     a.group_div = fast_div(a.group);
     a.page_size = std::array<int, 6>{1, 6, 16, 24, 64, 256}[pick(6)];
     a.page_div = fast_div(a.page_size);
-    a.B = spread(rng, 1, 200);
+    a.B = spread(rng, 1, pick(10) == 0 ? 600 : 200);
     a.max_pages = spread(rng, 1, std::max(1, 40000 / a.page_size));
     a.cap = a.page_size * a.max_pages;
-    a.shared = pick(3) == 0;
+    a.shared = kShared;
     a.causal = !a.shared && pick(3) > 0;
     a.min_steps = 1 + pick(8);
     a.min_rounds = 1 + pick(2);
@@ -117,12 +124,9 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     a.max_many = t.many > 0 ? (a.wgs ? room : int(t.many)) : 0;
     a.max_few = a.wgs ? room : int(t.few);
 
-    using Plan = PagedPlan<Shape, HostWave>;
-    const auto first = Plan::batch(a, 0);
-    const int cut = Plan::cut(a, first);
-    int items = 0;
-    for (int u0 = 0; u0 < paged_units(a); u0 += 64)
-        items += HostWave::lane(HostWave::scan(Plan::items(a, Plan::batch(a, u0), cut)), 63);
+    const PagedPlan<Shape, kShared, HostWave> plan(a);
+    const int items =
+        HostWave::lane(plan.many, 63) + HostWave::lane(plan.few, 63) + plan.pre_items;
     CHECK(items <= room);
     std::vector<int4> noted(paged_units(a), make_int4(-1, -1, -1, -1));
     bool chunked = false;
@@ -131,7 +135,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     std::map<std::pair<bool, int>, int> slots;
     const int grid = room;
     for (int x = 0; x < grid + 3; ++x) {
-        const PagedItem it = paged_item<Shape, HostWave>(a, x);
+        const PagedItem it = paged_item<Shape, kShared, HostWave>(a, x);
         CHECK(it.found == (x < items));
         if (!it.found) continue;
         CHECK(x < grid);
@@ -207,12 +211,19 @@ int main(int argc, char** argv) {
     for (int i = 0; i < 200000; ++i) {
         const int d = 1 + int(rng() >> (1 + rng() % 31)), v = int(rng() >> 1);
         const FastDiv f = fast_div(std::max(1, d));
+        const UniformDiv u(std::max(1, d));
+        for (int x : {v, 0x7fffffff, 0, v / d * d, std::max(0, v / d * d - 1)}) CHECK(u(x) == x / d);
         for (int x : {v, 0x7fffffff, 0, v / d * d, std::max(0, v / d * d - 1)}) CHECK(f(x) == x / d);
     }
     int chunked = 0;
     for (g_case = 0; g_case < n; ++g_case) {
-        chunked += g_case % 2 ? launch<PagedShape<256, 64, 256, 2>>(rng)
-                              : launch<PagedShape<128, 32, 128, 1>>(rng);
+        using A = PagedShape<256, 64, 256, 2>;
+        using B = PagedShape<128, 32, 128, 1>;
+        const int kind = rng() % 6;
+        chunked += kind == 0   ? launch<A, true>(rng)
+                   : kind == 1 ? launch<B, true>(rng)
+                   : kind % 2  ? launch<A, false>(rng)
+                               : launch<B, false>(rng);
     }
     std::printf("%d launches, %d of them with chunks\n", n, chunked);
     return chunked > n / 10 ? 0 : 1;
