@@ -31,6 +31,16 @@
 namespace cuflash {
 namespace dev {
 
+// LDS-DMA load from a scalar base (lds_dma16_async_s) with the non-temporal hint.
+__device__ __forceinline__ void lds_dma16_once_s(const void* sbase, unsigned voff,
+                                                 unsigned char* lds_base) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                 :
+                 : "v"(voff), "s"(sbase),
+                   "{m0}"(__builtin_amdgcn_readfirstlane(lds_address(lds_base)))
+                 : "memory");
+}
+
 // What differs between the types: tiles of 32 keys in LDS and the block over one of them.
 template <typename T_, int D_, int NW>
 struct PagedEngine {
@@ -41,6 +51,7 @@ struct PagedEngine {
     static constexpr int kWaves = NW;
     static constexpr int kPerCu = D <= 64 || NW <= 4 ? 2 : 1;  // workgroups (LDS)
     static constexpr int kRoundCost = 2;
+    static constexpr bool kInTurn = NW == 8 && D == 128;
     static constexpr int kStepBlocks = 2;              // 32-key blocks of a step (many rows)
     static constexpr int kGroupRows = Lay::kRows;      // key rows of one load
     static constexpr int kGroups = 32 / kGroupRows;    // loads of a tile
@@ -87,6 +98,7 @@ struct PagedEngine<float, D_, NW> {
     static constexpr int kWaves = NW;
     static constexpr int kPerCu = D <= 64 ? 2 : 1;
     static constexpr int kRoundCost = 1;
+    static constexpr bool kInTurn = false;
     static constexpr int kStepBlocks = 1;
     static constexpr int kGroupRows = 256 / D;
     static constexpr int kGroups = 32 / kGroupRows;
@@ -192,16 +204,14 @@ struct CacheRows {
     FastDiv page_div;
     int page_size;
     size_t pitch;  // elements from key to key
-    __device__ __forceinline__ size_t at(int t, int j, int page) const {
-        return (static_cast<size_t>(page) * page_size + (t - j * page_size)) * pitch;
+    __device__ __forceinline__ int entry(int j) const { return ((ConstInts)table)[j]; }
+    __device__ __forceinline__ int page(int t) const { return entry(page_div(t)); }
+    __device__ __forceinline__ size_t from_page(int t, int page) const {
+        return (static_cast<size_t>(page) * page_size + (t - page_div(t) * page_size)) * pitch;
     }
-    __device__ __forceinline__ size_t uniform(int t) const {
-        const int j = page_div(t);
-        return at(t, j, ((ConstInts)table)[j]);
-    }
+    __device__ __forceinline__ size_t uniform(int t) const { return from_page(t, page(t)); }
     __device__ __forceinline__ size_t lane(int t) const {
-        const int j = page_div(t);
-        return at(t, j, table[j]);
+        return from_page(t, table[page_div(t)]);
     }
 };
 
@@ -231,7 +241,10 @@ struct PagedWork {
         return min(it.kend, paged_limit(a, it.u, it.unit, a.group_div(r)));
     }
     // Group g of the tile that begins at key0, from K and V alike.
-    template <int N>
+    // kOnce: no other workgroup reads these keys, so they should not displace other lines (16 x 5 tokens
+    // of up to 8196 keys 63.6 -> 56.0 us; keys that several workgroups share, 61 tokens of 8253, 26.5
+    // -> 32.6).
+    template <int N, bool kOnce = false>
     __device__ __forceinline__ void load_groups(const E* src, int key0, int tile_end, int g0,
                                                 int step, unsigned char* dst) const {
         const int lane = threadIdx.x & 63;
@@ -242,9 +255,12 @@ struct PagedWork {
             for (int i = 0; i < N; ++i) {
                 const int g = g0 + step * i;
                 const E* base = src + rows.uniform(key0 + Eng::kGroupRows * g);
-                lds_dma16_async_s(base,
-                                  static_cast<unsigned>((row + Eng::ld_col(lane, g)) * sizeof(E)),
-                                  dst + g * Eng::kGroupBytes);
+                const unsigned voff =
+                    static_cast<unsigned>((row + Eng::ld_col(lane, g)) * sizeof(E));
+                if constexpr (kOnce)
+                    lds_dma16_once_s(base, voff, dst + g * Eng::kGroupBytes);
+                else
+                    lds_dma16_async_s(base, voff, dst + g * Eng::kGroupBytes);
             }
         } else {
             size_t off[N];
@@ -274,77 +290,22 @@ struct PagedWork {
     }
 
     __device__ __forceinline__ void many_rows(unsigned char* smem) const;
+    __device__ __forceinline__ void many_rows_in_turn(unsigned char* smem) const;
+    __device__ __forceinline__ void store_many(unsigned char* smem, const f32x16 (&o)[D / 32],
+                                               float m, float l, bool on, int orow) const;
     __device__ __forceinline__ void few_rows(unsigned char* smem, float (*s_m)[32],
                                              float (*s_l)[32]) const;
 };
 
+// The outputs or partial results of a wave's rows, from its accumulators.
 template <class Eng>
-__device__ __forceinline__ void PagedWork<Eng>::many_rows(unsigned char* smem) const {
-    constexpr int kBlocks = Eng::kStepBlocks;
-    constexpr int kStep = 32 * kBlocks;
-    constexpr int kBytes = kBlocks * Eng::kTile;  // of a step's K or V
-    constexpr int kParts = kBlocks * Eng::kGroups / Eng::kWaves;
+__device__ __forceinline__ void PagedWork<Eng>::store_many(unsigned char* smem,
+                                                           const f32x16 (&o)[D / 32], float m,
+                                                           float l, bool on, int orow) const {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31;
     const int g2 = lane >> 5;
-    const int row = it.r0 + wave * 32 + l32;
-    const bool on = row < it.rows;
-    const int orow = on ? out_row(row) : -1;
-
-    typename Eng::Query q;
-    Eng::load(q, Q + static_cast<size_t>(on ? orow : 0) * D, on, g2);
-    // This lane's keys, and the least and the greatest end of the wave's rows.
-    const int kend = on ? row_end(row) : it.kend;
-    int least = kend, most = on ? kend : 0;
-#pragma unroll
-    for (int w = 16; w >= 1; w >>= 1) {
-        least = min(least, __shfl_xor(least, w, 64));
-        most = max(most, __shfl_xor(most, w, 64));
-    }
-    const int mask_from = __builtin_amdgcn_readfirstlane(least);
-    const int wave_end = __builtin_amdgcn_readfirstlane(most);
-    const int nsteps = it.kend > it.kbeg ? (it.kend - it.kbeg + kStep - 1) / kStep : 0;
-
-    unsigned char* const k0 = smem;
-    unsigned char* const v0 = smem + kBytes;
-    unsigned char* const k1 = smem + 2 * kBytes;
-    unsigned char* const v1 = smem + 3 * kBytes;
-    auto load = [&](int j, unsigned char* kt, unsigned char* vt) {
-        const int key0 = it.kbeg + j * kStep;
-        load_groups<kParts>(K, key0, key0 + kStep, wave, Eng::kWaves, kt);
-        load_groups<kParts>(V, key0, key0 + kStep, wave, Eng::kWaves, vt);
-    };
-    const auto at = Eng::offsets(lane);
-    f32x16 o[D / 32];
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) o[dt] = f32x16{};
-    float m = -INFINITY, l = 0.0f;
-    const float cs = fmaxf(a.c, kFltMin);  // scale 0: -inf * 0 would make the masked scores NaN
-    auto step = [&](int j, const unsigned char* kt, const unsigned char* vt) {
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            const int key0 = it.kbeg + j * kStep + 32 * b;
-            if (key0 < wave_end)
-                Eng::block(kt + b * Eng::kTile, vt + b * Eng::kTile, at, key0, mask_from, kend, g2,
-                           cs, q, o, m, l, [] {});
-        }
-    };
-    // Step j in buffers j & 1: the loads of step j + 1 are issued behind the barrier that ends every
-    // wave's reads of step j - 1.
-    if (nsteps > 0) load(0, k0, v0);
-    for (int j = 0; j < nsteps; j += 2) {
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (j + 1 < nsteps) load(j + 1, k1, v1);
-        step(j, k0, v0);
-        if (j + 1 >= nsteps) break;
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (j + 2 < nsteps) load(j + 2, k0, v0);
-        step(j + 1, k1, v1);
-    }
-
     l = pair_sum(l);
     if (!it.direct) {
         if (!on) return;
@@ -403,6 +364,346 @@ __device__ __forceinline__ void PagedWork<Eng>::many_rows(unsigned char* smem) c
 }
 
 template <class Eng>
+__device__ __forceinline__ void PagedWork<Eng>::many_rows(unsigned char* smem) const {
+    constexpr int kBlocks = Eng::kStepBlocks;
+    constexpr int kStep = 32 * kBlocks;
+    constexpr int kBytes = kBlocks * Eng::kTile;  // of a step's K or V
+    constexpr int kParts = kBlocks * Eng::kGroups / Eng::kWaves;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31;
+    const int g2 = lane >> 5;
+    const int row = it.r0 + wave * 32 + l32;
+    const bool on = row < it.rows;
+    const int orow = on ? out_row(row) : -1;
+
+    typename Eng::Query q;
+    Eng::load(q, Q + static_cast<size_t>(on ? orow : 0) * D, on, g2);
+    // This lane's keys, and the least and the greatest end of the wave's rows.
+    const int kend = on ? row_end(row) : it.kend;
+    int least = kend, most = on ? kend : 0;
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1) {
+        least = min(least, __shfl_xor(least, w, 64));
+        most = max(most, __shfl_xor(most, w, 64));
+    }
+    const int mask_from = __builtin_amdgcn_readfirstlane(least);
+    const int wave_end = __builtin_amdgcn_readfirstlane(most);
+    const int nsteps = it.kend > it.kbeg ? (it.kend - it.kbeg + kStep - 1) / kStep : 0;
+
+    unsigned char* const k0 = smem;
+    unsigned char* const v0 = smem + kBytes;
+    unsigned char* const k1 = smem + 2 * kBytes;
+    unsigned char* const v1 = smem + 3 * kBytes;
+    auto load = [&](int j, unsigned char* kt, unsigned char* vt) {
+        const int key0 = it.kbeg + j * kStep;
+        load_groups<kParts>(K, key0, key0 + kStep, wave, Eng::kWaves, kt);
+        load_groups<kParts>(V, key0, key0 + kStep, wave, Eng::kWaves, vt);
+    };
+    const auto lds_at = Eng::offsets(lane);
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) o[dt] = f32x16{};
+    float m = -INFINITY, l = 0.0f;
+    const float cs = fmaxf(a.c, kFltMin);  // scale 0: -inf * 0 would make the masked scores NaN
+    auto step = [&](int j, const unsigned char* kt, const unsigned char* vt) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            const int key0 = it.kbeg + j * kStep + 32 * b;
+            if (key0 < wave_end)
+                Eng::block(kt + b * Eng::kTile, vt + b * Eng::kTile, lds_at, key0, mask_from, kend, g2,
+                           cs, q, o, m, l, [] {});
+        }
+    };
+    // Step j in buffers j & 1: the loads of step j + 1 are issued behind the barrier that ends every
+    // wave's reads of step j - 1.
+    if (nsteps > 0) load(0, k0, v0);
+    for (int j = 0; j < nsteps; j += 2) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (j + 1 < nsteps) load(j + 1, k1, v1);
+        step(j, k0, v0);
+        if (j + 1 >= nsteps) break;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (j + 2 < nsteps) load(j + 2, k0, v0);
+        step(j + 1, k1, v1);
+    }
+
+    store_many(smem, o, m, l, on, orow);
+}
+
+// The same with the two waves of a SIMD in turn on the matrix and the vector unit. Left to themselves
+// they form scores at the same time and then their softmax, so that each unit waits for the other. Here
+// waves 4 to 7 (waves 0 to 3 sit on the same SIMDs) start half a step late, and a barrier after each half
+// holds them there:
+//   half 2 j:      waves 0-3  softmax of S_j                                  waves 4-7  products of step j
+//   half 2 j + 1:  waves 0-3  O += V_j^T P_j, S_{j+1} = K_{j+1} Q^T           waves 4-7  softmax of S_j
+// K and V tiles rotate through three buffers each. Products j + 1 read V_j and K_{j+1}, in the halves
+// 2 j + 1 and 2 j + 2. A wave issues its share of later tiles before its softmax of S_j: waves 0-3 in half
+// 2 j, of V_{j+1} and K_{j+2}, whose buffers were last read in half 2 j - 2 (V_{j-2}, K_{j-1}); waves 4-7 in
+// half 2 j + 1, one step further, V_{j+2} and K_{j+3}, last read in half 2 j (V_{j-1}, K_j). Behind its next
+// softmax it waits until these have landed: half 2 j + 2 or 2 j + 3, before the half that reads them, 2 j + 3
+// or 2 j + 5.
+template <class Eng>
+__device__ __forceinline__ void PagedWork<Eng>::many_rows_in_turn(unsigned char* smem) const {
+    using Lay = typename Eng::Lay;
+    using Frag = typename Eng::Frag;
+    constexpr int NW = Eng::kWaves;
+    constexpr int kStep = 64;
+    constexpr int kBytes = 2 * Eng::kTile;             // of a step's K or V
+    constexpr int kParts = 2 * Eng::kGroups / NW;      // loads of a wave per tile
+    constexpr int KS = D / 16;
+    constexpr int NDT = D / 32;
+    constexpr int kMma = 4 * NDT;                      // MFMAs of either product per step
+    static_assert(NW == 8 && Eng::kStepBlocks == 2 && 6 * kBytes <= 2 * NW * Eng::kTile, "shape");
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31;
+    const int g2 = lane >> 5;
+    const int row = it.r0 + wave * 32 + l32;
+    const bool on = row < it.rows;
+    const int orow = on ? out_row(row) : -1;
+
+    typename Eng::Query q;
+    Eng::load(q, Q + static_cast<size_t>(on ? orow : 0) * D, on, g2);
+    const int kend = on ? row_end(row) : it.kend;
+    int least = kend, most = on ? kend : 0;
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1) {
+        least = min(least, __shfl_xor(least, w, 64));
+        most = max(most, __shfl_xor(most, w, 64));
+    }
+    const int mask_from = __builtin_amdgcn_readfirstlane(least);
+    const int wave_end = __builtin_amdgcn_readfirstlane(most);
+    const int n = it.kend > it.kbeg ? (it.kend - it.kbeg + kStep - 1) / kStep : 0;
+    // Steps in which this wave has keys to see.
+    const int nw = min(n, wave_end > it.kbeg ? (wave_end - it.kbeg + kStep - 1) / kStep : 0);
+
+    const int k_base[2] = {Lay::row_base(lane, 0), Lay::row_base(lane, 1)};
+    const int v_base = Lay::tr_off(lane);
+    f32x16 o[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x16{};
+    f32x16 s[2];
+    s[0] = s[1] = f32x16{};
+    Frag p[4];
+    float m = -INFINITY, l = 0.0f;
+    const float cs = fmaxf(a.c, kFltMin);  // scale 0: -inf * 0 would make the masked scores NaN
+
+    // A wave's share of a whole tile is kParts neighbouring groups of rows on one page: one scalar base,
+    // found by walking the page table a step ahead of K, and V_j comes from where K_j came a step before.
+    // (Scalar instructions take their time, 8 cycles where they depend on each other: with a base and a
+    // division for each load, the four loads took 950 cycles of each half's 2400; the loads themselves
+    // want to be few per half, too. Between the MFMAs they cost as much and delay these.)
+    constexpr int kShare = Eng::kGroupRows * kParts;  // rows
+    const bool shares_whole = whole && rows.page_size % kShare == 0 && it.kbeg % kShare == 0;
+    const int whole_tiles = shares_whole ? (it.kend - it.kbeg) / kStep : 0;
+    const unsigned row_bytes = static_cast<unsigned>(rows.pitch * sizeof(E));
+    const uint64_t page_bytes = static_cast<uint64_t>(row_bytes) * rows.page_size;
+    unsigned voff[kParts];
+#pragma unroll
+    for (int i = 0; i < kParts; ++i)
+        voff[i] = (Eng::ld_row(lane) + Eng::kGroupRows * i) * row_bytes +
+                  static_cast<unsigned>(Eng::ld_col(lane, 0) * sizeof(E));
+    // Place of this wave's share of the next tile to ask for: entry of the page table, row of the page.
+    const int first_key = it.kbeg + kShare * wave;
+    int entry = rows.page_div(first_key);
+    int in_page = first_key - entry * rows.page_size;
+    const int last_entry = rows.page_div(max(first_key, first_key + (whole_tiles - 1) * kStep));
+    const int step_pages = rows.page_div(kStep);
+    const int step_rows = kStep - step_pages * rows.page_size;
+    int page = 0, page_row = 0;  // of the tile asked for
+    uint64_t at = 0;             // place of the last whole K tile, in bytes
+    auto ask = [&] {
+        page = rows.entry(min(entry, last_entry));  // behind the last whole tile: any
+        page_row = in_page;
+        entry += step_pages;
+        in_page += step_rows;
+        if (in_page >= rows.page_size) {
+            in_page -= rows.page_size;
+            ++entry;
+        }
+    };
+    auto place = [&] {
+        at = static_cast<uint64_t>(static_cast<unsigned>(page)) * page_bytes +
+             static_cast<uint64_t>(static_cast<unsigned>(page_row)) * row_bytes;
+    };
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(smem)) +
+                          static_cast<unsigned>(wave * kParts * Eng::kGroupBytes);
+    auto load_whole = [&](const E* src, int buffer) {
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                         :
+                         : "v"(voff[i]), "s"(reinterpret_cast<const char*>(src) + at),
+                           "{m0}"(lds0 + buffer + Eng::kGroupBytes * i)
+                         : "memory");
+    };
+    auto load = [&](const E* src, int j, int buffer) {
+        if (j < whole_tiles) {
+            load_whole(src, buffer);
+        } else {
+            const int key0 = it.kbeg + j * kStep;
+            load_groups<kParts>(src, key0, key0 + kStep, wave * kParts, 1, smem + buffer);
+        }
+    };
+    auto v_frag = [&](const unsigned char* vt, int i) {
+        const unsigned char* at = vt + v_base + (i / NDT) * Lay::kTrRows16 + Lay::dtile_off(i % NDT);
+        return tr_frag_at<T>(at, at + Lay::kTrHigh);
+    };
+    auto k_frag = [&](const unsigned char* kt, int i) {
+        return as_frag<T>(
+            ld16(kt + k_base[(i % KS) & 1] + (i / KS) * Eng::kTile + Lay::k_off(i % KS)));
+    };
+    constexpr int kAhead = 4;  // MFMAs ahead of which an operand is read
+    auto scores = [&](const unsigned char* kt) {
+        Frag f[kMma];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) f[i] = k_frag(kt, i);
+#pragma unroll
+        for (int i = 0; i < kMma; ++i) {
+            if (i + kAhead < kMma) f[i + kAhead] = k_frag(kt, i + kAhead);
+            s[i / KS] = Elem<T>::mma(f[i], q.f[i % KS], s[i / KS]);
+        }
+    };
+    // O += V^T P, then the next scores, in one chain. (Behind the last step these come from an old
+    // tile and are not used.)
+    auto products = [&](const unsigned char* vt, const unsigned char* kt) {
+        Frag f[2 * kMma];
+        auto frag_of = [&](int i) { return i < kMma ? v_frag(vt, i) : k_frag(kt, i - kMma); };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) f[i] = frag_of(i);
+#pragma unroll
+        for (int i = 0; i < 2 * kMma; ++i) {
+            if (i + kAhead < 2 * kMma) f[i + kAhead] = frag_of(i + kAhead);
+            if (i < kMma) {
+                o[i % NDT] = Elem<T>::mma(f[i], p[i / NDT], o[i % NDT]);
+            } else {
+                const int k = i - kMma;
+                if (k == 0) s[0] = s[1] = f32x16{};
+                s[k / KS] = Elem<T>::mma(f[i], q.f[k % KS], s[k / KS]);
+            }
+        }
+    };
+    // The softmax of S_j: masks, the lazily raised maximum, P_j rounded to T, the row sum in fp32.
+    auto softmax = [&](int j) {
+        const int key0 = it.kbeg + j * kStep;
+        if (key0 + kStep > mask_from) {
+            const int lim = kend - key0 - 4 * g2;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) < lim ? s[t][r] : -INFINITY;
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 2)
+                mx = __builtin_elementwise_maximum(__builtin_elementwise_maximum(mx, s[t][r]),
+                                                   s[t][r + 1]);
+        }
+        const float m_new = fmaxf(m, pair_max(mx) * cs);
+        const bool grow = m_new > m + kLazyRescale;
+        if (__ballot(grow) != 0) {
+            const float alpha = grow ? fast_exp2(m_new == -INFINITY ? 0.0f : m - m_new) : 1.0f;
+            m = grow ? m_new : m;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
+        }
+        const float m_use = (m == -INFINITY) ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f32x16& x = s[i >> 1];
+            const int r0 = 8 * (i & 1);
+#pragma unroll
+            for (int r = r0; r < r0 + 8; ++r) x[r] = fast_exp2(fmaf(x[r], cs, -m_use));
+#pragma unroll
+            for (int r = r0; r < r0 + 8; r += 2) sum += x[r] + x[r + 1];
+            p[i] = pack_frag<T>(x[r0], x[r0 + 1], x[r0 + 2], x[r0 + 3], x[r0 + 4], x[r0 + 5],
+                                x[r0 + 6], x[r0 + 7]);
+        }
+        l += sum;
+    };
+    auto barrier = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    if (n > 0) {
+        // V_j and K_{j+1}, for j in turn, into the buffers at vd and kd; the loads issued.
+        int kd = kBytes, vd = 3 * kBytes;
+        auto rotate = [&] {
+            kd = kd == 2 * kBytes ? 0 : kd + kBytes;
+            vd = vd == 5 * kBytes ? 3 * kBytes : vd + kBytes;
+        };
+        auto load_kv = [&](int j) {
+            int count = 2 * kParts;
+            if (j + 1 < whole_tiles) {
+                load_whole(V, vd);
+                place();
+                load_whole(K, kd);
+                ask();
+            } else {
+                if (j < n) load(V, j, vd);
+                if (j + 1 < n)
+                    load(K, j + 1, kd);
+                else
+                    count = j < n ? kParts : 0;
+            }
+            rotate();
+            return count;
+        };
+        // Until only the newest loads, so many, are in flight.
+        auto wait_for_older = [&](int newest) {
+            if (newest == 2 * kParts)
+                wait_loads<2 * kParts>();
+            else if (newest == kParts)
+                wait_loads<kParts>();
+            else
+                wait_loads<0>();
+        };
+        if (whole_tiles > 0) {
+            ask();
+            place();
+            ask();
+        }
+        const int late = wave >> 2;  // 1: half a step behind
+        load(K, 0, 0);
+        load_kv(0);
+        int newest = 0;
+        if (late) newest = load_kv(1);
+        wait_for_older(newest);
+        barrier();
+        scores(smem);
+        if (late) barrier();
+        int kb = kBytes, vb = 3 * kBytes;  // buffers of K_{j+1} and V_j
+        for (int j = 0; j < n; ++j) {
+            newest = load_kv(j + 1 + late);
+            if (j < nw) softmax(j);
+            wait_for_older(newest);
+            barrier();
+            if (j < nw) {
+                __builtin_amdgcn_s_setprio(1);
+                products(smem + vb, smem + kb);
+                __builtin_amdgcn_s_setprio(0);
+            }
+            barrier();
+            kb = kb == 2 * kBytes ? 0 : kb + kBytes;
+            vb = vb == 5 * kBytes ? 3 * kBytes : vb + kBytes;
+        }
+        if (!late) barrier();  // as many as the others
+    }
+    store_many(smem, o, m, l, on, orow);
+}
+
+template <class Eng>
 __device__ __forceinline__ void PagedWork<Eng>::few_rows(unsigned char* smem, float (*s_m)[32],
                                                           float (*s_l)[32]) const {
     constexpr int NW = Eng::kWaves;
@@ -427,7 +728,10 @@ __device__ __forceinline__ void PagedWork<Eng>::few_rows(unsigned char* smem, fl
     unsigned char* vt = kt + Eng::kTile;
     auto load = [&](const E* src, int b, unsigned char* dst) {
         const int key0 = it.kbeg + 32 * b;
-        load_groups<kLoads>(src, key0, key0 + 32, 0, 1, dst);
+        if (it.of.tiles == 1)
+            load_groups<kLoads, true>(src, key0, key0 + 32, 0, 1, dst);
+        else
+            load_groups<kLoads>(src, key0, key0 + 32, 0, 1, dst);
     };
     // After the Q loads (see the waits of the loop below).
     asm volatile("" ::: "memory");
@@ -435,7 +739,7 @@ __device__ __forceinline__ void PagedWork<Eng>::few_rows(unsigned char* smem, fl
         load(K, wave, kt);
         load(V, wave, vt);
     }
-    const auto at = Eng::offsets(lane);
+    const auto lds_at = Eng::offsets(lane);
     f32x16 o[D / 32];
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) o[dt] = f32x16{};
@@ -447,7 +751,7 @@ __device__ __forceinline__ void PagedWork<Eng>::few_rows(unsigned char* smem, fl
     for (int b = wave; b < nblk; b += NW) {
         const bool next = b + NW < nblk;
         wait_loads<kLoads>();
-        Eng::block(kt, vt, at, it.kbeg + 32 * b, mask_from, kend, g2, cs, q, o, m, l, [&] {
+        Eng::block(kt, vt, lds_at, it.kbeg + 32 * b, mask_from, kend, g2, cs, q, o, m, l, [&] {
             if (next) {
                 wait_lds();
                 load(K, b + NW, kt);
@@ -583,16 +887,21 @@ __global__ void __launch_bounds__((64 * Eng::kWaves), (Eng::kPerCu * Eng::kWaves
                                 static_cast<size_t>(a.Hkv) * D},
                                // Tiles begin at the unit's first key: behind a prefix, anywhere.
                                a.whole_groups && it.unit.kbeg % Eng::kGroupRows == 0};
-    if (it.many)
-        work.many_rows(smem);
-    else
+    if (it.many) {
+        if constexpr (Eng::kInTurn)
+            work.many_rows_in_turn(smem);
+        else
+            work.many_rows(smem);
+    } else {
         work.few_rows(smem, s_m, s_l);
+    }
 }
 
 // Merges the parts of each row: O = sum O_i 2^(m_i - M) / l with M = max m_i and l = sum l_i
-// 2^(m_i - M), L = (M + log2 l) ln 2. One workgroup per token and 256 / (D / 4) query heads, D / 4
-// lanes a row, four columns each; kBatch parts of a row in flight.
-template <class Eng>
+// 2^(m_i - M), L = (M + log2 l) ln 2. D / 4 lanes hold a row, four columns each; kWays groups of them
+// take every kWays-th part, kBatch in flight, and are merged through LDS in order. One workgroup per token
+// and 256 / (kWays D / 4) query heads.
+template <class Eng, int kWays>
 __global__ void __launch_bounds__(256)
     paged_combine_kernel(typename Mma<typename Eng::T>::elem* __restrict__ O,
                          float* __restrict__ L, PagedArgs a) {
@@ -601,19 +910,23 @@ __global__ void __launch_bounds__(256)
     using Shape = PagedShapeOf<Eng>;
     constexpr int D = Eng::D;
     constexpr int LPR = D / 4;
-    constexpr int kRows = 256 / LPR;
-    constexpr int kBatch = 16;
+    constexpr int kRows = 256 / LPR / kWays;
+    constexpr int kBatch = 8;
+    __shared__ f32x4 s_acc[256];
+    __shared__ float2 s_ml[256 / LPR];
     const int t = blockIdx.x;
-    const int h = blockIdx.y * kRows + threadIdx.x / LPR;
+    const int slot = threadIdx.x / LPR;
+    const int way = slot % kWays;
+    const int h = blockIdx.y * kRows + slot / kWays;
     const int part = threadIdx.x % LPR;
     int u = t + 1;
     if (!a.shared) {
         u = sequence_of(a.starts, a.B, t);
         if (u == a.B) return;  // padding
     }
-    if (h >= a.H) return;
-    const int hk = a.group_div(h);
-    const int g = h - hk * a.group;
+    const bool on = h < a.H;
+    const int hk = a.group_div(on ? h : 0);
+    const int g = (on ? h : 0) - hk * a.group;
     // The parts of unit v's row r: `n` of them, from row `at` of acc and ml on, `step` rows apart.
     struct Parts {
         int n;
@@ -639,16 +952,16 @@ __global__ void __launch_bounds__(256)
         own = parts_of(u, (t - a.starts[u]) * a.group + g);
         if (own.n == 1) return;  // written already
     }
-    const int parts = pre.n + own.n;
+    const int parts = on ? pre.n + own.n : 0;
     float M = -INFINITY, l = 0.0f;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p0 = 0; p0 < parts; p0 += kBatch) {
+    for (int p0 = way; p0 < parts; p0 += kBatch * kWays) {
         float2 v[kBatch];
         f32x4 x[kBatch];
         float M2 = M;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int p = p0 + i;
+            const int p = p0 + i * kWays;
             v[i] = make_float2(-INFINITY, 0.0f);
             x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             if (p < parts) {
@@ -675,6 +988,23 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[c] = fmaf(x[i][c], f, acc[c]);
         }
+    }
+    s_acc[threadIdx.x] = acc;
+    if (part == 0) s_ml[slot] = make_float2(M, l);
+    __syncthreads();
+    if (way != 0 || !on) return;
+#pragma unroll
+    for (int w = 1; w < kWays; ++w) M = fmaxf(M, s_ml[slot + w].x);
+    l = 0.0f;
+    acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWays; ++w) {
+        const float2 v = s_ml[slot + w];
+        const f32x4 x = s_acc[threadIdx.x + w * LPR];
+        const float f = v.x == -INFINITY ? 0.0f : fast_exp2(v.x - M);
+        l = fmaf(v.y, f, l);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] = fmaf(x[c], f, acc[c]);
     }
     const bool none = l == 0.0f;
     const float inv = none ? 0.0f : 1.0f / l;
@@ -774,7 +1104,7 @@ FlashAttentionError run_paged(const PagedCall& call, bool chunks, hipStream_t st
     a.whole_groups = a.page_size % Eng::kGroupRows == 0 &&
                      static_cast<long long>(a.Hkv) * D * Eng::kGroupRows * 4 < (1LL << 31);
     a.c = call.scale * dev::kLog2e;
-    a.min_steps = 8;
+    a.min_steps = 6;
     a.min_rounds = 1;
 
     const PagedGrid<Eng> grid(call, shared, chunks);
@@ -809,46 +1139,68 @@ FlashAttentionError run_paged(const PagedCall& call, bool chunks, hipStream_t st
         go(dev::paged_kernel<Eng, false>);
     FlashAttentionError err = from_hip(hipGetLastError());
     if (err != FlashAttentionError::SUCCESS || !chunks) return err;
-    constexpr int kRows = 256 / (D / 4);
     tok = profile_kernel<T, D>("paged_combine");
-    launch_kernel(tok, (dev::paged_combine_kernel<Eng>),
-                  dim3(static_cast<unsigned>(a.T),
-                       static_cast<unsigned>((a.H + kRows - 1) / kRows)),
-                  dim3(256), 0, stream, static_cast<E*>(call.O), call.L, a);
+    auto merge = [&](auto kernel, int ways) {
+        const int rows = 256 / (D / 4) / ways;
+        launch_kernel(tok, kernel,
+                      dim3(static_cast<unsigned>(a.T),
+                           static_cast<unsigned>((a.H + rows - 1) / rows)),
+                      dim3(256), 0, stream, static_cast<E*>(call.O), call.L, a);
+    };
+    // Few rows have many parts each and want more loads in flight: 61 tokens of 8253 keys, 32 heads,
+    // 9.2 -> 7.0 us; 250 tokens 8.8 -> 11.3.
+    if (static_cast<long long>(a.T) * a.H * D <= (1 << 20))
+        merge(dev::paged_combine_kernel<Eng, 4>, 4);
+    else
+        merge(dev::paged_combine_kernel<Eng, 1>, 1);
     return from_hip(hipGetLastError());
 }
 
-// Workgroups of a launch with chunks and of one without.
+// Workgroups: eight waves (four in fp32), and at head_dim 128 four, two workgroups a CU, where most
+// sequences have few rows: the start of one workgroup then hides behind the other. Kernel times, us, eight
+// waves -> four: 64 sequences behind 2048 keys 46.0 -> 41.5; 250 tokens of 8442 keys 44.3 -> 55.9, 4 x 61
+// tokens of 8253 keys 38.5 -> 43.1.
 template <typename T, int D>
 struct PagedEngines {
     static constexpr int kWaves = std::is_same<T, float>::value ? 4 : 8;
-    using Chunked = dev::PagedEngine<T, D, D == 128 ? 4 : kWaves>;
-    using Whole = dev::PagedEngine<T, D, kWaves>;
+    using Rows = dev::PagedEngine<T, D, kWaves>;
+    using Few = dev::PagedEngine<T, D, D == 128 ? 4 : kWaves>;
+    static bool few(const PagedCall& call, bool shared) {
+        return shared || static_cast<long long>(call.num_tokens) *
+                                 (call.num_heads / call.num_kv_heads) <=
+                             static_cast<long long>(call.batch_size) * dev::kManyRows;
+    }
 };
 
 template <typename T, int D>
 FlashAttentionError run_paged_dim(const PagedCall& call, hipStream_t stream) {
     using Engines = PagedEngines<T, D>;
     const bool shared = call.query_starts == nullptr;
-    if (shared || !fills_chip<typename Engines::Whole>(call)) {
+    if (shared || !fills_chip<typename Engines::Rows>(call)) {
         // A graph's replays need memory that is theirs: the caller's. (Memory that the graph itself
         // allocates, a recorded hipMallocAsync, was not there in the replay of two graphs in a row.)
-        if (call.workspace != nullptr || !stream_capturing(stream))
-            return shared ? run_paged<typename Engines::Chunked, true>(call, true, stream)
-                          : run_paged<typename Engines::Chunked, false>(call, true, stream);
+        if (call.workspace != nullptr || !stream_capturing(stream)) {
+            if (shared) return run_paged<typename Engines::Few, true>(call, true, stream);
+            return Engines::few(call, false)
+                       ? run_paged<typename Engines::Few, false>(call, true, stream)
+                       : run_paged<typename Engines::Rows, false>(call, true, stream);
+        }
         if (shared) return FlashAttentionError::OUT_OF_MEMORY;
     }
-    return run_paged<typename Engines::Whole, false>(call, false, stream);
+    return run_paged<typename Engines::Rows, false>(call, false, stream);
 }
 
 template <typename T, int D>
 long long workspace_of(const PagedCall& call) {
     using Engines = PagedEngines<T, D>;
     const bool shared = call.prefix_len > 0;
-    if (!shared && fills_chip<typename Engines::Whole>(call))
-        return PagedGrid<typename Engines::Whole>(call, false, false).too_large() ? -1 : 0;
-    const PagedGrid<typename Engines::Chunked> grid(call, shared, true);
-    return grid.too_large() ? -1 : static_cast<long long>(grid.bytes());
+    const bool chunks = shared || !fills_chip<typename Engines::Rows>(call);
+    auto bytes = [](const auto& grid) {
+        return grid.too_large() ? -1 : static_cast<long long>(grid.bytes());
+    };
+    if (chunks && Engines::few(call, shared))
+        return bytes(PagedGrid<typename Engines::Few>(call, shared, true));
+    return bytes(PagedGrid<typename Engines::Rows>(call, shared, chunks));
 }
 
 }  // namespace

@@ -393,36 +393,49 @@ def flash_attention_decode_paged(q, k_cache, v_cache, block_table, seq_lens,
 
 def _check_paged(tensors, k_cache, v_cache, block_table, seq_lens, query_starts=None):
     """What the calls on a paged cache have in common: one device, the current one; K and V cache
-    [P, page, Hkv, D] and contiguous; int32 tables. -> B, pages, page size, Hkv, D."""
+    [P, page, Hkv, D] and contiguous; int32 tables. -> device, B, pages, page size, Hkv, D.
+    Small calls wait for the host, so what is right is passed in one look at each tensor
+    (2 us for eight of them); which rule is broken is found out afterwards."""
     torch = _torch()
-    dtype = k_cache.dtype
-    _suffix(k_cache)
-    ints = [t for t in (block_table, seq_lens, query_starts) if t is not None]
-    for t in (*tensors, k_cache, v_cache, *ints):
-        if not t.is_cuda:
-            raise ValueError("tensors must be on the GPU")
     device = torch.cuda.current_device()
-    for t in (*tensors, k_cache, v_cache, *ints):
-        if t.device.index != device:
-            raise ValueError("tensors must be on the current device")
-    for t in (*tensors, v_cache):
-        if t.dtype != dtype:
-            raise ValueError("all tensors must share one dtype")
+    dtype, int32 = k_cache.dtype, torch.int32
+    ints = ((block_table, seq_lens) if query_starts is None
+            else (block_table, seq_lens, query_starts))
+    good = k_cache.is_contiguous() and v_cache.is_contiguous()
+    for t in (k_cache, v_cache, *tensors):
+        if t.get_device() != device or t.dtype is not dtype or t.data_ptr() & 15:
+            good = False
     for t in ints:
-        if t.dtype != torch.int32:
-            raise TypeError("block_table, seq_lens and query_starts must be int32")
+        if t.get_device() != device or t.dtype is not int32 or not t.is_contiguous():
+            good = False
+    if not good:
+        _refuse_paged(tensors, k_cache, v_cache, ints, device)
+    shape, B = k_cache.shape, block_table.shape[0]
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError("expected k_cache, v_cache [P,page,Hkv,D]")
+    if block_table.dim() != 2 or seq_lens.shape != (B,):
+        raise ValueError("expected block_table [B,max_pages] and seq_lens [B]")
+    if query_starts is not None and query_starts.shape != (B + 1,):
+        raise ValueError("expected query_starts [B+1]")
+    return (device, B, *shape)
+
+
+def _refuse_paged(tensors, k_cache, v_cache, ints, device):
+    torch = _torch()
+    _suffix(k_cache)
+    every = (*tensors, k_cache, v_cache, *ints)
+    if not all(t.is_cuda for t in every):
+        raise ValueError("tensors must be on the GPU")
+    if any(t.device.index != device for t in every):
+        raise ValueError("tensors must be on the current device")
+    if any(t.dtype != k_cache.dtype for t in (*tensors, v_cache)):
+        raise ValueError("all tensors must share one dtype")
+    if any(t.dtype != torch.int32 for t in ints):
+        raise TypeError("block_table, seq_lens and query_starts must be int32")
     if not all(t.is_contiguous() for t in (k_cache, v_cache, *ints)):
         raise ValueError("the caches and int32 tensors must be contiguous")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
-        raise ValueError("expected k_cache, v_cache [P,page,Hkv,D]")
-    if block_table.dim() != 2 or tuple(seq_lens.shape) != block_table.shape[:1]:
-        raise ValueError("expected block_table [B,max_pages] and seq_lens [B]")
-    B = block_table.shape[0]
-    if query_starts is not None and tuple(query_starts.shape) != (B + 1,):
-        raise ValueError("expected query_starts [B+1]")
     if any(t.data_ptr() % 16 for t in (*tensors, k_cache, v_cache)):
         raise ValueError("tensors must start at a multiple of 16 bytes")
-    return (B, *k_cache.shape)
 
 
 def _output(given, like, shape, dtype, stream, name):
@@ -456,14 +469,15 @@ def _captured_workspace(lib, kind, like, stream, *sizes):
 def _token_stride(x, name):
     """Elements from token to token of x [T, heads, D], whose heads lie side by side."""
     T, heads, D = x.shape
-    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != D):
+    apart, head, one = x.stride()
+    if one != 1 or (heads > 1 and head != D):
         raise ValueError(f"the heads of a token of {name} must be contiguous")
     if T == 1:
         return heads * D
-    if x.stride(0) < heads * D or x.stride(0) * x.element_size() % 16:
+    if apart < heads * D or apart * x.element_size() % 16:
         raise ValueError(f"the tokens of {name} must be a multiple of 16 bytes apart and not "
                          "overlap")
-    return x.stride(0)
+    return apart
 
 
 def flash_attention_append_paged(k, v, k_cache, v_cache, block_table, seq_lens,
@@ -480,11 +494,12 @@ def flash_attention_append_paged(k, v, k_cache, v_cache, block_table, seq_lens,
     torch = _torch()
     lib = lib or load_library()
     given = (k, v) if q is None else (k, v, q)
-    B, pages, page_size, Hkv, D = _check_paged(given, k_cache, v_cache, block_table, seq_lens,
-                                               query_starts)
+    device, B, pages, page_size, Hkv, D = _check_paged(given, k_cache, v_cache, block_table,
+                                                       seq_lens, query_starts)
     T = k.shape[0]
-    if any(x.dim() != 3 or x.shape[0] != T or x.shape[2] != D for x in given) \
-            or k.shape[1] != Hkv or v.shape[1] != Hkv:
+    H = 0 if q is None else q.shape[1]
+    if k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D) \
+            or (q is not None and q.shape != (T, H, D)):
         raise ValueError("expected k, v [T,Hkv,D] and q [T,H,D] of the cache's Hkv and D")
     R = positions = 0
     if (cos is None) != (sin is None):
@@ -493,24 +508,25 @@ def flash_attention_append_paged(k, v, k_cache, v_cache, block_table, seq_lens,
         if cos.dim() != 2 or sin.shape != cos.shape:
             raise ValueError("expected cos, sin [positions, R / 2]")
         for x in (cos, sin):
-            if x.dtype != torch.float32 or x.device != k.device or not x.is_contiguous() \
-                    or x.data_ptr() % 16:
+            if x.dtype is not torch.float32 or x.get_device() != device \
+                    or not x.is_contiguous() or x.data_ptr() & 15:
                 raise ValueError("cos and sin must be contiguous float32 tensors on the inputs' "
                                  "device")
         positions, R = cos.shape[0], 2 * cos.shape[1]
-    strides = [_token_stride(x, n) for x, n in zip(given, ("k", "v", "q"))]
-    H = 0
+    k_stride, v_stride, q_stride = _token_stride(k, "k"), _token_stride(v, "v"), 0
     if q is not None:
-        H = q.shape[1]
+        q_stride = _token_stride(q, "q")
         out = _output(out, q, (T, H, D), q.dtype, stream, "out")
     elif out is not None:
         raise ValueError("out is the rotated q: it needs q")
-    ptr = lambda x: None if x is None else x.data_ptr()  # noqa: E731
+    q_ptr, out_ptr = (None, None) if q is None else (q.data_ptr(), out.data_ptr())
+    cos_ptr, sin_ptr = (None, None) if cos is None else (cos.data_ptr(), sin.data_ptr())
     status = lib.fn("append_paged", _suffix(k))(
-        ptr(q), k.data_ptr(), v.data_ptr(), ptr(out), k_cache.data_ptr(), v_cache.data_ptr(),
-        block_table.data_ptr(), seq_lens.data_ptr(), ptr(query_starts), ptr(cos), ptr(sin), T, B,
-        H, Hkv, strides[2] if q is not None else 0, strides[0], strides[1], pages, page_size,
-        block_table.shape[1], D, R, positions, bool(interleaved), _stream_ptr(stream))
+        q_ptr, k.data_ptr(), v.data_ptr(), out_ptr, k_cache.data_ptr(), v_cache.data_ptr(),
+        block_table.data_ptr(), seq_lens.data_ptr(),
+        None if query_starts is None else query_starts.data_ptr(), cos_ptr, sin_ptr, T, B, H, Hkv,
+        q_stride, k_stride, v_stride, pages, page_size, block_table.shape[1], D, R, positions,
+        bool(interleaved), _stream_ptr(stream))
     _raise(lib, status)
     return out
 
@@ -525,8 +541,8 @@ def flash_attention_forward_paged(q, k_cache, v_cache, block_table, seq_lens, qu
     -> O [T, H, D], L float32 [T, H] (cuflash_attention_forward_paged_*)."""
     torch = _torch()
     lib = lib or load_library()
-    B, _, page_size, Hkv, D = _check_paged((q,), k_cache, v_cache, block_table, seq_lens,
-                                           query_starts)
+    _, B, _, page_size, Hkv, D = _check_paged((q,), k_cache, v_cache, block_table, seq_lens,
+                                              query_starts)
     if q.dim() != 3 or q.shape[2] != D or not q.is_contiguous():
         raise ValueError("expected contiguous q [T,H,D] of the cache's D")
     T, H = q.shape[:2]
@@ -552,13 +568,13 @@ def flash_attention_decode_shared(q, k_cache, v_cache, prefix_table, prefix_len:
     -> O [B, H, 1, D], L [B, H, 1] (cuflash_attention_decode_shared_*)."""
     torch = _torch()
     lib = lib or load_library()
-    B, _, page_size, Hkv, D = _check_paged((q,), k_cache, v_cache, block_table, seq_lens)
+    device, B, _, page_size, Hkv, D = _check_paged((q,), k_cache, v_cache, block_table, seq_lens)
     if q.dim() != 4 or q.shape[0] != B or q.shape[2] != 1 or q.shape[3] != D \
             or not q.is_contiguous():
         raise ValueError("expected contiguous q [B,H,1,D] of the cache's D")
-    if prefix_table.dtype != torch.int32:
+    if prefix_table.dtype is not torch.int32:
         raise TypeError("prefix_table must be int32")
-    if prefix_table.device != q.device or prefix_table.dim() != 1 \
+    if prefix_table.get_device() != device or prefix_table.dim() != 1 \
             or not prefix_table.is_contiguous() \
             or prefix_table.shape[0] * page_size < prefix_len:
         raise ValueError("prefix_table must name the pages of prefix_len keys, on q's device")
