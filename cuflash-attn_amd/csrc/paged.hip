@@ -781,7 +781,7 @@ __device__ __forceinline__ void PagedWork<Eng>::few_rows(unsigned char* smem, fl
     for (int w = 0; w < NW; ++w) M = fmaxf(M, s_m[w][l32]);
     const float f = m == -INFINITY ? 0.0f : fast_exp2(m - M);
     float* mrg = reinterpret_cast<float*>(smem);
-    {
+    if (on) {
         float* dst = mrg + (wave * 32 + l32) * P + 4 * g2;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) {
@@ -860,9 +860,13 @@ __global__ void __launch_bounds__((64 * Eng::kWaves), (Eng::kPerCu * Eng::kWaves
     // The items of a key/value head stay on one XCD where the heads can be dealt out evenly.
     int hk, x;
     head_rank_order(blockIdx.x, a.Hkv, hk, x);
-    const PagedItem it = paged_item<PagedShapeOf<Eng>, kShared, GpuWave>(a, x);
+    PagedItem it;
+    if constexpr (kShared)
+        it = shared_item<PagedShapeOf<Eng>>(a, x);
+    else
+        it = paged_item<PagedShapeOf<Eng>, GpuWave>(a, x);
     if (!it.found) return;
-    if (a.wgs > 0 && it.first && hk == 0 && threadIdx.x == 0)
+    if (!kShared && a.wgs > 0 && it.first && hk == 0 && threadIdx.x == 0)
         a.units[it.u] = make_int4(it.of.first, it.of.tiles, it.of.chunks, it.many);
     if (!it.direct && it.kend <= it.kbeg) {
         // No keys of this chunk for these rows (a causal mask): nothing but the mark of an empty part.
@@ -919,7 +923,7 @@ __global__ void __launch_bounds__(256)
     const int way = slot % kWays;
     const int h = blockIdx.y * kRows + slot / kWays;
     const int part = threadIdx.x % LPR;
-    int u = t + 1;
+    int u = 0;
     if (!a.shared) {
         u = sequence_of(a.starts, a.B, t);
         if (u == a.B) return;  // padding
@@ -946,8 +950,22 @@ __global__ void __launch_bounds__(256)
     };
     Parts pre{0, 0, 0}, own{0, 0, 0};
     if (a.shared) {
-        pre = parts_of(0, t * a.group + g);
-        if (paged_seq_len(a, t) > a.prefix) own = parts_of(u, g);
+        // Slots as shared_item numbers them.
+        const SharedCut& c = a.cut;
+        auto cut_parts = [&](bool many, int first, int tiles, int n, int r) {
+            const int tile = many ? r / Shape::kTile : r / 32;
+            const int in = many ? r % Shape::kTile : r % 32;
+            return Parts{n, paged_slot_row<Shape>(a, hk, many, first + tile, in),
+                         static_cast<size_t>(tiles) * (many ? Shape::kTile : 32)};
+        };
+        pre = cut_parts(c.pre_many, 0, c.pre_tiles, c.pre_chunks, t * a.group + g);
+        const int keys = paged_seq_len(a, t) - a.prefix;
+        if (keys > 0) {
+            const int len = shared_own_len(a, keys);
+            const int before = c.pre_many == c.own_many ? c.pre_tiles * c.pre_chunks : 0;
+            own = cut_parts(c.own_many, before + t * c.own_chunks * c.own_tiles, c.own_tiles,
+                            (keys + len - 1) / len, g);
+        }
     } else {
         own = parts_of(u, (t - a.starts[u]) * a.group + g);
         if (own.n == 1) return;  // written already
@@ -1026,6 +1044,10 @@ __global__ void __launch_bounds__(256)
 namespace detail {
 namespace {
 
+// Steps and rounds that a chunk has at least: a part of 256 rows is 133 KB to write and to read again.
+constexpr int kMinSteps = 6;
+constexpr int kMinRounds = 1;
+
 // The sizes of one launch: grid and slots.
 template <class Eng>
 struct PagedGrid {
@@ -1036,24 +1058,30 @@ struct PagedGrid {
     long long units;
     int kv_heads;
 
+    dev::SharedCut cut;
+
     PagedGrid(const PagedCall& call, bool shared, bool chunks) {
         kv_heads = call.num_kv_heads;
-        units = call.batch_size + (shared ? 1LL : 0LL);
-        const long long tokens = call.num_tokens;
         const int group = call.num_heads / kv_heads;
-        dev::PagedTiles tiles =
-            dev::paged_tiles<Shape>(tokens, shared ? 1 : call.batch_size, group);
-        if (shared) {
-            const dev::PagedTiles own = dev::paged_tiles<Shape>(1, 1, group);
-            tiles.many += tokens * own.many;
-            tiles.few += tokens * own.few;
-        }
         wgs = chunks ? (Eng::kPerCu * compute_units() + kv_heads - 1) / kv_heads : 0;
+        if (shared) {
+            cut = dev::shared_cut<Shape>(call.batch_size, group, call.prefix_len, wgs, kMinSteps);
+            const long long pre = static_cast<long long>(cut.pre_tiles) * cut.pre_chunks;
+            const long long own =
+                static_cast<long long>(call.batch_size) * cut.own_chunks * cut.own_tiles;
+            items = pre + own;
+            many = (cut.pre_many ? pre : 0) + (cut.own_many ? own : 0);
+            few = items - many;
+            units = 0;
+            return;
+        }
+        const dev::PagedTiles tiles =
+            dev::paged_tiles<Shape>(call.num_tokens, call.batch_size, group);
         items = tiles.many + tiles.few;
         many = few = 0;
+        units = call.batch_size;
         if (chunks) {
-            const long long total = items;
-            items = (total + wgs / 2 + wgs) / wgs * wgs;  // paged_room, in 64 bits
+            items = (items + wgs / 2 + wgs) / wgs * wgs;  // paged_room, in 64 bits
             many = tiles.many ? items : 0;
             few = items;
         }
@@ -1104,12 +1132,13 @@ FlashAttentionError run_paged(const PagedCall& call, bool chunks, hipStream_t st
     a.whole_groups = a.page_size % Eng::kGroupRows == 0 &&
                      static_cast<long long>(a.Hkv) * D * Eng::kGroupRows * 4 < (1LL << 31);
     a.c = call.scale * dev::kLog2e;
-    a.min_steps = 6;
-    a.min_rounds = 1;
+    a.min_steps = kMinSteps;
+    a.min_rounds = kMinRounds;
 
     const PagedGrid<Eng> grid(call, shared, chunks);
     if (grid.too_large()) return FlashAttentionError::INVALID_DIMENSION;
     a.wgs = grid.wgs;
+    a.cut = grid.cut;
     a.max_many = static_cast<int>(grid.many);
     a.max_few = static_cast<int>(grid.few);
     StreamWorkspace ws(stream, true);
@@ -1149,7 +1178,7 @@ FlashAttentionError run_paged(const PagedCall& call, bool chunks, hipStream_t st
     };
     // Few rows have many parts each and want more loads in flight: 61 tokens of 8253 keys, 32 heads,
     // 9.2 -> 7.0 us; 250 tokens 8.8 -> 11.3.
-    if (static_cast<long long>(a.T) * a.H * D <= (1 << 20))
+    if (static_cast<long long>(a.T) * a.H * D <= (1 << 19))
         merge(dev::paged_combine_kernel<Eng, 4>, 4);
     else
         merge(dev::paged_combine_kernel<Eng, 1>, 1);
@@ -1157,18 +1186,18 @@ FlashAttentionError run_paged(const PagedCall& call, bool chunks, hipStream_t st
 }
 
 // Workgroups: eight waves (four in fp32), and at head_dim 128 four, two workgroups a CU, where most
-// sequences have few rows: the start of one workgroup then hides behind the other. Kernel times, us, eight
-// waves -> four: 64 sequences behind 2048 keys 46.0 -> 41.5; 250 tokens of 8442 keys 44.3 -> 55.9, 4 x 61
-// tokens of 8253 keys 38.5 -> 43.1.
+// sequences (in a shared decode the batch) have few rows: the start of one workgroup then hides behind the
+// other. Kernel times, us, eight waves -> four: 4 sequences behind 1000 keys 8.3 -> 7.7, 16 x 5 tokens of
+// up to 8196 keys 64.5 -> 63.0; 250 tokens of 8442 keys 44.3 -> 55.9, 4 x 61 tokens of 8253 keys 38.5 ->
+// 43.1, 128 sequences behind 32768 keys 125 -> 130.
 template <typename T, int D>
 struct PagedEngines {
     static constexpr int kWaves = std::is_same<T, float>::value ? 4 : 8;
     using Rows = dev::PagedEngine<T, D, kWaves>;
     using Few = dev::PagedEngine<T, D, D == 128 ? 4 : kWaves>;
     static bool few(const PagedCall& call, bool shared) {
-        return shared || static_cast<long long>(call.num_tokens) *
-                                 (call.num_heads / call.num_kv_heads) <=
-                             static_cast<long long>(call.batch_size) * dev::kManyRows;
+        return static_cast<long long>(call.num_tokens) * (call.num_heads / call.num_kv_heads) <=
+               static_cast<long long>(shared ? 1 : call.batch_size) * dev::kManyRows;
     }
 };
 
@@ -1180,9 +1209,11 @@ FlashAttentionError run_paged_dim(const PagedCall& call, hipStream_t stream) {
         // A graph's replays need memory that is theirs: the caller's. (Memory that the graph itself
         // allocates, a recorded hipMallocAsync, was not there in the replay of two graphs in a row.)
         if (call.workspace != nullptr || !stream_capturing(stream)) {
-            if (shared) return run_paged<typename Engines::Few, true>(call, true, stream);
-            return Engines::few(call, false)
-                       ? run_paged<typename Engines::Few, false>(call, true, stream)
+            const bool few = Engines::few(call, shared);
+            if (shared)
+                return few ? run_paged<typename Engines::Few, true>(call, true, stream)
+                           : run_paged<typename Engines::Rows, true>(call, true, stream);
+            return few ? run_paged<typename Engines::Few, false>(call, true, stream)
                        : run_paged<typename Engines::Rows, false>(call, true, stream);
         }
         if (shared) return FlashAttentionError::OUT_OF_MEMORY;

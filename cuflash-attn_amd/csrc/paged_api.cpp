@@ -102,7 +102,7 @@ long long workspace_impl(int num_tokens, int batch_size, int num_heads, int num_
     c.num_heads = num_heads;
     c.num_kv_heads = num_kv_heads;
     c.head_dim = head_dim;
-    c.prefix_len = shared ? 1 : 0;
+    c.prefix_len = shared ? 1 << 30 : 0;  // no prefix is cut into more chunks than a long one
     return detail::paged_workspace<T>(c);
 }
 

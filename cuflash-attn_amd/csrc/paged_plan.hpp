@@ -9,6 +9,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace cuflash {
 namespace dev {
 
@@ -31,15 +33,17 @@ inline FastDiv fast_div(int d) {
 // A unit is the tokens of one sequence over its keys; in a shared decode unit 0 is the whole batch
 // over the shared keys and unit b + 1 sequence b over its own ones. The rows of a unit are its
 // tokens times the query heads of one key/value head (row r: token r / group, head r % group).
+// Work comes in items, one workgroup's tile of rows over a chunk of keys:
 //  * More than kManyRows rows: tiles of kTile rows, one 32-row strip per wave, whose waves share the
 //    keys, kStep at a time.
 //  * Fewer: tiles of 32 rows whose keys are spread over the waves, kRound keys in each round. A round
 //    brings as many bytes as kRoundCost steps take time for.
-// Where the tiles alone do not fill the chip (`wgs` > 0), the keys of every unit are cut into chunks
-// that cost at most `s`, with the least s that leaves the items of one key/value head at whole rounds
-// of the workgroups that run at once: the next multiple of wgs beyond tiles + wgs / 2. Chunks leave
-// partial results in slots of their own, numbered like the items, and the first item of a unit notes
-// where they are.
+// A shared decode is cut by the host, but for the own keys of a sequence, whose length a workgroup
+// reads (SharedCut). In a forward, where the tiles alone do not fill the chip (`wgs` > 0), the keys of
+// every unit are cut into chunks that cost at most `s`, with the least s that leaves the items of one
+// key/value head at whole rounds of the workgroups that run at once: the next multiple of wgs beyond
+// tiles + wgs / 2. Chunks leave partial results in slots of their own, numbered like the items of
+// their kind, and the first item of a forward's unit notes where they are.
 constexpr int kManyRows = 96;
 
 template <int TILE, int STEP, int ROUND, int COST>
@@ -48,6 +52,16 @@ struct PagedShape {
     static constexpr int kStep = STEP;
     static constexpr int kRound = ROUND;
     static constexpr int kRoundCost = COST;
+};
+
+// The cut of a shared decode: unit 0 in `pre_chunks` chunks of pre_len keys; the own keys of every
+// sequence in at most own_chunks, of own_least keys or more. Items: unit 0, chunk by chunk, then
+// sequence by sequence.
+struct SharedCut {
+    int pre_tiles, pre_chunks, pre_len;
+    int own_tiles, own_chunks, own_least;
+    FastDiv own_items_div, own_tiles_div, pre_tiles_div;
+    bool pre_many, own_many;
 };
 
 struct PagedArgs {
@@ -67,7 +81,8 @@ struct PagedArgs {
     float c;                    // scale * log2(e)
     float* acc;   // [Hkv, max_many, kTile, D], then [Hkv, max_few, 32, D]
     float2* ml;   // the same without D: m in log2 units, l
-    int4* units;  // [units]: see PagedUnitItems
+    int4* units;  // [B], forward: see PagedUnitItems
+    SharedCut cut;
 };
 
 struct PagedUnit {
@@ -139,20 +154,16 @@ struct UniformDiv {
 
 // The cut of one launch, found by every wave for itself: a few hundred instructions and two loads that
 // need each other, which every workgroup waits for. W: the 64 lanes of a wave, one int each in W::Int.
-// Lane i has the `per` sequences from i per on, the first of them in registers. A shared decode's unit 0
-// stands apart.
-template <class Shape, bool kShared, class W>
+// Lane i has the `per` sequences from i per on, the first of them in registers.
+template <class Shape, class W>
 struct PagedPlan {
     using Int = typename W::Int;
 
     const PagedArgs& a;
     int per;
     Int rows0, keys0;
-    int pre_tiles, pre_steps;  // unit 0 of a shared decode
-    bool pre_many;
     UniformDiv most_many, most_few;  // steps, rounds of a chunk
     Int many, few;                   // items of either kind up to and with the lane's
-    int pre_items;
 
     __host__ __device__ __forceinline__ static int up(int x, int by) {
         return static_cast<int>((static_cast<uint32_t>(x) + (by - 1)) / by);
@@ -163,13 +174,8 @@ struct PagedPlan {
     __host__ __device__ __forceinline__ static int steps(int rows, int keys) {
         return rows > kManyRows ? up(keys, Shape::kStep) : up(keys, Shape::kRound);
     }
-    // Rows and keys of sequence b's unit; no rows: it has no items.
-    __host__ __device__ __forceinline__ int keys_of(int b) const {
-        const int len = paged_seq_len(a, b);
-        return !kShared ? len : len > a.prefix ? len - a.prefix : 0;
-    }
-    __host__ __device__ __forceinline__ int rows_of(int b, int keys) const {
-        if (kShared) return keys > 0 ? a.group : 0;
+    __host__ __device__ __forceinline__ int keys_of(int b) const { return paged_seq_len(a, b); }
+    __host__ __device__ __forceinline__ int rows_of(int b) const {
         const int t0 = paged_clamp(a.starts[b], 0, a.T);
         return (paged_clamp(a.starts[b + 1], t0, a.T) - t0) * a.group;
     }
@@ -188,8 +194,7 @@ struct PagedPlan {
             sum = W::add(sum, W::each([&](int lane) {
                              int x = 0;
                              for (int j = 1; j < per && lane * per + j < a.B; ++j) {
-                                 const int keys = keys_of(lane * per + j);
-                                 x += f(rows_of(lane * per + j, keys), keys);
+                                 x += f(rows_of(lane * per + j), keys_of(lane * per + j));
                              }
                              return x;
                          }));
@@ -200,20 +205,13 @@ struct PagedPlan {
         const int few_s = s / Shape::kRoundCost;
         most_many = UniformDiv(s > a.min_steps ? s : a.min_steps);
         most_few = UniformDiv(few_s > a.min_rounds ? few_s : a.min_rounds);
-        pre_items = kShared ? pre_tiles * chunks(pre_many, pre_steps) : 0;
     }
 
     __host__ __device__ __forceinline__ explicit PagedPlan(const PagedArgs& args)
         : a(args), most_many(1), most_few(1) {
         per = (a.B + 63) / 64;
         keys0 = W::each([&](int lane) { return lane * per < a.B ? keys_of(lane * per) : 0; });
-        rows0 = W::map1(keys0, [&](int lane, int keys) {
-            return lane * per < a.B ? rows_of(lane * per, keys) : 0;
-        });
-        const int pre_rows = kShared ? a.B * a.group : 0;
-        pre_many = pre_rows > kManyRows;
-        pre_tiles = tiles(pre_rows);
-        pre_steps = steps(pre_rows, a.prefix);
+        rows0 = W::each([&](int lane) { return lane * per < a.B ? rows_of(lane * per) : 0; });
         const int room = choose();
         for (int s = 0;; s = s ? 2 * s : most_many.d) {
             if (s) set(s);
@@ -222,7 +220,7 @@ struct PagedPlan {
             few = W::scan(per_lane(
                 [&](int rows, int keys) { return rows > kManyRows ? 0 : items(rows, keys); }));
             // Only units whose work was cut off (choose) can leave more than there is room for.
-            if (a.wgs == 0 || W::lane(many, 63) + W::lane(few, 63) + pre_items <= room ||
+            if (a.wgs == 0 || W::lane(many, 63) + W::lane(few, 63) <= room ||
                 s > 1 << 28)
                 return;
         }
@@ -243,10 +241,8 @@ struct PagedPlan {
                             (rows > kManyRows ? 1 : Shape::kRoundCost);
             return x > static_cast<float>(cap) ? cap : static_cast<int>(x);
         });
-        const int total = W::lane(W::scan(n_tiles), 63) + pre_tiles;
-        const float work = static_cast<float>(W::lane(W::scan(cost), 63)) +
-                           static_cast<float>(pre_tiles) * static_cast<float>(pre_steps) *
-                               (pre_many ? 1 : Shape::kRoundCost);
+        const int total = W::lane(W::scan(n_tiles), 63);
+        const float work = static_cast<float>(W::lane(W::scan(cost), 63));
         // Chunks of at most s: at most work / s + total items, on average work / s + total / 2. So
         // the least s that leaves no more than there is room for lies between work / room and
         // work / (room - total), rounded up (a round is not divided: the bound holds for multiples of
@@ -262,9 +258,7 @@ struct PagedPlan {
         auto count = [&](int s) {
             set(s);
             return W::lane(
-                       W::scan(per_lane([&](int rows, int keys) { return items(rows, keys); })),
-                       63) +
-                   pre_items;
+                W::scan(per_lane([&](int rows, int keys) { return items(rows, keys); })), 63);
         };
         const int n1 = count(s1), n2 = count(s2), n3 = count(s3);
         set(n1 <= room ? s1 : n2 <= room ? s2 : n3 <= room ? s3 : hi);
@@ -292,48 +286,36 @@ struct PagedItem {
     PagedUnitItems of;  // the unit's items
 };
 
-template <class Shape, bool kShared, class W>
+template <class Shape, class W>
 __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int x) {
     PagedItem r{};
-    const PagedPlan<Shape, kShared, W> plan(a);
-    using Plan = PagedPlan<Shape, kShared, W>;
-    // Items of many rows come first: they take longest. Those of unit 0 come before its kind's others.
-    const int pre_many = plan.pre_many ? plan.pre_items : 0;
-    const int pre_few = plan.pre_items - pre_many;
-    const int total_many = W::lane(plan.many, 63) + pre_many;
-    if (x >= total_many + W::lane(plan.few, 63) + pre_few) return r;
+    const PagedPlan<Shape, W> plan(a);
+    using Plan = PagedPlan<Shape, W>;
+    // Items of many rows come first: they take longest.
+    const int total_many = W::lane(plan.many, 63);
+    if (x >= total_many + W::lane(plan.few, 63)) return r;
     r.many = x < total_many;
     if (!r.many) x -= total_many;
     r.index = x;
-    const int pre = r.many ? pre_many : pre_few;
-    int at = x, keys = 0;
-    if (kShared && x < pre) {
-        r.u = 0;
-        r.rows = a.B * a.group;
-        keys = a.prefix;
-        r.unit = PagedUnit{0, a.B, 0, a.prefix};
-    } else {
-        const auto& incl = r.many ? plan.many : plan.few;
-        const int i = W::first(incl, [&](int n) { return pre + n > x; });
-        at -= pre + (i > 0 ? W::lane(incl, i > 0 ? i - 1 : 0) : 0);
-        // The sequence among the lane's.
-        r.rows = W::lane(plan.rows0, i);
-        keys = W::lane(plan.keys0, i);
-        int b = i * plan.per;
-        for (;;) {
-            const int own = (r.rows > kManyRows) == r.many ? plan.items(r.rows, keys) : 0;
-            if (at < own) break;
-            at -= own;
-            if (++b >= a.B) return r;  // not reached
-            keys = plan.keys_of(b);
-            r.rows = plan.rows_of(b, keys);
-        }
-        r.u = kShared ? b + 1 : b;
-        r.unit.n = kShared ? 1 : a.group_div(r.rows);
-        r.unit.t0 = kShared ? b : paged_clamp(a.starts[b], 0, a.T);
-        r.unit.kbeg = kShared ? a.prefix : 0;
-        r.unit.kend = r.unit.kbeg + keys;
+    const auto& incl = r.many ? plan.many : plan.few;
+    const int i = W::first(incl, [&](int n) { return n > x; });
+    int at = x - (i > 0 ? W::lane(incl, i > 0 ? i - 1 : 0) : 0);
+    // The sequence among the lane's.
+    r.rows = W::lane(plan.rows0, i);
+    int keys = W::lane(plan.keys0, i);
+    int b = i * plan.per;
+    for (;;) {
+        const int own = (r.rows > kManyRows) == r.many ? plan.items(r.rows, keys) : 0;
+        if (at < own) break;
+        at -= own;
+        if (++b >= a.B) return r;  // not reached
+        keys = plan.keys_of(b);
+        r.rows = plan.rows_of(b);
     }
+    r.u = b;
+    r.unit.n = a.group_div(r.rows);
+    r.unit.t0 = paged_clamp(a.starts[b], 0, a.T);
+    r.unit.kend = keys;
     r.of.first = x - at;
     r.of.many = r.many;
     r.of.tiles = Plan::tiles(r.rows);
@@ -345,21 +327,101 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
     const int in = at - chunk * r.of.tiles;
     r.first = at == 0;
     r.r0 = (a.causal ? r.of.tiles - 1 - in : in) * (r.many ? Shape::kTile : 32);
-    r.direct = r.of.chunks == 1 && !kShared;
+    r.direct = r.of.chunks == 1;
     // (chunks - 1) each <= (chunks - 1) most < steps: the last chunk has keys as well.
     if (r.of.chunks > 1) each = (each + r.of.chunks - 1) / r.of.chunks;
     const int64_t len = static_cast<int64_t>(each) * (r.many ? Shape::kStep : Shape::kRound);
-    const int64_t beg = r.unit.kbeg + chunk * len;
+    const int64_t beg = chunk * len;
     r.kbeg = static_cast<int>(beg);
     r.kend = beg + len < r.unit.kend ? static_cast<int>(beg + len) : r.unit.kend;
     // With a causal mask, no further than the last row of the tile sees.
-    if (!kShared && a.causal) {
+    if (a.causal) {
         const int last = (r.many ? Shape::kTile : 32) + r.r0;
         const int lim =
             paged_limit(a, r.u, r.unit, a.group_div((last < r.rows ? last : r.rows) - 1));
         if (lim < r.kend) r.kend = lim;
     }
     return r;
+}
+
+// Keys of each chunk of a sequence's own `keys` in a shared decode.
+__host__ __device__ __forceinline__ int shared_own_len(const PagedArgs& a, int keys) {
+    const uint32_t part = (static_cast<uint32_t>(keys) + (a.cut.own_chunks - 1)) / a.cut.own_chunks;
+    const uint32_t len = (part + 31) / 32 * 32;
+    return len > 0x7fffffe0u                                   ? 0x7fffffff
+           : len > static_cast<uint32_t>(a.cut.own_least) ? static_cast<int>(len)
+                                                          : a.cut.own_least;
+}
+
+// Item x of a shared decode. Its slot among those of its kind: unit 0's come first.
+template <class Shape>
+__host__ __device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, int x) {
+    PagedItem r{};
+    const SharedCut& c = a.cut;
+    const int pre = c.pre_tiles * c.pre_chunks;
+    r.index = x;
+    int chunk, tile, len;
+    if (x < pre) {
+        r.many = c.pre_many;
+        r.rows = a.B * a.group;
+        chunk = c.pre_tiles_div(x);
+        tile = x - chunk * c.pre_tiles;
+        len = c.pre_len;
+        r.of.tiles = c.pre_tiles;
+    } else {
+        x -= pre;
+        if (x >= a.B * c.own_chunks * c.own_tiles) return r;
+        if (c.own_many != c.pre_many) r.index = x;
+        r.many = c.own_many;
+        r.rows = a.group;
+        const int b = c.own_items_div(x);
+        x -= b * c.own_chunks * c.own_tiles;
+        chunk = c.own_tiles_div(x);
+        tile = x - chunk * c.own_tiles;
+        r.u = b + 1;
+        r.of.tiles = c.own_tiles;
+    }
+    r.found = true;
+    r.unit = paged_unit(a, r.u);
+    if (r.u > 0) len = shared_own_len(a, r.unit.kend - r.unit.kbeg);
+    r.r0 = tile * (r.many ? Shape::kTile : 32);
+    const int64_t beg = r.unit.kbeg + static_cast<int64_t>(chunk) * len;
+    r.kbeg = beg < r.unit.kend ? static_cast<int>(beg) : r.unit.kend;
+    r.kend = beg + len < r.unit.kend ? static_cast<int>(beg + len) : r.unit.kend;
+    return r;
+}
+
+// The cut, for `wgs` workgroups per key/value head at once: unit 0 in items for three of four of them (the
+// others start on own keys), of at least min_steps steps or one round; own keys in chunks where the tiles of
+// all sequences leave workgroups free.
+template <class Shape>
+inline SharedCut shared_cut(int B, int group, int prefix, int wgs, int min_steps) {
+    SharedCut c{};
+    auto tiles = [](long long rows) {
+        return static_cast<int>(rows > kManyRows ? (rows + Shape::kTile - 1) / Shape::kTile
+                                                 : (rows + 31) / 32);
+    };
+    auto ceil_div = [](long long x, long long by) { return (x + by - 1) / by; };
+    const long long rows = static_cast<long long>(B) * group;
+    c.pre_many = rows > kManyRows;
+    c.own_many = group > kManyRows;
+    c.pre_tiles = tiles(rows);
+    c.own_tiles = tiles(group);
+    const int unit = c.pre_many ? Shape::kStep : Shape::kRound;
+    const long long steps = ceil_div(prefix, unit);
+    const long long chunks =
+        std::max(1LL, std::min<long long>(ceil_div(3LL * wgs, 4LL * c.pre_tiles),
+                                          steps / (c.pre_many ? min_steps : 1)));
+    const long long each = ceil_div(steps, chunks);
+    c.pre_chunks = static_cast<int>(ceil_div(steps, each));
+    c.pre_len = static_cast<int>(std::min<long long>(each * unit, 0x7fffffffLL));
+    c.own_chunks = static_cast<int>(
+        std::max(1LL, std::min<long long>(64, wgs / (static_cast<long long>(B) * c.own_tiles))));
+    c.own_least = c.own_many ? Shape::kStep * min_steps : Shape::kRound;
+    c.pre_tiles_div = fast_div(c.pre_tiles);
+    c.own_tiles_div = fast_div(c.own_tiles);
+    c.own_items_div = fast_div(c.own_chunks * c.own_tiles);
+    return c;
 }
 
 // Row of `acc` and `ml` that item `index`'s row r has.

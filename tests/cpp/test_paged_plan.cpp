@@ -112,34 +112,48 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     a.starts = starts.data();
     a.prefix = a.shared ? spread(rng, 1, a.cap) : 0;
 
-    PagedTiles t = a.shared ? paged_tiles<Shape>(a.B, 1, a.group)
-                            : paged_tiles<Shape>(a.T, a.B, a.group);
-    if (a.shared) {
-        const PagedTiles own = paged_tiles<Shape>(1, 1, a.group);
-        t.many += a.B * own.many;
-        t.few += a.B * own.few;
+    PagedTiles t{};
+    int items, room;
+    if constexpr (kShared) {
+        a.wgs = spread(rng, 1, 300);
+        a.cut = shared_cut<Shape>(a.B, a.group, a.prefix, a.wgs, a.min_steps);
+        const SharedCut& c = a.cut;
+        const int pre = c.pre_tiles * c.pre_chunks, own = a.B * c.own_chunks * c.own_tiles;
+        CHECK(c.pre_len > 0 && int64_t(c.pre_len) * c.pre_chunks >= a.prefix);
+        CHECK(int64_t(c.pre_len) * (c.pre_chunks - 1) < a.prefix);
+        a.max_many = (c.pre_many ? pre : 0) + (c.own_many ? own : 0);
+        a.max_few = pre + own - a.max_many;
+        items = room = pre + own;
+        // The workspace's bound, for any prefix.
+        const SharedCut most = shared_cut<Shape>(a.B, a.group, 1 << 30, a.wgs, a.min_steps);
+        CHECK(c.pre_chunks <= most.pre_chunks && c.own_chunks == most.own_chunks);
+    } else {
+        t = paged_tiles<Shape>(a.T, a.B, a.group);
+        a.wgs = pick(4) == 0 ? 0 : spread(rng, 1, 300);
+        room = a.wgs ? paged_room(int(t.many + t.few), a.wgs) : int(t.many + t.few);
+        a.max_many = t.many > 0 ? (a.wgs ? room : int(t.many)) : 0;
+        a.max_few = a.wgs ? room : int(t.few);
+        const PagedPlan<Shape, HostWave> plan(a);
+        items = HostWave::lane(plan.many, 63) + HostWave::lane(plan.few, 63);
     }
-    a.wgs = pick(4) == 0 ? 0 : spread(rng, 1, 300);
-    const int room = a.wgs ? paged_room(int(t.many + t.few), a.wgs) : int(t.many + t.few);
-    a.max_many = t.many > 0 ? (a.wgs ? room : int(t.many)) : 0;
-    a.max_few = a.wgs ? room : int(t.few);
-
-    const PagedPlan<Shape, kShared, HostWave> plan(a);
-    const int items =
-        HostWave::lane(plan.many, 63) + HostWave::lane(plan.few, 63) + plan.pre_items;
     CHECK(items <= room);
-    std::vector<int4> noted(paged_units(a), make_int4(-1, -1, -1, -1));
+    const int units = a.shared ? a.B + 1 : a.B;
+    std::vector<int4> noted(units, make_int4(-1, -1, -1, -1));
     bool chunked = false;
     // (unit, tile row) -> the key ranges of its items; slots taken.
     std::map<std::pair<int, int>, std::vector<std::array<int, 2>>> met;
     std::map<std::pair<bool, int>, int> slots;
     const int grid = room;
     for (int x = 0; x < grid + 3; ++x) {
-        const PagedItem it = paged_item<Shape, kShared, HostWave>(a, x);
+        PagedItem it;
+        if constexpr (kShared)
+            it = shared_item<Shape>(a, x);
+        else
+            it = paged_item<Shape, HostWave>(a, x);
         CHECK(it.found == (x < items));
         if (!it.found) continue;
         CHECK(x < grid);
-        CHECK(it.u >= 0 && it.u < paged_units(a));
+        CHECK(it.u >= 0 && it.u < units);
         const PagedUnit u = paged_unit(a, it.u);
         CHECK(u.t0 >= 0 && u.n > 0 && u.t0 + u.n <= a.T && it.rows == u.n * a.group);
         CHECK(it.many == (it.rows > kManyRows));
@@ -151,10 +165,28 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         CHECK(taken == 1);
         const int last = a.group_div(std::min(it.rows, it.r0 + tile) - 1);
         if (a.causal) CHECK(it.kend <= paged_limit(a, it.u, u, last));
+        // Parts of the unit's rows, as the combine counts them.
+        PagedUnitItems ui = it.of;
+        if (kShared) {
+            const SharedCut& c = a.cut;
+            const int keys = u.kend - u.kbeg;
+            const int pre = c.pre_tiles * c.pre_chunks;
+            ui.many = it.u == 0 ? c.pre_many : c.own_many;
+            ui.chunks = it.u == 0 ? c.pre_chunks : keys / shared_own_len(a, keys) + (keys % shared_own_len(a, keys) > 0);
+            ui.first = it.u == 0 ? 0
+                                 : (c.pre_many == c.own_many ? pre : 0) +
+                                       (it.u - 1) * c.own_chunks * c.own_tiles;
+            CHECK(ui.chunks <= (it.u == 0 ? c.pre_chunks : c.own_chunks));
+            // Chunks past a sequence's keys are empty items that nobody reads.
+            if (it.index - ui.first >= ui.chunks * ui.tiles) {
+                CHECK(it.kbeg >= it.kend);
+                continue;
+            }
+            noted[it.u] = make_int4(ui.first, ui.tiles, ui.chunks, ui.many);
+        }
         auto& ranges = met[{it.u, it.r0}];
         CHECK(!it.direct || ranges.empty());
         ranges.push_back({it.kbeg, it.kend});
-        const PagedUnitItems ui = it.of;
         if (it.first) {
             CHECK(noted[it.u].x == -1);
             noted[it.u] = make_int4(ui.first, ui.tiles, ui.chunks, ui.many);
@@ -170,7 +202,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         CHECK(row < static_cast<size_t>(a.Hkv) * a.max_many * Shape::kTile +
                         static_cast<size_t>(a.Hkv) * a.max_few * 32);
     }
-    for (int u = 0; u < paged_units(a); ++u) {
+    for (int u = 0; u < units; ++u) {
         const PagedUnit pu = paged_unit(a, u);
         const int rows = pu.n * a.group;
         const int tile = rows > kManyRows ? Shape::kTile : 32;
