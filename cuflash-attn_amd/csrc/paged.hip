@@ -51,7 +51,10 @@ struct PagedEngine {
     static constexpr int kWaves = NW;
     static constexpr int kPerCu = D <= 64 || NW <= 4 ? 2 : 1;  // workgroups (LDS)
     static constexpr int kRoundCost = 2;
-    static constexpr bool kInTurn = NW == 8 && D == 128;
+    // Rows from which on waves have rows of their own. A few-rows item loads its keys for 32 rows: 4 x 61
+    // tokens of 8253 keys, 32 heads over 8, 244 rows a sequence, take 52 us so, and 79 as eight of these.
+    static constexpr int kManyRows = 96;
+    static constexpr bool kInTurn = NW == 8;
     static constexpr int kStepBlocks = 2;              // 32-key blocks of a step (many rows)
     static constexpr int kGroupRows = Lay::kRows;      // key rows of one load
     static constexpr int kGroups = 32 / kGroupRows;    // loads of a tile
@@ -98,6 +101,9 @@ struct PagedEngine<float, D_, NW> {
     static constexpr int kWaves = NW;
     static constexpr int kPerCu = D <= 64 ? 2 : 1;
     static constexpr int kRoundCost = 1;
+    // Few-rows items only: the products take so long that a wave's own loads hide behind them, and tiles of
+    // 32 rows spread better (700 tokens, 16 heads over 4, head_dim 128: 69 -> 53 us).
+    static constexpr int kManyRows = 1 << 28;
     static constexpr bool kInTurn = false;
     static constexpr int kStepBlocks = 1;
     static constexpr int kGroupRows = 256 / D;
@@ -193,7 +199,8 @@ struct PagedEngine<float, D_, NW> {
 
 template <class Eng>
 using PagedShapeOf =
-    PagedShape<32 * Eng::kWaves, 32 * Eng::kStepBlocks, 32 * Eng::kWaves, Eng::kRoundCost>;
+    PagedShape<32 * Eng::kWaves, 32 * Eng::kStepBlocks, 32 * Eng::kWaves, Eng::kRoundCost,
+               Eng::kManyRows>;
 
 // The rows of one key/value head in the cache, from their position in a sequence.
 template <typename E>
@@ -891,13 +898,13 @@ __global__ void __launch_bounds__((64 * Eng::kWaves), (Eng::kPerCu * Eng::kWaves
                                 static_cast<size_t>(a.Hkv) * D},
                                // Tiles begin at the unit's first key: behind a prefix, anywhere.
                                a.whole_groups && it.unit.kbeg % Eng::kGroupRows == 0};
-    if (it.many) {
+    if (std::is_same<typename Eng::T, float>::value || !it.many) {
+        work.few_rows(smem, s_m, s_l);
+    } else if constexpr (!std::is_same<typename Eng::T, float>::value) {
         if constexpr (Eng::kInTurn)
             work.many_rows_in_turn(smem);
         else
             work.many_rows(smem);
-    } else {
-        work.few_rows(smem, s_m, s_l);
     }
 }
 
@@ -1100,7 +1107,8 @@ template <class Eng>
 bool fills_chip(const PagedCall& call) {
     const long long rows =
         static_cast<long long>(call.num_tokens) * (call.num_heads / call.num_kv_heads);
-    return rows / dev::PagedShapeOf<Eng>::kTile * call.num_kv_heads >=
+    const int tile = rows > Eng::kManyRows ? 32 * Eng::kWaves : 32;
+    return rows / tile * call.num_kv_heads >=
            static_cast<long long>(Eng::kPerCu) * compute_units();
 }
 
@@ -1197,7 +1205,7 @@ struct PagedEngines {
     using Few = dev::PagedEngine<T, D, D == 128 ? 4 : kWaves>;
     static bool few(const PagedCall& call, bool shared) {
         return static_cast<long long>(call.num_tokens) * (call.num_heads / call.num_kv_heads) <=
-               static_cast<long long>(shared ? 1 : call.batch_size) * dev::kManyRows;
+               static_cast<long long>(shared ? 1 : call.batch_size) * Rows::kManyRows;
     }
 };
 

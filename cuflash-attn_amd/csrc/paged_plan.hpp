@@ -34,7 +34,7 @@ inline FastDiv fast_div(int d) {
 // over the shared keys and unit b + 1 sequence b over its own ones. The rows of a unit are its
 // tokens times the query heads of one key/value head (row r: token r / group, head r % group).
 // Work comes in items, one workgroup's tile of rows over a chunk of keys:
-//  * More than kManyRows rows: tiles of kTile rows, one 32-row strip per wave, whose waves share the
+//  * More than kMany rows: tiles of kTile rows, one 32-row strip per wave, whose waves share the
 //    keys, kStep at a time.
 //  * Fewer: tiles of 32 rows whose keys are spread over the waves, kRound keys in each round. A round
 //    brings as many bytes as kRoundCost steps take time for.
@@ -44,10 +44,9 @@ inline FastDiv fast_div(int d) {
 // key/value head at whole rounds of the workgroups that run at once: the next multiple of wgs beyond
 // tiles + wgs / 2. Chunks leave partial results in slots of their own, numbered like the items of
 // their kind, and the first item of a forward's unit notes where they are.
-constexpr int kManyRows = 96;
-
-template <int TILE, int STEP, int ROUND, int COST>
+template <int TILE, int STEP, int ROUND, int COST, int MANY>
 struct PagedShape {
+    static constexpr int kMany = MANY;
     static constexpr int kTile = TILE;
     static constexpr int kStep = STEP;
     static constexpr int kRound = ROUND;
@@ -169,10 +168,10 @@ struct PagedPlan {
         return static_cast<int>((static_cast<uint32_t>(x) + (by - 1)) / by);
     }
     __host__ __device__ __forceinline__ static int tiles(int rows) {
-        return rows > kManyRows ? up(rows, Shape::kTile) : up(rows, 32);
+        return rows > Shape::kMany ? up(rows, Shape::kTile) : up(rows, 32);
     }
     __host__ __device__ __forceinline__ static int steps(int rows, int keys) {
-        return rows > kManyRows ? up(keys, Shape::kStep) : up(keys, Shape::kRound);
+        return rows > Shape::kMany ? up(keys, Shape::kStep) : up(keys, Shape::kRound);
     }
     __host__ __device__ __forceinline__ int keys_of(int b) const { return paged_seq_len(a, b); }
     __host__ __device__ __forceinline__ int rows_of(int b) const {
@@ -184,7 +183,7 @@ struct PagedPlan {
         return n == 0 ? 1 : (is_many ? most_many : most_few)(n - 1) + 1;
     }
     __host__ __device__ __forceinline__ int items(int rows, int keys) const {
-        return tiles(rows) * chunks(rows > kManyRows, steps(rows, keys));
+        return tiles(rows) * chunks(rows > Shape::kMany, steps(rows, keys));
     }
     // f(rows, keys) summed over the sequences of each lane, f(0, 0) = 0.
     template <class F>
@@ -216,9 +215,9 @@ struct PagedPlan {
         for (int s = 0;; s = s ? 2 * s : most_many.d) {
             if (s) set(s);
             many = W::scan(per_lane(
-                [&](int rows, int keys) { return rows > kManyRows ? items(rows, keys) : 0; }));
+                [&](int rows, int keys) { return rows > Shape::kMany ? items(rows, keys) : 0; }));
             few = W::scan(per_lane(
-                [&](int rows, int keys) { return rows > kManyRows ? 0 : items(rows, keys); }));
+                [&](int rows, int keys) { return rows > Shape::kMany ? 0 : items(rows, keys); }));
             // Only units whose work was cut off (choose) can leave more than there is room for.
             if (a.wgs == 0 || W::lane(many, 63) + W::lane(few, 63) <= room ||
                 s > 1 << 28)
@@ -238,7 +237,7 @@ struct PagedPlan {
         const Int cost = per_lane([&](int rows, int keys) {
             const float x = static_cast<float>(tiles(rows)) *
                             static_cast<float>(steps(rows, keys)) *
-                            (rows > kManyRows ? 1 : Shape::kRoundCost);
+                            (rows > Shape::kMany ? 1 : Shape::kRoundCost);
             return x > static_cast<float>(cap) ? cap : static_cast<int>(x);
         });
         const int total = W::lane(W::scan(n_tiles), 63);
@@ -286,6 +285,69 @@ struct PagedItem {
     PagedUnitItems of;  // the unit's items
 };
 
+// Tiles of a unit of many rows that have more than `steps` steps: with a causal mask tile t sees the keys
+// below len - n + min(n, ((t + 1) kTile - 1) / group + 1), so those from (64 steps - len + n) group / kTile on.
+template <class Shape>
+__host__ __device__ __forceinline__ int longer_tiles(const PagedArgs& a, int rows, int keys,
+                                                     int steps) {
+    if (rows <= Shape::kMany) return 0;
+    const int tiles = (rows + Shape::kTile - 1) / Shape::kTile;
+    if (steps < 0) return tiles;
+    const int n = a.group_div(rows);
+    const int64_t q = static_cast<int64_t>(steps) * Shape::kStep - keys + (a.causal ? n : 0);
+    if (!a.causal) return q < 0 ? tiles : 0;
+    if (q < 0) return tiles;
+    if (q >= n) return 0;
+    return tiles - static_cast<int>(q) * a.group / Shape::kTile;
+}
+
+// Tile x in the order of their steps, longest first, of the tiles of all units of many rows: the
+// workgroups of a launch without chunks, where a long tile started last would run on alone (7 prompts of
+// 285 to 2001 tokens, head_dim 64: 120.6 -> 114.9 us; 2 of 2048 and 4096, head_dim 32: 96.4 -> 88.0). The steps of the tile are the least s with no more
+// than x longer tiles.
+template <class Shape, class W>
+__host__ __device__ __forceinline__ void tile_by_length(const PagedArgs& a,
+                                                        const PagedPlan<Shape, W>& plan, int x,
+                                                        PagedItem& r, int& keys, int& tile) {
+    auto longer = [&](int steps) {
+        return W::lane(W::scan(plan.per_lane([&](int rows, int k) {
+                           return longer_tiles<Shape>(a, rows, k, steps);
+                       })),
+                       63);
+    };
+    int lo = 0, hi = a.cap / Shape::kStep + 1;
+    while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (longer(mid) <= x)
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    // Its place among those of as many steps.
+    int at = x - longer(lo);
+    auto as_long = [&](int rows, int k) {
+        return longer_tiles<Shape>(a, rows, k, lo - 1) - longer_tiles<Shape>(a, rows, k, lo);
+    };
+    const auto incl = W::scan(plan.per_lane(as_long));
+    const int i = W::first(incl, [&](int n) { return n > at; });
+    at -= i > 0 ? W::lane(incl, i > 0 ? i - 1 : 0) : 0;
+    r.rows = W::lane(plan.rows0, i);
+    keys = W::lane(plan.keys0, i);
+    for (r.u = i * plan.per;;) {
+        const int own = as_long(r.rows, keys);
+        if (at < own) break;
+        at -= own;
+        if (++r.u >= a.B) {  // not reached
+            r.u = a.B - 1;
+            break;
+        }
+        keys = plan.keys_of(r.u);
+        r.rows = plan.rows_of(r.u);
+    }
+    const int tiles = (r.rows + Shape::kTile - 1) / Shape::kTile;
+    tile = tiles - longer_tiles<Shape>(a, r.rows, keys, lo) - 1 - at;
+}
+
 template <class Shape, class W>
 __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int x) {
     PagedItem r{};
@@ -297,24 +359,28 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
     r.many = x < total_many;
     if (!r.many) x -= total_many;
     r.index = x;
-    const auto& incl = r.many ? plan.many : plan.few;
-    const int i = W::first(incl, [&](int n) { return n > x; });
-    int at = x - (i > 0 ? W::lane(incl, i > 0 ? i - 1 : 0) : 0);
-    // The sequence among the lane's.
-    r.rows = W::lane(plan.rows0, i);
-    int keys = W::lane(plan.keys0, i);
-    int b = i * plan.per;
-    for (;;) {
-        const int own = (r.rows > kManyRows) == r.many ? plan.items(r.rows, keys) : 0;
-        if (at < own) break;
-        at -= own;
-        if (++b >= a.B) return r;  // not reached
-        keys = plan.keys_of(b);
-        r.rows = plan.rows_of(b);
+    int at = 0, keys = 0, by_length = -1;
+    if (r.many && a.wgs == 0 && a.B > 1) {
+        tile_by_length<Shape, W>(a, plan, x, r, keys, by_length);
+    } else {
+        const auto& incl = r.many ? plan.many : plan.few;
+        const int i = W::first(incl, [&](int n) { return n > x; });
+        at = x - (i > 0 ? W::lane(incl, i > 0 ? i - 1 : 0) : 0);
+        // The sequence among the lane's.
+        r.rows = W::lane(plan.rows0, i);
+        keys = W::lane(plan.keys0, i);
+        r.u = i * plan.per;
+        for (;;) {
+            const int own = (r.rows > Shape::kMany) == r.many ? plan.items(r.rows, keys) : 0;
+            if (at < own) break;
+            at -= own;
+            if (++r.u >= a.B) return r;  // not reached
+            keys = plan.keys_of(r.u);
+            r.rows = plan.rows_of(r.u);
+        }
     }
-    r.u = b;
     r.unit.n = a.group_div(r.rows);
-    r.unit.t0 = paged_clamp(a.starts[b], 0, a.T);
+    r.unit.t0 = paged_clamp(a.starts[r.u], 0, a.T);
     r.unit.kend = keys;
     r.of.first = x - at;
     r.of.many = r.many;
@@ -326,7 +392,8 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
     const int chunk = r.of.chunks == 1 ? 0 : at / r.of.tiles;
     const int in = at - chunk * r.of.tiles;
     r.first = at == 0;
-    r.r0 = (a.causal ? r.of.tiles - 1 - in : in) * (r.many ? Shape::kTile : 32);
+    const int tile = by_length >= 0 ? by_length : a.causal ? r.of.tiles - 1 - in : in;
+    r.r0 = tile * (r.many ? Shape::kTile : 32);
     r.direct = r.of.chunks == 1;
     // (chunks - 1) each <= (chunks - 1) most < steps: the last chunk has keys as well.
     if (r.of.chunks > 1) each = (each + r.of.chunks - 1) / r.of.chunks;
@@ -398,13 +465,13 @@ template <class Shape>
 inline SharedCut shared_cut(int B, int group, int prefix, int wgs, int min_steps) {
     SharedCut c{};
     auto tiles = [](long long rows) {
-        return static_cast<int>(rows > kManyRows ? (rows + Shape::kTile - 1) / Shape::kTile
+        return static_cast<int>(rows > Shape::kMany ? (rows + Shape::kTile - 1) / Shape::kTile
                                                  : (rows + 31) / 32);
     };
     auto ceil_div = [](long long x, long long by) { return (x + by - 1) / by; };
     const long long rows = static_cast<long long>(B) * group;
-    c.pre_many = rows > kManyRows;
-    c.own_many = group > kManyRows;
+    c.pre_many = rows > Shape::kMany;
+    c.own_many = group > Shape::kMany;
     c.pre_tiles = tiles(rows);
     c.own_tiles = tiles(group);
     const int unit = c.pre_many ? Shape::kStep : Shape::kRound;
@@ -443,8 +510,8 @@ template <class Shape>
 inline PagedTiles paged_tiles(long long tokens, long long units, int group) {
     const long long rows = tokens * group;
     const long long with = units < tokens ? units : tokens;  // sequences that have tokens
-    const long long big = rows / (kManyRows + 1) < with ? rows / (kManyRows + 1) : with;
-    const long long a = rows / 32 + with, b = with * ((kManyRows + 31) / 32);
+    const long long big = rows / (Shape::kMany + 1LL) < with ? rows / (Shape::kMany + 1LL) : with;
+    const long long a = rows / 32 + with, b = with * ((Shape::kMany + 31LL) / 32);
     return {big ? rows / Shape::kTile + big : 0, a < b ? a : b};
 }
 

@@ -140,6 +140,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     const int units = a.shared ? a.B + 1 : a.B;
     std::vector<int4> noted(units, make_int4(-1, -1, -1, -1));
     bool chunked = false;
+    int64_t longest = int64_t(1) << 40;  // tiles of many rows without chunks: longest first
     // (unit, tile row) -> the key ranges of its items; slots taken.
     std::map<std::pair<int, int>, std::vector<std::array<int, 2>>> met;
     std::map<std::pair<bool, int>, int> slots;
@@ -156,11 +157,16 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         CHECK(it.u >= 0 && it.u < units);
         const PagedUnit u = paged_unit(a, it.u);
         CHECK(u.t0 >= 0 && u.n > 0 && u.t0 + u.n <= a.T && it.rows == u.n * a.group);
-        CHECK(it.many == (it.rows > kManyRows));
+        CHECK(it.many == (it.rows > Shape::kMany));
         const int tile = it.many ? Shape::kTile : 32;
         CHECK(it.r0 >= 0 && it.r0 % tile == 0 && it.r0 < it.rows);
         CHECK(it.kbeg >= u.kbeg && it.kend <= u.kend);
-        CHECK(it.index >= 0 && it.index < (it.many ? a.max_many : a.max_few));
+        if (!kShared && a.wgs == 0 && a.B > 1 && it.many) {
+            const int64_t n = (std::max(0, it.kend) + Shape::kStep - 1) / Shape::kStep;
+            CHECK(n <= longest);
+            longest = n;
+        }
+        if (kShared || a.wgs > 0) CHECK(it.index >= 0 && it.index < (it.many ? a.max_many : a.max_few));
         const int taken = ++slots[{it.many, it.index}];
         CHECK(taken == 1);
         const int last = a.group_div(std::min(it.rows, it.r0 + tile) - 1);
@@ -187,15 +193,16 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         auto& ranges = met[{it.u, it.r0}];
         CHECK(!it.direct || ranges.empty());
         ranges.push_back({it.kbeg, it.kend});
-        if (it.first) {
+        if (it.first && a.wgs > 0) {
             CHECK(noted[it.u].x == -1);
             noted[it.u] = make_int4(ui.first, ui.tiles, ui.chunks, ui.many);
         }
-        CHECK(ui.many == it.many && ui.first >= 0);
+        CHECK(ui.many == it.many);
         CHECK(it.direct == (ui.chunks == 1 && !a.shared));
         chunked |= ui.chunks > 1;
         const int i = it.r0 / tile;
         const int at = it.index - ui.first;
+        if (!kShared && a.wgs == 0) continue;  // no slots
         CHECK(at >= 0 && at < ui.tiles * ui.chunks);
         CHECK(at % ui.tiles == (a.causal ? ui.tiles - 1 - i : i));
         const size_t row = paged_slot_row<Shape>(a, a.Hkv - 1, it.many, it.index, tile - 1);
@@ -205,14 +212,15 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     for (int u = 0; u < units; ++u) {
         const PagedUnit pu = paged_unit(a, u);
         const int rows = pu.n * a.group;
-        const int tile = rows > kManyRows ? Shape::kTile : 32;
+        const int tile = rows > Shape::kMany ? Shape::kTile : 32;
         // What the combine finds: noted by the unit's first item, but where there is none.
         const int4 n = noted[u];
-        const PagedUnitItems ui = n.x >= 0 ? PagedUnitItems{n.x, n.y, n.z, n.w != 0}
+        PagedUnitItems ui = n.x >= 0 ? PagedUnitItems{n.x, n.y, n.z, n.w != 0}
                                            : PagedUnitItems{0, 0, 0, false};
-        if (n.x < 0) CHECK(pu.n == 0 || (a.shared && pu.kend == pu.kbeg));
-        if (n.x >= 0) {
-            CHECK(ui.tiles == (rows + tile - 1) / tile && ui.many == (rows > kManyRows));
+        if (!kShared && a.wgs == 0) ui = PagedUnitItems{0, 0, pu.n > 0 ? 1 : 0, false};
+        else if (n.x < 0) CHECK(pu.n == 0 || (a.shared && pu.kend == pu.kbeg));
+        if (n.x >= 0 && (kShared || a.wgs > 0)) {
+            CHECK(ui.tiles == (rows + tile - 1) / tile && ui.many == (rows > Shape::kMany));
             CHECK(ui.first + ui.tiles * ui.chunks <= (ui.many ? a.max_many : a.max_few));
         }
         for (int r0 = 0; r0 < rows; r0 += tile) {
@@ -249,8 +257,8 @@ int main(int argc, char** argv) {
     }
     int chunked = 0;
     for (g_case = 0; g_case < n; ++g_case) {
-        using A = PagedShape<256, 64, 256, 2>;
-        using B = PagedShape<128, 32, 128, 1>;
+        using A = PagedShape<256, 64, 256, 2, 96>;
+        using B = PagedShape<128, 32, 128, 1, 1 << 28>;
         const int kind = rng() % 6;
         chunked += kind == 0   ? launch<A, true>(rng)
                    : kind == 1 ? launch<B, true>(rng)
