@@ -317,7 +317,7 @@ __device__ __forceinline__ void PagedWork<Eng>::store_many(unsigned char* smem,
     if (!it.direct) {
         if (!on) return;
         const size_t slot =
-            paged_slot_row<PagedShapeOf<Eng>>(a, hk, true, it.index, wave * 32 + l32);
+            paged_slot_row<PagedShapeOf<Eng>>(a, hk, true, it.slot, wave * 32 + l32);
         float* dst = a.acc + slot * D + 4 * g2;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) {
@@ -831,7 +831,7 @@ __device__ __forceinline__ void PagedWork<Eng>::few_rows(unsigned char* smem, fl
             }
         }
         if (!it.direct) {
-            const size_t slot = paged_slot_row<PagedShapeOf<Eng>>(a, hk, false, it.index, r);
+            const size_t slot = paged_slot_row<PagedShapeOf<Eng>>(a, hk, false, it.slot, r);
 #pragma unroll
             for (int u = 0; u < kPiece; u += 4)
                 st16(a.acc + slot * D + cc + u,
@@ -879,7 +879,7 @@ __global__ void __launch_bounds__((64 * Eng::kWaves), (Eng::kPerCu * Eng::kWaves
         // No keys of this chunk for these rows (a causal mask): nothing but the mark of an empty part.
         const int n = min(it.rows - it.r0, it.many ? PagedShapeOf<Eng>::kTile : 32);
         for (int r = threadIdx.x; r < n; r += 64 * Eng::kWaves)
-            a.ml[paged_slot_row<PagedShapeOf<Eng>>(a, hk, it.many, it.index, r)] =
+            a.ml[paged_slot_row<PagedShapeOf<Eng>>(a, hk, it.many, it.slot, r)] =
                 make_float2(-INFINITY, 0.0f);
         return;
     }
@@ -953,7 +953,7 @@ __global__ void __launch_bounds__(256)
         const bool ok = d.x >= 0 && d.z >= 0 && tile < d.y &&
                         d.x + static_cast<long long>(d.y) * d.z <= (many ? a.max_many : a.max_few);
         return Parts{ok ? d.z : 0, ok ? paged_slot_row<Shape>(a, hk, many, first, in) : 0,
-                     static_cast<size_t>(d.y) * (many ? Shape::kTile : 32)};
+                     static_cast<size_t>(d.y) * (many ? Shape::kTile : a.few_rows)};
     };
     Parts pre{0, 0, 0}, own{0, 0, 0};
     if (a.shared) {
@@ -963,7 +963,7 @@ __global__ void __launch_bounds__(256)
             const int tile = many ? r / Shape::kTile : r / 32;
             const int in = many ? r % Shape::kTile : r % 32;
             return Parts{n, paged_slot_row<Shape>(a, hk, many, first + tile, in),
-                         static_cast<size_t>(tiles) * (many ? Shape::kTile : 32)};
+                         static_cast<size_t>(tiles) * (many ? Shape::kTile : a.few_rows)};
         };
         pre = cut_parts(c.pre_many, 0, c.pre_tiles, c.pre_chunks, t * a.group + g);
         const int keys = paged_seq_len(a, t) - a.prefix;
@@ -1063,7 +1063,7 @@ struct PagedGrid {
     int wgs;                     // 0: keys are not cut into chunks
     long long items, many, few;  // per key/value head: items, and slots of either kind
     long long units;
-    int kv_heads;
+    int kv_heads, few_rows;
 
     dev::SharedCut cut;
 
@@ -1080,22 +1080,26 @@ struct PagedGrid {
             many = (cut.pre_many ? pre : 0) + (cut.own_many ? own : 0);
             few = items - many;
             units = 0;
+            few_rows = cut.pre_many && !cut.own_many && cut.own_tiles == 1 ? group : 32;
             return;
         }
         const dev::PagedTiles tiles =
             dev::paged_tiles<Shape>(call.num_tokens, call.batch_size, group);
-        items = tiles.many + tiles.few;
+        items = tiles.all;
         many = few = 0;
+        few_rows = 32;
         units = call.batch_size;
         if (chunks) {
             items = (items + wgs / 2 + wgs) / wgs * wgs;  // paged_room, in 64 bits
-            many = tiles.many ? items : 0;
-            few = items;
+            // Items of units with several chunks: at most 3/2 wgs more than tiles (paged_room), and no
+            // more tiles than that, as each adds one at least.
+            few = std::min(items, 3LL * wgs);
+            many = tiles.many ? std::min(few, tiles.many + 2LL * wgs) : 0;
         }
     }
     bool too_large() const { return items * kv_heads > 0x7fffffffLL; }
     size_t slots() const {  // rows of partial results
-        return static_cast<size_t>(kv_heads) * (many * Shape::kTile + few * 32);
+        return static_cast<size_t>(kv_heads) * (many * Shape::kTile + few * few_rows);
     }
     size_t bytes() const {
         return wgs ? slots() * (D * sizeof(float) + sizeof(float2)) + units * sizeof(int4) : 0;
@@ -1151,6 +1155,7 @@ FlashAttentionError run_paged(const PagedCall& call, bool chunks, hipStream_t st
     a.cut = grid.cut;
     a.max_many = static_cast<int>(grid.many);
     a.max_few = static_cast<int>(grid.few);
+    a.few_rows = grid.few_rows;
     StreamWorkspace ws(stream, true);
     if (chunks) {
         void* base = call.workspace;

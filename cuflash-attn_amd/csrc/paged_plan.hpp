@@ -42,8 +42,8 @@ inline FastDiv fast_div(int d) {
 // reads (SharedCut). In a forward, where the tiles alone do not fill the chip (`wgs` > 0), the keys of
 // every unit are cut into chunks that cost at most `s`, with the least s that leaves the items of one
 // key/value head at whole rounds of the workgroups that run at once: the next multiple of wgs beyond
-// tiles + wgs / 2. Chunks leave partial results in slots of their own, numbered like the items of
-// their kind, and the first item of a forward's unit notes where they are.
+// tiles + wgs / 2. The items of units with several chunks leave partial results in slots, numbered in
+// their order among their kind, and the first item of a forward's unit notes where they are.
 template <int TILE, int STEP, int ROUND, int COST, int MANY>
 struct PagedShape {
     static constexpr int kMany = MANY;
@@ -78,7 +78,8 @@ struct PagedArgs {
     int min_steps, min_rounds;  // least per chunk
     int max_many, max_few;      // slots per key/value head for the items of either kind
     float c;                    // scale * log2(e)
-    float* acc;   // [Hkv, max_many, kTile, D], then [Hkv, max_few, 32, D]
+    int few_rows;               // rows of a slot for an item of few rows
+    float* acc;   // [Hkv, max_many, kTile, D], then [Hkv, max_few, few_rows, D]
     float2* ml;   // the same without D: m in log2 units, l
     int4* units;  // [B], forward: see PagedUnitItems
     SharedCut cut;
@@ -265,7 +266,7 @@ struct PagedPlan {
     }
 };
 
-// A unit's items in one launch: `first` is the index of its first one among those of its kind; item
+// A unit's items in one launch: `first` is the slot of its first one, where it has several chunks; slot
 // first + chunk * tiles + i is chunk `chunk` of tile i (of tile tiles - 1 - i with a causal mask:
 // the longest tiles start first). As noted in PagedArgs::units: {first, tiles, chunks, many}.
 struct PagedUnitItems {
@@ -280,7 +281,7 @@ struct PagedItem {
     bool first;   // the first item of its unit
     int u, rows, r0;
     int kbeg, kend;
-    int index;  // among the items of its kind: the slot
+    int slot;  // for its partial results, among those of its kind
     PagedUnit unit;
     PagedUnitItems of;  // the unit's items
 };
@@ -358,14 +359,22 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
     if (x >= total_many + W::lane(plan.few, 63)) return r;
     r.many = x < total_many;
     if (!r.many) x -= total_many;
-    r.index = x;
-    int at = 0, keys = 0, by_length = -1;
+    int at = 0, keys = 0, by_length = -1, slot = 0;
     if (r.many && a.wgs == 0 && a.B > 1) {
         tile_by_length<Shape, W>(a, plan, x, r, keys, by_length);
     } else {
         const auto& incl = r.many ? plan.many : plan.few;
         const int i = W::first(incl, [&](int n) { return n > x; });
         at = x - (i > 0 ? W::lane(incl, i > 0 ? i - 1 : 0) : 0);
+        // Slots before the lane's units: the items of units with several chunks.
+        auto slots = [&](int rows, int n) {
+            const int own = (rows > Shape::kMany) == r.many ? plan.items(rows, n) : 0;
+            return own > Plan::tiles(rows) ? own : 0;
+        };
+        if (a.wgs > 0) {
+            const auto before = W::scan(plan.per_lane(slots));
+            slot = i > 0 ? W::lane(before, i > 0 ? i - 1 : 0) : 0;
+        }
         // The sequence among the lane's.
         r.rows = W::lane(plan.rows0, i);
         keys = W::lane(plan.keys0, i);
@@ -374,6 +383,7 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
             const int own = (r.rows > Shape::kMany) == r.many ? plan.items(r.rows, keys) : 0;
             if (at < own) break;
             at -= own;
+            slot += slots(r.rows, keys);
             if (++r.u >= a.B) return r;  // not reached
             keys = plan.keys_of(r.u);
             r.rows = plan.rows_of(r.u);
@@ -382,13 +392,14 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
     r.unit.n = a.group_div(r.rows);
     r.unit.t0 = paged_clamp(a.starts[r.u], 0, a.T);
     r.unit.kend = keys;
-    r.of.first = x - at;
+    r.of.first = slot;
+    r.slot = slot + at;
     r.of.many = r.many;
     r.of.tiles = Plan::tiles(r.rows);
     int each = Plan::steps(r.rows, keys);
     r.of.chunks = plan.chunks(r.many, each);
-    r.found = a.wgs == 0 ||
-              r.of.first + r.of.tiles * r.of.chunks <= (r.many ? a.max_many : a.max_few);
+    r.found = r.of.chunks == 1 ||
+              slot + r.of.tiles * r.of.chunks <= (r.many ? a.max_many : a.max_few);
     const int chunk = r.of.chunks == 1 ? 0 : at / r.of.tiles;
     const int in = at - chunk * r.of.tiles;
     r.first = at == 0;
@@ -426,7 +437,7 @@ __host__ __device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, in
     PagedItem r{};
     const SharedCut& c = a.cut;
     const int pre = c.pre_tiles * c.pre_chunks;
-    r.index = x;
+    r.slot = x;
     int chunk, tile, len;
     if (x < pre) {
         r.many = c.pre_many;
@@ -438,7 +449,7 @@ __host__ __device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, in
     } else {
         x -= pre;
         if (x >= a.B * c.own_chunks * c.own_tiles) return r;
-        if (c.own_many != c.pre_many) r.index = x;
+        if (c.own_many != c.pre_many) r.slot = x;
         r.many = c.own_many;
         r.rows = a.group;
         const int b = c.own_items_div(x);
@@ -491,28 +502,29 @@ inline SharedCut shared_cut(int B, int group, int prefix, int wgs, int min_steps
     return c;
 }
 
-// Row of `acc` and `ml` that item `index`'s row r has.
+// Row of `acc` and `ml` that row r of a slot has.
 template <class Shape>
 __host__ __device__ __forceinline__ size_t paged_slot_row(const PagedArgs& a, int hk, bool many,
-                                                          int index, int r) {
+                                                          int slot, int r) {
     if (many)
-        return (static_cast<size_t>(hk) * a.max_many + index) * Shape::kTile + r;
+        return (static_cast<size_t>(hk) * a.max_many + slot) * Shape::kTile + r;
     return static_cast<size_t>(a.Hkv) * a.max_many * Shape::kTile +
-           (static_cast<size_t>(hk) * a.max_few + index) * 32 + r;
+           (static_cast<size_t>(hk) * a.max_few + slot) * a.few_rows + r;
 }
 
-// Sizes that the host knows: the tiles of either kind that `units` sequences with `tokens` tokens in
-// all can have at most.
+// What the host knows of a forward: the tiles, of many rows and in all, that `units` sequences with
+// `tokens` tokens in all can have at most.
 struct PagedTiles {
-    long long many, few;
+    long long many, all;
 };
 template <class Shape>
 inline PagedTiles paged_tiles(long long tokens, long long units, int group) {
     const long long rows = tokens * group;
-    const long long with = units < tokens ? units : tokens;  // sequences that have tokens
-    const long long big = rows / (Shape::kMany + 1LL) < with ? rows / (Shape::kMany + 1LL) : with;
-    const long long a = rows / 32 + with, b = with * ((Shape::kMany + 31LL) / 32);
-    return {big ? rows / Shape::kTile + big : 0, a < b ? a : b};
+    const long long with = std::min(units, tokens);  // sequences that have tokens
+    const long long big = std::min(rows / (Shape::kMany + 1LL), with);
+    const long long few = (Shape::kMany + 31LL) / 32;  // most tiles of a unit of few rows
+    return {big ? rows / Shape::kTile + big : 0,
+            std::min(rows / 32 + with, few * with + (big ? rows / Shape::kTile : 0))};
 }
 
 }  // namespace dev

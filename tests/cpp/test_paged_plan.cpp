@@ -123,6 +123,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         CHECK(int64_t(c.pre_len) * (c.pre_chunks - 1) < a.prefix);
         a.max_many = (c.pre_many ? pre : 0) + (c.own_many ? own : 0);
         a.max_few = pre + own - a.max_many;
+        a.few_rows = c.pre_many && !c.own_many && c.own_tiles == 1 ? a.group : 32;
         items = room = pre + own;
         // The workspace's bound, for any prefix.
         const SharedCut most = shared_cut<Shape>(a.B, a.group, 1 << 30, a.wgs, a.min_steps);
@@ -130,9 +131,10 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     } else {
         t = paged_tiles<Shape>(a.T, a.B, a.group);
         a.wgs = pick(4) == 0 ? 0 : spread(rng, 1, 300);
-        room = a.wgs ? paged_room(int(t.many + t.few), a.wgs) : int(t.many + t.few);
-        a.max_many = t.many > 0 ? (a.wgs ? room : int(t.many)) : 0;
-        a.max_few = a.wgs ? room : int(t.few);
+        room = a.wgs ? paged_room(int(t.all), a.wgs) : int(t.all);
+        a.max_few = a.wgs ? std::min(room, 3 * a.wgs) : 0;
+        a.max_many = t.many > 0 ? int(std::min<long long>(a.max_few, t.many + 2LL * a.wgs)) : 0;
+        a.few_rows = 32;
         const PagedPlan<Shape, HostWave> plan(a);
         items = HostWave::lane(plan.many, 63) + HostWave::lane(plan.few, 63);
     }
@@ -166,9 +168,11 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
             CHECK(n <= longest);
             longest = n;
         }
-        if (kShared || a.wgs > 0) CHECK(it.index >= 0 && it.index < (it.many ? a.max_many : a.max_few));
-        const int taken = ++slots[{it.many, it.index}];
-        CHECK(taken == 1);
+        if (!it.direct) CHECK(it.slot >= 0 && it.slot < (it.many ? a.max_many : a.max_few));
+        if (!it.direct) {
+            const int taken = ++slots[{it.many, it.slot}];
+            CHECK(taken == 1);
+        }
         const int last = a.group_div(std::min(it.rows, it.r0 + tile) - 1);
         if (a.causal) CHECK(it.kend <= paged_limit(a, it.u, u, last));
         // Parts of the unit's rows, as the combine counts them.
@@ -184,7 +188,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
                                        (it.u - 1) * c.own_chunks * c.own_tiles;
             CHECK(ui.chunks <= (it.u == 0 ? c.pre_chunks : c.own_chunks));
             // Chunks past a sequence's keys are empty items that nobody reads.
-            if (it.index - ui.first >= ui.chunks * ui.tiles) {
+            if (it.slot - ui.first >= ui.chunks * ui.tiles) {
                 CHECK(it.kbeg >= it.kend);
                 continue;
             }
@@ -201,13 +205,15 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         CHECK(it.direct == (ui.chunks == 1 && !a.shared));
         chunked |= ui.chunks > 1;
         const int i = it.r0 / tile;
-        const int at = it.index - ui.first;
-        if (!kShared && a.wgs == 0) continue;  // no slots
+        const int at = it.slot - ui.first;
+        if (it.direct) continue;  // no slot
         CHECK(at >= 0 && at < ui.tiles * ui.chunks);
         CHECK(at % ui.tiles == (a.causal ? ui.tiles - 1 - i : i));
-        const size_t row = paged_slot_row<Shape>(a, a.Hkv - 1, it.many, it.index, tile - 1);
+        const int used = std::min(tile, it.rows - it.r0);
+        CHECK(it.many || used <= a.few_rows);
+        const size_t row = paged_slot_row<Shape>(a, a.Hkv - 1, it.many, it.slot, used - 1);
         CHECK(row < static_cast<size_t>(a.Hkv) * a.max_many * Shape::kTile +
-                        static_cast<size_t>(a.Hkv) * a.max_few * 32);
+                        static_cast<size_t>(a.Hkv) * a.max_few * a.few_rows);
     }
     for (int u = 0; u < units; ++u) {
         const PagedUnit pu = paged_unit(a, u);
@@ -221,7 +227,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         else if (n.x < 0) CHECK(pu.n == 0 || (a.shared && pu.kend == pu.kbeg));
         if (n.x >= 0 && (kShared || a.wgs > 0)) {
             CHECK(ui.tiles == (rows + tile - 1) / tile && ui.many == (rows > Shape::kMany));
-            CHECK(ui.first + ui.tiles * ui.chunks <= (ui.many ? a.max_many : a.max_few));
+            CHECK(ui.chunks <= 1 || ui.first + ui.tiles * ui.chunks <= (ui.many ? a.max_many : a.max_few));
         }
         for (int r0 = 0; r0 < rows; r0 += tile) {
             auto ranges = met[{u, r0}];
