@@ -869,7 +869,7 @@ __global__ void __launch_bounds__((64 * Eng::kWaves), (Eng::kPerCu * Eng::kWaves
     head_rank_order(blockIdx.x, a.Hkv, hk, x);
     PagedItem it;
     if constexpr (kShared)
-        it = shared_item<PagedShapeOf<Eng>>(a, x);
+        it = shared_item<PagedShapeOf<Eng>, GpuWave>(a, x);
     else
         it = paged_item<PagedShapeOf<Eng>, GpuWave>(a, x);
     if (!it.found) return;

@@ -35,12 +35,12 @@ struct GpuWave {
         return f(v);
     }
     template <class F>
-    __device__ static Int map1(Int v, F f) {
-        return f(static_cast<int>(threadIdx.x & 63), v);
-    }
-    template <class F>
     __device__ static Int map2(Int v, Int w, F f) {
         return f(v, w);
+    }
+    template <class F>
+    __device__ static Int map3(Int v, Int w, F f) {
+        return f(static_cast<int>(threadIdx.x & 63), v, w);
     }
     __device__ static Int add(Int a, Int b) { return a + b; }
     // Inclusive sum over the lanes.

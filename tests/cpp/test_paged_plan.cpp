@@ -36,8 +36,8 @@ struct HostWave {
         return each([&](int i) { return x[i] + y[i]; });
     }
     template <class F>
-    static Int map1(const Int& x, F f) {
-        return each([&](int i) { return f(i, x[i]); });
+    static Int map3(const Int& x, const Int& y, F f) {
+        return each([&](int i) { return f(i, x[i], y[i]); });
     }
     template <class F>
     static Int map2(const Int& x, const Int& y, F f) {
@@ -150,7 +150,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     for (int x = 0; x < grid + 3; ++x) {
         PagedItem it;
         if constexpr (kShared)
-            it = shared_item<Shape>(a, x);
+            it = shared_item<Shape, HostWave>(a, x);
         else
             it = paged_item<Shape, HostWave>(a, x);
         CHECK(it.found == (x < items));
