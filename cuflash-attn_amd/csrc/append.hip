@@ -184,6 +184,9 @@ FlashAttentionError run_append(const AppendCall& c, hipStream_t stream) {
     constexpr int kUnits = D * static_cast<int>(sizeof(E)) / 32;  // per row
     const long long units = (static_cast<long long>(a.H) + 2LL * a.Hkv) * kUnits;
     const int threads = static_cast<int>(std::min(1024LL, (units + 63) / 64 * 64));
+    // A launch has at most 2^32 - 1 threads in x.
+    if (static_cast<long long>(c.num_tokens) * threads > 0xffffffffLL)
+        return FlashAttentionError::INVALID_DIMENSION;
     ProfileEvents tok = profile_kernel<T, D>("append");
     auto go = [&](auto kernel) {
         launch_kernel(tok, kernel, dim3(static_cast<unsigned>(c.num_tokens)),

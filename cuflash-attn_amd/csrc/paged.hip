@@ -103,7 +103,7 @@ struct PagedEngine<float, D_, NW> {
     static constexpr int kRoundCost = 1;
     // Few-rows items only: the products take so long that a wave's own loads hide behind them, and tiles of
     // 32 rows spread better (700 tokens, 16 heads over 4, head_dim 128: 69 -> 53 us).
-    static constexpr int kManyRows = 1 << 28;
+    static constexpr int kManyRows = 0x7fffffff;
     static constexpr bool kInTurn = false;
     static constexpr int kStepBlocks = 1;
     static constexpr int kGroupRows = 256 / D;
@@ -1063,12 +1063,12 @@ struct PagedGrid {
     int wgs;                     // 0: keys are not cut into chunks
     long long items, many, few;  // per key/value head: items, and slots of either kind
     long long units;
-    int kv_heads, few_rows;
-
+    int kv_heads, few_rows, tokens;
     dev::SharedCut cut;
 
     PagedGrid(const PagedCall& call, bool shared, bool chunks) {
         kv_heads = call.num_kv_heads;
+        tokens = call.num_tokens;
         const int group = call.num_heads / kv_heads;
         wgs = chunks ? (Eng::kPerCu * compute_units() + kv_heads - 1) / kv_heads : 0;
         if (shared) {
@@ -1097,7 +1097,11 @@ struct PagedGrid {
             many = tiles.many ? std::min(few, tiles.many + 2LL * wgs) : 0;
         }
     }
-    bool too_large() const { return items * kv_heads > 0x7fffffffLL; }
+    // A launch has at most 2^32 - 1 threads in x; the merge has a workgroup per token.
+    bool too_large() const {
+        return items * kv_heads * 64 * Eng::kWaves > 0xffffffffLL ||
+               (wgs && 256LL * tokens > 0xffffffffLL);
+    }
     size_t slots() const {  // rows of partial results
         return static_cast<size_t>(kv_heads) * (many * Shape::kTile + few * few_rows);
     }
@@ -1231,7 +1235,10 @@ FlashAttentionError run_paged_dim(const PagedCall& call, hipStream_t stream) {
             return few ? run_paged<typename Engines::Few, false>(call, true, stream)
                        : run_paged<typename Engines::Rows, false>(call, true, stream);
         }
-        if (shared) return FlashAttentionError::OUT_OF_MEMORY;
+        if (shared)
+            return PagedGrid<typename Engines::Rows>(call, true, true).too_large()
+                       ? FlashAttentionError::INVALID_DIMENSION
+                       : FlashAttentionError::OUT_OF_MEMORY;
     }
     return run_paged<typename Engines::Rows, false>(call, false, stream);
 }

@@ -14,6 +14,8 @@ namespace {
 using E = FlashAttentionError;
 
 constexpr long long kIntMax = 0x7fffffffLL;
+constexpr long long kMaxKeys = kIntMax - 1023;  // key positions some tiles past the end stay in 32 bits
+constexpr int kMaxHeads = 65535;                // the merge's grid has the query heads in y
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -28,7 +30,7 @@ E check_sizes(int num_tokens, int batch_size, int num_heads, int num_kv_heads, i
 }
 E check_relations(int num_heads, int num_kv_heads, int page_size, int max_pages) {
     if (num_heads % num_kv_heads != 0) return E::DIMENSION_MISMATCH;
-    if (static_cast<long long>(page_size) * max_pages > kIntMax) return E::INVALID_DIMENSION;
+    if (static_cast<long long>(page_size) * max_pages > kMaxKeys) return E::INVALID_DIMENSION;
     return E::SUCCESS;
 }
 
@@ -65,6 +67,9 @@ E check_append(const detail::AppendCall& c, int elem_bytes) {
                           static_cast<const void*>(c.rope_cos),
                           static_cast<const void*>(c.rope_sin)})
         if (!aligned16(p)) return E::INVALID_DIMENSION;
+    // In place, a token's rotated queries must not reach another token's.
+    if (c.Q && c.Q_out == c.Q && c.num_tokens > 1 && c.q_stride != q_row)
+        return E::DIMENSION_MISMATCH;
     return E::SUCCESS;
 }
 
@@ -81,7 +86,8 @@ E check_attention(const detail::PagedCall& c, bool shared) {
     err = check_relations(c.num_heads, c.num_kv_heads, c.page_size, c.max_pages);
     if (err != E::SUCCESS) return err;
     if (c.prefix_len > c.page_size * c.max_pages) return E::DIMENSION_MISMATCH;
-    if (static_cast<long long>(c.num_tokens) * c.num_heads > kIntMax) return E::INVALID_DIMENSION;
+    if (static_cast<long long>(c.num_tokens) * c.num_heads > kIntMax || c.num_heads > kMaxHeads)
+        return E::INVALID_DIMENSION;
     for (const void* p : {c.Q, c.K_cache, c.V_cache, static_cast<const void*>(c.O)})
         if (!aligned16(p)) return E::INVALID_DIMENSION;
     if (reinterpret_cast<uintptr_t>(c.workspace) % 256) return E::INVALID_DIMENSION;
@@ -94,7 +100,8 @@ long long workspace_impl(int num_tokens, int batch_size, int num_heads, int num_
                          int head_dim, bool shared) {
     if (check_sizes(num_tokens, batch_size, num_heads, num_kv_heads, 1, 1, head_dim) !=
             E::SUCCESS ||
-        num_heads % num_kv_heads != 0 || static_cast<long long>(num_tokens) * num_heads > kIntMax)
+        num_heads % num_kv_heads != 0 || static_cast<long long>(num_tokens) * num_heads > kIntMax ||
+        num_heads > kMaxHeads)
         return -1;
     detail::PagedCall c{};
     c.num_tokens = num_tokens;
@@ -117,7 +124,8 @@ template <typename T>
 E shared_impl(const detail::PagedCall& c, hipStream_t stream) {
     E err = check_attention(c, true);
     if (err != E::SUCCESS) return err;
-    if (c.prefix_len == 0)
+    // A captured call needs memory that is the caller's, which that entry point has no argument for.
+    if (c.prefix_len == 0 && !detail::stream_capturing(stream))
         return detail::launch_decode_paged<T>(
             static_cast<const T*>(c.Q), static_cast<const T*>(c.K_cache),
             static_cast<const T*>(c.V_cache), static_cast<T*>(c.O), c.L, c.block_table, c.seq_lens,

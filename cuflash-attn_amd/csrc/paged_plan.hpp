@@ -96,9 +96,6 @@ __host__ __device__ __forceinline__ int paged_clamp(int x, int lo, int hi) {
 __host__ __device__ __forceinline__ int paged_seq_len(const PagedArgs& a, int b) {
     return paged_clamp(a.seq_lens[b], 0, a.cap);
 }
-__host__ __device__ __forceinline__ int paged_units(const PagedArgs& a) {
-    return a.shared ? a.B + 1 : a.B;
-}
 __host__ __device__ __forceinline__ PagedUnit paged_unit(const PagedArgs& a, int u) {
     if (a.shared) {
         if (u == 0) return {0, a.B, 0, a.prefix};
@@ -512,8 +509,8 @@ inline SharedCut shared_cut(int B, int group, int prefix, int wgs, int min_steps
     const long long chunks =
         std::max(1LL, std::min<long long>(ceil_div(3LL * wgs, 4LL * c.pre_tiles),
                                           steps / (c.pre_many ? min_steps : 1)));
-    const long long each = ceil_div(steps, chunks);
-    c.pre_chunks = static_cast<int>(ceil_div(steps, each));
+    const long long each = std::max(1LL, ceil_div(steps, chunks));
+    c.pre_chunks = prefix > 0 ? static_cast<int>(ceil_div(steps, each)) : 0;
     c.pre_len = static_cast<int>(std::min<long long>(each * unit, 0x7fffffffLL));
     c.own_chunks = static_cast<int>(
         std::max(1LL, std::min<long long>(64, wgs / (static_cast<long long>(B) * c.own_tiles))));

@@ -474,9 +474,9 @@ def _token_stride(x, name):
         raise ValueError(f"the heads of a token of {name} must be contiguous")
     if T == 1:
         return heads * D
-    if apart < heads * D or apart * x.element_size() % 16:
-        raise ValueError(f"the tokens of {name} must be a multiple of 16 bytes apart and not "
-                         "overlap")
+    if apart < heads * D or apart > 0x7fffffff or apart * x.element_size() % 16:
+        raise ValueError(f"the tokens of {name} must be a multiple of 16 bytes apart, less than 2^31 "
+                         "elements, and not overlap")
     return apart
 
 

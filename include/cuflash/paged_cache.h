@@ -18,15 +18,18 @@
 //    are padding: their outputs are left as they were.
 //  * seq_lens [batch_size] (int32) counts a sequence's keys WITH its new tokens, so token t of
 //    sequence b stands at position seq_lens[b] - (query_starts[b + 1] - t), and the same array
-//    goes to the append and to the attention after it.
+//    goes to the append and to the attention after it. The attentions take a length past the block
+//    table's max_pages_per_seq * page_size keys for that many.
 //  * head_dim 32, 64 or 128; num_heads a multiple of num_kv_heads (query head h reads key/value
 //    head h / (num_heads / num_kv_heads)).
 //  * Pointers and token strides are multiples of 16 bytes. Every pointer is a device pointer.
 //    Calls are asynchronous on `stream` and can be captured into a HIP graph (see Workspaces).
 // Validation, in this order: null pointers (NULL_POINTER), dimensions that are not positive
 // (INVALID_DIMENSION), head_dim (UNSUPPORTED_HEAD_DIM), scale (INVALID_DIMENSION), then the
-// relations between sizes (DIMENSION_MISMATCH), sizes whose products exceed 32 bits and alignment
-// (INVALID_DIMENSION).
+// relations between sizes (DIMENSION_MISMATCH), sizes that are too large and alignment
+// (INVALID_DIMENSION). Too large: page_size * max_pages_per_seq beyond 2^31 - 1024, num_tokens *
+// num_heads beyond 2^31 - 1, num_heads beyond 65535 (the attentions), more than 2^32 - 1 threads in one
+// launch.
 
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -46,13 +49,13 @@ namespace cuflash {
 // are rotated by row p = position: the pair (x1, x2) = elements (i, i + rotary_dim / 2), or (2 i,
 // 2 i + 1) if `interleaved`, becomes (x1 cos - x2 sin, x2 cos + x1 sin), computed in float and
 // rounded once. Rotated queries go to Q_out [num_tokens, num_heads, head_dim], which may be Q itself
-// where Q is packed (q_stride = num_heads * head_dim). Q and Q_out may both be null.
+// where Q is packed (q_stride = num_heads * head_dim; otherwise DIMENSION_MISMATCH). Q and Q_out may both be null.
 // query_starts may be null: then token t is the one new token of sequence t (num_tokens ==
 // batch_size).
 // What the host cannot see is not an error but left out: a token whose position is negative or past
 // the block table, and one whose page is not in [0, num_pages) (so -1 marks rows that have none), is
 // not written; a query whose position is outside the rotation's tables becomes NaN, and its token is
-// not written. Two tokens for one cache row: one of them is kept.
+// not written. Where tables name one cache row for two tokens, it holds parts of either afterwards.
 CUFLASH_EXPORT FlashAttentionError flash_attention_append_paged(
     const float* Q, const float* K, const float* V, float* Q_out, float* K_cache, float* V_cache,
     const int* block_table, const int* seq_lens, const int* query_starts, const float* rope_cos,
@@ -90,8 +93,10 @@ CUFLASH_EXPORT FlashAttentionError flash_attention_append_paged(
 // head_dim], L [num_tokens, num_heads] float. Token t of sequence b sees all seq_lens[b] keys (fewer
 // where the block table ends before), with `causal` those up to its own position. A query that sees
 // no key, or whose scores are all -inf, has O = 0 and L = -inf. Cache rows from seq_lens[b] on and
-// table entries past a sequence's pages are not read. A sequence whose pages are wanted must name
-// pages of the cache (they are not range-checked).
+// table entries past a sequence's pages are not read. The entries of a sequence's keys must name pages
+// of the cache (they are not range-checked). Keys that a query does not see do not reach it, whatever
+// they hold; of values that it does not see it takes 0 times those in the same block of 64 keys, so a
+// NaN or an infinity there (the value of a later token of its own sequence) may make its output NaN.
 CUFLASH_EXPORT FlashAttentionError flash_attention_forward_paged(
     const float* Q, const float* K_cache, const float* V_cache, float* O, float* L,
     const int* block_table, const int* seq_lens, const int* query_starts, int num_tokens,
@@ -118,8 +123,9 @@ CUFLASH_EXPORT FlashAttentionError flash_attention_forward_paged(
 // num_heads] float. seq_lens counts all keys of a sequence, the shared ones among them; positions stay
 // what they are, so block_table[b][j / page_size] is read for the keys j >= prefix_len only (where the
 // prefix ends inside a page, that entry is the sequence's own page, whose first rows are not read). A
-// sequence shorter than the prefix sees its first seq_lens[b] keys. prefix_len 0 is
-// flash_attention_decode_paged; prefix_len past the block table's capacity is DIMENSION_MISMATCH.
+// sequence shorter than the prefix sees its first seq_lens[b] keys (non-finite values behind these: as in
+// the forward). prefix_len 0 is flash_attention_decode_paged (captured: the same result up to rounding,
+// in the caller's workspace); prefix_len past the block table's capacity is DIMENSION_MISMATCH.
 CUFLASH_EXPORT FlashAttentionError flash_attention_decode_shared(
     const float* Q, const float* K_cache, const float* V_cache, float* O, float* L,
     const int* prefix_table, const int* block_table, const int* seq_lens, int batch_size,

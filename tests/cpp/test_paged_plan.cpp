@@ -110,7 +110,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     if (!a.shared && pick(8) == 0) a.T = std::max(1, a.T - pick(50));  // starts past the tokens
     a.seq_lens = lens.data();
     a.starts = starts.data();
-    a.prefix = a.shared ? spread(rng, 1, a.cap) : 0;
+    a.prefix = a.shared && rng() % 8 ? spread(rng, 1, a.cap) : 0;
 
     PagedTiles t{};
     int items, room;
@@ -264,7 +264,7 @@ int main(int argc, char** argv) {
     int chunked = 0;
     for (g_case = 0; g_case < n; ++g_case) {
         using A = PagedShape<256, 64, 256, 2, 96>;
-        using B = PagedShape<128, 32, 128, 1, 1 << 28>;
+        using B = PagedShape<128, 32, 128, 1, 0x7fffffff>;
         const int kind = rng() % 6;
         chunked += kind == 0   ? launch<A, true>(rng)
                    : kind == 1 ? launch<B, true>(rng)

@@ -144,7 +144,7 @@ class PagedCase:
         pg, row = self.keys[b]
         return self.k[pg, row], self.v[pg, row]
 
-    def check(self, q, new, causal, o, lse, scale=None, left_alone=None):
+    def check(self, q, new, causal, o, lse, scale=None):
         """Compares O [T, heads, d] and L [T, heads] of packed queries q, new[b] of sequence b."""
         scale = self.d ** -0.5 if scale is None else scale
         group, t0 = self.heads // self.kv_heads, 0

@@ -89,6 +89,29 @@ def test_no_prefix_is_the_paged_decode(torch_gpu, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_no_prefix_captured(torch_gpu, dtype):
+    """A server's graph without a prefix yet: its memory is the caller's here, too."""
+    torch = torch_gpu
+    c = PagedCase(dtype, 64, 8, 2, 16, lens=[340, 0, 33, 1])
+    q = torch.randn((4, 8, 1, 64), device="cuda").to(c.t_k.dtype)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, lse = cuflash_attn.flash_attention_decode_shared(q, c.t_k, c.t_v, none, 0, c.t_table,
+                                                            c.t_lens)
+    torch.cuda.synchronize()
+    for rep in range(3):
+        print(f"[no prefix, captured] replay {rep}", flush=True)
+        q.normal_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(synth.to_numpy(q)[:, :, 0], [1] * 4, False, synth.to_numpy(o)[:, :, 0],
+                synth.to_numpy(lse)[:, :, 0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_non_finite_scores(torch_gpu, dtype):
     """Shared keys of -inf leave the own ones; a NaN among the shared keys reaches the sequences that
     see it, not those that end before it."""

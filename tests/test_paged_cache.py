@@ -72,6 +72,10 @@ def test_append_refusals(lib, sfx):
                 v_stride=1 << 30) == DIMENSION_MISMATCH  # rows longer than any stride
     for name in ("q", "k", "v", "q_out", "k_cache", "v_cache", "cos", "sin"):
         assert call(**{name: P + 8}) == INVALID_DIMENSION, name
+    assert call(q_stride=768) == DIMENSION_MISMATCH  # rotated in place, but not packed
+    assert call(page=1 << 10, max_pages=1 << 21) == INVALID_DIMENSION
+    assert call(tokens=1 << 26, batch=1, heads=64, kv_heads=64, d=128, q_stride=1 << 13,
+                k_stride=1 << 13, v_stride=1 << 13) == INVALID_DIMENSION  # 2^32 threads and more
     # Order: null, dimension, head_dim, relations.
     assert call(k=None, d=48, tokens=0) == NULL_POINTER
     assert call(tokens=0, d=48) == INVALID_DIMENSION
@@ -125,6 +129,12 @@ def test_grids_beyond_32_bits_are_refused(lib, sfx):
     n = 1 << 22
     assert _call(lib, "forward_paged", sfx, FORWARD, tokens=n, batch=n, heads=500, kv_heads=500,
                  d=32) == INVALID_DIMENSION
+    assert _call(lib, "decode_shared", sfx, SHARED, batch=1 << 24) == INVALID_DIMENSION  # the merge
+    assert lib.fn("decode_shared_workspace", sfx)(1 << 24, 8, 2, 64) == -1
+    for kind, ok in (("forward_paged", FORWARD), ("decode_shared", SHARED)):
+        assert _call(lib, kind, sfx, ok, heads=65536) == INVALID_DIMENSION
+        assert _call(lib, kind, sfx, ok, page=1 << 10, max_pages=1 << 21) == INVALID_DIMENSION
+    assert lib.fn("forward_paged_workspace", sfx)(4, 2, 65536, 2, 64) == -1
 
 
 @pytest.mark.parametrize("sfx", ["f32", "f16", "bf16"])
@@ -187,6 +197,8 @@ def test_append_helper_refusals(monkeypatch):
     refused("float32", cos=f(9, 16, dtype=torch.float16), sin=f(9, 16, dtype=torch.float16))
     refused("heads of a token", k=_Fake(torch.zeros(4, 64, 2).transpose(1, 2)))
     refused("tokens of v", v=_Fake(torch.zeros(1, 2, 64).expand(4, 2, 64)))
+    refused("tokens of k", k=_Fake(torch.empty((4, 2, 64), device="meta").as_strided(
+        (4, 2, 64), (1 << 31, 64, 1))))
     refused("multiple of 16 bytes", k=_Fake(torch.zeros(4 * 2 * 64 + 1)[1:].view(4, 2, 64)))
     refused("needs q", out=f(4, 2, 64))
     with pytest.raises(cuflash_attn.CuFlashError):
