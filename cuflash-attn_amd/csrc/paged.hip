@@ -868,10 +868,22 @@ __global__ void __launch_bounds__((64 * Eng::kWaves), (Eng::kPerCu * Eng::kWaves
     int hk, x;
     head_rank_order(blockIdx.x, a.Hkv, hk, x);
     PagedItem it;
-    if constexpr (kShared)
+    if constexpr (kShared) {
         it = shared_item<PagedShapeOf<Eng>, GpuWave>(a, x);
-    else
-        it = paged_item<PagedShapeOf<Eng>, GpuWave>(a, x);
+    } else {
+        // The sequences of more than 64 (see PagedPlan), where they fit.
+        PagedSeq* seqs = reinterpret_cast<PagedSeq*>(smem);
+        const int per = (a.B + 63) / 64;
+        const bool staged = per > 1 && per < kBytes / static_cast<int>(64 * sizeof(PagedSeq));
+        if (staged) {
+            const int lane = threadIdx.x & 63;
+            for (int j = threadIdx.x >> 6; j < per && lane * per + j < a.B; j += Eng::kWaves)
+                seqs[lane * (per + 1) + j] = paged_seq(a, lane * per + j);
+            __syncthreads();
+        }
+        it = paged_item<PagedShapeOf<Eng>, GpuWave>(a, x, seqs, staged);
+        if (staged) __syncthreads();  // the tiles go to the same place
+    }
     if (!it.found) return;
     if (!kShared && a.wgs > 0 && it.first && hk == 0 && threadIdx.x == 0)
         a.units[it.u] = make_int4(it.of.first, it.of.tiles, it.of.chunks, it.many);

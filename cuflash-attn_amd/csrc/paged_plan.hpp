@@ -149,18 +149,36 @@ struct UniformDiv {
     }
 };
 
+// Rows and keys of a sequence in a forward.
+struct PagedSeq {
+    int rows, keys;
+};
+__host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
+    const int t0 = paged_clamp(a.starts[b], 0, a.T);
+    return {(paged_clamp(a.starts[b + 1], t0, a.T) - t0) * a.group, paged_seq_len(a, b)};
+}
+
 // The cut of one launch, found by every wave for itself: a few hundred instructions and two loads that
 // need each other, which every workgroup waits for. W: the 64 lanes of a wave, one int each in W::Int.
-// Lane i has the `per` sequences from i per on, the first of them in registers.
+// Lane i has the `per` sequences from i per on, the first of them in registers. Where there are several,
+// the workgroup has put them side by side in LDS (`seqs`: sequence i per + j at i (per + 1) + j, so that
+// the lanes meet different banks), as they are gone through several times: one token each, 32 heads over 8,
+// head_dim 128, of 512 sequences with up to 500 keys 309 -> 179 us, of 1024 with up to 60 keys 809 -> 222.
 template <class Shape, class W>
 struct PagedPlan {
     using Int = typename W::Int;
+    struct Most {  // steps, rounds of a chunk
+        UniformDiv many, few;
+    };
 
     const PagedArgs& a;
     int per;
+    const PagedSeq* seqs;
+    bool staged;
     Int rows0, keys0;
-    UniformDiv most_many, most_few;  // steps, rounds of a chunk
-    Int many, few;                   // items of either kind up to and with the lane's
+    Most most;
+    Int many, few;              // items of either kind up to and with the lane's
+    Int many_slots, few_slots;  // the lane's items of units with several chunks
 
     __host__ __device__ __forceinline__ static int up(int x, int by) {
         return static_cast<int>((static_cast<uint32_t>(x) + (by - 1)) / by);
@@ -171,51 +189,91 @@ struct PagedPlan {
     __host__ __device__ __forceinline__ static int steps(int rows, int keys) {
         return rows > Shape::kMany ? up(keys, Shape::kStep) : up(keys, Shape::kRound);
     }
-    __host__ __device__ __forceinline__ int keys_of(int b) const { return paged_seq_len(a, b); }
-    __host__ __device__ __forceinline__ int rows_of(int b) const {
-        const int t0 = paged_clamp(a.starts[b], 0, a.T);
-        return (paged_clamp(a.starts[b + 1], t0, a.T) - t0) * a.group;
+    // Sequence j of a lane.
+    __host__ __device__ __forceinline__ PagedSeq seq(int lane, int j) const {
+        return staged ? seqs[lane * (per + 1) + j] : paged_seq(a, lane * per + j);
     }
     // Chunks of n steps, items of a unit. A unit with rows but no keys has outputs all the same.
-    __host__ __device__ __forceinline__ int chunks(bool is_many, int n) const {
-        return n == 0 ? 1 : (is_many ? most_many : most_few)(n - 1) + 1;
+    __host__ __device__ __forceinline__ static int chunks(const Most& m, bool is_many, int n) {
+        const UniformDiv& most = is_many ? m.many : m.few;
+        return n <= most.d ? 1 : most(n - 1) + 1;
     }
-    __host__ __device__ __forceinline__ int items(int rows, int keys) const {
-        return tiles(rows) * chunks(rows > Shape::kMany, steps(rows, keys));
+    __host__ __device__ __forceinline__ static int items(const Most& m, int rows, int keys) {
+        return tiles(rows) * chunks(m, rows > Shape::kMany, steps(rows, keys));
     }
-    // f(rows, keys) summed over the sequences of each lane, f(0, 0) = 0.
+    // Each lane's sums over its sequences: f(rows, keys, sums) adds to N of them, and nothing where both
+    // are 0.
+    template <int N, class F>
+    __host__ __device__ __forceinline__ void sums(Int (&out)[N], F f) const {
+        W::fill(out, rows0, keys0, [&](int lane, int rows, int keys, int (&x)[N]) {
+            f(rows, keys, x);
+            for (int j = 1; j < per && lane * per + j < a.B; ++j) {
+                const PagedSeq s = seq(lane, j);
+                f(s.rows, s.keys, x);
+            }
+        });
+    }
     template <class F>
-    __host__ __device__ __forceinline__ Int per_lane(F f) const {
-        Int sum = W::map2(rows0, keys0, f);
-        if (per > 1)
-            sum = W::add(sum, W::each([&](int lane) {
-                             int x = 0;
-                             for (int j = 1; j < per && lane * per + j < a.B; ++j) {
-                                 x += f(rows_of(lane * per + j), keys_of(lane * per + j));
-                             }
-                             return x;
-                         }));
-        return sum;
+    __host__ __device__ __forceinline__ Int sum(F f) const {
+        Int x[1];
+        sums(x, [&](int rows, int keys, int* to) { to[0] += f(rows, keys); });
+        return x[0];
+    }
+    // Among lane i's sequences, with f(rows, keys) places each, the one that has place `at`: its number, rows
+    // and keys. `at` is left within it; `sum` gains g(rows, keys) of those before it.
+    template <class F, class G>
+    __host__ __device__ __forceinline__ PagedSeq place(int i, F f, G g, int& u, int& at,
+                                                       int& sum) const {
+        u = i * per;
+        if (per == 1) return {W::lane(rows0, i), W::lane(keys0, i)};
+        for (int j0 = 0;; j0 += 64) {
+            auto here = [&](int lane) { return j0 + lane < per && u + j0 + lane < a.B; };
+            const Int rows = W::each([&](int lane) { return here(lane) ? seq(i, j0 + lane).rows : 0; });
+            const Int keys = W::each([&](int lane) { return here(lane) ? seq(i, j0 + lane).keys : 0; });
+            const Int n = W::scan(W::map2(rows, keys, f)), m = W::scan(W::map2(rows, keys, g));
+            if (at >= W::lane(n, 63) && j0 + 64 < per) {
+                at -= W::lane(n, 63);
+                sum += W::lane(m, 63);
+                continue;
+            }
+            const int k = W::first(n, [&](int x) { return x > at; });
+            if (k > 0) {
+                at -= W::lane(n, k - 1);
+                sum += W::lane(m, k - 1);
+            }
+            u += j0 + (k > 0 ? k : 0);
+            return {W::lane(rows, k > 0 ? k : 0), W::lane(keys, k > 0 ? k : 0)};
+        }
     }
     // Chunks that cost at most s.
-    __host__ __device__ __forceinline__ void set(int s) {
+    __host__ __device__ __forceinline__ Most at_most(int s) const {
         const int few_s = s / Shape::kRoundCost;
-        most_many = UniformDiv(s > a.min_steps ? s : a.min_steps);
-        most_few = UniformDiv(few_s > a.min_rounds ? few_s : a.min_rounds);
+        return {UniformDiv(s > a.min_steps ? s : a.min_steps),
+                UniformDiv(few_s > a.min_rounds ? few_s : a.min_rounds)};
     }
 
-    __host__ __device__ __forceinline__ explicit PagedPlan(const PagedArgs& args)
-        : a(args), most_many(1), most_few(1) {
+    __host__ __device__ __forceinline__ PagedPlan(const PagedArgs& args, const PagedSeq* in_lds,
+                                                  bool are_staged)
+        : a(args), seqs(in_lds), staged(are_staged), most{UniformDiv(1), UniformDiv(1)} {
         per = (a.B + 63) / 64;
-        keys0 = W::each([&](int lane) { return lane * per < a.B ? keys_of(lane * per) : 0; });
-        rows0 = W::each([&](int lane) { return lane * per < a.B ? rows_of(lane * per) : 0; });
+        rows0 = W::each([&](int lane) { return lane * per < a.B ? seq(lane, 0).rows : 0; });
+        keys0 = W::each([&](int lane) { return lane * per < a.B ? seq(lane, 0).keys : 0; });
         const int room = choose();
-        for (int s = 0;; s = s ? 2 * s : most_many.d) {
-            if (s) set(s);
-            many = W::scan(per_lane(
-                [&](int rows, int keys) { return rows > Shape::kMany ? items(rows, keys) : 0; }));
-            few = W::scan(per_lane(
-                [&](int rows, int keys) { return rows > Shape::kMany ? 0 : items(rows, keys); }));
+        for (int s = 0;; s = s ? 2 * s : most.many.d) {
+            if (s) most = at_most(s);
+            Int x[4];
+            sums(x, [&](int rows, int keys, int* to) {
+                const int n = items(most, rows, keys), slots = n > tiles(rows) ? n : 0;
+                const bool is_many = rows > Shape::kMany;
+                to[0] += is_many ? n : 0;
+                to[1] += is_many ? 0 : n;
+                to[2] += is_many ? slots : 0;
+                to[3] += is_many ? 0 : slots;
+            });
+            many = W::scan(x[0]);
+            few = W::scan(x[1]);
+            many_slots = x[2];
+            few_slots = x[3];
             // Only units whose work was cut off (choose) can leave more than there is room for.
             if (a.wgs == 0 || W::lane(many, 63) + W::lane(few, 63) <= room ||
                 s > 1 << 28)
@@ -226,20 +284,21 @@ struct PagedPlan {
     // Sets the chunks; the room for items.
     __host__ __device__ __forceinline__ int choose() {
         if (a.wgs == 0) {
-            set(0x7fffffff);
+            most = at_most(0x7fffffff);
             return 0;
         }
-        const Int n_tiles = per_lane([](int rows, int) { return tiles(rows); });
         // A lane's work, cut off where the sum would pass 2^30.
         const int cap = per > 64 ? (1 << 24) / per : 1 << 18;
-        const Int cost = per_lane([&](int rows, int keys) {
-            const float x = static_cast<float>(tiles(rows)) *
-                            static_cast<float>(steps(rows, keys)) *
-                            (rows > Shape::kMany ? 1 : Shape::kRoundCost);
-            return x > static_cast<float>(cap) ? cap : static_cast<int>(x);
+        Int x[2];
+        sums(x, [&](int rows, int keys, int* to) {
+            const int n = tiles(rows);
+            const float cost = static_cast<float>(n) * static_cast<float>(steps(rows, keys)) *
+                               (rows > Shape::kMany ? 1 : Shape::kRoundCost);
+            to[0] += n;
+            to[1] += cost > static_cast<float>(cap) ? cap : static_cast<int>(cost);
         });
-        const int total = W::lane(W::scan(n_tiles), 63);
-        const float work = static_cast<float>(W::lane(W::scan(cost), 63));
+        const int total = W::lane(W::scan(x[0]), 63);
+        const float work = static_cast<float>(W::lane(W::scan(x[1]), 63));
         // Chunks of at most s: at most work / s + total items, on average work / s + total / 2. So
         // the least s that leaves no more than there is room for lies between work / room and
         // work / (room - total), rounded up (a round is not divided: the bound holds for multiples of
@@ -251,14 +310,21 @@ struct PagedPlan {
             return s < Shape::kRoundCost ? Shape::kRoundCost : s;
         };
         const int lo = over(room), hi = over(room - total) + Shape::kRoundCost;
-        const int s1 = lo + (hi - lo) / 4, s2 = lo + (hi - lo) / 2, s3 = hi - (hi - lo) / 4;
-        auto count = [&](int s) {
-            set(s);
-            return W::lane(
-                W::scan(per_lane([&](int rows, int keys) { return items(rows, keys); })), 63);
-        };
-        const int n1 = count(s1), n2 = count(s2), n3 = count(s3);
-        set(n1 <= room ? s1 : n2 <= room ? s2 : n3 <= room ? s3 : hi);
+        if (total > 4 * a.wgs) {  // a few more or less are nothing beside so many
+            most = at_most(hi);
+            return room;
+        }
+        const Most m1 = at_most(lo + (hi - lo) / 4), m2 = at_most(lo + (hi - lo) / 2),
+                   m3 = at_most(hi - (hi - lo) / 4);
+        Int n[3];
+        sums(n, [&](int rows, int keys, int* to) {
+            to[0] += items(m1, rows, keys);
+            to[1] += items(m2, rows, keys);
+            to[2] += items(m3, rows, keys);
+        });
+        const int n1 = W::lane(W::scan(n[0]), 63), n2 = W::lane(W::scan(n[1]), 63),
+                  n3 = W::lane(W::scan(n[2]), 63);
+        most = n1 <= room ? m1 : n2 <= room ? m2 : n3 <= room ? m3 : at_most(hi);
         return room;
     }
 };
@@ -308,7 +374,7 @@ __host__ __device__ __forceinline__ void tile_by_length(const PagedArgs& a,
                                                         const PagedPlan<Shape, W>& plan, int x,
                                                         PagedItem& r, int& keys, int& tile) {
     auto longer = [&](int steps) {
-        return W::lane(W::scan(plan.per_lane([&](int rows, int k) {
+        return W::lane(W::scan(plan.sum([&](int rows, int k) {
                            return longer_tiles<Shape>(a, rows, k, steps);
                        })),
                        63);
@@ -326,30 +392,22 @@ __host__ __device__ __forceinline__ void tile_by_length(const PagedArgs& a,
     auto as_long = [&](int rows, int k) {
         return longer_tiles<Shape>(a, rows, k, lo - 1) - longer_tiles<Shape>(a, rows, k, lo);
     };
-    const auto incl = W::scan(plan.per_lane(as_long));
+    const auto incl = W::scan(plan.sum(as_long));
     const int i = W::first(incl, [&](int n) { return n > at; });
     at -= i > 0 ? W::lane(incl, i > 0 ? i - 1 : 0) : 0;
-    r.rows = W::lane(plan.rows0, i);
-    keys = W::lane(plan.keys0, i);
-    for (r.u = i * plan.per;;) {
-        const int own = as_long(r.rows, keys);
-        if (at < own) break;
-        at -= own;
-        if (++r.u >= a.B) {  // not reached
-            r.u = a.B - 1;
-            break;
-        }
-        keys = plan.keys_of(r.u);
-        r.rows = plan.rows_of(r.u);
-    }
+    int none = 0;
+    const PagedSeq s = plan.place(i, as_long, [](int, int) { return 0; }, r.u, at, none);
+    r.rows = s.rows;
+    keys = s.keys;
     const int tiles = (r.rows + Shape::kTile - 1) / Shape::kTile;
     tile = tiles - longer_tiles<Shape>(a, r.rows, keys, lo) - 1 - at;
 }
 
 template <class Shape, class W>
-__host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int x) {
+__host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int x,
+                                                         const PagedSeq* seqs, bool staged) {
     PagedItem r{};
-    const PagedPlan<Shape, W> plan(a);
+    const PagedPlan<Shape, W> plan(a, seqs, staged);
     using Plan = PagedPlan<Shape, W>;
     // Items of many rows come first: they take longest.
     const int total_many = W::lane(plan.many, 63);
@@ -363,28 +421,22 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
         const auto& incl = r.many ? plan.many : plan.few;
         const int i = W::first(incl, [&](int n) { return n > x; });
         at = x - (i > 0 ? W::lane(incl, i > 0 ? i - 1 : 0) : 0);
-        // Slots before the lane's units: the items of units with several chunks.
-        auto slots = [&](int rows, int n) {
-            const int own = (rows > Shape::kMany) == r.many ? plan.items(rows, n) : 0;
-            return own > Plan::tiles(rows) ? own : 0;
-        };
+        // Slots before the lane's units.
         if (a.wgs > 0) {
-            const auto before = W::scan(plan.per_lane(slots));
+            const auto before = W::scan(r.many ? plan.many_slots : plan.few_slots);
             slot = i > 0 ? W::lane(before, i > 0 ? i - 1 : 0) : 0;
         }
         // The sequence among the lane's.
-        r.rows = W::lane(plan.rows0, i);
-        keys = W::lane(plan.keys0, i);
-        r.u = i * plan.per;
-        for (;;) {
-            const int own = (r.rows > Shape::kMany) == r.many ? plan.items(r.rows, keys) : 0;
-            if (at < own) break;
-            at -= own;
-            slot += slots(r.rows, keys);
-            if (++r.u >= a.B) return r;  // not reached
-            keys = plan.keys_of(r.u);
-            r.rows = plan.rows_of(r.u);
-        }
+        auto own = [&](int rows, int n) {
+            return (rows > Shape::kMany) == r.many ? Plan::items(plan.most, rows, n) : 0;
+        };
+        auto slots = [&](int rows, int n) {
+            const int x = own(rows, n);
+            return x > Plan::tiles(rows) ? x : 0;
+        };
+        const PagedSeq s = plan.place(i, own, slots, r.u, at, slot);
+        r.rows = s.rows;
+        keys = s.keys;
     }
     r.unit.n = a.group_div(r.rows);
     r.unit.t0 = paged_clamp(a.starts[r.u], 0, a.T);
@@ -394,7 +446,7 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
     r.of.many = r.many;
     r.of.tiles = Plan::tiles(r.rows);
     int each = Plan::steps(r.rows, keys);
-    r.of.chunks = plan.chunks(r.many, each);
+    r.of.chunks = Plan::chunks(plan.most, r.many, each);
     r.found = r.of.chunks == 1 ||
               slot + r.of.tiles * r.of.chunks <= (r.many ? a.max_many : a.max_few);
     const int chunk = r.of.chunks == 1 ? 0 : at / r.of.tiles;

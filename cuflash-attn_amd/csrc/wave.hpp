@@ -43,6 +43,13 @@ struct GpuWave {
         return f(static_cast<int>(threadIdx.x & 63), v, w);
     }
     __device__ static Int add(Int a, Int b) { return a + b; }
+    // f(lane, v, w, sums) forms N numbers of each lane, from 0.
+    template <int N, class F>
+    __device__ static void fill(Int (&out)[N], Int v, Int w, F f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = 0;
+        f(static_cast<int>(threadIdx.x & 63), v, w, out);
+    }
     // Inclusive sum over the lanes.
     __device__ static Int scan(Int v) {
         v += __builtin_amdgcn_update_dpp(0, v, kDppRowShr + 1, 0xF, 0xF, false);

@@ -32,9 +32,6 @@ struct HostWave {
         for (int i = 0; i < 64; ++i) v[i] = f(i);
         return v;
     }
-    static Int add(const Int& x, const Int& y) {
-        return each([&](int i) { return x[i] + y[i]; });
-    }
     template <class F>
     static Int map3(const Int& x, const Int& y, F f) {
         return each([&](int i) { return f(i, x[i], y[i]); });
@@ -42,6 +39,14 @@ struct HostWave {
     template <class F>
     static Int map2(const Int& x, const Int& y, F f) {
         return each([&](int i) { return f(x[i], y[i]); });
+    }
+    template <int N, class F>
+    static void fill(Int (&out)[N], const Int& x, const Int& y, F f) {
+        for (int i = 0; i < 64; ++i) {
+            int sums[N] = {};
+            f(i, x[i], y[i], sums);
+            for (int j = 0; j < N; ++j) out[j][i] = sums[j];
+        }
     }
     static Int scan(Int v) {
         for (int i = 1; i < 64; ++i) {
@@ -85,7 +90,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     a.group_div = fast_div(a.group);
     a.page_size = std::array<int, 6>{1, 6, 16, 24, 64, 256}[pick(6)];
     a.page_div = fast_div(a.page_size);
-    a.B = spread(rng, 1, pick(10) == 0 ? 600 : 200);
+    a.B = spread(rng, 1, pick(300) == 0 ? 6000 : pick(10) == 0 ? 600 : 200);
     a.max_pages = spread(rng, 1, std::max(1, 40000 / a.page_size));
     a.cap = a.page_size * a.max_pages;
     a.shared = kShared;
@@ -112,6 +117,12 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     a.starts = starts.data();
     a.prefix = a.shared && rng() % 8 ? spread(rng, 1, a.cap) : 0;
 
+    // As the workgroups put them into LDS.
+    const bool staged = !a.shared && pick(4) != 0;
+    const int per = (a.B + 63) / 64;
+    std::vector<PagedSeq> seqs(staged ? 64 * (per + 1) : 0, PagedSeq{1 << 20, 1 << 20});
+    for (int b = 0; staged && b < a.B; ++b) seqs[b / per * (per + 1) + b % per] = paged_seq(a, b);
+
     PagedTiles t{};
     int items, room;
     if constexpr (kShared) {
@@ -135,7 +146,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         a.max_few = a.wgs ? std::min(room, 3 * a.wgs) : 0;
         a.max_many = t.many > 0 ? int(std::min<long long>(a.max_few, t.many + 2LL * a.wgs)) : 0;
         a.few_rows = 32;
-        const PagedPlan<Shape, HostWave> plan(a);
+        const PagedPlan<Shape, HostWave> plan(a, nullptr, false);
         items = HostWave::lane(plan.many, 63) + HostWave::lane(plan.few, 63);
     }
     CHECK(items <= room);
@@ -152,7 +163,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         if constexpr (kShared)
             it = shared_item<Shape, HostWave>(a, x);
         else
-            it = paged_item<Shape, HostWave>(a, x);
+            it = paged_item<Shape, HostWave>(a, x, seqs.data(), staged);
         CHECK(it.found == (x < items));
         if (!it.found) continue;
         CHECK(x < grid);

@@ -83,6 +83,29 @@ def test_many_sequences(torch_gpu, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch", [700, 4200])
+def test_hundreds_of_sequences(torch_gpu, dtype, batch):
+    """So many that a workgroup keeps their lengths in LDS, and more than it has room for."""
+    lens = [(37 * b) % 90 for b in range(batch)]
+    new = [min(n, (b * 7) % 3) for b, n in enumerate(lens)]
+    for b, n in ((batch // 2, 2000), (batch - 1, 700), (3, 300)):
+        lens[b], new[b] = n, min(n, 150) if b > 3 else 1
+    c = PagedCase(dtype, 32, 2, 1, 16, lens=lens)
+    run(c, new)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_of_a_hundred_sequences(torch_gpu, dtype):
+    """Rows that fill the chip, so that no keys are cut."""
+    lens = [100 + (53 * b) % 130 for b in range(100)]
+    lens[40] = 1500
+    c = PagedCase(dtype, 32, 8, 8, 16, lens=lens)
+    run(c, [n - b % 3 for b, n in enumerate(lens)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [32, 128])
 def test_rows_without_keys_and_padding(torch_gpu, dtype, d):
     """Lengths of zero and below, fewer keys than tokens (the first ones see nothing), a length past
