@@ -957,6 +957,7 @@ __global__ void __launch_bounds__(256)
     };
     auto parts_of = [&](int v, int r) {
         const int4 d = a.units[v];
+        if (d.z == 1) return Parts{1, 0, 0};
         const bool many = d.w != 0;
         const int tile = many ? r / Shape::kTile : r / 32;
         const int in = many ? r % Shape::kTile : r % 32;

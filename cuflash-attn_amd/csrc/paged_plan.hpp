@@ -149,6 +149,8 @@ struct UniformDiv {
     }
 };
 
+constexpr int kNoChunks = 0x7fffffff;
+
 // Rows and keys of a sequence in a forward.
 struct PagedSeq {
     int rows, keys;
@@ -284,18 +286,23 @@ struct PagedPlan {
     // Sets the chunks; the room for items.
     __host__ __device__ __forceinline__ int choose() {
         if (a.wgs == 0) {
-            most = at_most(0x7fffffff);
+            most = at_most(kNoChunks);
             return 0;
         }
         // A lane's work, cut off where the sum would pass 2^30.
         const int cap = per > 64 ? (1 << 24) / per : 1 << 18;
-        Int x[2];
+        Int x[4];
         sums(x, [&](int rows, int keys, int* to) {
+            const bool is_many = rows > Shape::kMany;
             const int n = tiles(rows);
-            const float cost = static_cast<float>(n) * static_cast<float>(steps(rows, keys)) *
-                               (rows > Shape::kMany ? 1 : Shape::kRoundCost);
+            const float each = static_cast<float>(steps(rows, keys)) *
+                               (is_many ? 1 : Shape::kRoundCost);
+            const float cost = static_cast<float>(n) * each;
             to[0] += n;
             to[1] += cost > static_cast<float>(cap) ? cap : static_cast<int>(cost);
+            to[2] += is_many ? n : 0;
+            const int own = n == 0 ? 0 : each < 1e9f ? static_cast<int>(each) : 1000000000;
+            to[3] = to[3] > own ? to[3] : own;
         });
         const int total = W::lane(W::scan(x[0]), 63);
         const float work = static_cast<float>(W::lane(W::scan(x[1]), 63));
@@ -325,6 +332,17 @@ struct PagedPlan {
         const int n1 = W::lane(W::scan(n[0]), 63), n2 = W::lane(W::scan(n[1]), 63),
                   n3 = W::lane(W::scan(n[2]), 63);
         most = n1 <= room ? m1 : n2 <= room ? m2 : n3 <= room ? m3 : at_most(hi);
+        // Where the tiles run all at once and the longest takes no more steps than the rounds of chunks and
+        // what these cost beside, there are no chunks. Of many rows: the partial results of as many tiles
+        // as run at once are written, read and merged in the time of 16 steps, and a chunk's start and end
+        // take that of 4 (bf16, us: 1000 tokens, 32 heads over 8, head_dim 128, 41 -> 36; 6 x 1024 tokens
+        // of 12 heads, head_dim 64, 55 -> 42; 3000 tokens of 8 heads, head_dim 128, 70 without, 55 with).
+        const int n_many = W::lane(W::scan(x[2]), 63);
+        const int beside = n_many > 0 ? 4 + 16 * n_many / a.wgs : 1;
+        const int rounds = room / a.wgs;
+        if (total <= a.wgs &&
+            W::most(x[3]) <= static_cast<int64_t>(rounds) * most.many.d + beside)
+            most = at_most(kNoChunks);
         return room;
     }
 };

@@ -60,6 +60,16 @@ struct GpuWave {
         v += __builtin_amdgcn_update_dpp(0, v, kDppRowBcast31, 0xC, 0xF, false);
         return v;
     }
+    // The largest of numbers from 0 on.
+    __device__ static int most(Int v) {
+        v = max(v, __builtin_amdgcn_update_dpp(0, v, kDppRowShr + 1, 0xF, 0xF, false));
+        v = max(v, __builtin_amdgcn_update_dpp(0, v, kDppRowShr + 2, 0xF, 0xF, false));
+        v = max(v, __builtin_amdgcn_update_dpp(0, v, kDppRowShr + 4, 0xF, 0xF, false));
+        v = max(v, __builtin_amdgcn_update_dpp(0, v, kDppRowShr + 8, 0xF, 0xF, false));
+        v = max(v, __builtin_amdgcn_update_dpp(0, v, kDppRowBcast15, 0xA, 0xF, false));
+        v = max(v, __builtin_amdgcn_update_dpp(0, v, kDppRowBcast31, 0xC, 0xF, false));
+        return lane(v, 63);
+    }
     __device__ static int lane(Int v, int i) { return __builtin_amdgcn_readlane(v, i); }
     // The first lane where f is not 0, or -1.
     template <class F>

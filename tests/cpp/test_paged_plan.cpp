@@ -54,6 +54,7 @@ struct HostWave {
         }
         return v;
     }
+    static int most(const Int& v) { return std::max(0, *std::max_element(v.begin(), v.end())); }
     static int lane(const Int& v, int i) {
         if (i < 0 || i >= 64) std::abort();
         return v[i];
