@@ -367,37 +367,42 @@ struct PagedItem {
     PagedUnitItems of;  // the unit's items
 };
 
-// Tiles of a unit of many rows that have more than `steps` steps: with a causal mask tile t sees the keys
-// below len - n + min(n, ((t + 1) kTile - 1) / group + 1), so those from (64 steps - len + n) group / kTile on.
+// Tiles of a unit of many rows, or of few, that have more than `steps` steps or rounds: with a causal mask
+// tile t of h rows sees the keys below len - n + min(n, ((t + 1) h - 1) / group + 1), so those from
+// (kStep steps - len + n) group / h on.
 template <class Shape>
-__host__ __device__ __forceinline__ int longer_tiles(const PagedArgs& a, int rows, int keys,
-                                                     int steps) {
-    if (rows <= Shape::kMany) return 0;
-    const int tiles = (rows + Shape::kTile - 1) / Shape::kTile;
+__host__ __device__ __forceinline__ int longer_tiles(const PagedArgs& a, bool many, int rows,
+                                                     int keys, int steps) {
+    if ((rows > Shape::kMany) != many) return 0;
+    const int height = many ? Shape::kTile : 32;
+    const int tiles = static_cast<int>((static_cast<uint32_t>(rows) + (height - 1)) / height);
     if (steps < 0) return tiles;
     const int n = a.group_div(rows);
-    const int64_t q = static_cast<int64_t>(steps) * Shape::kStep - keys + (a.causal ? n : 0);
+    const int64_t q = static_cast<int64_t>(steps) * (many ? Shape::kStep : Shape::kRound) - keys +
+                      (a.causal ? n : 0);
     if (!a.causal) return q < 0 ? tiles : 0;
     if (q < 0) return tiles;
     if (q >= n) return 0;
-    return tiles - static_cast<int>(q) * a.group / Shape::kTile;
+    return tiles - static_cast<int>(q) * a.group / height;
 }
 
-// Tile x in the order of their steps, longest first, of the tiles of all units of many rows: the
+// Tile x in the order of their steps, longest first, of the tiles of all units of many rows, or of few: the
 // workgroups of a launch without chunks, where a long tile started last would run on alone (7 prompts of
-// 285 to 2001 tokens, head_dim 64: 120.6 -> 114.9 us; 2 of 2048 and 4096, head_dim 32: 96.4 -> 88.0). The steps of the tile are the least s with no more
-// than x longer tiles.
+// 285 to 2001 tokens, head_dim 64: 120.6 -> 114.9 us; 2 of 2048 and 4096, head_dim 32: 96.4 -> 88.0; fp32,
+// 1024 + 700 tokens of 8 heads, head_dim 64: 44.5 -> 38.0; 6 of 400 tokens, where it only costs: 46.0 -> 47.9).
+// The steps of the tile are the least s with no more than x longer tiles.
 template <class Shape, class W>
 __host__ __device__ __forceinline__ void tile_by_length(const PagedArgs& a,
                                                         const PagedPlan<Shape, W>& plan, int x,
                                                         PagedItem& r, int& keys, int& tile) {
+    const bool many = r.many;
     auto longer = [&](int steps) {
         return W::lane(W::scan(plan.sum([&](int rows, int k) {
-                           return longer_tiles<Shape>(a, rows, k, steps);
+                           return longer_tiles<Shape>(a, many, rows, k, steps);
                        })),
                        63);
     };
-    int lo = 0, hi = a.cap / Shape::kStep + 1;
+    int lo = 0, hi = a.cap / (many ? Shape::kStep : Shape::kRound) + 1;
     while (lo < hi) {
         const int mid = lo + (hi - lo) / 2;
         if (longer(mid) <= x)
@@ -408,7 +413,8 @@ __host__ __device__ __forceinline__ void tile_by_length(const PagedArgs& a,
     // Its place among those of as many steps.
     int at = x - longer(lo);
     auto as_long = [&](int rows, int k) {
-        return longer_tiles<Shape>(a, rows, k, lo - 1) - longer_tiles<Shape>(a, rows, k, lo);
+        return longer_tiles<Shape>(a, many, rows, k, lo - 1) -
+               longer_tiles<Shape>(a, many, rows, k, lo);
     };
     const auto incl = W::scan(plan.sum(as_long));
     const int i = W::first(incl, [&](int n) { return n > at; });
@@ -417,8 +423,8 @@ __host__ __device__ __forceinline__ void tile_by_length(const PagedArgs& a,
     const PagedSeq s = plan.place(i, as_long, [](int, int) { return 0; }, r.u, at, none);
     r.rows = s.rows;
     keys = s.keys;
-    const int tiles = (r.rows + Shape::kTile - 1) / Shape::kTile;
-    tile = tiles - longer_tiles<Shape>(a, r.rows, keys, lo) - 1 - at;
+    tile = PagedPlan<Shape, W>::tiles(r.rows) -
+           longer_tiles<Shape>(a, many, r.rows, keys, lo) - 1 - at;
 }
 
 template <class Shape, class W>
@@ -433,7 +439,7 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
     r.many = x < total_many;
     if (!r.many) x -= total_many;
     int at = 0, keys = 0, by_length = -1, slot = 0;
-    if (r.many && a.wgs == 0 && a.B > 1) {
+    if (a.wgs == 0 && a.B > 1 && (r.many || plan.per == 1)) {
         tile_by_length<Shape, W>(a, plan, x, r, keys, by_length);
     } else {
         const auto& incl = r.many ? plan.many : plan.few;

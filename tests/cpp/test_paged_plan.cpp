@@ -154,7 +154,7 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
     const int units = a.shared ? a.B + 1 : a.B;
     std::vector<int4> noted(units, make_int4(-1, -1, -1, -1));
     bool chunked = false;
-    int64_t longest = int64_t(1) << 40;  // tiles of many rows without chunks: longest first
+    int64_t longest[2] = {int64_t(1) << 40, int64_t(1) << 40};  // without chunks: longest tiles first
     // (unit, tile row) -> the key ranges of its items; slots taken.
     std::map<std::pair<int, int>, std::vector<std::array<int, 2>>> met;
     std::map<std::pair<bool, int>, int> slots;
@@ -175,10 +175,11 @@ bool launch(std::mt19937& rng) {  // whether something was cut into chunks
         const int tile = it.many ? Shape::kTile : 32;
         CHECK(it.r0 >= 0 && it.r0 % tile == 0 && it.r0 < it.rows);
         CHECK(it.kbeg >= u.kbeg && it.kend <= u.kend);
-        if (!kShared && a.wgs == 0 && a.B > 1 && it.many) {
-            const int64_t n = (std::max(0, it.kend) + Shape::kStep - 1) / Shape::kStep;
-            CHECK(n <= longest);
-            longest = n;
+        if (!kShared && a.wgs == 0 && a.B > 1 && (it.many || a.B <= 64)) {
+            const int step = it.many ? Shape::kStep : Shape::kRound;
+            const int64_t n = (std::max(0, it.kend) + step - 1) / step;
+            CHECK(n <= longest[it.many]);
+            longest[it.many] = n;
         }
         if (!it.direct) CHECK(it.slot >= 0 && it.slot < (it.many ? a.max_many : a.max_few));
         if (!it.direct) {
