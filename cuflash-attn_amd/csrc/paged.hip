@@ -1228,18 +1228,22 @@ FlashAttentionError run_paged(const PagedCall& call, bool chunks, hipStream_t st
 }
 
 // Workgroups: eight waves (four in fp32), and at head_dim 128 four, two workgroups a CU, where most
-// sequences (in a shared decode the batch) have few rows: the start of one workgroup then hides behind the
-// other. Kernel times, us, eight waves -> four: 4 sequences behind 1000 keys 8.3 -> 7.7, 16 x 5 tokens of
-// up to 8196 keys 64.5 -> 63.0; 250 tokens of 8442 keys 44.3 -> 55.9, 4 x 61 tokens of 8253 keys 38.5 ->
-// 43.1, 128 sequences behind 32768 keys 125 -> 130.
+// sequences have few rows: the start of one workgroup then hides behind the other. In a shared decode, where
+// the batch has few rows or the prefix is not so long that the products over it take most of the time. Kernel
+// times, us, eight waves -> four: 16 x 5 tokens of up to 8196 keys 64.5 -> 63.0; 250 tokens of 8442 keys
+// 44.3 -> 55.9, 4 x 61 tokens of 8253 keys 38.5 -> 43.1. Shared, 32 heads over 8, up to 300 own keys: 4
+// sequences behind 1000 keys 8.3 -> 7.7, 128 behind 500 40.8 -> 31.8, behind 4000 55.0 -> 48.0, behind 16000
+// 76.9 -> 78.1, 512 behind 4000 155.7 -> 130.6, behind 16000 227.9 -> 230.5, 128 with up to 512 own keys
+// behind 32768 113 -> 124.
 template <typename T, int D>
 struct PagedEngines {
     static constexpr int kWaves = std::is_same<T, float>::value ? 4 : 8;
     using Rows = dev::PagedEngine<T, D, kWaves>;
     using Few = dev::PagedEngine<T, D, D == 128 ? 4 : kWaves>;
     static bool few(const PagedCall& call, bool shared) {
-        return static_cast<long long>(call.num_tokens) * (call.num_heads / call.num_kv_heads) <=
-               static_cast<long long>(shared ? 1 : call.batch_size) * Rows::kManyRows;
+        return (shared && call.prefix_len <= 8192) ||
+               static_cast<long long>(call.num_tokens) * (call.num_heads / call.num_kv_heads) <=
+                   static_cast<long long>(shared ? 1 : call.batch_size) * Rows::kManyRows;
     }
 };
 
@@ -1274,8 +1278,13 @@ long long workspace_of(const PagedCall& call) {
     auto bytes = [](const auto& grid) {
         return grid.too_large() ? -1 : static_cast<long long>(grid.bytes());
     };
-    if (chunks && Engines::few(call, shared))
-        return bytes(PagedGrid<typename Engines::Few>(call, shared, true));
+    if (shared) {  // of any prefix
+        const long long few = bytes(PagedGrid<typename Engines::Few>(call, true, true));
+        const long long rows = bytes(PagedGrid<typename Engines::Rows>(call, true, true));
+        return few < 0 || rows < 0 ? -1 : std::max(few, rows);
+    }
+    if (chunks && Engines::few(call, false))
+        return bytes(PagedGrid<typename Engines::Few>(call, false, true));
     return bytes(PagedGrid<typename Engines::Rows>(call, shared, chunks));
 }
 

@@ -504,14 +504,15 @@ __host__ __device__ __forceinline__ int shared_own_len(const PagedArgs& a, int k
                                                           : a.cut.own_least;
 }
 
-// The sequence at place i of a batch of at most 64 where one has more than four rounds of own keys: in the
-// order of the lengths, longest first, every lane counting the sequences before its own (40 sequences with 17
-// to 700 own keys in fp32 56.6 -> 48.1 us, 64 with 62 to 4000 112.8 -> 94.3). Shorter ones keep their order:
-// the counting costs more than a late long sequence there (64 with 16 to 1024 38.4 -> 42.6).
+// The sequence at place i of a batch of at most 64 in few chunks where one has more than 1024 own keys (512 in
+// fp32): in the order of the lengths, longest first, every lane counting the sequences before its own (40
+// sequences with 17 to 700 own keys in fp32 50.8 -> 48.5 us, 64 with 62 to 4000 101.7 -> 96.4). Shorter ones
+// keep their order: the counting costs more than a late long sequence there (64 with 16 to 1024 40.0 -> 46.1).
 template <class Shape, class W>
 __host__ __device__ __forceinline__ int by_length(const PagedArgs& a, int i) {
+    constexpr int kLong = std::min(1024, 4 * Shape::kRoundCost * Shape::kRound);
     const auto len = W::each([&](int lane) { return lane < a.B ? paged_seq_len(a, lane) : -1; });
-    if (W::first(len, [&](int n) { return n > a.prefix && n - a.prefix > 4 * Shape::kRound; }) < 0)
+    if (W::first(len, [&](int n) { return n > a.prefix && n - a.prefix > kLong; }) < 0)
         return i;
     auto place = W::each([](int) { return 0; });
     for (int b = 0; b < a.B; ++b) {
@@ -547,7 +548,7 @@ __host__ __device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, in
         r.rows = a.group;
         int b = c.own_items_div(x);
         x -= b * c.own_chunks * c.own_tiles;
-        if (a.B <= 64 && c.own_chunks == 1) b = by_length<Shape, W>(a, b);
+        if (a.B <= 64 && c.own_chunks <= 4) b = by_length<Shape, W>(a, b);
         r.slot = (c.own_many == c.pre_many ? pre : 0) + b * c.own_chunks * c.own_tiles + x;
         chunk = c.own_tiles_div(x);
         tile = x - chunk * c.own_tiles;
@@ -566,7 +567,11 @@ __host__ __device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, in
 
 // The cut, for `wgs` workgroups per key/value head at once: unit 0 in items for three of four of them (the
 // others start on own keys), of at least min_steps steps or one round; own keys in chunks where the tiles of
-// all sequences leave workgroups free.
+// all sequences leave workgroups free, or fill them at most twice: so a long sequence among short ones ends
+// sooner (bf16, 32 heads over 8, head_dim 128, us: 8 sequences with up to 8000 own keys 39.6 -> 34.5, 32 with
+// up to 3000 50.5 -> 45.2, 64 with up to 4000 112 -> 102; but 40 with up to 500 24.2 -> 24.3, 96 of 4
+// key/value heads 27.0 -> 28.3). No more than 16 for that: 4 sequences with up to 200 own keys 11.2 -> 12.0
+// with 32.
 template <class Shape>
 inline SharedCut shared_cut(int B, int group, int prefix, int wgs, int min_steps) {
     SharedCut c{};
@@ -588,8 +593,9 @@ inline SharedCut shared_cut(int B, int group, int prefix, int wgs, int min_steps
     const long long each = std::max(1LL, ceil_div(steps, chunks));
     c.pre_chunks = prefix > 0 ? static_cast<int>(ceil_div(steps, each)) : 0;
     c.pre_len = static_cast<int>(std::min<long long>(each * unit, 0x7fffffffLL));
+    const long long own = static_cast<long long>(B) * c.own_tiles;
     c.own_chunks = static_cast<int>(
-        std::max(1LL, std::min<long long>(64, wgs / (static_cast<long long>(B) * c.own_tiles))));
+        std::max({1LL, std::min<long long>(64, wgs / own), std::min<long long>(16, 2LL * wgs / own)}));
     c.own_least = c.own_many ? Shape::kStep * min_steps : Shape::kRound;
     c.pre_tiles_div = fast_div(c.pre_tiles);
     c.own_tiles_div = fast_div(c.own_tiles);

@@ -59,6 +59,17 @@ def test_batches(torch_gpu, dtype, batch, heads, kv_heads):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("prefix", [900, 8192, 8300])
+def test_long_prefixes(torch_gpu, dtype, prefix):
+    """Many shared rows at head_dim 128, on either side of the prefix from which other workgroups take
+    them; own keys in chunks, one of them long."""
+    c = PagedCase(dtype, 128, 8, 2, 16, prefix=prefix,
+                  lens=[prefix + (29 * b) % 300 for b in range(37)] + [prefix + 1500, 70, 0])
+    run(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("heads", [40, 128])
 def test_many_heads_over_one(torch_gpu, dtype, heads):
     """More query heads of a key/value head than a tile's rows, and so many that a sequence alone
