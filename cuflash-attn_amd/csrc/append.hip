@@ -7,7 +7,7 @@
 // on the token's place in the cache, so their loads run beside the walk to it: query_starts ->
 // seq_lens -> block_table, three loads that need each other.
 // Bound by memory: the rows are read and written once, 3 operations per rotated element. 36856 tokens of 48
-// heads, head_dim 128, bf16: 155 us, 5.9 TB/s (a copy of 1 GiB runs at 5.1); one token 2.6 us.
+// heads, head_dim 128, bf16: 155 us, 5.9 TB/s (a copy of 1 GiB runs at 5.1); one token 2.4 us.
 
 #include <algorithm>
 #include <type_traits>

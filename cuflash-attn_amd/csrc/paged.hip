@@ -20,7 +20,7 @@
 // maxima, sums and O are fp32.
 //
 // Bound by MFMA where a sequence has many rows (one prompt of 16384 tokens, 32 heads
-// over 8, head_dim 128, bf16: 1.9 ms, 1158 TFLOP/s), at head_dim 64 by the softmax beside it (seven prompts
+// over 8, head_dim 128, bf16: 1.85 to 1.9 ms, 1158 to 1191 TFLOP/s), at head_dim 64 by the softmax beside it (seven prompts
 // of 285 to 2001 tokens 106 us, 700 TFLOP/s), by HBM where it has few (16 x 5 tokens of up to 8196 keys:
 // 55 us, 5.2 TB/s).
 
