@@ -306,3 +306,56 @@ def test_cache_past_32_bit_offsets(torch_gpu, tokens):
     assert all(torch.equal(a, b) for a, b in zip(*results))
     del k, v
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_captured_step(torch_gpu):
+    """A server's captured step: append, then both attentions, replayed as the sequences grow. The graph's
+    cache and the eager one stay the same bit for bit, and so do the outputs."""
+    torch = torch_gpu
+    c = PagedCase("bfloat16", 128, 16, 4, 16, prefix=200, lens=[230, 900, 205, 411], capacity=1024)
+    c.t_table[:, :12] = c.t_prefix[:12]
+    spare = torch.full((60,) + tuple(c.t_k.shape[1:]), float("nan"), device="cuda", dtype=c.t_k.dtype)
+    caches = [[torch.cat([x, spare]) for x in (c.t_k, c.t_v)] for _ in range(2)]
+    pages = c.t_k.shape[0]
+    for b in range(4):  # rows to grow into, and each sequence's own copy of the page the prefix ends in
+        have = -(-c.lens[b] // 16)
+        c.t_table[b, have:have + 2] = torch.arange(pages + 10 * b, pages + 10 * b + 2)
+        for k, v in caches:
+            own, shared = int(c.t_table[b, 12]), int(c.t_prefix[12])
+            k[own, :8], v[own, :8] = k[shared, :8], v[shared, :8]
+    lens, starts = c.t_lens.clone(), c.ints([0, 1, 2, 3, 4])
+    qkv = torch.randn((4, 24, 128), device="cuda").bfloat16()
+    angle = torch.arange(1024, device="cuda")[:, None] * 1e4 ** (-torch.arange(64, device="cuda") / 64)
+    cos, sin = angle.cos().contiguous(), angle.sin().contiguous()
+
+    def step(k, v):
+        q = cuflash_attn.flash_attention_append_paged(
+            qkv[:, 16:20], qkv[:, 20:], k, v, c.t_table, lens, q=qkv[:, :16], cos=cos, sin=sin)
+        return (q, *cuflash_attn.flash_attention_forward_paged(q, k, v, c.t_table, lens, starts,
+                                                               causal=True),
+                *cuflash_attn.flash_attention_decode_shared(q.unsqueeze(2), k, v, c.t_prefix, 200,
+                                                            c.t_table, lens))
+
+    graph = torch.cuda.CUDAGraph()
+    lens += 1
+    with torch.cuda.graph(graph):
+        out = step(*caches[0])
+    torch.cuda.synchronize()
+    for rep in range(4):
+        print(f"[captured step] replay {rep}", flush=True)
+        qkv.normal_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in out]
+        want = step(*caches[1])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), rep
+        assert bool(torch.isfinite(got[1].float()).all() and torch.isfinite(got[3].float()).all())
+        # One query per sequence: both attentions see the same keys.
+        off = (got[1].float() - got[3][:, :, 0].float()).abs().max()
+        assert float(off) <= 8 * HALF_STEP["bfloat16"] * 6
+        for a, b in zip(*caches):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16)), rep
+        lens += 1
