@@ -1076,6 +1076,10 @@ namespace {
 
 // Steps and rounds that a chunk has at least: a part of 256 rows is 133 KB to write and to read again.
 constexpr int kMinSteps = 6;
+// In a shared decode own keys wait for the prefix's items, so these are longer (bf16, 32 heads over 8, us, of 6,
+// 8 and 12 steps: 64 sequences behind 2048 keys 41.6, 40.9, 41.6, 128 behind 4000 47.1, 44.1, 41.9, 256 of 2
+// key/value heads behind 2000 44.2, 40.5, 42.2, 40 behind 2000 24.2, 25.0, 37.8).
+constexpr int kSharedSteps = 8;
 constexpr int kMinRounds = 1;
 
 // The sizes of one launch: grid and slots.
@@ -1095,7 +1099,7 @@ struct PagedGrid {
         const int group = call.num_heads / kv_heads;
         wgs = chunks ? (Eng::kPerCu * compute_units() + kv_heads - 1) / kv_heads : 0;
         if (shared) {
-            cut = dev::shared_cut<Shape>(call.batch_size, group, call.prefix_len, wgs, kMinSteps);
+            cut = dev::shared_cut<Shape>(call.batch_size, group, call.prefix_len, wgs, kSharedSteps);
             const long long pre = static_cast<long long>(cut.pre_tiles) * cut.pre_chunks;
             const long long own =
                 static_cast<long long>(call.batch_size) * cut.own_chunks * cut.own_tiles;
