@@ -991,10 +991,9 @@ __global__ void __launch_bounds__(256)
         pre = cut_parts(c.pre_many, 0, c.pre_tiles, c.pre_chunks, t * a.group + g);
         const int keys = paged_seq_len(a, t) - a.prefix;
         if (keys > 0) {
-            const int len = shared_own_len(a, keys);
             const int before = c.pre_many == c.own_many ? c.pre_tiles * c.pre_chunks : 0;
             own = cut_parts(c.own_many, before + t * c.own_chunks * c.own_tiles, c.own_tiles,
-                            (keys + len - 1) / len, g);
+                            shared_own_parts(a, keys), g);
         }
     } else {
         own = parts_of(u, (t - a.starts[u]) * a.group + g);

@@ -503,6 +503,10 @@ __host__ __device__ __forceinline__ int shared_own_len(const PagedArgs& a, int k
            : len > static_cast<uint32_t>(a.cut.own_least) ? static_cast<int>(len)
                                                           : a.cut.own_least;
 }
+// Chunks that a sequence's own `keys`, at least one, fill. (keys + len may pass 2^31.)
+__host__ __device__ __forceinline__ int shared_own_parts(const PagedArgs& a, int keys) {
+    return (keys - 1) / shared_own_len(a, keys) + 1;
+}
 
 // The sequence at place i of a batch of at most 64 in few chunks where one has more than 1024 own keys (512 in
 // fp32): in the order of the lengths, longest first, every lane counting the sequences before its own (40
