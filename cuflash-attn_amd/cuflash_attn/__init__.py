@@ -453,11 +453,20 @@ def _output(given, like, shape, dtype, stream, name):
         return like.new_empty(shape, dtype=dtype)
 
 
+def _capturing(stream):
+    """Whether the call's stream, torch's current one where that is None, is being captured."""
+    torch = _torch()
+    if stream is None:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _captured_workspace(lib, kind, like, stream, *sizes):
     """Pointer and bytes of the workspace of a call that is being captured: torch's allocator gives it
     from the graph's own pool. Eager calls use the library's: None, 0. The third value keeps it."""
     torch = _torch()
-    if not torch.cuda.is_current_stream_capturing():
+    if not _capturing(stream):
         return None, 0, None
     need = lib.fn(f"{kind}_workspace", _suffix(like))(*sizes)
     if need <= 0:
