@@ -796,7 +796,10 @@ __device__ __forceinline__ void PagedWork<Eng>::few_rows(unsigned char* smem, fl
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) M = fmaxf(M, s_m[w][l32]);
-    const float f = m == -INFINITY ? 0.0f : fast_exp2(m - M);
+    // No key of this row among the wave's, or every score -inf: such a part has no say, also where 0 times
+    // a value made it NaN.
+    const bool none = m == -INFINITY;
+    const float f = none ? 0.0f : fast_exp2(m - M);
     float* mrg = reinterpret_cast<float*>(smem);
     if (on) {
         float* dst = mrg + (wave * 32 + l32) * P + 4 * g2;
@@ -806,7 +809,7 @@ __device__ __forceinline__ void PagedWork<Eng>::few_rows(unsigned char* smem, fl
             for (int i = 0; i < 4; ++i) {
                 f32x4 w;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) w[u] = o[dt][4 * i + u] * f;
+                for (int u = 0; u < 4; ++u) w[u] = none ? 0.0f : o[dt][4 * i + u] * f;
                 st16(dst + 32 * dt + 8 * i, __builtin_bit_cast(u32x4, w));
             }
         }

@@ -95,8 +95,9 @@ CUFLASH_EXPORT FlashAttentionError flash_attention_append_paged(
 // no key, or whose scores are all -inf, has O = 0 and L = -inf. Cache rows from seq_lens[b] on and
 // table entries past a sequence's pages are not read. The entries of a sequence's keys must name pages
 // of the cache (they are not range-checked). Keys that a query does not see do not reach it, whatever
-// they hold; of values that it does not see it takes 0 times those in the same block of 64 keys, so a
-// NaN or an infinity there (the value of a later token of its own sequence) may make its output NaN.
+// they hold. Of the values that `causal` hides from it it may take 0 times those of up to 94 positions past
+// its own (the 32 rows that share a wave end up to 31 positions later, in blocks of 64 keys): a NaN or an
+// infinity there makes its output NaN. A query that sees no key has O = 0 whatever the cache holds.
 CUFLASH_EXPORT FlashAttentionError flash_attention_forward_paged(
     const float* Q, const float* K_cache, const float* V_cache, float* O, float* L,
     const int* block_table, const int* seq_lens, const int* query_starts, int num_tokens,
@@ -123,8 +124,9 @@ CUFLASH_EXPORT FlashAttentionError flash_attention_forward_paged(
 // num_heads] float. seq_lens counts all keys of a sequence, the shared ones among them; positions stay
 // what they are, so block_table[b][j / page_size] is read for the keys j >= prefix_len only (where the
 // prefix ends inside a page, that entry is the sequence's own page, whose first rows are not read). A
-// sequence shorter than the prefix sees its first seq_lens[b] keys (non-finite values behind these: as in
-// the forward). prefix_len 0 is flash_attention_decode_paged (captured: the same result up to rounding,
+// sequence shorter than the prefix sees its first seq_lens[b] keys; of the shared values behind these it may
+// take 0 times any, which a NaN or an infinity there makes NaN (a length of 0: O = 0 all the same).
+// prefix_len 0 is flash_attention_decode_paged (captured: the same result up to rounding,
 // in the caller's workspace); prefix_len past the block table's capacity is DIMENSION_MISMATCH.
 CUFLASH_EXPORT FlashAttentionError flash_attention_decode_shared(
     const float* Q, const float* K_cache, const float* V_cache, float* O, float* L,
