@@ -18,6 +18,14 @@
 // and nothing synchronizes the host; kernel execution errors surface at the caller's next
 // synchronizing call, as in the reference.
 //
+// HIP graphs: calls can be captured. A captured backward, and a captured decode that is cut into splits
+// (but for cuflash_attention_decode_noalloc_f16), has its workspace from an allocation and a free that the
+// graph records (hipMallocAsync, hipFreeAsync). This is tested with one such graph at a time, the device
+// waited for between its replays. With several of them caution is due: an early form of the paged forward,
+// whose workspace was such memory, faulted the GPU in the first replay of two graphs one right after the
+// other; it does not since its workspace is the caller's (paged_cache.h). That the recorded memory was the
+// cause is inferred, not shown. Forwards and the calls of paged_cache.h record no memory.
+//
 // Additive entry points (no counterpart in the reference, which lists split-KV decoding as a
 // roadmap item, ROADMAP.md:24-25): flash_attention_decode / cuflash_attention_decode_*.
 
