@@ -1088,6 +1088,8 @@ constexpr int kMinRounds = 1;
 template <class Eng>
 struct PagedGrid {
     using Shape = dev::PagedShapeOf<Eng>;
+    static_assert(dev::is_paged_shape<Shape>(static_cast<dev::PagedShapes*>(nullptr)),
+                  "the cut is tested on the host for PagedShapes");
     static constexpr int D = Eng::D;
     int wgs;                     // 0: keys are not cut into chunks
     long long items, many, few;  // per key/value head: items, and slots of either kind

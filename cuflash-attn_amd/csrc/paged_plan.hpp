@@ -10,6 +10,8 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <tuple>
+#include <type_traits>
 
 namespace cuflash {
 namespace dev {
@@ -52,6 +54,14 @@ struct PagedShape {
     static constexpr int kRound = ROUND;
     static constexpr int kRoundCost = COST;
 };
+
+// The shapes that paged.hip's engines have: 16 bits with eight and with four waves, fp32.
+using PagedShapes = std::tuple<PagedShape<256, 64, 256, 2, 96>, PagedShape<128, 64, 128, 2, 96>,
+                               PagedShape<128, 32, 128, 1, 0x7fffffff>>;
+template <class Shape, class... Known>
+constexpr bool is_paged_shape(const std::tuple<Known...>*) {
+    return (std::is_same<Shape, Known>::value || ...);
+}
 
 // The cut of a shared decode: unit 0 in `pre_chunks` chunks of pre_len keys; the own keys of every
 // sequence in at most own_chunks, of own_least keys or more. Items: unit 0, chunk by chunk, then

@@ -6,6 +6,7 @@ from __future__ import annotations
 from test_host_rules import run_program
 
 
-def test_shared_cut_up_to_the_key_limit(tmp_path):
-    """Lengths up to 2^31 - 1024 (tests/cpp/test_paged_limits.cpp)."""
+def test_every_shape_up_to_the_key_limit(tmp_path):
+    """The shapes of all engines, lengths up to 2^31 - 1024, more than 96 query heads over a key/value
+    head (tests/cpp/test_paged_limits.cpp)."""
     run_program("test_paged_limits", tmp_path, 300, 1)
