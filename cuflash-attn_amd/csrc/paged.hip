@@ -17,12 +17,13 @@
 //
 // P is rounded to the inputs' type before P V, as in the forward kernels (at most half a step of it per
 // value: 2^-8 of p |v| in bf16), as the 16-bit matrix instructions take no wider operand; scores,
-// maxima, sums and O are fp32.
+// maxima, sums and O are fp32. Against 64-bit results bf16 outputs are off by 0.0023 of their size so, and by
+// 0.0017 with P in fp32 (fp16 0.00029 and 0.00021).
 //
 // Bound by MFMA where a sequence has many rows (one prompt of 16384 tokens, 32 heads
-// over 8, head_dim 128, bf16: 1.85 to 1.9 ms, 1158 to 1191 TFLOP/s), at head_dim 64 by the softmax beside it (seven prompts
-// of 285 to 2001 tokens 106 us, 700 TFLOP/s), by HBM where it has few (16 x 5 tokens of up to 8196 keys:
-// 55 us, 5.2 TB/s).
+// over 8, head_dim 128, bf16: 1.85 to 1.96 ms a call, 1120 to 1191 TFLOP/s), at head_dim 64 by the softmax
+// beside it (seven prompts of 285 to 2001 tokens 97 to 102 us a call, 736 to 770 TFLOP/s), by HBM where it
+// has few (16 x 5 tokens of up to 8196 keys: 60 us a call, the first kernel 57 us, 5.05 TB/s).
 
 #include <algorithm>
 #include <type_traits>
@@ -40,7 +41,9 @@
 namespace cuflash {
 namespace dev {
 
-// LDS-DMA load from a scalar base (lds_dma16_async_s) with the non-temporal hint.
+// LDS-DMA load from a scalar base (lds_dma16_async_s) with the non-temporal hint. As there, one wait state is
+// enough because base and LDS address are SALU values: pages come by scalar loads here, where the decode's
+// come from a lane (lds_dma16_nt_s, five). tests/test_code_hazards.py checks the built code.
 __device__ __forceinline__ void lds_dma16_once_s(const void* sbase, unsigned voff,
                                                  unsigned char* lds_base) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
@@ -548,6 +551,7 @@ __device__ __forceinline__ void PagedWork<Eng>::many_rows_in_turn(unsigned char*
     };
     const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(smem)) +
                           static_cast<unsigned>(wave * kParts * Eng::kGroupBytes);
+    // lds_dma16_async_s with the LDS address as a number.
     auto load_whole = [&](const E* src, int buffer) {
 #pragma unroll
         for (int i = 0; i < kParts; ++i)
@@ -1143,7 +1147,11 @@ struct PagedGrid {
 
 // Whether the tiles alone, at least so many, take three of four workgroup places: chunks cost the partial
 // results and the merge (fp32, 512 + 1024 tokens of 8 heads, head_dim 64, 384 tiles for 512 places: 40.7
-// -> 31 us without).
+// -> 31 us without). From num_tokens alone, as the host knows no more: beside
+// prompts that fill the chip a token with a long cache has all its keys in one workgroup per key/value head,
+// which starts after the prompts' tiles (bf16, 32 heads over 8, head_dim 128, us in one call and in two: 5000
+// tokens and one behind 8000 keys 292 and 229, behind 100000 keys 1260 and 302; 4 x 2000 tokens and 32 behind
+// 4000 keys 258 and 251).
 template <class Eng>
 bool fills_chip(const PagedCall& call) {
     const long long rows =

@@ -443,7 +443,7 @@ __host__ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a, int
     PagedItem r{};
     const PagedPlan<Shape, W> plan(a, seqs, staged);
     using Plan = PagedPlan<Shape, W>;
-    // Items of many rows come first: they take longest.
+    // Items of many rows come first: of sequences of like lengths they take longest.
     const int total_many = W::lane(plan.many, 63);
     if (x >= total_many + W::lane(plan.few, 63)) return r;
     r.many = x < total_many;

@@ -54,8 +54,8 @@ namespace cuflash {
 // batch_size).
 // What the host cannot see is not an error but left out: a token whose position is negative or past
 // the block table, and one whose page is not in [0, num_pages) (so -1 marks rows that have none), is
-// not written; a query whose position is outside the rotation's tables becomes NaN, and its token is
-// not written. Where tables name one cache row for two tokens, it holds parts of either afterwards.
+// not written; the rotated elements of a query whose position is outside the rotation's tables become NaN,
+// and its token is not written. Where tables name one cache row for two tokens, it holds parts of either afterwards.
 CUFLASH_EXPORT FlashAttentionError flash_attention_append_paged(
     const float* Q, const float* K, const float* V, float* Q_out, float* K_cache, float* V_cache,
     const int* block_table, const int* seq_lens, const int* query_starts, const float* rope_cos,
@@ -90,9 +90,13 @@ CUFLASH_EXPORT FlashAttentionError flash_attention_append_paged(
 // is OUT_OF_MEMORY, one that is not aligned INVALID_DIMENSION.
 // ---- Several new tokens of every sequence ----
 // O = softmax(scale Q K^T) V over the cache, L the logsumexp: Q, O [num_tokens, num_heads,
-// head_dim], L [num_tokens, num_heads] float. Token t of sequence b sees all seq_lens[b] keys (fewer
+// head_dim], L [num_tokens, num_heads] float. In 16 bits the softmax's weights are rounded to that type
+// before they meet V (the shared decode's too), as in the library's matrix-core kernels; scores and sums are
+// float. Token t of sequence b sees all seq_lens[b] keys (fewer
 // where the block table ends before), with `causal` those up to its own position. A query that sees
-// no key, or whose scores are all -inf, has O = 0 and L = -inf. Cache rows from seq_lens[b] on and
+// no key, or whose scores are all -inf, has O = 0 and L = -inf. How keys are cut goes by num_tokens: beside
+// prompts that fill the chip, or padding as long, a token with a cache much longer than these is faster in a
+// call of its own. Cache rows from seq_lens[b] on and
 // table entries past a sequence's pages are not read. The entries of a sequence's keys must name pages
 // of the cache (they are not range-checked). Keys that a query does not see do not reach it, whatever
 // they hold. Of the values that `causal` hides from it it may take 0 times those of up to 94 positions past
@@ -126,8 +130,8 @@ CUFLASH_EXPORT FlashAttentionError flash_attention_forward_paged(
 // prefix ends inside a page, that entry is the sequence's own page, whose first rows are not read). A
 // sequence shorter than the prefix sees its first seq_lens[b] keys; of the shared values behind these it may
 // take 0 times any, which a NaN or an infinity there makes NaN (a length of 0: O = 0 all the same).
-// prefix_len 0 is flash_attention_decode_paged (captured: the same result up to rounding,
-// in the caller's workspace); prefix_len past the block table's capacity is DIMENSION_MISMATCH.
+// prefix_len 0 is flash_attention_decode_paged, which does not use the workspace (captured: the same result
+// up to rounding, in the caller's workspace); prefix_len past the block table's capacity is DIMENSION_MISMATCH.
 CUFLASH_EXPORT FlashAttentionError flash_attention_decode_shared(
     const float* Q, const float* K_cache, const float* V_cache, float* O, float* L,
     const int* prefix_table, const int* block_table, const int* seq_lens, int batch_size,
