@@ -76,6 +76,16 @@ _FWD_PAGED_ARGS = ([ctypes.c_void_p] * 8 + [ctypes.c_int] * 7 +
 _DEC_SHARED_ARGS = ([ctypes.c_void_p] * 8 + [ctypes.c_int] * 7 +
                     [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p])
 
+_APPEND_PAGED_Q8_ARGS = ([ctypes.c_void_p] * 13 + [ctypes.c_int] * 13 +
+                         [ctypes.c_bool, ctypes.c_int, ctypes.c_void_p])
+_READ_PAGED_Q8_ARGS = [ctypes.c_void_p] * 9 + [ctypes.c_int] * 8 + [ctypes.c_void_p]
+_DEC_PAGED_Q8_ARGS = ([ctypes.c_void_p] * 9 + [ctypes.c_int] * 6 +
+                      [ctypes.c_float, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t,
+                       ctypes.c_void_p])
+_FWD_PAGED_Q8_ARGS = ([ctypes.c_void_p] * 10 + [ctypes.c_int] * 7 +
+                      [ctypes.c_float, ctypes.c_bool, ctypes.c_int, ctypes.c_void_p,
+                       ctypes.c_size_t, ctypes.c_void_p])
+
 EXPORTED_SYMBOLS = (
     "cuflash_attention_forward_f32", "cuflash_attention_forward_f16",
     "cuflash_attention_forward_bf16", "cuflash_attention_backward_f32",
@@ -97,6 +107,14 @@ PAGED_CACHE_SYMBOLS = tuple(f"cuflash_attention_{kind}_{sfx}"
                             for kind in ("append_paged", "forward_paged", "decode_shared",
                                          "forward_paged_workspace", "decode_shared_workspace")
                             for sfx in ("f32", "f16", "bf16"))
+
+
+# Declared in include/cuflash/paged_cache_q8.h.
+PAGED_CACHE_Q8_SYMBOLS = tuple(f"cuflash_attention_{kind}_{sfx}"
+                               for kind in ("append_paged_q8", "read_paged_q8", "decode_paged_q8",
+                                            "forward_paged_q8", "decode_paged_q8_workspace",
+                                            "forward_paged_q8_workspace")
+                               for sfx in ("f32", "f16", "bf16"))
 
 
 class CuFlashLibrary:
@@ -127,6 +145,15 @@ class CuFlashLibrary:
             shared = getattr(library, f"cuflash_attention_decode_shared_{sfx}")
             shared.argtypes, shared.restype = _DEC_SHARED_ARGS, ctypes.c_int
             for kind, n in (("forward_paged", 5), ("decode_shared", 4)):
+                size = getattr(library, f"cuflash_attention_{kind}_workspace_{sfx}")
+                size.argtypes, size.restype = [ctypes.c_int] * n, ctypes.c_longlong
+            for kind, args in (("append_paged_q8", _APPEND_PAGED_Q8_ARGS),
+                               ("read_paged_q8", _READ_PAGED_Q8_ARGS),
+                               ("decode_paged_q8", _DEC_PAGED_Q8_ARGS),
+                               ("forward_paged_q8", _FWD_PAGED_Q8_ARGS)):
+                q8 = getattr(library, f"cuflash_attention_{kind}_{sfx}")
+                q8.argtypes, q8.restype = args, ctypes.c_int
+            for kind, n in (("forward_paged_q8", 5), ("decode_paged_q8", 4)):
                 size = getattr(library, f"cuflash_attention_{kind}_workspace_{sfx}")
                 size.argtypes, size.restype = [ctypes.c_int] * n, ctypes.c_longlong
         noalloc = library.cuflash_attention_decode_noalloc_f16
@@ -489,6 +516,22 @@ def _token_stride(x, name):
     return apart
 
 
+def _rotation(cos, sin, device):
+    """Positions and rotated elements of the tables of an append, checked; 0, 0 without."""
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    if cos is None:
+        return 0, 0
+    if cos.dim() != 2 or sin.shape != cos.shape:
+        raise ValueError("expected cos, sin [positions, R / 2]")
+    for x in (cos, sin):
+        if x.dtype is not _torch().float32 or x.get_device() != device \
+                or not x.is_contiguous() or x.data_ptr() & 15:
+            raise ValueError("cos and sin must be contiguous float32 tensors on the inputs' "
+                             "device")
+    return cos.shape[0], 2 * cos.shape[1]
+
+
 def flash_attention_append_paged(k, v, k_cache, v_cache, block_table, seq_lens,
                                  query_starts=None, q=None, cos=None, sin=None,
                                  interleaved: bool = False, out=None, stream=None,
@@ -510,18 +553,7 @@ def flash_attention_append_paged(k, v, k_cache, v_cache, block_table, seq_lens,
     if k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D) \
             or (q is not None and q.shape != (T, H, D)):
         raise ValueError("expected k, v [T,Hkv,D] and q [T,H,D] of the cache's Hkv and D")
-    R = positions = 0
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin come together")
-    if cos is not None:
-        if cos.dim() != 2 or sin.shape != cos.shape:
-            raise ValueError("expected cos, sin [positions, R / 2]")
-        for x in (cos, sin):
-            if x.dtype is not torch.float32 or x.get_device() != device \
-                    or not x.is_contiguous() or x.data_ptr() & 15:
-                raise ValueError("cos and sin must be contiguous float32 tensors on the inputs' "
-                                 "device")
-        positions, R = cos.shape[0], 2 * cos.shape[1]
+    positions, R = _rotation(cos, sin, device)
     k_stride, v_stride, q_stride = _token_stride(k, "k"), _token_stride(v, "v"), 0
     if q is not None:
         q_stride = _token_stride(q, "q")
@@ -601,12 +633,173 @@ def flash_attention_decode_shared(q, k_cache, v_cache, prefix_table, prefix_len:
     return out, lse
 
 
+def _check_q8(tensors, k_cache, v_cache, k_exp, v_exp, block_table, seq_lens, starts=None):
+    """What the calls on an 8-bit paged cache have in common (see _check_paged): codes [P, page, Hkv,
+    D] of one type, exponents [P, Hkv, page] uint8, and `tensors` of one floating type.
+    -> code, device, B, pages, page size, Hkv, D."""
+    torch = _torch()
+    device = torch.cuda.current_device()
+    code = {torch.int8: 0, torch.float8_e4m3fn: 1}.get(k_cache.dtype)
+    if code is None or v_cache.dtype != k_cache.dtype or k_exp.dtype != torch.uint8 \
+            or v_exp.dtype != torch.uint8:
+        raise TypeError("the caches must both be int8 or float8_e4m3fn, their exponents uint8")
+    if tensors:
+        _suffix(tensors[0])
+    ints = (block_table, seq_lens) if starts is None else (block_table, seq_lens, starts)
+    whole = (k_cache, v_cache, k_exp, v_exp)
+    for t in (*tensors, *whole, *ints):
+        if t.get_device() != device:
+            raise ValueError("tensors must be on the GPU, on the current device")
+    for t in tensors:
+        if t.dtype != tensors[0].dtype:
+            raise ValueError("all tensors must share one dtype")
+    for t in ints:
+        if t.dtype != torch.int32:
+            raise TypeError("block_table, seq_lens and query_starts must be int32")
+    for t in (*whole, *ints):
+        if not t.is_contiguous():
+            raise ValueError("the caches, exponents and int32 tensors must be contiguous")
+    for t in (*tensors, *whole):
+        if t.data_ptr() & 15:
+            raise ValueError("tensors must start at a multiple of 16 bytes")
+    shape, B = k_cache.shape, block_table.shape[0]
+    if len(shape) != 4 or v_cache.shape != shape \
+            or k_exp.shape != (shape[0], shape[2], shape[1]) or v_exp.shape != k_exp.shape:
+        raise ValueError("expected k_cache, v_cache [P,page,Hkv,D] and k_exp, v_exp [P,Hkv,page]")
+    if block_table.dim() != 2 or seq_lens.shape != (B,):
+        raise ValueError("expected block_table [B,max_pages] and seq_lens [B]")
+    if starts is not None and starts.shape != (B + 1,):
+        raise ValueError("expected starts [B+1]")
+    return (code, device, B, *shape)
+
+
+def flash_attention_append_paged_q8(k, v, k_cache, v_cache, k_exp, v_exp, block_table, seq_lens,
+                                    query_starts=None, q=None, cos=None, sin=None,
+                                    interleaved: bool = False, out=None, stream=None,
+                                    lib: Optional[CuFlashLibrary] = None):
+    """flash_attention_append_paged into a cache of one byte an element: k_cache, v_cache [P, page,
+    Hkv, D] int8 or float8_e4m3fn, k_exp, v_exp [P, Hkv, page] uint8; an element is its code times
+    2^(exponent - 127). A head's row of a token gets the least exponent that its largest element allows
+    and codes rounded to the nearest. -> rotated q [T, H, D] or None
+    (cuflash_attention_append_paged_q8_*)."""
+    lib = lib or load_library()
+    given = (k, v) if q is None else (k, v, q)
+    code, device, B, pages, page_size, Hkv, D = _check_q8(given, k_cache, v_cache, k_exp, v_exp,
+                                                          block_table, seq_lens, query_starts)
+    T, H = k.shape[0], 0 if q is None else q.shape[1]
+    if k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D) \
+            or (q is not None and q.shape != (T, H, D)):
+        raise ValueError("expected k, v [T,Hkv,D] and q [T,H,D] of the cache's Hkv and D")
+    positions, R = _rotation(cos, sin, device)
+    k_stride, v_stride, q_stride = _token_stride(k, "k"), _token_stride(v, "v"), 0
+    if q is not None:
+        q_stride = _token_stride(q, "q")
+        out = _output(out, q, (T, H, D), q.dtype, stream, "out")
+    elif out is not None:
+        raise ValueError("out is the rotated q: it needs q")
+    q_ptr, out_ptr = (None, None) if q is None else (q.data_ptr(), out.data_ptr())
+    cos_ptr, sin_ptr = (None, None) if cos is None else (cos.data_ptr(), sin.data_ptr())
+    status = lib.fn("append_paged_q8", _suffix(k))(
+        q_ptr, k.data_ptr(), v.data_ptr(), out_ptr, k_cache.data_ptr(), v_cache.data_ptr(),
+        k_exp.data_ptr(), v_exp.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+        None if query_starts is None else query_starts.data_ptr(), cos_ptr, sin_ptr, T, B, H, Hkv,
+        q_stride, k_stride, v_stride, pages, page_size, block_table.shape[1], D, R, positions,
+        bool(interleaved), code, _stream_ptr(stream))
+    _raise(lib, status)
+    return out
+
+
+def flash_attention_read_paged_q8(k_cache, v_cache, k_exp, v_exp, block_table, seq_lens, key_starts,
+                                  num_tokens: int, dtype=None, k_out=None, v_out=None, stream=None,
+                                  lib: Optional[CuFlashLibrary] = None):
+    """The keys and values that an 8-bit paged cache holds, as numbers of `dtype` (bfloat16 if not
+    given): tokens key_starts[b] .. key_starts[b + 1] - 1 are the newest of sequence b, as in
+    flash_attention_append_paged_q8, of whose tokens it gives back what the cache has. num_tokens:
+    rows of the outputs, those from key_starts[B] on are left as they are. -> k, v [num_tokens, Hkv, D]
+    (cuflash_attention_read_paged_q8_*)."""
+    torch = _torch()
+    lib = lib or load_library()
+    code, _, B, pages, page_size, Hkv, D = _check_q8((), k_cache, v_cache, k_exp, v_exp,
+                                                     block_table, seq_lens, key_starts)
+    if key_starts is None:
+        raise ValueError("expected key_starts [B+1]")
+    dtype = dtype or (torch.bfloat16 if k_out is None else k_out.dtype)
+    T = int(num_tokens)
+    if T < 1:
+        raise CuFlashError(INVALID_DIMENSION, lib.error_string(INVALID_DIMENSION))
+    k_out = _output(k_out, k_exp, (T, Hkv, D), dtype, stream, "k_out")
+    v_out = _output(v_out, k_exp, (T, Hkv, D), dtype, stream, "v_out")
+    status = lib.fn("read_paged_q8", _suffix(k_out))(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(),
+        k_out.data_ptr(), v_out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+        key_starts.data_ptr(), T, B, Hkv, pages, page_size, block_table.shape[1], D, code,
+        _stream_ptr(stream))
+    _raise(lib, status)
+    return k_out, v_out
+
+
+def flash_attention_decode_paged_q8(q, k_cache, v_cache, k_exp, v_exp, block_table, seq_lens,
+                                    scale: Optional[float] = None, out=None, lse=None, stream=None,
+                                    lib: Optional[CuFlashLibrary] = None):
+    """flash_attention_decode_paged over a cache of one byte an element (see
+    flash_attention_append_paged_q8): q [B, H, 1, D] -> O [B, H, 1, D], L float32 [B, H, 1]
+    (cuflash_attention_decode_paged_q8_*)."""
+    torch = _torch()
+    lib = lib or load_library()
+    code, _, B, _, page_size, Hkv, D = _check_q8((q,), k_cache, v_cache, k_exp, v_exp, block_table,
+                                                 seq_lens)
+    if q.dim() != 4 or q.shape[0] != B or q.shape[2] != 1 or q.shape[3] != D \
+            or not q.is_contiguous():
+        raise ValueError("expected contiguous q [B,H,1,D] of the cache's D")
+    H = q.shape[1]
+    scale = float(D ** -0.5) if scale is None else float(scale)
+    out = _output(out, q, (B, H, 1, D), q.dtype, stream, "out")
+    lse = _output(lse, q, (B, H, 1), torch.float32, stream, "lse")
+    ws, ws_bytes, _keep = _captured_workspace(lib, "decode_paged_q8", q, stream, B, H, Hkv, D)
+    status = lib.fn("decode_paged_q8", _suffix(q))(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(),
+        out.data_ptr(), lse.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), B, H, Hkv,
+        page_size, block_table.shape[1], D, scale, code, ws, ws_bytes, _stream_ptr(stream))
+    _raise(lib, status)
+    return out, lse
+
+
+def flash_attention_forward_paged_q8(q, k_cache, v_cache, k_exp, v_exp, block_table, seq_lens,
+                                     query_starts, scale: Optional[float] = None,
+                                     causal: bool = False, out=None, lse=None, stream=None,
+                                     lib: Optional[CuFlashLibrary] = None):
+    """flash_attention_forward_paged over a cache of one byte an element (see
+    flash_attention_append_paged_q8): q [T, H, D] -> O [T, H, D], L float32 [T, H]
+    (cuflash_attention_forward_paged_q8_*)."""
+    torch = _torch()
+    lib = lib or load_library()
+    code, _, B, _, page_size, Hkv, D = _check_q8((q,), k_cache, v_cache, k_exp, v_exp, block_table,
+                                                 seq_lens, query_starts)
+    if query_starts is None or q.dim() != 3 or q.shape[2] != D or not q.is_contiguous():
+        raise ValueError("expected contiguous q [T,H,D] of the cache's D and query_starts [B+1]")
+    T, H = q.shape[:2]
+    scale = float(D ** -0.5) if scale is None else float(scale)
+    out = _output(out, q, (T, H, D), q.dtype, stream, "out")
+    lse = _output(lse, q, (T, H), torch.float32, stream, "lse")
+    ws, ws_bytes, _keep = _captured_workspace(lib, "forward_paged_q8", q, stream, T, B, H, Hkv, D)
+    status = lib.fn("forward_paged_q8", _suffix(q))(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(),
+        out.data_ptr(), lse.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+        query_starts.data_ptr(), T, B, H, Hkv, page_size, block_table.shape[1], D, scale,
+        bool(causal), code, ws, ws_bytes, _stream_ptr(stream))
+    _raise(lib, status)
+    return out, lse
+
+
 __all__ = [
     "CuFlashError", "CuFlashLibrary", "EXPORTED_SYMBOLS", "load_library",
     "candidate_library_paths", "flash_attention_forward", "flash_attention_backward",
     "flash_attention_forward_ext", "flash_attention_backward_ext", "flash_attention_decode",
     "flash_attention_decode_paged", "flash_attention_append_paged",
     "flash_attention_forward_paged", "flash_attention_decode_shared", "PAGED_CACHE_SYMBOLS",
+    "flash_attention_append_paged_q8", "flash_attention_read_paged_q8",
+    "flash_attention_decode_paged_q8", "flash_attention_forward_paged_q8",
+    "PAGED_CACHE_Q8_SYMBOLS",
     "SUCCESS", "INVALID_DIMENSION", "DIMENSION_MISMATCH",
     "NULL_POINTER", "CUDA_ERROR", "OUT_OF_MEMORY", "UNSUPPORTED_HEAD_DIM", "UNSUPPORTED_DTYPE",
 ]
