@@ -35,7 +35,7 @@ RELEASE_LINK = os.path.join(BUILD_DIR, "release", LIB_NAME)
 
 SOURCES = ["api.cpp", "paged_api.cpp", "profile.cpp", "workspace.cpp", "forward.hip",
            "backward.hip", "decode.hip", "append.hip", "paged.hip",
-           "paged_q8_api.cpp", "append_q8.hip", "attention_q8.hip",
+           "paged_q8_api.cpp", "append_q8.hip", "attention_q8.hip", "prompt_q8.hip",
            "primitives.hip"]
 # C++ test programs linked against the library (sources under tests/cpp, binaries in build/).
 TEST_PROGRAMS = {"test_primitives": "test_primitives.cpp"}

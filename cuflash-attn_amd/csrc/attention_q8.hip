@@ -15,39 +15,13 @@
 // library's other matrix-core kernels), float ones taken apart into three bf16 numbers without a loss.
 // Codes of the next block are asked for before this one is worked on. The waves of neighbouring key/value
 // heads have the same share and so read the same cache rows at the same time.
-// combine_q8_kernel merges the rows that several waves have and writes those without a key.
+// combine_q8_kernel (attention_q8.hpp) merges the rows that several waves have and writes those without a
+// key. Where sequences have many 16-bit rows prompt_q8.hip takes over.
 
-#include <algorithm>
-#include <type_traits>
-
-#include "common.hpp"
-#include "launch.hpp"
-#include "paged_q8_launch.hpp"
-#include "paged_q8_plan.hpp"
-#include "profile.hpp"
-#include "q8.hpp"
-#include "softmax.hpp"
-#include "wave.hpp"
+#include "attention_q8.hpp"
 
 namespace cuflash {
 namespace dev {
-
-struct AttentionQ8Args {
-    Q8PlanArgs plan;
-    const int* block_table;  // [B, max_pages]
-    int H, Hkv;
-    int page_size, max_pages;
-    FastDiv page_div;
-    float c;          // scale * log2(e)
-    int slot_rows;    // rows of a partial result
-    float* acc;       // [shares, 2, Hkv, slot_rows, D]
-    float2* ml;       // the same without D: m in log2 units, l
-};
-
-// The row in acc and ml of row r of a tile.
-__device__ __forceinline__ size_t q8_slot_row(const AttentionQ8Args& a, int p, int slot, int hk, int r) {
-    return ((static_cast<size_t>(p) * 2 + slot) * a.Hkv + hk) * a.slot_rows + r;
-}
 
 template <typename M>
 __device__ __forceinline__ f32x4 mma16(typename Elem<M>::frag a, typename Elem<M>::frag b, f32x4 c) {
@@ -483,219 +457,65 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
         work.segment(s, a.block_table + static_cast<size_t>(s.b) * a.max_pages, p);
 }
 
-// Merges the parts of each row: O = sum O_i 2^(m_i - M) / l with M = max m_i and l = sum l_i
-// 2^(m_i - M), L = (M + log2 l) ln 2. D / 4 lanes have a row's columns, four each, and the kWays groups of
-// them every kWays-th part; they are merged through LDS in order. One workgroup per token.
-template <typename T, int D, int R>
-__global__ void __launch_bounds__(256)
-    combine_q8_kernel(typename Mma<T>::elem* __restrict__ O, float* __restrict__ L,
-                      AttentionQ8Args a) {
-    using E = typename Mma<T>::elem;
-    constexpr int LPR = D / 4;
-    constexpr int kWays = 256 / LPR;
-    constexpr int kBatch = 4;
-    __shared__ f32x4 s_acc[256];
-    __shared__ float2 s_ml[kWays];
-    const int t = blockIdx.x;
-    const int way = threadIdx.x / LPR;
-    const int part = threadIdx.x % LPR;
-    const int b = a.plan.starts ? sequence_of(a.plan.starts, a.plan.B, t) : t;
-    if (b == a.plan.B) return;  // padding
-    const Q8Seq s = q8_seq(a.plan, b);
-    if (t - s.t0 >= s.n) return;  // starts that decrease
-    const Q8Total total = q8_total<R, GpuWave>(a.plan);
-    const int first = q8_begin_of<R, GpuWave>(a.plan, b);
-    const Q8Line<R> line(a.plan, s);
-    for (int h = blockIdx.y; h < a.H; h += gridDim.y) {
-        const int hk = h / a.plan.group;
-        const int r = (t - s.t0) * a.plan.group + (h - hk * a.plan.group);
-        const int tile = r / R;
-        const Q8Parts parts =
-            q8_parts(a.plan, total, first + line.begin(a.plan, s, tile),
-                     Q8Line<R>::grains(a.plan, line.keys(a.plan, s, tile)));
-        if (parts.from == parts.to) continue;  // written already
-        float M = -INFINITY, l = 0.0f;
-        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int p0 = parts.from + way; p0 <= parts.to; p0 += kBatch * kWays) {
-            float2 v[kBatch];
-            f32x4 x[kBatch];
-            float M2 = M;
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int p = p0 + i * kWays;
-                v[i] = make_float2(-INFINITY, 0.0f);
-                x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (p <= parts.to) {
-                    const size_t at =
-                        q8_slot_row(a, p, p == parts.from ? parts.slot : 0, hk, r - tile * R);
-                    v[i] = a.ml[at];
-                    x[i] = __builtin_bit_cast(f32x4, ld16(a.acc + at * D + 4 * part));
-                    // No key of this row, or every score -inf: such a part has no say, also where
-                    // 0 times a value made it NaN.
-                    if (v[i].x == -INFINITY) x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) M2 = fmaxf(M2, v[i].x);
-            auto weight = [&](float mi) { return mi == -INFINITY ? 0.0f : fast_exp2(mi - M2); };
-            const float f0 = weight(M);
-            l *= f0;
-            acc *= f0;
-            M = M2;
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const float f = weight(v[i].x);
-                l = fmaf(v[i].y, f, l);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[c] = fmaf(x[i][c], f, acc[c]);
-            }
-        }
-        s_acc[threadIdx.x] = acc;
-        if (part == 0) s_ml[way] = make_float2(M, l);
-        __syncthreads();
-        if (way == 0) {
-#pragma unroll
-            for (int w = 1; w < kWays; ++w) M = fmaxf(M, s_ml[w].x);
-            l = 0.0f;
-            acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < kWays; ++w) {
-                const float2 v = s_ml[w];
-                const f32x4 x = s_acc[threadIdx.x + w * LPR];
-                const float f = v.x == -INFINITY ? 0.0f : fast_exp2(v.x - M);
-                l = fmaf(v.y, f, l);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[c] = fmaf(x[c], f, acc[c]);
-            }
-            const bool none = l == 0.0f;
-            const float inv = none ? 0.0f : 1.0f / l;
-            float y[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) y[c] = none ? 0.0f : acc[c] * inv;
-            const size_t row = static_cast<size_t>(t) * a.H + h;
-            E* dst = O + row * D + 4 * part;
-            if constexpr (std::is_same<T, float>::value)
-                st16(dst, u32x4{__float_as_uint(y[0]), __float_as_uint(y[1]),
-                                __float_as_uint(y[2]), __float_as_uint(y[3])});
-            else
-                st8(dst, u32x2{Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3])});
-            if (part == 0) L[row] = none ? -INFINITY : (M + fast_log2(l)) * kLn2;
-        }
-        __syncthreads();  // before the next row's
-    }
-}
-
 }  // namespace dev
 
 namespace detail {
 namespace {
 
-// The sizes of one launch.
-struct Q8Grid {
-    int rows;       // of a tile: 16, or 32 where a sequence has more
-    int shares;     // waves per key/value head
-    int slot_rows;  // of a partial result
-    int kv_heads, head_dim, tokens;
-
-    // `wide`: tiles of 32 rows have registers enough.
-    Q8Grid(const PagedCall& c, bool wide) {
-        kv_heads = c.num_kv_heads;
-        head_dim = c.head_dim;
-        tokens = c.num_tokens;
-        const int group = c.num_heads / c.num_kv_heads;
-        const long long all = static_cast<long long>(tokens) * group;
-        rows = !wide || all <= 16LL * c.batch_size ? 16 : 32;
-        // Two waves a SIMD (registers); of 32 rows a little fewer, whose partial results then fit the
-        // library's workspace of a stream.
-        const int waves = compute_units() * 8;
-        shares = std::max(1, (rows == 16 ? waves : waves / 16 * 15) / kv_heads);
-        const long long most = c.query_starts ? all : group;
-        slot_rows = static_cast<int>(std::min<long long>(rows, most));
-    }
-    size_t slots() const { return static_cast<size_t>(shares) * 2 * kv_heads * slot_rows; }
-    size_t bytes() const { return slots() * (head_dim * sizeof(float) + sizeof(float2)); }
-    unsigned groups() const {
-        return static_cast<unsigned>((static_cast<long long>(shares) * kv_heads + dev::kQ8Waves - 1) /
-                                     dev::kQ8Waves);
-    }
-    // A launch has at most 2^32 - 1 threads in x; the merge has a workgroup per token.
-    bool too_large() const { return 256LL * tokens > 0xffffffffLL; }
-};
-
-// float queries of 128 elements in three parts are too many for 32 rows.
+// Where most sequences have more rows than this, workgroups share the keys (prompt_q8.hip).
+constexpr long long kManyRows = 96;
 template <typename T>
-constexpr bool wide_tiles(int head_dim) {
-    return !std::is_same<T, float>::value || head_dim < 128;
+bool many_rows(const PagedCall& c) {
+    return !std::is_same<T, float>::value && c.query_starts &&
+           static_cast<long long>(c.num_tokens) * (c.num_heads / c.num_kv_heads) >
+               kManyRows * c.batch_size;
+}
+
+// Tiles of 16 rows, or of 32 where sequences have more and registers suffice (float queries of 128 elements
+// in three parts are too many). Two waves a SIMD (registers); with 32 rows a little fewer, whose partial
+// results then fit the library's workspace of a stream.
+template <typename T>
+Q8Grid waves_grid(const PagedCall& c) {
+    const bool wide = (!std::is_same<T, float>::value || c.head_dim < 128) &&
+                      static_cast<long long>(c.num_tokens) * (c.num_heads / c.num_kv_heads) >
+                          16LL * c.batch_size;
+    const int waves = compute_units() * 8;
+    return Q8Grid(c, wide ? 32 : 16, (wide ? waves / 16 * 15 : waves) / c.num_kv_heads, 0);
 }
 
 template <typename T, int D, QuantCode C>
 FlashAttentionError run_attention(const PagedQ8Call& q8, hipStream_t stream) {
     using E = typename dev::Mma<T>::elem;
     const PagedCall& c = q8.call;
-    const Q8Grid grid(c, wide_tiles<T>(D));
-    if (grid.too_large()) return FlashAttentionError::INVALID_DIMENSION;
-    dev::AttentionQ8Args a{};
-    a.plan.seq_lens = c.seq_lens;
-    a.plan.starts = c.query_starts;
-    a.plan.B = c.batch_size;
-    a.plan.T = c.num_tokens;
-    a.plan.group = c.num_heads / c.num_kv_heads;
-    a.plan.cap = c.page_size * c.max_pages;
-    a.plan.shares = grid.shares;
-    a.plan.shift = dev::q8_shift(c.num_tokens, c.batch_size, a.plan.group, grid.rows, a.plan.cap);
-    a.plan.causal = c.causal;
-    a.plan.group_div = dev::fast_div(a.plan.group);
-    a.block_table = c.block_table;
-    a.H = c.num_heads;
-    a.Hkv = c.num_kv_heads;
-    a.page_size = c.page_size;
-    a.max_pages = c.max_pages;
-    a.page_div = dev::fast_div(c.page_size);
-    a.c = c.scale * dev::kLog2e;
-    a.slot_rows = grid.slot_rows;
-    StreamWorkspace ws(stream, true);
-    void* base = c.workspace;
-    if (base == nullptr) {
-        // A graph's replays need memory that is theirs: the caller's.
-        if (stream_capturing(stream)) return FlashAttentionError::OUT_OF_MEMORY;
-        FlashAttentionError err = ws.alloc(grid.bytes());
-        if (err != FlashAttentionError::SUCCESS) return err;
-        base = ws.get();
-    } else if (c.workspace_bytes < grid.bytes()) {
-        return FlashAttentionError::OUT_OF_MEMORY;
+    if (many_rows<T>(c)) {
+        if constexpr (!std::is_same<T, float>::value) return launch_prompt_q8<T>(q8, stream);
     }
-    a.acc = static_cast<float*>(base);
-    a.ml = reinterpret_cast<float2*>(a.acc + grid.slots() * D);
-    ProfileEvents tok = profile_kernel<T, D>(c.query_starts ? "forward_q8" : "decode_q8");
-    auto go = [&](auto kernel) {
-        launch_kernel(tok, kernel, dim3(grid.groups()), dim3(64 * dev::kQ8Waves), 0, stream,
-                      static_cast<const E*>(c.Q), static_cast<const uint8_t*>(c.K_cache),
-                      static_cast<const uint8_t*>(c.V_cache), q8.K_exp, q8.V_exp,
-                      static_cast<E*>(c.O), c.L, a);
-    };
+    const Q8Grid grid = waves_grid<T>(c);
     const bool whole = c.page_size % 16 == 0;  // half a block's rows lie on one page
-    if (grid.rows == 16) {
-        whole ? go(dev::attention_q8_kernel<T, D, C, 1, true>)
-              : go(dev::attention_q8_kernel<T, D, C, 1, false>);
-    } else if constexpr (wide_tiles<T>(D)) {
-        whole ? go(dev::attention_q8_kernel<T, D, C, 2, true>)
-              : go(dev::attention_q8_kernel<T, D, C, 2, false>);
-    }
-    FlashAttentionError err = from_hip(hipGetLastError());
-    if (err != FlashAttentionError::SUCCESS) return err;
-    tok = profile_kernel<T, D>("combine_q8");
-    auto merge = [&](auto kernel) {
-        // Every workgroup finds its token's place first: with many tokens it takes all heads.
-        const int heads = std::min(c.num_heads, std::max(1, 8 * compute_units() / c.num_tokens));
-        launch_kernel(tok, kernel,
-                      dim3(static_cast<unsigned>(c.num_tokens), static_cast<unsigned>(heads)),
-                      dim3(256), 0, stream, static_cast<E*>(c.O), c.L, a);
+    auto run = [&](auto nr) {
+        constexpr int NR = decltype(nr)::value;
+        return run_q8<T, D, 16 * NR>(c, grid, stream, [&](const dev::AttentionQ8Args& a) {
+            const long long waves = static_cast<long long>(grid.shares) * grid.kv_heads;
+            auto go = [&](auto kernel) {
+                launch_kernel(profile_kernel<T, D>(c.query_starts ? "forward_q8" : "decode_q8"),
+                              kernel,
+                              dim3(static_cast<unsigned>((waves + dev::kQ8Waves - 1) /
+                                                         dev::kQ8Waves)),
+                              dim3(64 * dev::kQ8Waves), 0, stream, static_cast<const E*>(c.Q),
+                              static_cast<const uint8_t*>(c.K_cache),
+                              static_cast<const uint8_t*>(c.V_cache), q8.K_exp, q8.V_exp,
+                              static_cast<E*>(c.O), c.L, a);
+            };
+            if (whole)
+                go(dev::attention_q8_kernel<T, D, C, NR, true>);
+            else
+                go(dev::attention_q8_kernel<T, D, C, NR, false>);
+        });
     };
-    if (grid.rows == 16)
-        merge(dev::combine_q8_kernel<T, D, 16>);
-    else if constexpr (wide_tiles<T>(D))
-        merge(dev::combine_q8_kernel<T, D, 32>);
-    return from_hip(hipGetLastError());
+    if constexpr (!std::is_same<T, float>::value || D < 128) {
+        if (grid.rows == 32) return run(std::integral_constant<int, 2>{});
+    }
+    return run(std::integral_constant<int, 1>{});
 }
 
 template <typename T, QuantCode C>
@@ -715,8 +535,13 @@ FlashAttentionError run_dim(const PagedQ8Call& c, hipStream_t stream) {
 
 template <typename T>
 long long paged_q8_workspace(const PagedCall& c) {
-    const Q8Grid grid(c, wide_tiles<T>(c.head_dim));
-    return grid.too_large() ? -1 : static_cast<long long>(grid.bytes());
+    auto grid = [&] {
+        if constexpr (!std::is_same<T, float>::value) {
+            if (many_rows<T>(c)) return prompt_q8_grid<T>(c);
+        }
+        return waves_grid<T>(c);
+    }();
+    return static_cast<long long>(grid.bytes());
 }
 
 template <typename T>

@@ -37,7 +37,7 @@ struct PagedQ8Call {
     QuantCode code;
 };
 // Bytes of the partial results of a call of these sizes (query_starts: null for a decode; the others are
-// not read), -1 where its grid would be too large.
+// not read).
 template <typename T>
 long long paged_q8_workspace(const PagedCall& call);
 template <typename T>

@@ -14,7 +14,8 @@
 // With a causal mask a later tile sees more keys. Tiles stand in pairs in the line, the first with the last,
 // the second with the last but one, so that every pair has as many grains, and where a pair begins is a
 // product. (With f(e) = max(0, keys - n + e), convex, and e_i <= (i + 1) R / group + 1 tokens up to tile i, a
-// pair has at most f(e_first) + f(e_last) + R / group + 2 keys: up to 3 grains more than the first pair.)
+// pair has at most f(e_first) + f(e_last) + R / group + 2 keys, and so, in grains of g keys, at most
+// 2 + floor(R / (group g)) more than the first pair: the `slack`.)
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -30,6 +31,7 @@ struct Q8PlanArgs {
     int B, T, group, cap;
     int shares;  // waves per key/value head
     int shift;   // a grain has 32 << shift keys
+    int slack;   // grains between pairs
     bool causal;
     FastDiv group_div;
 };
@@ -51,13 +53,11 @@ __host__ __device__ __forceinline__ int q8_limit(const Q8PlanArgs& a, const Q8Se
     return lim > 0 ? lim : 0;
 }
 
-constexpr int kQ8PairSlack = 3;
 constexpr int kQ8Line = 1 << 30;  // grains of a line, and waves of a launch, are fewer
 
 // The tiles of a sequence in the line.
 template <int R>
 struct Q8Line {
-    static_assert(R <= 32, "the slack of a pair");
     int rows, tiles;
     int pairs;  // the last of them may have one tile; without a mask every one has
     int pair;   // grains from pair to pair
@@ -72,7 +72,7 @@ struct Q8Line {
             size = pairs * pair;
         } else {
             pairs = tiles / 2;
-            pair = grains(a, keys(a, s, 0)) + last + kQ8PairSlack;
+            pair = grains(a, keys(a, s, 0)) + last + a.slack;
             size = pairs * pair;
             if (tiles % 2) size += grains(a, keys(a, s, pairs++));
         }
@@ -209,6 +209,14 @@ struct Q8Walk {
     }
 };
 
+// Rows of a sequence that lie in tiles without a key: the first ones.
+template <int R>
+__host__ __device__ __forceinline__ int q8_rows_without_keys(const Q8PlanArgs& a, const Q8Seq& s) {
+    if (s.keys == 0) return s.n * a.group;
+    if (!a.causal || s.n <= s.keys) return 0;
+    return (s.n - s.keys) * a.group / R * R;
+}
+
 // The waves that have a part of a tile, `from` .. `to`, and the slot of wave `from`'s; from > to: the tile
 // has no keys (or, with starts that decrease, no wave).
 struct Q8Parts {
@@ -222,12 +230,13 @@ __host__ __device__ __forceinline__ Q8Parts q8_parts(const Q8PlanArgs& a, const 
     return {from, to, begin > from * total.share ? 1 : 0};
 }
 
-// What the host knows: the most grains that a line can have stay below 2^30 with this shift.
-inline int q8_shift(long long tokens, long long batch, int group, int rows_per_tile, long long cap) {
-    const long long tiles = tokens * group / rows_per_tile + 2 * batch;
-    int shift = 0;
-    while (shift < 26 && tiles * (((cap + 31) / 32 >> shift) + 1 + kQ8PairSlack) >= kQ8Line) ++shift;
-    return shift;
+// The grains of a launch, of 32 << least keys or more: what the host knows keeps the line below 2^30 of them.
+inline void q8_set_grains(Q8PlanArgs& a, int rows_per_tile, int least) {
+    const long long tiles = static_cast<long long>(a.T) * a.group / rows_per_tile + 2LL * a.B;
+    for (a.shift = least;; ++a.shift) {
+        a.slack = 2 + static_cast<int>(rows_per_tile / (static_cast<long long>(a.group) << (5 + a.shift)));
+        if (a.shift >= 26 || tiles * (((a.cap + 31LL) / 32 >> a.shift) + 1 + a.slack) < kQ8Line) return;
+    }
 }
 
 }  // namespace dev

@@ -82,9 +82,9 @@ bool launch(std::mt19937& rng) {  // whether a tile was cut
     a.seq_lens = lens.data();
     a.starts = decode ? nullptr : starts.data();
     a.T = decode ? a.B : std::max(1, starts.back() + (pick(4) == 0 ? 5 : 0) - (pick(6) == 0 ? 1 : 0));
-    a.shift = q8_shift(a.T, a.B, a.group, R, a.cap);
-    CHECK(far || a.shift == 0);
-    if (pick(5) == 0) a.shift += 1 + pick(2);
+    const int least = R == 256 ? 1 : pick(5) == 0 ? 1 + pick(2) : 0;
+    q8_set_grains(a, R, least);
+    CHECK(far || a.shift == least);
 
     const Q8Total total = q8_total<R, HostWave>(a);
     int sum = 0;
@@ -111,7 +111,7 @@ bool launch(std::mt19937& rng) {  // whether a tile was cut
             CHECK(s.kbeg >= 0 && s.kbeg < s.kend && s.kend <= q.keys && s.kbeg % 32 == 0);
             grains += (s.kend - s.kbeg - 1) / (32 << a.shift) + 1;
             if (s.slot >= 0) {
-                CHECK(s.slot < 2 && !used[s.slot]);
+                CHECK(s.slot < 2 && !used[s.slot] && (s.slot == 0 || p < a.shares - 1));
                 used[s.slot] = true;
                 cut = true;
             }
@@ -123,7 +123,9 @@ bool launch(std::mt19937& rng) {  // whether a tile was cut
         const Q8Seq q = q8_seq(a, b);
         const Q8Line<R> line(a, q);
         CHECK(line.tiles == (q.n * a.group + R - 1) / R);
+        const int without = q8_rows_without_keys<R>(a, q);
         for (int tile = 0; tile < line.tiles; ++tile) {
+            CHECK((line.keys(a, q, tile) == 0) == (tile * R < without));
             // The keys that some row of the tile sees.
             int keys = 0;
             for (int r = tile * R; r < std::min((tile + 1) * R, line.rows); ++r)
@@ -142,6 +144,14 @@ bool launch(std::mt19937& rng) {  // whether a tile was cut
                 CHECK(got[i][3] == (got.size() == 1 ? -1 : i == 0 ? parts.slot : 0));
             }
             CHECK(at == keys);
+            // The merge by shares finds a cut tile from the share that it begins in.
+            if (got.size() > 1) {
+                const int end = std::min((parts.from + 1) * total.share, total.grains);
+                int first = 0, in = 0, grain = 0;
+                CHECK((q8_sequence_at<R, HostWave>(a, end - 1, first) == b));
+                CHECK(line.find(a, q, end - 1 - first, in, grain) && in == tile);
+                CHECK(end - 1 - grain == first + line.begin(a, q, tile));
+            }
         }
     }
     return cut;
@@ -166,7 +176,7 @@ void disorder(std::mt19937& rng) {
     }
     a.seq_lens = lens.data();
     a.starts = starts.data();
-    a.shift = q8_shift(a.T, a.B, a.group, R, a.cap);
+    q8_set_grains(a, R, R == 256 ? 1 : 0);
     const Q8Total total = q8_total<R, HostWave>(a);
     for (int p = 0; p < a.shares; ++p) {
         Q8Walk<R, HostWave> walk(a, p);
@@ -187,8 +197,9 @@ int main(int argc, char** argv) {
     std::mt19937 rng(argc > 2 ? std::atoi(argv[2]) : 1);
     int cut = 0;
     for (g_case = 0; g_case < launches; ++g_case) {
-        cut += g_case % 2 ? launch<16>(rng) : launch<32>(rng);
-        g_case % 2 ? disorder<32>(rng) : disorder<16>(rng);
+        const int kind = g_case % 3;
+        cut += kind == 0 ? launch<16>(rng) : kind == 1 ? launch<32>(rng) : launch<256>(rng);
+        kind == 0 ? disorder<32>(rng) : kind == 1 ? disorder<16>(rng) : disorder<256>(rng);
     }
     CHECK(cut > launches / 3);
     std::printf("%d launches, %d with tiles that several waves have\n", launches, cut);
