@@ -13,7 +13,8 @@
 // Codes become 16-bit numbers in registers (q8.hpp) and stay exact; scores, maxima, sums and O are
 // float, the weights are rounded to T before they meet V (half a step, 2^-8 of p |v| in bf16, as in the
 // library's other matrix-core kernels), float ones taken apart into three bf16 numbers without a loss.
-// Codes of the next block are asked for before this one is worked on. The waves of neighbouring key/value
+// Codes of the next block are asked for before this one is worked on, or where registers are short as
+// its own have been used. The waves of neighbouring key/value
 // heads have the same share and so read the same cache rows at the same time.
 // combine_q8_kernel (attention_q8.hpp) merges the rows that several waves have and writes those without a
 // key. Where sequences have many 16-bit rows prompt_q8.hip takes over.
@@ -88,20 +89,22 @@ struct AttentionQ8 {
     struct Codes {
         uint32_t k[2][KI][KB / 4];
         uint32_t v[8][VW];
-        uint32_t kx[2];  // the exponent of the lane's key of each half block
-        uint32_t vx[2];  // of its four keys
+        uint32_t kx[2];  // the exponents of the lane's four keys of each half block (kScaleK: of its one)
+        uint32_t vx[2];
     };
-    // The table entries of a block's halves (kWhole).
     typedef const __attribute__((address_space(4))) int* ConstInts;
+    // Two blocks in registers, or one, whose keys and then values give way to the next as they have been used.
+    static constexpr bool kDouble = NR == 1 && kParts == 1;
+    // e4m3 codes are scaled as they are converted; for int8 codes that would be an instruction an element, so
+    // their scores are scaled instead.
+    static constexpr bool kScaleK = C == QuantCode::E4M3;
 
     template <int N>
     static __device__ __forceinline__ void copy(uint32_t (&to)[N], const uint8_t* from, int bytes) {
         if constexpr (N == 4) {
             const u32x4 v = ld16(from);
-            to[0] = v[0];
-            to[1] = v[1];
-            to[2] = v[2];
-            to[3] = v[3];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[i] = v[i];
         } else if constexpr (N == 2) {
             const u32x2 v = *reinterpret_cast<const u32x2*>(from);
             to[0] = v[0];
@@ -111,64 +114,141 @@ struct AttentionQ8 {
                                : *reinterpret_cast<const uint32_t*>(from);
         }
     }
-
-    // Entries of the table for the halves of the block at key0 of a segment that ends at kend.
-    __device__ __forceinline__ void entries(const int* table, int key0, int kend, int (&page)[2]) const {
-        const int last = (kend - 1) & ~15;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-            page[t] = ((ConstInts)table)[a.page_div(min(key0 + 16 * t, last))];
+    // The same for lines that one load reads whole and nothing reads again (64 sequences of up to 8192 keys,
+    // int8: 111 -> 99 us; K, half a line a load, so 100 -> 123).
+    template <int N>
+    static __device__ __forceinline__ void copy_once(uint32_t (&to)[N], const uint8_t* from, int bytes) {
+        if constexpr (N == 2) {
+            const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(from));
+            to[0] = v[0];
+            to[1] = v[1];
+        } else {
+            copy(to, from, bytes);
+        }
     }
-    // The codes of the block at key0. Of a half that lies behind the end another's rows are read, and of
-    // one that ends inside it the page's rows behind the end; neither is used.
-    __device__ __forceinline__ void load(const int* table, const int (&page)[2], int key0, int kend,
-                                         Codes& x) const {
+
+    // The place of the half block that is loaded next (kWhole: its rows lie on one page): the walk over a
+    // segment's halves, the table read one ahead. Behind the last it stays there.
+    struct Place {
+        const int* table;
+        int entry, in_page;  // of the next half
+        int page;
+        int left;  // halves behind it
+    };
+    __device__ __forceinline__ Place place_of(const int* table, int kbeg, int kend) const {
+        Place at;
+        at.table = table;
+        at.entry = a.page_div(kbeg);
+        at.in_page = kbeg - at.entry * a.page_size;
+        at.page = ((ConstInts)table)[at.entry];
+        at.left = (kend - kbeg - 1) >> 4;
+        return at;
+    }
+    __device__ __forceinline__ void advance(Place& at) const {
+        if (at.left == 0) return;
+        --at.left;
+        at.in_page += 16;
+        if (at.in_page >= a.page_size) {
+            at.in_page = 0;
+            ++at.entry;
+            at.page = ((ConstInts)at.table)[at.entry];
+        }
+    }
+
+    // base + offset as a load from a scalar base and a 32-bit lane offset: seen as a constant of the loop the
+    // offset would be widened in front of it, to two registers and an addition a load.
+    static __device__ __forceinline__ const uint8_t* lane_at(const uint8_t* base, uint32_t offset) {
+        asm volatile("" : "+v"(offset));
+        return base + offset;
+    }
+
+    // Where the halves of a block lie (kWhole): their first row, in bytes, and its exponent.
+    struct Rows {
+        uint64_t row[2], ex[2];
+        int key0;
+    };
+    __device__ __forceinline__ Rows rows_of(Place& next, int key0) const {
+        Rows at;
+        at.key0 = key0;
+        if constexpr (kWhole) {
+            const uint32_t pitch = static_cast<uint32_t>(a.Hkv) * D;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint64_t pg = static_cast<uint32_t>(next.page);
+                at.row[t] = pg * a.page_bytes + static_cast<uint64_t>(next.in_page) * pitch;
+                at.ex[t] = pg * a.page_exps + next.in_page;
+                advance(next);
+            }
+        }
+        return at;
+    }
+    // The same of one key, that of a lane.
+    __device__ __forceinline__ void row_of(const int* table, int key, uint64_t& row, uint64_t& ex) const {
+        const int entry = a.page_div(key);
+        const uint32_t in_page = key - entry * a.page_size;
+        const uint64_t pg = static_cast<uint32_t>(table[entry]);
+        row = pg * a.page_bytes + static_cast<uint64_t>(in_page) * (static_cast<uint32_t>(a.Hkv) * D);
+        ex = pg * a.page_exps + in_page;
+    }
+    // The codes of a block. Of a half that lies behind the end another's rows are read, and of one that ends
+    // inside it the page's rows behind the end; neither is used.
+    __device__ __forceinline__ void load_k(const Rows& at, const int* table, int kend, Codes& x) const {
         const int lane = threadIdx.x & 63;
         const int l16 = lane & 15, q = lane >> 4;
-        const size_t pitch = static_cast<size_t>(a.Hkv) * D;
-        if constexpr (kWhole) {
-            const int last = (kend - 1) & ~15;
+        const uint32_t pitch = static_cast<uint32_t>(a.Hkv) * D;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int at = min(key0 + 16 * t, last);
-                const int in_page = at - a.page_div(at) * a.page_size;
-                const size_t row = (static_cast<size_t>(page[t]) * a.page_size + in_page) * pitch;
-                const size_t ex = static_cast<size_t>(page[t]) * a.Hkv * a.page_size + in_page;
-                const uint32_t k_at = l16 * static_cast<uint32_t>(pitch) + q * KB;
+        for (int t = 0; t < 2; ++t) {
+            if constexpr (kWhole) {
 #pragma unroll
-                for (int i = 0; i < KI; ++i) copy(x.k[t][i], K + row + (k_at + 64u * i), KB);
-                const uint32_t v_at = 4 * q * static_cast<uint32_t>(pitch) + l16 * VB;
+                for (int i = 0; i < KI; ++i)
+                    copy(x.k[t][i], lane_at(K + at.row[t] + 64 * i, l16 * pitch + q * KB), KB);
+                x.kx[t] = kScaleK
+                              ? *lane_at(Kx + at.ex[t], l16)
+                              : *reinterpret_cast<const uint32_t*>(lane_at(Kx + at.ex[t], 4 * q));
+            } else {
+                uint64_t row, ex;
+                row_of(table, min(at.key0 + 16 * t + l16, kend - 1), row, ex);
+#pragma unroll
+                for (int i = 0; i < KI; ++i) copy(x.k[t][i], K + row + (q * KB + 64 * i), KB);
+                x.kx[t] = kScaleK ? Kx[ex] : 0;
+                if constexpr (!kScaleK) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        row_of(table, min(at.key0 + 16 * t + 4 * q + r, kend - 1), row, ex);
+                        x.kx[t] |= static_cast<uint32_t>(Kx[ex]) << (8 * r);
+                    }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(const Rows& at, const int* table, int kend, Codes& x) const {
+        const int lane = threadIdx.x & 63;
+        const int l16 = lane & 15, q = lane >> 4;
+        const uint32_t pitch = static_cast<uint32_t>(a.Hkv) * D;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            if constexpr (kWhole) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    copy(x.v[4 * t + r], V + row + r * pitch + v_at, VB);
-                x.kx[t] = *(Kx + ex + l16);
-                x.vx[t] = *reinterpret_cast<const uint32_t*>(Vx + ex + 4 * q);
-            }
-        } else {
-            auto place = [&](int key, size_t& row, size_t& ex) {
-                key = min(key, kend - 1);
-                const int entry = a.page_div(key);
-                const int in_page = key - entry * a.page_size;
-                const size_t pg = static_cast<size_t>(table[entry]);
-                row = (pg * a.page_size + in_page) * pitch;
-                ex = pg * a.Hkv * a.page_size + in_page;
-            };
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                size_t row, ex;
-                place(key0 + 16 * t + l16, row, ex);
-#pragma unroll
-                for (int i = 0; i < KI; ++i) copy(x.k[t][i], K + row + q * KB + 64 * i, KB);
-                x.kx[t] = Kx[ex];
+                    copy_once(x.v[4 * t + r],
+                              lane_at(V + at.row[t] + static_cast<uint64_t>(r) * pitch,
+                                      4 * q * pitch + l16 * VB),
+                              VB);
+                x.vx[t] = *reinterpret_cast<const uint32_t*>(lane_at(Vx + at.ex[t], 4 * q));
+            } else {
                 x.vx[t] = 0;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    place(key0 + 16 * t + 4 * q + r, row, ex);
+                    uint64_t row, ex;
+                    row_of(table, min(at.key0 + 16 * t + 4 * q + r, kend - 1), row, ex);
                     copy(x.v[4 * t + r], V + row + l16 * VB, VB);
                     x.vx[t] |= static_cast<uint32_t>(Vx[ex]) << (8 * r);
                 }
             }
         }
+    }
+    static __device__ __forceinline__ float factor(uint32_t four, int i) {
+        return Q8<C>::factor((four >> (8 * i)) & 0xffu);
     }
 
     // The outputs of a segment's rows, or their partial results, those of wave p.
@@ -241,20 +321,19 @@ struct AttentionQ8 {
         }
         const float cs = fmaxf(a.c, kFltMin);  // scale 0: -inf * 0 would make the masked scores NaN
 
-        auto block = [&](const Codes& x, int key0) {
-            f32x4 sc[NR][2];
+        f32x4 sc[NR][2];
+        auto scores = [&](const Codes& x) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) sc[nr][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                const float by = Q8<C>::factor(x.kx[t]);
+                const float by = kScaleK ? Q8<C>::factor(x.kx[t]) : 1.0f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const uint32_t* w = &x.k[t][ks / (KB / 8)][ks % (KB / 8) * 2];
-                    const Frag k = as_frag<M>(u32x4{Q8<C>::template expand<M, 0>(w[0], by),
-                                                    Q8<C>::template expand<M, 1>(w[0], by),
-                                                    Q8<C>::template expand<M, 0>(w[1], by),
-                                                    Q8<C>::template expand<M, 1>(w[1], by)});
+                    const u32x2 lo = Q8<C>::template four<M, kScaleK>(w[0], by);
+                    const u32x2 hi = Q8<C>::template four<M, kScaleK>(w[1], by);
+                    const Frag k = as_frag<M>(u32x4{lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
                     for (int part = kParts - 1; part >= 0; --part) {
 #pragma unroll
@@ -262,7 +341,17 @@ struct AttentionQ8 {
                             sc[nr][t] = mma16<M>(k, f[nr][part][ks], sc[nr][t]);
                     }
                 }
+                if constexpr (!kScaleK) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float k_by = factor(x.kx[t], r);
+#pragma unroll
+                        for (int nr = 0; nr < NR; ++nr) sc[nr][t][r] *= k_by;
+                    }
+                }
             }
+        };
+        auto values = [&](const Codes& x, int key0) {
             if (key0 + 32 > mask_from) {
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
@@ -318,19 +407,17 @@ struct AttentionQ8 {
             }
             float by[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) by[e] = Q8<C>::factor((x.vx[e >> 2] >> (8 * (e & 3))) & 0xffu);
+            for (int e = 0; e < 8; ++e) by[e] = factor(x.vx[e >> 2], e & 3);
             // The codes of columns 2 j and 2 j + 1 of the lane's 8 keys: 8 pairs, turned.
             auto columns = [&](auto jc) {
                 constexpr int j = decltype(jc)::value;
-                uint32_t w[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    w[e] = Q8<C>::template expand<M, (j & 1)>(x.v[e][j >> 1], by[e]);
                 u32x4 lo, hi;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    lo[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
-                    hi[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+                    const u32x2 two = Q8<C>::template turned<M, (j & 1)>(
+                        x.v[2 * i][j >> 1], by[2 * i], x.v[2 * i + 1][j >> 1], by[2 * i + 1]);
+                    lo[i] = two[0];
+                    hi[i] = two[1];
                 }
 #pragma unroll
                 for (int part = kParts - 1; part >= 0; --part) {
@@ -362,24 +449,48 @@ struct AttentionQ8 {
             }
         };
 
-        Codes x[2];
-        int page[2] = {0, 0};
-        if constexpr (kWhole) entries(table, kbeg, kend, page);
-        load(table, page, kbeg, kend, x[0]);
-        if constexpr (kWhole) entries(table, kbeg + 32, kend, page);
-        for (int key0 = kbeg; key0 < kend; key0 += 64) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = key0 + 32 * h;
-                if (h == 1 && at >= kend) break;
-                if (at + 32 < kend) {
-                    load(table, page, at + 32, kend, x[1 - h]);
-                    if constexpr (kWhole) entries(table, at + 64, kend, page);
+        Place next = place_of(table, kbeg, kend);
+        int key0 = kbeg;
+        Codes last;
+        if constexpr (kDouble) {
+            Codes x[2];
+            auto load = [&](int at, Codes& to) {
+                const Rows rows = rows_of(next, at);
+                load_k(rows, table, kend, to);
+                load_v(rows, table, kend, to);
+            };
+            load(kbeg, x[0]);
+            while (key0 + 32 < kend) {
+                load(key0 + 32, x[1]);
+                scores(x[0]);
+                values(x[0], key0);
+                key0 += 32;
+                if (key0 + 32 >= kend) {
+                    x[0] = x[1];
+                    break;
                 }
-                cut(x[h], at);
-                block(x[h], at);
+                load(key0 + 32, x[0]);
+                scores(x[1]);
+                values(x[1], key0);
+                key0 += 32;
+            }
+            last = x[0];
+        } else {
+            const Rows first = rows_of(next, kbeg);
+            load_k(first, table, kend, last);
+            load_v(first, table, kend, last);
+            while (key0 + 32 < kend) {
+                scores(last);
+                const Rows rows = rows_of(next, key0 + 32);
+                load_k(rows, table, kend, last);
+                values(last, key0);
+                load_v(rows, table, kend, last);
+                key0 += 32;
             }
         }
+        cut(last, key0);
+        scores(last);
+        values(last, key0);
 
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
@@ -427,7 +538,9 @@ struct AttentionQ8 {
     }
 };
 
-constexpr int kQ8Waves = 4;  // of a workgroup: each for itself
+// Of a workgroup, each for itself: the eight key/value heads of a common model then read their shares of the
+// cache's rows from one CU.
+constexpr int kQ8Waves = 8;
 
 template <typename T, int D, QuantCode C, int NR, bool kWhole>
 __global__ void __launch_bounds__((64 * kQ8Waves), 2)
@@ -480,7 +593,8 @@ Q8Grid waves_grid(const PagedCall& c) {
                       static_cast<long long>(c.num_tokens) * (c.num_heads / c.num_kv_heads) >
                           16LL * c.batch_size;
     const int waves = compute_units() * 8;
-    return Q8Grid(c, wide ? 32 : 16, (wide ? waves / 16 * 15 : waves) / c.num_kv_heads, 0);
+    return Q8Grid(c, wide ? 32 : 16, (wide ? waves / 16 * 15 : waves) / c.num_kv_heads, 0,
+                  1);
 }
 
 template <typename T, int D, QuantCode C>

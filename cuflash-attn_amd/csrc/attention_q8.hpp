@@ -23,6 +23,7 @@ struct AttentionQ8Args {
     const int* block_table;  // [B, max_pages]
     int H, Hkv;
     int page_size, max_pages;
+    uint64_t page_bytes, page_exps;  // codes and exponents of a page
     FastDiv page_div;
     float c;          // scale * log2(e)
     int slot_rows;    // rows of a partial result
@@ -78,19 +79,20 @@ struct Q8Merge {
     }
 };
 
-// The merge, row by row: one workgroup per token and every gridDim.y-th head. D / 4 lanes have a row, and the
-// kWays groups of them every kWays-th part; they are merged through LDS in order.
-template <typename T, int D, int R>
+// The merge, row by row: one workgroup per token and gridDim.y-th part of its heads. D / 4 lanes have a row,
+// and kWays groups of them every kWays-th part of it; they are merged through LDS in order.
+template <typename T, int D, int R, int kWays>
 __global__ void __launch_bounds__(256)
     combine_q8_kernel(typename Mma<T>::elem* __restrict__ O, float* __restrict__ L,
                       AttentionQ8Args a) {
     constexpr int LPR = D / 4;
-    constexpr int kWays = 256 / LPR;
+    constexpr int kRows = 256 / LPR / kWays;  // at a time
     constexpr int kBatch = 4;
     __shared__ f32x4 s_acc[256];
-    __shared__ float2 s_ml[kWays];
+    __shared__ float2 s_ml[256 / LPR];
     const int t = blockIdx.x;
-    const int way = threadIdx.x / LPR;
+    const int slot = threadIdx.x / LPR;
+    const int way = slot % kWays;
     const int part = threadIdx.x % LPR;
     const int b = a.plan.starts ? sequence_of(a.plan.starts, a.plan.B, t) : t;
     if (b == a.plan.B) return;  // padding
@@ -99,16 +101,18 @@ __global__ void __launch_bounds__(256)
     const Q8Total total = q8_total<R, GpuWave>(a.plan);
     const int first = q8_begin_of<R, GpuWave>(a.plan, b);
     const Q8Line<R> line(a.plan, s);
-    for (int h = blockIdx.y; h < a.H; h += gridDim.y) {
-        const int hk = a.plan.group_div(h);
-        const int r = (t - s.t0) * a.plan.group + (h - hk * a.plan.group);
+    for (int h0 = blockIdx.y * kRows; h0 < a.H; h0 += gridDim.y * kRows) {
+        const int h = h0 + slot / kWays;
+        const bool on = h < a.H;
+        const int hk = a.plan.group_div(on ? h : 0);
+        const int r = (t - s.t0) * a.plan.group + ((on ? h : 0) - hk * a.plan.group);
         const int tile = r / R;
         const Q8Parts parts =
             q8_parts(a.plan, total, first + line.begin(a.plan, s, tile),
                      Q8Line<R>::grains(a.plan, line.keys(a.plan, s, tile)));
-        if (parts.from == parts.to) continue;  // written already
+        const bool mine = on && parts.from != parts.to;  // else written already
         Q8Merge sum;
-        for (int p0 = parts.from + way; p0 <= parts.to; p0 += kBatch * kWays) {
+        for (int p0 = parts.from + way; mine && p0 <= parts.to; p0 += kBatch * kWays) {
             float2 v[kBatch];
             f32x4 x[kBatch];
 #pragma unroll
@@ -125,23 +129,27 @@ __global__ void __launch_bounds__(256)
             }
             sum.add(v, x);
         }
-        s_acc[threadIdx.x] = sum.acc;
-        if (part == 0) s_ml[way] = make_float2(sum.M, sum.l);
-        __syncthreads();
-        if (way == 0) {
-            float2 v[kWays];
-            f32x4 x[kWays];
+        if constexpr (kWays > 1) {
+            s_acc[threadIdx.x] = sum.acc;
+            if (part == 0) s_ml[slot] = make_float2(sum.M, sum.l);
+            __syncthreads();
+            if (way == 0) {
+                float2 v[kWays];
+                f32x4 x[kWays];
 #pragma unroll
-            for (int w = 0; w < kWays; ++w) {
-                v[w] = s_ml[w];
-                x[w] = s_acc[threadIdx.x + w * LPR];
+                for (int w = 0; w < kWays; ++w) {
+                    v[w] = s_ml[slot + w];
+                    x[w] = s_acc[threadIdx.x + w * LPR];
+                }
+                sum = Q8Merge();
+                sum.add(v, x);
             }
-            Q8Merge all;
-            all.add(v, x);
-            const size_t row = static_cast<size_t>(t) * a.H + h;
-            all.store<T>(O + row * D + 4 * part, L + row, part == 0);
         }
-        __syncthreads();  // before the next row's
+        if (mine && way == 0) {
+            const size_t row = static_cast<size_t>(t) * a.H + h;
+            sum.store<T>(O + row * D + 4 * part, L + row, part == 0);
+        }
+        if constexpr (kWays > 1) __syncthreads();  // before the next rows'
     }
 }
 
@@ -218,11 +226,12 @@ namespace detail {
 struct Q8Grid {
     int rows, shares;
     int least_shift;  // grains of at least 32 << least_shift keys
+    int least;        // such grains of a share
     int slot_rows;    // of a partial result
     int heads, kv_heads, head_dim, tokens;
 
-    Q8Grid(const PagedCall& c, int tile_rows, int parts, int shift)
-        : rows(tile_rows), shares(std::max(1, parts)), least_shift(shift), heads(c.num_heads),
+    Q8Grid(const PagedCall& c, int tile_rows, int parts, int shift, int grains)
+        : rows(tile_rows), shares(std::max(1, parts)), least_shift(shift), least(grains), heads(c.num_heads),
           kv_heads(c.num_kv_heads), head_dim(c.head_dim), tokens(c.num_tokens) {
         const long long group = c.num_heads / c.num_kv_heads;
         slot_rows = static_cast<int>(
@@ -247,11 +256,14 @@ struct Q8Grid {
         a.plan.causal = c.causal;
         a.plan.group_div = dev::fast_div(a.plan.group);
         dev::q8_set_grains(a.plan, rows, least_shift);
+        a.plan.least = least;
         a.block_table = c.block_table;
         a.H = c.num_heads;
         a.Hkv = c.num_kv_heads;
         a.page_size = c.page_size;
         a.max_pages = c.max_pages;
+        a.page_exps = static_cast<uint64_t>(c.page_size) * c.num_kv_heads;
+        a.page_bytes = a.page_exps * c.head_dim;
         a.page_div = dev::fast_div(c.page_size);
         a.c = c.scale * dev::kLog2e;
         a.slot_rows = slot_rows;
@@ -291,10 +303,19 @@ FlashAttentionError run_q8(const PagedCall& c, const Q8Grid& grid, hipStream_t s
                    static_cast<unsigned>(c.num_kv_heads),
                    static_cast<unsigned>((grid.slot_rows + dev::kMergeRows - 1) / dev::kMergeRows)));
     } else {
-        // Every workgroup finds its token's place first: with many tokens it takes all heads.
-        const int heads = std::min(c.num_heads, std::max(1, 8 * compute_units() / c.num_tokens));
-        merge(dev::combine_q8_kernel<T, D, R>,
-              dim3(static_cast<unsigned>(c.num_tokens), static_cast<unsigned>(heads)));
+        // Few rows have many parts each and want more loads in flight. Every workgroup finds its token's
+        // place first: with many tokens it takes several rounds of heads.
+        constexpr int kAll = 256 / (D / 4);
+        auto rows = [&](auto kernel, int at_once) {
+            const int rounds = (c.num_heads + at_once - 1) / at_once;
+            const int most = std::max(1, 8 * compute_units() / c.num_tokens);
+            merge(kernel, dim3(static_cast<unsigned>(c.num_tokens),
+                               static_cast<unsigned>(std::min(rounds, most))));
+        };
+        if (static_cast<long long>(c.num_tokens) * c.num_heads <= 512)
+            rows(dev::combine_q8_kernel<T, D, R, kAll>, 1);
+        else
+            rows(dev::combine_q8_kernel<T, D, R, kAll / 4>, 4);
     }
     return from_hip(hipGetLastError());
 }

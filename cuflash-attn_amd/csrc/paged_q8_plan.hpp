@@ -32,6 +32,7 @@ struct Q8PlanArgs {
     int shares;  // waves per key/value head
     int shift;   // a grain has 32 << shift keys
     int slack;   // grains between pairs
+    int least;   // grains of a share, where there are that many
     bool causal;
     FastDiv group_div;
 };
@@ -128,7 +129,7 @@ __host__ __device__ __forceinline__ Q8Total q8_total(const Q8PlanArgs& a) {
     // Only starts that decrease lead past what q8_shift() leaves room for; they are undefined, not unsafe.
     if (sum < 0 || sum > kQ8Line) sum = 0;
     const int share = (sum + (a.shares - 1)) / a.shares;
-    return {sum, share > 0 ? share : 1};
+    return {sum, share > a.least ? share : a.least};
 }
 
 // The sequence that has place x of the line (x < total), and where it begins.

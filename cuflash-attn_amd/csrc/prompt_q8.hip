@@ -13,10 +13,10 @@
 // late, and a barrier after each half holds them there:
 //   half 2 j:      waves 0-3  softmax of S_j                                  waves 4-7  products of step j
 //   half 2 j + 1:  waves 0-3  O += V_j^T P_j, S_{j+1} = K_{j+1} Q^T           waves 4-7  softmax of S_j
-// Products j read V_j and K_{j+1}, in the halves 2 j + 1 and 2 j + 2. A wave asks for its share of the pair
-// (V_i, K_{i+1}) before a softmax and puts it into LDS behind its next: waves 0-3 pair j in half 2 j, waves
-// 4-7 pair j + 1 in half 2 j + 1. Two buffers each are enough: V_{j+1} and K_{j+2}, written in half 2 j + 1 at
-// the earliest, take the place of V_{j-1} and K_j, last read in half 2 j.
+// Products j read V_j and K_{j+1}, in the halves 2 j + 1 and 2 j + 2. Behind its softmax a wave puts its share
+// of a later step's keys and values into LDS, waves 0-3 that of step j + 1 in half 2 j, waves 4-7 that of step
+// j + 2 in half 2 j + 1, and asks for the next, which has until the next softmax to arrive. K_{j+2} takes the
+// place of K_j, last read in half 2 j, and V_{j+2} that of V_{j-1}, too: two buffers for K and three for V.
 
 #include "attention_q8.hpp"
 #include "tile_groups.hpp"
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
     constexpr int P = 2 * D + 16;  // pitch of a staged row of O
     constexpr int kStage = kPromptRows * P;
     __shared__ __attribute__((aligned(1024))) unsigned char
-        smem[4 * kBytes > kStage ? 4 * kBytes : kStage];
+        smem[5 * kBytes > kStage ? 5 * kBytes : kStage];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31;
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
     // The items of a key/value head stay on one XCD where the heads can be dealt out evenly.
     int hk, share;
     head_rank_order(blockIdx.x, a.Hkv, hk, share);
-    const size_t pitch = static_cast<size_t>(a.Hkv) * D;
+    const uint32_t pitch = static_cast<uint32_t>(a.Hkv) * D;
 
     // This thread's codes of a step.
     const int my_key = 8 * wave + Tile::key(lane);
@@ -95,9 +95,6 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
     struct Codes {
         uint32_t w[kWords];
         uint32_t x;
-    };
-    struct Pair {
-        Codes v, k;
     };
     auto get = [](Codes& to, const uint8_t* codes, const uint8_t* exps, size_t row, size_t ex) {
         if constexpr (kWords == 4) {
@@ -169,34 +166,35 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
         // Steps in which this wave has keys to see.
         const int nw = wave_end > s.kbeg ? min(n, (wave_end - s.kbeg + kStep - 1) / kStep) : 0;
 
-        // The place of this thread's key of step j; of a step behind the last, and of keys behind the end,
-        // that of the last key. The table is read a step ahead.
+        // This thread's key of step j; for a step behind the last, and a key behind the end, the last key.
+        // The table is read a step ahead.
         auto key_of = [&](int j) { return min(s.kbeg + kStep * j + my_key, s.kend - 1); };
         int entry = table[a.page_div(key_of(0))];
-        auto place = [&](int j, size_t& at, size_t& ex) {
+        Codes k_codes, v_codes;
+        auto ask = [&](int j) {
             const int key = key_of(j);
-            const int in_page = key - a.page_div(key) * a.page_size;
-            at = (static_cast<size_t>(entry) * a.page_size + in_page) * pitch;
-            ex = static_cast<size_t>(entry) * a.Hkv * a.page_size + in_page;
+            const uint32_t in_page = key - a.page_div(key) * a.page_size;
+            const uint64_t row = static_cast<uint64_t>(static_cast<uint32_t>(entry)) *
+                                     static_cast<uint32_t>(a.page_size) +
+                                 in_page;
+            const uint64_t ex = static_cast<uint64_t>(static_cast<uint32_t>(entry)) *
+                                    static_cast<uint32_t>(a.Hkv) * a.page_size +
+                                in_page;
+            get(k_codes, k_src, kx_src, row * pitch, ex);
+            get(v_codes, v_src, vx_src, row * pitch, ex);
             entry = table[a.page_div(key_of(j + 1))];
         };
-        size_t v_at, v_ex, k_at, k_ex;  // of V_i; of K_{i+1}
-        auto ask = [&](int i, Pair& to) {
-            v_at = k_at;
-            v_ex = k_ex;
-            place(i + 1, k_at, k_ex);
-            get(to.v, v_src, vx_src, v_at, v_ex);
-            get(to.k, k_src, kx_src, k_at, k_ex);
-        };
-        auto give = [&](int i, Pair& from) {
+        int v_to = 2 * kBytes;  // buffer of the next values to give
+        auto give = [&](int j) {
             // Values behind the end may be anything: 0, as 0 times an infinity or a NaN would be seen.
-            if (s.kbeg + kStep * i + my_key >= s.kend) {
+            if (s.kbeg + kStep * j + my_key >= s.kend) {
 #pragma unroll
-                for (int w = 0; w < kWords; ++w) from.v.w[w] = 0;
-                from.v.x = 127;
+                for (int w = 0; w < kWords; ++w) v_codes.w[w] = 0;
+                v_codes.x = 127;
             }
-            turn(from.v, smem + 2 * kBytes + (i & 1) * kBytes + put);
-            turn(from.k, smem + ((i + 1) & 1) * kBytes + put);
+            turn(k_codes, smem + (j & 1) * kBytes + put);
+            turn(v_codes, smem + v_to + put);
+            v_to = v_to == 4 * kBytes ? 2 * kBytes : v_to + kBytes;
         };
 
         f32x16 o[NDT];
@@ -291,33 +289,29 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
             l += sum;
         };
 
-        // Pair -1 is K_0 alone. Every thread has asked for one pair more than it gave.
-        Codes first;
-        Pair pairs[2];
-        place(0, k_at, k_ex);
-        get(first, k_src, kx_src, k_at, k_ex);
-        ask(0, pairs[0]);
-        turn(first, smem + put);
+        ask(0);
+        give(0);
+        ask(1);
         if (late) {
-            ask(1, pairs[1]);
-            give(0, pairs[0]);
-            pairs[0] = pairs[1];
+            give(1);
+            ask(2);
         }
         barrier();
         scores(smem);
         if (late) barrier();
+        int vb = 2 * kBytes;  // buffer of V_j
         for (int j = 0; j < n; ++j) {
-            ask(j + 1 + late, pairs[1]);
             if (j < nw) softmax(j);
-            give(j + late, pairs[0]);
-            pairs[0] = pairs[1];
+            give(j + 1 + late);
+            ask(j + 2 + late);
             barrier();
             if (j < nw) {
                 __builtin_amdgcn_s_setprio(1);
-                products(smem + 2 * kBytes + (j & 1) * kBytes, smem + ((j + 1) & 1) * kBytes);
+                products(smem + vb, smem + ((j + 1) & 1) * kBytes);
                 __builtin_amdgcn_s_setprio(0);
             }
             barrier();
+            vb = vb == 4 * kBytes ? 2 * kBytes : vb + kBytes;
         }
         if (!late) barrier();  // as many as the others
 
@@ -383,7 +377,8 @@ Q8Grid grid_of(const PagedCall& c) {
                            (D * sizeof(float) + sizeof(float2));
     const long long fit = (static_cast<long long>(kStreamCacheBytes) / slot + 1) / 2;
     return Q8Grid(c, dev::kPromptRows,
-                  static_cast<int>(std::min<long long>(groups / c.num_kv_heads, fit)), 1);
+                  static_cast<int>(std::min<long long>(groups / c.num_kv_heads, fit)), 1,
+                  4);
 }
 
 template <typename T, int D, QuantCode C>

@@ -50,6 +50,17 @@ struct Q8<QuantCode::E4M3> {
             return __builtin_bit_cast(uint32_t,
                                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, f, i != 0));
     }
+    // All four, scaled or as they are.
+    template <typename M, bool kScaled>
+    static __device__ __forceinline__ u32x2 four(uint32_t codes, float f) {
+        return u32x2{expand<M, 0>(codes, kScaled ? f : 1.0f), expand<M, 1>(codes, kScaled ? f : 1.0f)};
+    }
+    // Codes 2 i and 2 i + 1 of two rows, scaled: the first ones as one pair, the second ones as another.
+    template <typename M, int i>
+    static __device__ __forceinline__ u32x2 turned(uint32_t a, float fa, uint32_t b, float fb) {
+        const uint32_t x = expand<M, i>(a, fa), y = expand<M, i>(b, fb);
+        return u32x2{__builtin_amdgcn_perm(y, x, 0x05040100u), __builtin_amdgcn_perm(y, x, 0x07060302u)};
+    }
     template <int i>
     static __device__ __forceinline__ f32x2 expand_f32(uint32_t codes, float f) {
         return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, f, i != 0);
@@ -70,18 +81,49 @@ struct Q8<QuantCode::INT8> {
         return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(0x38u, __uint_as_float(x << 23), false)[0];
     }
     template <int i>
-    static __device__ __forceinline__ float one(uint32_t codes, float f) {
-        return static_cast<float>(static_cast<int8_t>(codes >> (8 * i))) * f;
+    static __device__ __forceinline__ float plain(uint32_t codes) {
+        return static_cast<float>(static_cast<int8_t>(codes >> (8 * i)));
     }
-    template <typename M, int i>
-    static __device__ __forceinline__ uint32_t expand(uint32_t codes, float f) {
-        const float a = one<2 * i>(codes, f), b = one<2 * i + 1>(codes, f);
+    template <int i>
+    static __device__ __forceinline__ float one(uint32_t codes, float f) {
+        return plain<i>(codes) * f;
+    }
+    // Two numbers that M has (in fp16 rounded, where it has not).
+    template <typename M>
+    static __device__ __forceinline__ uint32_t pair(float a, float b) {
         if constexpr (std::is_same<M, __half>::value) {
             return Elem<__half>::pack2(a, b);
         } else {
             // The upper halves: what is cut off is 0.
             return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
         }
+    }
+    template <typename M, int i>
+    static __device__ __forceinline__ uint32_t expand(uint32_t codes, float f) {
+        return pair<M>(one<2 * i>(codes, f), one<2 * i + 1>(codes, f));
+    }
+    template <typename M, bool kScaled>
+    static __device__ __forceinline__ u32x2 four(uint32_t codes, float f) {
+        if constexpr (!kScaled && std::is_same<M, __half>::value) {
+            // code + 128 as the low byte of an fp16 number from 1024 on, whose steps are 1.
+            const f16x2 minus = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+            codes ^= 0x80808080u;
+            auto two = [&](uint32_t select) {
+                const uint32_t x = __builtin_amdgcn_perm(0x64646464u, codes, select);
+                return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, x) + minus);
+            };
+            return u32x2{two(0x04010400u), two(0x04030402u)};
+        } else if constexpr (!kScaled) {
+            return u32x2{pair<M>(plain<0>(codes), plain<1>(codes)),
+                         pair<M>(plain<2>(codes), plain<3>(codes))};
+        } else {
+            return u32x2{expand<M, 0>(codes, f), expand<M, 1>(codes, f)};
+        }
+    }
+    template <typename M, int i>
+    static __device__ __forceinline__ u32x2 turned(uint32_t a, float fa, uint32_t b, float fb) {
+        return u32x2{pair<M>(one<2 * i>(a, fa), one<2 * i>(b, fb)),
+                     pair<M>(one<2 * i + 1>(a, fa), one<2 * i + 1>(b, fb))};
     }
     template <int i>
     static __device__ __forceinline__ f32x2 expand_f32(uint32_t codes, float f) {

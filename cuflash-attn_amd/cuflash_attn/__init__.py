@@ -633,35 +633,36 @@ def flash_attention_decode_shared(q, k_cache, v_cache, prefix_table, prefix_len:
     return out, lse
 
 
+_Q8_CODES = _Q8_FLOATS = None
+
+
 def _check_q8(tensors, k_cache, v_cache, k_exp, v_exp, block_table, seq_lens, starts=None):
-    """What the calls on an 8-bit paged cache have in common (see _check_paged): codes [P, page, Hkv,
-    D] of one type, exponents [P, Hkv, page] uint8, and `tensors` of one floating type.
-    -> code, device, B, pages, page size, Hkv, D."""
+    """What the calls on an 8-bit paged cache have in common (as in _check_paged, with codes [P, page,
+    Hkv, D] of one type and exponents [P, Hkv, page] uint8): what is right is passed in one look at each
+    tensor. -> code, device, B, pages, page size, Hkv, D."""
+    global _Q8_CODES, _Q8_FLOATS
     torch = _torch()
+    if _Q8_CODES is None:
+        _Q8_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+        _Q8_FLOATS = {torch.float32, torch.float16, torch.bfloat16}
     device = torch.cuda.current_device()
-    code = {torch.int8: 0, torch.float8_e4m3fn: 1}.get(k_cache.dtype)
-    if code is None or v_cache.dtype != k_cache.dtype or k_exp.dtype != torch.uint8 \
-            or v_exp.dtype != torch.uint8:
-        raise TypeError("the caches must both be int8 or float8_e4m3fn, their exponents uint8")
-    if tensors:
-        _suffix(tensors[0])
+    kind, uint8, int32 = k_cache.dtype, torch.uint8, torch.int32
+    code = _Q8_CODES.get(kind)
     ints = (block_table, seq_lens) if starts is None else (block_table, seq_lens, starts)
-    whole = (k_cache, v_cache, k_exp, v_exp)
-    for t in (*tensors, *whole, *ints):
-        if t.get_device() != device:
-            raise ValueError("tensors must be on the GPU, on the current device")
-    for t in tensors:
-        if t.dtype != tensors[0].dtype:
-            raise ValueError("all tensors must share one dtype")
+    floating = tensors[0].dtype if tensors else torch.float32
+    good = (code is not None and v_cache.dtype is kind and k_exp.dtype is uint8
+            and v_exp.dtype is uint8 and floating in _Q8_FLOATS)
+    for t in (k_cache, v_cache, k_exp, v_exp):
+        if t.get_device() != device or not t.is_contiguous() or t.data_ptr() & 15:
+            good = False
     for t in ints:
-        if t.dtype != torch.int32:
-            raise TypeError("block_table, seq_lens and query_starts must be int32")
-    for t in (*whole, *ints):
-        if not t.is_contiguous():
-            raise ValueError("the caches, exponents and int32 tensors must be contiguous")
-    for t in (*tensors, *whole):
-        if t.data_ptr() & 15:
-            raise ValueError("tensors must start at a multiple of 16 bytes")
+        if t.get_device() != device or t.dtype is not int32 or not t.is_contiguous():
+            good = False
+    for t in tensors:
+        if t.get_device() != device or t.dtype is not floating or t.data_ptr() & 15:
+            good = False
+    if not good:
+        _refuse_q8(tensors, (k_cache, v_cache, k_exp, v_exp), ints, device)
     shape, B = k_cache.shape, block_table.shape[0]
     if len(shape) != 4 or v_cache.shape != shape \
             or k_exp.shape != (shape[0], shape[2], shape[1]) or v_exp.shape != k_exp.shape:
@@ -671,6 +672,24 @@ def _check_q8(tensors, k_cache, v_cache, k_exp, v_exp, block_table, seq_lens, st
     if starts is not None and starts.shape != (B + 1,):
         raise ValueError("expected starts [B+1]")
     return (code, device, B, *shape)
+
+
+def _refuse_q8(tensors, cache, ints, device):
+    torch = _torch()
+    if cache[0].dtype not in _Q8_CODES or cache[1].dtype != cache[0].dtype \
+            or any(t.dtype != torch.uint8 for t in cache[2:]):
+        raise TypeError("the caches must both be int8 or float8_e4m3fn, their exponents uint8")
+    if any(t.get_device() != device for t in (*tensors, *cache, *ints)):
+        raise ValueError("tensors must be on the GPU, on the current device")
+    if tensors:
+        _suffix(tensors[0])
+    if any(t.dtype != tensors[0].dtype for t in tensors):
+        raise ValueError("all tensors must share one dtype")
+    if any(t.dtype != torch.int32 for t in ints):
+        raise TypeError("block_table, seq_lens and query_starts must be int32")
+    if not all(t.is_contiguous() for t in (*cache, *ints)):
+        raise ValueError("the caches, exponents and int32 tensors must be contiguous")
+    raise ValueError("tensors must start at a multiple of 16 bytes")
 
 
 def flash_attention_append_paged_q8(k, v, k_cache, v_cache, k_exp, v_exp, block_table, seq_lens,

@@ -71,6 +71,7 @@ bool launch(std::mt19937& rng) {  // whether a tile was cut
     a.B = far ? 1 + pick(3) : std::array<int, 6>{1, 2, 7, 64, 65, 200}[pick(6)];
     a.cap = far ? 0x7fffffff - 1023 : spread(rng, 1, a.B > 10 ? 500 : 5000);
     a.shares = spread(rng, 1, 2048);
+    a.least = 1 + pick(3) * pick(4);
     const bool decode = pick(3) == 0;
     std::vector<int> lens, starts{0};
     const int most = far ? 6 : spread(rng, 1, a.B > 10 ? 20 : 300);
@@ -169,6 +170,7 @@ void disorder(std::mt19937& rng) {
     a.cap = 1 + pick(3000);
     a.T = 1 + pick(40);
     a.shares = 1 + pick(600);
+    a.least = 1 + pick(3);
     std::vector<int> lens, starts;
     for (int b = 0; b <= a.B; ++b) {
         lens.push_back(pick(2 * a.cap) - 5);
