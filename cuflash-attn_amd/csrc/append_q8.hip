@@ -255,7 +255,10 @@ __global__ void __launch_bounds__(1024)
         u32x4 codes = {0u, 0u, 0u, 0u};
         uint32_t x = 255;  // every code is NaN
         if (at.page >= 0) {
-            codes = ld16((is_v ? V_cache : K_cache) + at.code(a, head, D) + c);
+            // Read once: 69620 keys of 8 heads, head_dim 128, to fp16 98.9 -> 81.3 us with the hint, 5.3 TB/s
+            // (124 with one for the stores).
+            codes = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(
+                (is_v ? V_cache : K_cache) + at.code(a, head, D) + c));
             x = (is_v ? V_exp : K_exp)[at.exponent(a, head)];
         }
         const float f = Q8<C>::factor(x);

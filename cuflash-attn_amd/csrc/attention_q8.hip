@@ -251,8 +251,10 @@ struct AttentionQ8 {
         return Q8<C>::factor((four >> (8 * i)) & 0xffu);
     }
 
-    // The outputs of a segment's rows, or their partial results, those of wave p.
-    __device__ __forceinline__ void segment(const Q8Segment& g, const int* table, int p) const {
+    // The outputs of a segment's rows, or (slot >= 0) their partial results: part_of(r) says where those of row
+    // r of the tile go, D floats and (m, l).
+    template <class Part>
+    __device__ __forceinline__ void segment(const Q8Segment& g, const int* table, Part part_of) const {
         const Q8Seq& s = g.seq;
         const int kbeg = g.kbeg, kend = g.kend;
         const int lane = threadIdx.x & 63;
@@ -498,10 +500,9 @@ struct AttentionQ8 {
             if (orow[nr] < 0) continue;
             // Columns D / 4 q .. of the row, in order.
             if (g.slot >= 0) {
-                const size_t to = q8_slot_row(a, p, g.slot, hk, 16 * nr + l16);
-                float* dst = a.acc + to * D + q * (D / 4);
-                store(dst, o[nr], 1.0f);
-                if (q == 0) a.ml[to] = make_float2(m[nr], lt);
+                const auto part = part_of(16 * nr + l16);
+                store(part.acc + q * (D / 4), o[nr], 1.0f);
+                if (q == 0) *part.ml = make_float2(m[nr], lt);
                 continue;
             }
             const bool none = lt == 0.0f;  // no key, or every score -inf: O = 0, L = -inf
@@ -541,6 +542,10 @@ struct AttentionQ8 {
 // Of a workgroup, each for itself: the eight key/value heads of a common model then read their shares of the
 // cache's rows from one CU.
 constexpr int kQ8Waves = 8;
+struct Q8Part {
+    float* acc;
+    float2* ml;
+};
 
 template <typename T, int D, QuantCode C, int NR, bool kWhole>
 __global__ void __launch_bounds__((64 * kQ8Waves), 2)
@@ -567,7 +572,74 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
         hk};
     Q8Segment s;
     while (walk.next(a.plan, s))
-        work.segment(s, a.block_table + static_cast<size_t>(s.b) * a.max_pages, p);
+        work.segment(s, a.block_table + static_cast<size_t>(s.b) * a.max_pages, [&](int r) {
+            const size_t to = q8_slot_row(a, p, s.slot, hk, r);
+            return Q8Part{a.acc + to * D, a.ml + to};
+        });
+}
+
+// A decode from short tables in one launch: a workgroup has a tile of one sequence, each wave a piece of its keys,
+// and their parts are merged through LDS.
+template <typename T, int D, QuantCode C, int NR, bool kWhole>
+__global__ void __launch_bounds__((64 * kQ8Waves), 2)
+    decode_q8_short_kernel(const typename Mma<T>::elem* __restrict__ Q,
+                           const uint8_t* __restrict__ K, const uint8_t* __restrict__ V,
+                           const uint8_t* __restrict__ Kx, const uint8_t* __restrict__ Vx,
+                           typename Mma<T>::elem* __restrict__ O, float* __restrict__ L,
+                           AttentionQ8Args a) {
+    constexpr int R = 16 * NR;
+    constexpr int P = D + 4;  // floats from row to row
+    __shared__ __attribute__((aligned(16))) float s_acc[kQ8Waves][R][P];
+    __shared__ float2 s_ml[kQ8Waves][R];
+    const int tiles = (a.plan.group + R - 1) / R;
+    const int unit = blockIdx.x / tiles;
+    const int tile = blockIdx.x - unit * tiles;
+    const int b = unit / a.Hkv;
+    const int hk = unit - b * a.Hkv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const AttentionQ8<T, D, C, NR, kWhole> work{
+        a,
+        Q,
+        K + static_cast<size_t>(hk) * D,
+        V + static_cast<size_t>(hk) * D,
+        Kx + static_cast<size_t>(hk) * a.page_size,
+        Vx + static_cast<size_t>(hk) * a.page_size,
+        O,
+        L,
+        hk};
+    Q8Segment s;
+    s.seq = q8_seq(a.plan, b);
+    s.b = b;
+    s.rows = a.plan.group;
+    s.r0 = tile * R;
+    s.slot = 0;
+    const int blocks = (s.seq.keys + 31) / 32;
+    const int each = (blocks + kQ8Waves - 1) / kQ8Waves * 32;
+    s.kbeg = wave * each;
+    s.kend = min(s.kbeg + each, s.seq.keys);
+    if (s.kbeg < s.kend) {
+        work.segment(s, a.block_table + static_cast<size_t>(b) * a.max_pages,
+                     [&](int r) { return Q8Part{s_acc[wave][r], &s_ml[wave][r]}; });
+    } else if (lane < R) {
+        s_ml[wave][lane] = make_float2(-INFINITY, 0.0f);
+    }
+    __syncthreads();
+    constexpr int LPR = D / 4;
+    const int part = threadIdx.x % LPR;
+    for (int r = threadIdx.x / LPR; r < min(R, s.rows - s.r0); r += 64 * kQ8Waves / LPR) {
+        float2 v[kQ8Waves];
+        f32x4 x[kQ8Waves];
+#pragma unroll
+        for (int w = 0; w < kQ8Waves; ++w) {
+            v[w] = s_ml[w][r];
+            x[w] = __builtin_bit_cast(f32x4, ld16(&s_acc[w][r][4 * part]));
+        }
+        Q8Merge sum;
+        sum.add(v, x);
+        const size_t row = static_cast<size_t>(b) * a.H + hk * a.plan.group + s.r0 + r;
+        sum.store<T>(O + row * D + 4 * part, L + row, part == 0);
+    }
 }
 
 }  // namespace dev
@@ -597,6 +669,14 @@ Q8Grid waves_grid(const PagedCall& c) {
                   1);
 }
 
+// Decodes from tables of at most so many keys are one launch (bf16 over e4m3, 32 heads over 8, head_dim 128, us of
+// kernels in one and in two: one sequence of 500 keys 6.7 and 11.5, of 1000 9.8 and 12.1, of 2000 15.9 and 12.0; 64
+// of up to 500 13.5 and 17.4, of up to 1000 23.2 and 24.1, of up to 2000 37.7 and 33.0).
+constexpr long long kShortKeys = 1024;
+bool short_tables(const PagedCall& c) {
+    return !c.query_starts && static_cast<long long>(c.page_size) * c.max_pages <= kShortKeys;
+}
+
 template <typename T, int D, QuantCode C>
 FlashAttentionError run_attention(const PagedQ8Call& q8, hipStream_t stream) {
     using E = typename dev::Mma<T>::elem;
@@ -606,6 +686,30 @@ FlashAttentionError run_attention(const PagedQ8Call& q8, hipStream_t stream) {
     }
     const Q8Grid grid = waves_grid<T>(c);
     const bool whole = c.page_size % 16 == 0;  // half a block's rows lie on one page
+    if (short_tables(c)) {
+        auto run = [&](auto nr) {
+            constexpr int NR = decltype(nr)::value;
+            const long long groups = static_cast<long long>(c.batch_size) * c.num_kv_heads *
+                                     ((c.num_heads / c.num_kv_heads + 16 * NR - 1) / (16 * NR));
+            auto go = [&](auto kernel) {
+                launch_kernel(profile_kernel<T, D>("decode_q8_short"), kernel,
+                              dim3(static_cast<unsigned>(groups)), dim3(64 * dev::kQ8Waves), 0,
+                              stream, static_cast<const E*>(c.Q),
+                              static_cast<const uint8_t*>(c.K_cache),
+                              static_cast<const uint8_t*>(c.V_cache), q8.K_exp, q8.V_exp,
+                              static_cast<E*>(c.O), c.L, grid.args(c));
+            };
+            if (whole)
+                go(dev::decode_q8_short_kernel<T, D, C, NR, true>);
+            else
+                go(dev::decode_q8_short_kernel<T, D, C, NR, false>);
+            return from_hip(hipGetLastError());
+        };
+        if constexpr (!std::is_same<T, float>::value || D < 128) {
+            if (grid.rows == 32) return run(std::integral_constant<int, 2>{});
+        }
+        return run(std::integral_constant<int, 1>{});
+    }
     auto run = [&](auto nr) {
         constexpr int NR = decltype(nr)::value;
         return run_q8<T, D, 16 * NR>(c, grid, stream, [&](const dev::AttentionQ8Args& a) {

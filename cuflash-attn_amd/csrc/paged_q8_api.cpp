@@ -54,6 +54,9 @@ template <typename T>
 E attention_impl(const detail::PagedQ8Call& c, bool decode, hipStream_t stream) {
     const E err = check_cache(detail::check_attention(c.call, decode), c.K_exp, c.V_exp, c.code);
     if (err != E::SUCCESS) return err;
+    // The kernels' offsets in a page have 32 bits.
+    if (static_cast<long long>(c.call.page_size) * c.call.num_kv_heads > detail::kIntMax / c.call.head_dim)
+        return E::INVALID_DIMENSION;
     return detail::launch_paged_q8<T>(c, stream);
 }
 

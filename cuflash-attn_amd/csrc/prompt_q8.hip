@@ -13,10 +13,11 @@
 // late, and a barrier after each half holds them there:
 //   half 2 j:      waves 0-3  softmax of S_j                                  waves 4-7  products of step j
 //   half 2 j + 1:  waves 0-3  O += V_j^T P_j, S_{j+1} = K_{j+1} Q^T           waves 4-7  softmax of S_j
-// Products j read V_j and K_{j+1}, in the halves 2 j + 1 and 2 j + 2. Behind its softmax a wave puts its share
-// of a later step's keys and values into LDS, waves 0-3 that of step j + 1 in half 2 j, waves 4-7 that of step
-// j + 2 in half 2 j + 1, and asks for the next, which has until the next softmax to arrive. K_{j+2} takes the
-// place of K_j, last read in half 2 j, and V_{j+2} that of V_{j-1}, too: two buffers for K and three for V.
+// Products j read V_j and K_{j+1}, in the halves 2 j + 1 and 2 j + 2. Beside them, where its vector unit has
+// time, a wave turns its share of the keys and values of step j + 2 (behind the softmax, in the other half, this
+// took 3% longer), puts it into LDS and asks for the next.
+// K_{j+2} takes the place of K_j, last read in half 2 j, and V_{j+2} that of V_{j-1}, too: two buffers for K and
+// three for V.
 
 #include "attention_q8.hpp"
 #include "tile_groups.hpp"
@@ -56,7 +57,7 @@ struct PromptTile : TileGroups<D> {
 };
 
 template <typename T, int D, QuantCode C>
-__global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
+__global__ void __launch_bounds__((64 * kPromptWaves), (D == 32 ? 4 : 2))
     prompt_q8_kernel(const uint16_t* __restrict__ Q, const uint8_t* __restrict__ K,
                      const uint8_t* __restrict__ V, const uint8_t* __restrict__ Kx,
                      const uint8_t* __restrict__ Vx, uint16_t* __restrict__ O,
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
     const uint8_t* const v_src = V + static_cast<size_t>(hk) * D + my_part;
     const uint8_t* const kx_src = Kx + static_cast<size_t>(hk) * a.page_size;
     const uint8_t* const vx_src = Vx + static_cast<size_t>(hk) * a.page_size;
-    const int put = Tile::at(my_key, my_part);
+    const int put_at = Tile::at(my_key, my_part);
     struct Codes {
         uint32_t w[kWords];
         uint32_t x;
@@ -110,20 +111,27 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
         }
         to.x = exps[ex];
     };
-    auto turn = [&](const Codes& from, unsigned char* to) {
-        const float by = Q8<C>::factor(from.x);
+    struct Turned {
         uint32_t w[2 * kWords];
+    };
+    auto turn = [](const Codes& from) {
+        const float by = Q8<C>::factor(from.x);
+        Turned to;
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
-            w[2 * i] = Q8<C>::template expand<T, 0>(from.w[i], by);
-            w[2 * i + 1] = Q8<C>::template expand<T, 1>(from.w[i], by);
+            to.w[2 * i] = Q8<C>::template expand<T, 0>(from.w[i], by);
+            to.w[2 * i + 1] = Q8<C>::template expand<T, 1>(from.w[i], by);
         }
+        return to;
+    };
+    auto put = [&](const Turned& x, int buffer) {
+        unsigned char* to = smem + buffer + put_at;
         if constexpr (kWords == 1) {
-            st8(to, u32x2{w[0], w[1]});
+            st8(to, u32x2{x.w[0], x.w[1]});
         } else {
 #pragma unroll
             for (int i = 0; i < kWords; i += 2)
-                st16(to + 8 * i, u32x4{w[2 * i], w[2 * i + 1], w[2 * i + 2], w[2 * i + 3]});
+                st16(to + 8 * i, u32x4{x.w[2 * i], x.w[2 * i + 1], x.w[2 * i + 2], x.w[2 * i + 3]});
         }
     };
     const int k_base[2] = {Tile::row_base(lane, 0), Tile::row_base(lane, 1)};
@@ -135,6 +143,8 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
         __builtin_amdgcn_sched_barrier(0);
     };
 
+    const int step_pages = a.page_div(kStep);
+    const int step_rows = kStep - step_pages * a.page_size;
     Q8Walk<R, GpuWave> walk(a.plan, share);
     Q8Segment s;
     while (walk.next(a.plan, s)) {
@@ -166,35 +176,44 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
         // Steps in which this wave has keys to see.
         const int nw = wave_end > s.kbeg ? min(n, (wave_end - s.kbeg + kStep - 1) / kStep) : 0;
 
-        // This thread's key of step j; for a step behind the last, and a key behind the end, the last key.
-        // The table is read a step ahead.
-        auto key_of = [&](int j) { return min(s.kbeg + kStep * j + my_key, s.kend - 1); };
-        int entry = table[a.page_div(key_of(0))];
-        Codes k_codes, v_codes;
-        auto ask = [&](int j) {
-            const int key = key_of(j);
-            const uint32_t in_page = key - a.page_div(key) * a.page_size;
-            const uint64_t row = static_cast<uint64_t>(static_cast<uint32_t>(entry)) *
-                                     static_cast<uint32_t>(a.page_size) +
-                                 in_page;
-            const uint64_t ex = static_cast<uint64_t>(static_cast<uint32_t>(entry)) *
-                                    static_cast<uint32_t>(a.Hkv) * a.page_size +
-                                in_page;
-            get(k_codes, k_src, kx_src, row * pitch, ex);
-            get(v_codes, v_src, vx_src, row * pitch, ex);
-            entry = table[a.page_div(key_of(j + 1))];
+        // The place of this thread's key of the step to ask for, by walking from step to step (a division and its
+        // 64-bit products are an eighth of a step at head_dim 64); the table is read a step ahead. Behind the end it
+        // stands at the last key.
+        const int last = s.kend - 1;
+        const int last_index = a.page_div(last), last_row = last - last_index * a.page_size;
+        int key = s.kbeg + my_key;
+        int index = a.page_div(min(key, last));
+        int in_page = min(key, last) - index * a.page_size;
+        int entry = table[index];
+        struct Step {
+            Codes k, v;
         };
-        int v_to = 2 * kBytes;  // buffer of the next values to give
-        auto give = [&](int j) {
-            // Values behind the end may be anything: 0, as 0 times an infinity or a NaN would be seen.
+        auto ask = [&](Step& to) {
+            const uint64_t row = static_cast<uint64_t>(static_cast<uint32_t>(entry)) *
+                                     static_cast<uint32_t>(a.page_bytes) +
+                                 static_cast<uint32_t>(in_page) * pitch;
+            const uint64_t ex = static_cast<uint64_t>(static_cast<uint32_t>(entry)) *
+                                    static_cast<uint32_t>(a.page_exps) +
+                                static_cast<uint32_t>(in_page);
+            get(to.k, k_src, kx_src, row, ex);
+            get(to.v, v_src, vx_src, row, ex);
+            key += kStep;
+            in_page += step_rows;
+            const bool over = in_page >= a.page_size;
+            in_page -= over ? a.page_size : 0;
+            index += step_pages + (over ? 1 : 0);
+            const bool behind = key > last;
+            in_page = behind ? last_row : in_page;
+            index = behind ? last_index : index;
+            entry = table[index];
+        };
+        // Values behind the end may be anything: 0, as 0 times an infinity or a NaN would be seen.
+        auto cut = [&](int j, Step& x) {
             if (s.kbeg + kStep * j + my_key >= s.kend) {
 #pragma unroll
-                for (int w = 0; w < kWords; ++w) v_codes.w[w] = 0;
-                v_codes.x = 127;
+                for (int w = 0; w < kWords; ++w) x.v.w[w] = 0;
+                x.v.x = 127;
             }
-            turn(k_codes, smem + (j & 1) * kBytes + put);
-            turn(v_codes, smem + v_to + put);
-            v_to = v_to == 4 * kBytes ? 2 * kBytes : v_to + kBytes;
         };
 
         f32x16 o[NDT];
@@ -227,7 +246,9 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
         };
         // O += V^T P, then the next scores, in one chain. (Behind the last step these come from an old
         // tile and are not used.)
-        auto products = [&](const unsigned char* vt, const unsigned char* kt) {
+        auto products = [&](int v_from, int k_from) {
+            const unsigned char* vt = smem + v_from;
+            const unsigned char* kt = smem + k_from;
             Frag f[2 * kMma];
             auto frag_of = [&](int i) { return i < kMma ? v_frag(vt, i) : k_frag(kt, i - kMma); };
 #pragma unroll
@@ -289,29 +310,39 @@ __global__ void __launch_bounds__((64 * kPromptWaves), (D == 128 ? 2 : 4))
             l += sum;
         };
 
-        ask(0);
-        give(0);
-        ask(1);
-        if (late) {
-            give(1);
-            ask(2);
+        Step next;
+        {
+            Step first;
+            ask(first);
+            ask(next);
+            cut(0, first);
+            put(turn(first.k), 0);
+            put(turn(first.v), 2 * kBytes);
+            cut(1, next);
+            put(turn(next.k), kBytes);
+            put(turn(next.v), 3 * kBytes);
+            ask(next);
         }
         barrier();
         scores(smem);
         if (late) barrier();
-        int vb = 2 * kBytes;  // buffer of V_j
+        int v_from = 2 * kBytes, v_to = 4 * kBytes;  // buffers of V_j and V_{j+2}
         for (int j = 0; j < n; ++j) {
             if (j < nw) softmax(j);
-            give(j + 1 + late);
-            ask(j + 2 + late);
             barrier();
+            cut(j + 2, next);
+            const Turned k_next = turn(next.k), v_next = turn(next.v);
             if (j < nw) {
                 __builtin_amdgcn_s_setprio(1);
-                products(smem + vb, smem + ((j + 1) & 1) * kBytes);
+                products(v_from, ((j + 1) & 1) * kBytes);
                 __builtin_amdgcn_s_setprio(0);
             }
+            put(k_next, (j & 1) * kBytes);
+            put(v_next, v_to);
+            ask(next);
             barrier();
-            vb = vb == 4 * kBytes ? 2 * kBytes : vb + kBytes;
+            v_from = v_from == 4 * kBytes ? 2 * kBytes : v_from + kBytes;
+            v_to = v_to == 4 * kBytes ? 2 * kBytes : v_to + kBytes;
         }
         if (!late) barrier();  // as many as the others
 
@@ -372,7 +403,7 @@ namespace {
 template <int D>
 Q8Grid grid_of(const PagedCall& c) {
     // Workgroups that run at once, as far as their partial results fit the library's workspace of a stream.
-    const int groups = compute_units() * (D == 128 ? 1 : 2);
+    const int groups = compute_units() * (D == 32 ? 2 : 1);
     const long long slot = static_cast<long long>(c.num_kv_heads) * dev::kPromptRows *
                            (D * sizeof(float) + sizeof(float2));
     const long long fit = (static_cast<long long>(kStreamCacheBytes) / slot + 1) / 2;

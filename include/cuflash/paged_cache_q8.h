@@ -19,7 +19,7 @@
 //    The fp16 append writes none that is infinite.
 // Pages, tables, packed tokens, positions, padding, lengths, head_dim, head groups, alignment (of
 // the exponents' pointers too) and errors are as in cuflash/paged_cache.h; a QuantCode that is none is
-// UNSUPPORTED_DTYPE, found after null pointers.
+// UNSUPPORTED_DTYPE, found after null pointers, and a page of 2^31 bytes or more in an attention INVALID_DIMENSION.
 
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>

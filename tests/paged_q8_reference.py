@@ -108,7 +108,8 @@ class Q8Case:
         pages = sum(own) + 1
         rng = np.random.default_rng(seed)
         order = rng.permutation(pages)
-        self.table = np.full((B, self.max_pages), order[-1])
+        self.unused = order[-1]
+        self.table = np.full((B, self.max_pages), self.unused)
         at = 0
         for b in range(B):
             self.table[b, :own[b]] = order[at:at + own[b]]

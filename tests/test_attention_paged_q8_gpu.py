@@ -29,6 +29,19 @@ def queries(c, n, seed=9, std=1.0):
 
 
 def check_decode(c, scale=None, only=None):
+    """Twice: from a table of the sequences' length, and from one that is too long for a decode in one
+    launch."""
+    if c.max_pages * c.page <= 1024:
+        table = c.t_table
+        more = -(-1040 // c.page) - c.max_pages
+        c.t_table = c.ints(np.concatenate((c.table, np.repeat(c.table[:, :1] * 0 + c.unused, more, 1)), 1))
+        if (np.asarray(c.lens) <= c.max_pages * c.page).all():
+            _check_decode(c, scale, only)
+        c.t_table = table
+    _check_decode(c, scale, only)
+
+
+def _check_decode(c, scale, only):
     B = len(c.lens)
     x, q = queries(c, B)
     o, lse = decode(c, q.view(B, c.heads, 1, c.d), scale=scale)
@@ -102,6 +115,23 @@ def test_forward_of_prompts(torch_gpu, dtype, code, d, heads, kv_heads, page, ne
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,heads,kv_heads,page,new,lens", [
+    (64, 8, 8, 24, [700, 500, 2, 0, 60], [0, 120, 900, 40, 61]),
+    (128, 16, 2, 7, [600, 1, 1, 300], [650, 2000, 0, 299]),
+    (32, 24, 1, 16, [90, 257], [0, 100]), (128, 8, 8, 16, [1, 1100], [5, 1100])])
+def test_prompts_with_rows_that_see_no_key(torch_gpu, dtype, code, d, heads, kv_heads, page, new,
+                                           lens):
+    """So many rows that the merge goes by shares: empty sequences, more tokens than keys, tiles without a
+    key, single tokens between prompts, pages of any size."""
+    assert sum(new) * heads >= 8192
+    c = Q8Case(dtype, code, d, heads, kv_heads, page, lens)
+    check_forward(c, new, True, extra=3)
+    check_forward(c, new, False)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_lengths_past_the_table(torch_gpu, dtype):
     """A longer sequence is taken for as many keys as the table has."""
@@ -139,7 +169,8 @@ def test_small_and_large_rows(torch_gpu, dtype, code, std):
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_a_poisoned_row_reaches_those_that_see_it(torch_gpu, dtype):
     """x = 255 in a value row that one of two sequences has: NaN there, and only there. In a causal forward
-    at most the queries up to 30 tokens before it, whose block of 32 keys has it, may be NaN too."""
+    queries some tokens before it, whose block of keys has it, may be NaN too (up to 94; here the tokens of a
+    wave and the blocks begin at 192)."""
     torch = torch_gpu
     c = Q8Case(dtype, "int8", 64, 4, 2, 16, [300, 300])
     pg, row = c.places[1]
@@ -150,7 +181,7 @@ def test_a_poisoned_row_reaches_those_that_see_it(torch_gpu, dtype):
     assert bool(torch.isfinite(o[0]).all()) and bool(torch.isnan(o[1]).all())
     x, q = queries(c, 600)
     o, _ = forward(c, q, c.ints([0, 300, 600]), causal=True)
-    assert bool(torch.isfinite(o[:300 + 200 - 31]).all()) and bool(torch.isnan(o[500:]).all())
+    assert bool(torch.isfinite(o[:300 + 192]).all()) and bool(torch.isnan(o[500:]).all())
 
 
 @pytest.mark.gpu

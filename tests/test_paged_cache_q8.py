@@ -130,13 +130,15 @@ def test_attention_refusals(lib, sfx, kind, ok):
         assert call(scale=scale) == INVALID_DIMENSION
     assert call(kv_heads=3) == DIMENSION_MISMATCH
     assert call(page=1 << 16, max_pages=1 << 16) == INVALID_DIMENSION
+    assert call(page=1 << 24) == INVALID_DIMENSION  # a page of 2^31 bytes
     many = {"tokens": 1 << 28} if "tokens" in ok else {"batch": 1 << 28}
     assert call(**many) == INVALID_DIMENSION  # tokens times heads beyond 32 bits
     assert call(heads=65536) == INVALID_DIMENSION
     for name in ("q", "k_cache", "v_cache", "k_exp", "v_exp", "o"):
         assert call(**{name: P + 8}) == INVALID_DIMENSION, name
     assert call(ws=(P + 255) // 256 * 256 + 16, ws_bytes=1 << 30) == INVALID_DIMENSION
-    assert call(ws=(P + 255) // 256 * 256, ws_bytes=16) == OUT_OF_MEMORY
+    # (A decode from a short table has no workspace.)
+    assert call(ws=(P + 255) // 256 * 256, ws_bytes=16, max_pages=100) == OUT_OF_MEMORY
     assert call(k_exp=None, code=9, d=48) == NULL_POINTER
     assert call(code=9, heads=0) == UNSUPPORTED_DTYPE
     assert call(heads=0, d=48) == INVALID_DIMENSION
