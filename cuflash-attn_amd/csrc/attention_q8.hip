@@ -62,7 +62,7 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&to)[kParts])
     }
 }
 
-template <typename T, int D, QuantCode C, int NR, bool kWhole>
+template <typename T, int D, QuantCode C, int NR, int kPage>
 struct AttentionQ8 {
     using M = typename Q8Operand<T>::type;
     using E = typename Mma<T>::elem;
@@ -75,6 +75,7 @@ struct AttentionQ8 {
     static constexpr int VB = D / 16;                 // bytes of a lane's V codes of a key
     static constexpr int VW = VB >= 4 ? VB / 4 : 1;   // in dwords
     static constexpr int VT = VB;                     // tiles of O
+    static constexpr int kPitch = D + 4;              // floats from row to row in LDS
 
     const AttentionQ8Args& a;
     const E* Q;
@@ -86,18 +87,24 @@ struct AttentionQ8 {
     float* L;
     int hk;
 
+    // e4m3 codes are scaled as they are converted; for int8 codes that would be an instruction an element, so
+    // their scores are scaled instead.
+    static constexpr bool kScaleK = C == QuantCode::E4M3;
+    // The rows that surely lie on one page, from a multiple of their number on: of a page of 16 n rows those of
+    // half a block, found by one walk; of one of 4 n rows a lane's four keys.
+    static constexpr bool kWhole = kPage == 16, kFours = kPage >= 4;
+    static constexpr int XW = kFours ? 2 : 8;
     struct Codes {
         uint32_t k[2][KI][KB / 4];
         uint32_t v[8][VW];
-        uint32_t kx[2];  // the exponents of the lane's four keys of each half block (kScaleK: of its one)
-        uint32_t vx[2];
+        // The exponents of the lane's four keys of each half block, in one word or (!kFours) in one each;
+        // kScaleK: of its one key of each half.
+        uint32_t kx[kScaleK ? 2 : XW];
+        uint32_t vx[XW];
     };
     typedef const __attribute__((address_space(4))) int* ConstInts;
     // Two blocks in registers, or one, whose keys and then values give way to the next as they have been used.
     static constexpr bool kDouble = NR == 1 && kParts == 1;
-    // e4m3 codes are scaled as they are converted; for int8 codes that would be an instruction an element, so
-    // their scores are scaled instead.
-    static constexpr bool kScaleK = C == QuantCode::E4M3;
 
     template <int N>
     static __device__ __forceinline__ void copy(uint32_t (&to)[N], const uint8_t* from, int bytes) {
@@ -210,14 +217,25 @@ struct AttentionQ8 {
                 row_of(table, min(at.key0 + 16 * t + l16, kend - 1), row, ex);
 #pragma unroll
                 for (int i = 0; i < KI; ++i) copy(x.k[t][i], K + row + (q * KB + 64 * i), KB);
-                x.kx[t] = kScaleK ? Kx[ex] : 0;
-                if constexpr (!kScaleK) {
+                if constexpr (kScaleK)
+                    x.kx[t] = Kx[ex];
+                else
+                    load_x(at.key0 + 16 * t + 4 * q, table, kend, Kx, &x.kx[XW / 2 * t]);
+            }
+        }
+    }
+    // The exponents of keys key .. key + 3, where half a block is no walk.
+    __device__ __forceinline__ void load_x(int key, const int* table, int kend, const uint8_t* exps,
+                                           uint32_t* x) const {
+        uint64_t row, ex;
+        if constexpr (kFours) {
+            row_of(table, min(key, (kend - 1) & ~3), row, ex);
+            *x = *reinterpret_cast<const uint32_t*>(exps + ex);
+        } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        row_of(table, min(at.key0 + 16 * t + 4 * q + r, kend - 1), row, ex);
-                        x.kx[t] |= static_cast<uint32_t>(Kx[ex]) << (8 * r);
-                    }
-                }
+            for (int r = 0; r < 4; ++r) {
+                row_of(table, min(key + r, kend - 1), row, ex);
+                x[r] = exps[ex];
             }
         }
     }
@@ -236,25 +254,32 @@ struct AttentionQ8 {
                               VB);
                 x.vx[t] = *reinterpret_cast<const uint32_t*>(lane_at(Vx + at.ex[t], 4 * q));
             } else {
-                x.vx[t] = 0;
+                const int key = at.key0 + 16 * t + 4 * q;
+                uint64_t row, ex;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    uint64_t row, ex;
-                    row_of(table, min(at.key0 + 16 * t + 4 * q + r, kend - 1), row, ex);
-                    copy(x.v[4 * t + r], V + row + l16 * VB, VB);
-                    x.vx[t] |= static_cast<uint32_t>(Vx[ex]) << (8 * r);
+                    if (!kFours)
+                        row_of(table, min(key + r, kend - 1), row, ex);
+                    else if (r == 0)
+                        row_of(table, min(key, (kend - 1) & ~3), row, ex);
+                    copy(x.v[4 * t + r],
+                         V + row + (static_cast<uint64_t>(kFours ? r : 0) * pitch + l16 * VB), VB);
                 }
+                load_x(key, table, kend, Vx, &x.vx[XW / 2 * t]);
             }
         }
     }
-    static __device__ __forceinline__ float factor(uint32_t four, int i) {
-        return Q8<C>::factor((four >> (8 * i)) & 0xffu);
+    // Of key e of the lane's eight.
+    static __device__ __forceinline__ float factor(const uint32_t (&x)[XW], int e) {
+        return Q8<C>::factor(kFours ? (x[e >> 2] >> (8 * (e & 3))) & 0xffu : x[e]);
     }
 
-    // The outputs of a segment's rows, or (slot >= 0) their partial results: part_of(r) says where those of row
-    // r of the tile go, D floats and (m, l).
-    template <class Part>
-    __device__ __forceinline__ void segment(const Q8Segment& g, const int* table, Part part_of) const {
+    // The outputs of a segment's rows, or (slot >= 0) their partial results, those of row r of the tile D floats
+    // at acc_of(r) and (m, l) at ml_of(r). `stage`: 16 rows of the wave's in LDS; kKeep: R rows, and the partial
+    // results stay there.
+    template <bool kKeep, class Acc, class Ml>
+    __device__ __forceinline__ void segment(const Q8Segment& g, const int* table, float* stage,
+                                            Acc acc_of, Ml ml_of) const {
         const Q8Seq& s = g.seq;
         const int kbeg = g.kbeg, kend = g.kend;
         const int lane = threadIdx.x & 63;
@@ -346,7 +371,7 @@ struct AttentionQ8 {
                 if constexpr (!kScaleK) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float k_by = factor(x.kx[t], r);
+                        const float k_by = factor(x.kx, 4 * t + r);
 #pragma unroll
                         for (int nr = 0; nr < NR; ++nr) sc[nr][t][r] *= k_by;
                     }
@@ -409,7 +434,7 @@ struct AttentionQ8 {
             }
             float by[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) by[e] = factor(x.vx[e >> 2], e & 3);
+            for (int e = 0; e < 8; ++e) by[e] = factor(x.vx, e);
             // The codes of columns 2 j and 2 j + 1 of the lane's 8 keys: 8 pairs, turned.
             auto columns = [&](auto jc) {
                 constexpr int j = decltype(jc)::value;
@@ -446,8 +471,9 @@ struct AttentionQ8 {
                 const bool in = 16 * (e >> 2) + (e & 3) < n;
 #pragma unroll
                 for (int i = 0; i < VW; ++i) x.v[e][i] = in ? x.v[e][i] : 0u;
-                const uint32_t byte = 0xffu << (8 * (e & 3));
-                x.vx[e >> 2] = in ? x.vx[e >> 2] : (x.vx[e >> 2] & ~byte) | (0x7f7f7f7fu & byte);
+                const uint32_t byte = kFours ? 0xffu << (8 * (e & 3)) : 0xffu;
+                uint32_t& exps = x.vx[kFours ? e >> 2 : e];
+                exps = in ? exps : (exps & ~byte) | (0x7f7f7f7fu & byte);
             }
         };
 
@@ -494,47 +520,58 @@ struct AttentionQ8 {
         scores(last);
         values(last, key0);
 
+        // Rows leave through LDS, so that a store writes whole ones: from a lane's D / 4 columns it would write 16
+        // bytes of each of 64 lines (16 x 5 tokens of 8196 keys 57.4 -> 52.7 us).
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
             const float lt = quad_sum(l[nr]);
-            if (orow[nr] < 0) continue;
-            // Columns D / 4 q .. of the row, in order.
-            if (g.slot >= 0) {
-                const auto part = part_of(16 * nr + l16);
-                store(part.acc + q * (D / 4), o[nr], 1.0f);
-                if (q == 0) *part.ml = make_float2(m[nr], lt);
-                continue;
-            }
             const bool none = lt == 0.0f;  // no key, or every score -inf: O = 0, L = -inf
-            if (none) {
+            const bool part = kKeep || g.slot >= 0;
+            const float by = part ? 1.0f : none ? 0.0f : 1.0f / lt;
+            float* rows = stage + (kKeep ? 16 * nr * kPitch : 0);
+            // Columns (4 q + r) VT + j of the lane's row, in order.
 #pragma unroll
-                for (int j = 0; j < VT; ++j) o[nr][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < D / 4; i += 4) {
+                f32x4 w;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    w[u] = none && !part ? 0.0f : o[nr][(i + u) % VT][(i + u) / VT] * by;
+                st16(rows + l16 * kPitch + q * (D / 4) + i, __builtin_bit_cast(u32x4, w));
             }
-            store(O + static_cast<size_t>(orow[nr]) * D + q * (D / 4), o[nr],
-                  none ? 0.0f : 1.0f / lt);
-            if (q == 0) L[orow[nr]] = none ? -INFINITY : (m[nr] + fast_log2(lt)) * kLn2;
-        }
-    }
-
-    // A lane's D / 4 columns: (4 q + r) VT + j.
-    static __device__ __forceinline__ void store(float* dst, const f32x4 (&o)[VT], float by) {
+            if (part) {
+                if (q == 0 && orow[nr] >= 0) *ml_of(16 * nr + l16) = make_float2(m[nr], lt);
+            } else if (q == 0 && orow[nr] >= 0) {
+                L[orow[nr]] = none ? -INFINITY : (m[nr] + fast_log2(lt)) * kLn2;
+            }
+            if constexpr (kKeep) continue;
+            asm volatile("" ::: "memory");  // a wave's LDS accesses are performed in order
+            constexpr int VEC = 16 / static_cast<int>(sizeof(E));
+            if (part) {
 #pragma unroll
-        for (int i = 0; i < D / 4; i += 4) {
-            f32x4 w;
+                for (int i = 0; i < D / 16; ++i) {
+                    const int r = (64 * i + lane) / (D / 4), c = (64 * i + lane) % (D / 4) * 4;
+                    if (g.r0 + 16 * nr + r < g.rows)
+                        st16(acc_of(16 * nr + r) + c, ld16(rows + r * kPitch + c));
+                }
+            } else {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) w[u] = o[(i + u) % VT][(i + u) / VT] * by;
-            st16(dst + i, __builtin_bit_cast(u32x4, w));
-        }
-    }
-    static __device__ __forceinline__ void store(uint16_t* dst, const f32x4 (&o)[VT], float by) {
-#pragma unroll
-        for (int i = 0; i < D / 4; i += 8) {
-            u32x4 w;
-#pragma unroll
-            for (int u = 0; u < 8; u += 2)
-                w[u / 2] = Elem<M>::pack2(o[(i + u) % VT][(i + u) / VT] * by,
-                                          o[(i + u + 1) % VT][(i + u + 1) / VT] * by);
-            st16(dst + i, w);
+                for (int i = 0; i < 16 * (D / VEC) / 64; ++i) {
+                    const int r = (64 * i + lane) / (D / VEC), c = (64 * i + lane) % (D / VEC) * VEC;
+                    const int to = __shfl(orow[nr], r, 64);
+                    if (to < 0) continue;
+                    const f32x4 x = __builtin_bit_cast(f32x4, ld16(rows + r * kPitch + c));
+                    u32x4 w;
+                    if constexpr (VEC == 4) {
+                        w = __builtin_bit_cast(u32x4, x);
+                    } else {
+                        const f32x4 y = __builtin_bit_cast(f32x4, ld16(rows + r * kPitch + c + 4));
+                        w = u32x4{Elem<M>::pack2(x[0], x[1]), Elem<M>::pack2(x[2], x[3]),
+                                  Elem<M>::pack2(y[0], y[1]), Elem<M>::pack2(y[2], y[3])};
+                    }
+                    st16(O + static_cast<size_t>(to) * D + c, w);
+                }
+            }
+            asm volatile("" ::: "memory");
         }
     }
 };
@@ -542,12 +579,8 @@ struct AttentionQ8 {
 // Of a workgroup, each for itself: the eight key/value heads of a common model then read their shares of the
 // cache's rows from one CU.
 constexpr int kQ8Waves = 8;
-struct Q8Part {
-    float* acc;
-    float2* ml;
-};
 
-template <typename T, int D, QuantCode C, int NR, bool kWhole>
+template <typename T, int D, QuantCode C, int NR, int kPage>
 __global__ void __launch_bounds__((64 * kQ8Waves), 2)
     attention_q8_kernel(const typename Mma<T>::elem* __restrict__ Q,
                         const uint8_t* __restrict__ K, const uint8_t* __restrict__ V,
@@ -559,8 +592,10 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
     const int p = wave / a.Hkv;
     const int hk = wave - p * a.Hkv;
     if (p >= a.plan.shares) return;
+    using Work = AttentionQ8<T, D, C, NR, kPage>;
+    __shared__ __attribute__((aligned(16))) float s_rows[kQ8Waves][16 * Work::kPitch];
     Q8Walk<R, GpuWave> walk(a.plan, p);
-    const AttentionQ8<T, D, C, NR, kWhole> work{
+    const Work work{
         a,
         Q,
         K + static_cast<size_t>(hk) * D,
@@ -571,16 +606,18 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
         L,
         hk};
     Q8Segment s;
-    while (walk.next(a.plan, s))
-        work.segment(s, a.block_table + static_cast<size_t>(s.b) * a.max_pages, [&](int r) {
-            const size_t to = q8_slot_row(a, p, s.slot, hk, r);
-            return Q8Part{a.acc + to * D, a.ml + to};
-        });
+    while (walk.next(a.plan, s)) {
+        auto row = [&](int r) { return q8_slot_row(a, p, s.slot, hk, r); };
+        work.template segment<false>(
+            s, a.block_table + static_cast<size_t>(s.b) * a.max_pages,
+            s_rows[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)],
+            [&](int r) { return a.acc + row(r) * D; }, [&](int r) { return a.ml + row(r); });
+    }
 }
 
 // A decode from short tables in one launch: a workgroup has a tile of one sequence, each wave a piece of its keys,
 // and their parts are merged through LDS.
-template <typename T, int D, QuantCode C, int NR, bool kWhole>
+template <typename T, int D, QuantCode C, int NR, int kPage>
 __global__ void __launch_bounds__((64 * kQ8Waves), 2)
     decode_q8_short_kernel(const typename Mma<T>::elem* __restrict__ Q,
                            const uint8_t* __restrict__ K, const uint8_t* __restrict__ V,
@@ -588,8 +625,8 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
                            typename Mma<T>::elem* __restrict__ O, float* __restrict__ L,
                            AttentionQ8Args a) {
     constexpr int R = 16 * NR;
-    constexpr int P = D + 4;  // floats from row to row
-    __shared__ __attribute__((aligned(16))) float s_acc[kQ8Waves][R][P];
+    using Work = AttentionQ8<T, D, C, NR, kPage>;
+    __shared__ __attribute__((aligned(16))) float s_acc[kQ8Waves][R][Work::kPitch];
     __shared__ float2 s_ml[kQ8Waves][R];
     const int tiles = (a.plan.group + R - 1) / R;
     const int unit = blockIdx.x / tiles;
@@ -598,7 +635,7 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
     const int hk = unit - b * a.Hkv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    const AttentionQ8<T, D, C, NR, kWhole> work{
+    const Work work{
         a,
         Q,
         K + static_cast<size_t>(hk) * D,
@@ -619,8 +656,9 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
     s.kbeg = wave * each;
     s.kend = min(s.kbeg + each, s.seq.keys);
     if (s.kbeg < s.kend) {
-        work.segment(s, a.block_table + static_cast<size_t>(b) * a.max_pages,
-                     [&](int r) { return Q8Part{s_acc[wave][r], &s_ml[wave][r]}; });
+        work.template segment<true>(
+            s, a.block_table + static_cast<size_t>(b) * a.max_pages, s_acc[wave][0],
+            [&](int r) { return s_acc[wave][r]; }, [&](int r) { return &s_ml[wave][r]; });
     } else if (lane < R) {
         s_ml[wave][lane] = make_float2(-INFINITY, 0.0f);
     }
@@ -647,13 +685,17 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
 namespace detail {
 namespace {
 
-// Where most sequences have more rows than this, workgroups share the keys (prompt_q8.hip).
-constexpr long long kManyRows = 96;
+// Where sequences have more rows than this, 16-bit ones, workgroups share the keys (prompt_q8.hip): on average 48 a
+// sequence, 96 at head_dim 64 and 32, 16 for a single sequence, whose waves would have few blocks each and leave as
+// many partial results (bf16 over e4m3, us of kernels by waves and by workgroups; head_dim 128, 32 heads over 8: 16
+// sequences of 4000 keys, 32 rows each 41 and 61, 48 rows 63 and 66, 64 rows 80 and 67; one of 8000 keys, 32 rows 29
+// and 20; head_dim 64 over 4, 16 of 4000 keys: 96 rows 33 and 36, 128 rows 41 and 38).
 template <typename T>
 bool many_rows(const PagedCall& c) {
+    const long long most = c.batch_size == 1 ? 16 : c.head_dim == 128 ? 48 : 96;
     return !std::is_same<T, float>::value && c.query_starts &&
            static_cast<long long>(c.num_tokens) * (c.num_heads / c.num_kv_heads) >
-               kManyRows * c.batch_size;
+               most * c.batch_size;
 }
 
 // Tiles of 16 rows, or of 32 where sequences have more and registers suffice (float queries of 128 elements
@@ -685,7 +727,15 @@ FlashAttentionError run_attention(const PagedQ8Call& q8, hipStream_t stream) {
         if constexpr (!std::is_same<T, float>::value) return launch_prompt_q8<T>(q8, stream);
     }
     const Q8Grid grid = waves_grid<T>(c);
-    const bool whole = c.page_size % 16 == 0;  // half a block's rows lie on one page
+    // go(n) with n rows that lie on one page.
+    auto by_page = [&](auto go) {
+        if (c.page_size % 16 == 0)
+            go(std::integral_constant<int, 16>{});
+        else if (c.page_size % 4 == 0)
+            go(std::integral_constant<int, 4>{});
+        else
+            go(std::integral_constant<int, 1>{});
+    };
     if (short_tables(c)) {
         auto run = [&](auto nr) {
             constexpr int NR = decltype(nr)::value;
@@ -699,10 +749,9 @@ FlashAttentionError run_attention(const PagedQ8Call& q8, hipStream_t stream) {
                               static_cast<const uint8_t*>(c.V_cache), q8.K_exp, q8.V_exp,
                               static_cast<E*>(c.O), c.L, grid.args(c));
             };
-            if (whole)
-                go(dev::decode_q8_short_kernel<T, D, C, NR, true>);
-            else
-                go(dev::decode_q8_short_kernel<T, D, C, NR, false>);
+            by_page([&](auto page) {
+                go(dev::decode_q8_short_kernel<T, D, C, NR, decltype(page)::value>);
+            });
             return from_hip(hipGetLastError());
         };
         if constexpr (!std::is_same<T, float>::value || D < 128) {
@@ -724,10 +773,9 @@ FlashAttentionError run_attention(const PagedQ8Call& q8, hipStream_t stream) {
                               static_cast<const uint8_t*>(c.V_cache), q8.K_exp, q8.V_exp,
                               static_cast<E*>(c.O), c.L, a);
             };
-            if (whole)
-                go(dev::attention_q8_kernel<T, D, C, NR, true>);
-            else
-                go(dev::attention_q8_kernel<T, D, C, NR, false>);
+            by_page([&](auto page) {
+                go(dev::attention_q8_kernel<T, D, C, NR, decltype(page)::value>);
+            });
         });
     };
     if constexpr (!std::is_same<T, float>::value || D < 128) {

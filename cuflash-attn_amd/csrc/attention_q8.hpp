@@ -81,15 +81,15 @@ struct Q8Merge {
 
 // The merge, row by row: one workgroup per token and gridDim.y-th part of its heads. D / 4 lanes have a row,
 // and kWays groups of them every kWays-th part of it; they are merged through LDS in order.
-template <typename T, int D, int R, int kWays>
-__global__ void __launch_bounds__(256)
+template <typename T, int D, int R, int kWays, int kThreads>
+__global__ void __launch_bounds__(kThreads)
     combine_q8_kernel(typename Mma<T>::elem* __restrict__ O, float* __restrict__ L,
                       AttentionQ8Args a) {
     constexpr int LPR = D / 4;
-    constexpr int kRows = 256 / LPR / kWays;  // at a time
+    constexpr int kRows = kThreads / LPR / kWays;  // at a time
     constexpr int kBatch = 4;
-    __shared__ f32x4 s_acc[256];
-    __shared__ float2 s_ml[256 / LPR];
+    __shared__ f32x4 s_acc[kThreads];
+    __shared__ float2 s_ml[kThreads / LPR];
     const int t = blockIdx.x;
     const int slot = threadIdx.x / LPR;
     const int way = slot % kWays;
@@ -134,15 +134,18 @@ __global__ void __launch_bounds__(256)
             if (part == 0) s_ml[slot] = make_float2(sum.M, sum.l);
             __syncthreads();
             if (way == 0) {
-                float2 v[kWays];
-                f32x4 x[kWays];
-#pragma unroll
-                for (int w = 0; w < kWays; ++w) {
-                    v[w] = s_ml[slot + w];
-                    x[w] = s_acc[threadIdx.x + w * LPR];
-                }
                 sum = Q8Merge();
-                sum.add(v, x);
+                constexpr int kAtOnce = kWays < 4 ? kWays : 4;
+                for (int w0 = 0; w0 < kWays; w0 += kAtOnce) {
+                    float2 v[kAtOnce];
+                    f32x4 x[kAtOnce];
+#pragma unroll
+                    for (int w = 0; w < kAtOnce; ++w) {
+                        v[w] = s_ml[slot + w0 + w];
+                        x[w] = s_acc[threadIdx.x + (w0 + w) * LPR];
+                    }
+                    sum.add(v, x);
+                }
             }
         }
         if (mine && way == 0) {
@@ -163,6 +166,7 @@ __global__ void __launch_bounds__(256)
                     AttentionQ8Args a) {
     constexpr int LPR = D / 4;
     constexpr int kRows = 256 / LPR;  // at a time
+    constexpr int kBatch = 4;
     const int hk = blockIdx.y;
     const int part = threadIdx.x % LPR;
     auto row_of = [&](const Q8Seq& s, int r) {
@@ -197,11 +201,11 @@ __global__ void __launch_bounds__(256)
     const int rows = min(min(line.rows - tile * R, R), z + kMergeRows);
     for (int r = z + threadIdx.x / LPR; r < rows; r += kRows) {
         Q8Merge sum;
-        for (int p0 = parts.from; p0 <= parts.to; p0 += 2) {
-            float2 v[2];
-            f32x4 x[2];
+        for (int p0 = parts.from; p0 <= parts.to; p0 += kBatch) {
+            float2 v[kBatch];
+            f32x4 x[kBatch];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < kBatch; ++i) {
                 v[i] = make_float2(-INFINITY, 0.0f);
                 x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 if (p0 + i <= parts.to) {
@@ -293,29 +297,35 @@ FlashAttentionError run_q8(const PagedCall& c, const Q8Grid& grid, hipStream_t s
     attend(a);
     const FlashAttentionError err = from_hip(hipGetLastError());
     if (err != FlashAttentionError::SUCCESS) return err;
-    auto merge = [&](auto kernel, dim3 groups) {
-        launch_kernel(profile_kernel<T, D>("combine_q8"), kernel, groups, dim3(256), 0, stream,
-                      static_cast<E*>(c.O), c.L, a);
+    auto merge = [&](auto kernel, dim3 groups, int threads) {
+        launch_kernel(profile_kernel<T, D>("combine_q8"), kernel, groups,
+                      dim3(static_cast<unsigned>(threads)), 0, stream, static_cast<E*>(c.O), c.L, a);
     };
     if (grid.by_share()) {
         merge(dev::merge_q8_kernel<T, D, R>,
               dim3(static_cast<unsigned>(grid.shares + std::min(c.batch_size, 64)),
                    static_cast<unsigned>(c.num_kv_heads),
-                   static_cast<unsigned>((grid.slot_rows + dev::kMergeRows - 1) / dev::kMergeRows)));
+                   static_cast<unsigned>((grid.slot_rows + dev::kMergeRows - 1) / dev::kMergeRows)),
+              256);
     } else {
-        // Few rows have many parts each and want more loads in flight. Every workgroup finds its token's
-        // place first: with many tokens it takes several rounds of heads.
-        constexpr int kAll = 256 / (D / 4);
-        auto rows = [&](auto kernel, int at_once) {
+        // Few rows have many parts each and want more loads in flight: 32 rows of 256 parts 11.1 us with 256
+        // threads a row, 7.8 with 1024 (of 32 parts 4.2 and 5.9); 2048 rows of 5 parts 7.7 with 256, 4.7 with 64.
+        // Every workgroup finds its token's place first: with many tokens it takes several rounds of heads.
+        auto rows = [&](auto kernel, int at_once, int threads) {
             const int rounds = (c.num_heads + at_once - 1) / at_once;
             const int most = std::max(1, 8 * compute_units() / c.num_tokens);
-            merge(kernel, dim3(static_cast<unsigned>(c.num_tokens),
-                               static_cast<unsigned>(std::min(rounds, most))));
+            merge(kernel,
+                  dim3(static_cast<unsigned>(c.num_tokens),
+                       static_cast<unsigned>(std::min(rounds, most))),
+                  threads);
         };
-        if (static_cast<long long>(c.num_tokens) * c.num_heads <= 512)
-            rows(dev::combine_q8_kernel<T, D, R, kAll>, 1);
+        const long long all = static_cast<long long>(c.num_tokens) * c.num_heads;
+        if (all <= 256 && a.plan.cap >= 2048)
+            rows(dev::combine_q8_kernel<T, D, R, 1024 / (D / 4), 1024>, 1, 1024);
+        else if (all <= 1024)
+            rows(dev::combine_q8_kernel<T, D, R, 256 / (D / 4), 256>, 1, 256);
         else
-            rows(dev::combine_q8_kernel<T, D, R, kAll / 4>, 4);
+            rows(dev::combine_q8_kernel<T, D, R, 256 / D, 256>, 4, 256);
     }
     return from_hip(hipGetLastError());
 }

@@ -72,7 +72,8 @@ enum class QuantCode : int { INT8 = 0, E4M3 = 1 };
 // captured call needs the caller's, of the size that the *_workspace_* functions return, and is refused
 // without one (OUT_OF_MEMORY).
 // float queries take part as three bf16 numbers each, and so do the softmax's weights before they meet
-// V: what is lost is below float's own rounding, at five times the rate of the float matrix products.
+// V: what is lost is below float's own rounding, at more than the rate of the float matrix products (184 to 227
+// TFLOP/s in prompts of 4096 tokens, where a large product of float matrices runs at 151).
 #define CUFLASH_Q8_DECODE(T)                                                                      \
     CUFLASH_EXPORT FlashAttentionError flash_attention_decode_paged_q8(                           \
         const T* Q, const void* K_cache, const void* V_cache, const uint8_t* K_exp,               \
