@@ -2,8 +2,9 @@
 // flash_attention_forward_paged_q8 (cuflash/paged_cache_q8.h).
 //
 // attention_q8_kernel: a wave takes an equal share of all keys of all tiles of rows (paged_q8_plan.hpp),
-// by itself: no LDS, no barrier. Tiles have 16 or 32 rows, the query heads of one key/value head over a few
-// tokens, so that a key is read once for all of them. Blocks of 32 keys, in 16 x 16 x 32 products:
+// by itself, without a barrier: keys and values go from memory to registers, and LDS only turns results into
+// whole rows. Tiles have 16 or 32 rows, the query heads of one key/value head over a few tokens, so that a key
+// is read once for all of them. Blocks of 32 keys, in 16 x 16 x 32 products:
 //   S^T = K Q^T   A: lane l has key l % 16 of a half block, of its codes the 16 bytes at 64 i + 16 (l / 16):
 //                 two k-steps from one load; Q is laid out alike. C: lane l has row l % 16 and the keys
 //                 4 (l / 16) + r of both halves, 8 in all.
@@ -14,10 +15,13 @@
 // float, the weights are rounded to T before they meet V (half a step, 2^-8 of p |v| in bf16, as in the
 // library's other matrix-core kernels), float ones taken apart into three bf16 numbers without a loss.
 // Codes of the next block are asked for before this one is worked on, or where registers are short as
-// its own have been used. The waves of neighbouring key/value
-// heads have the same share and so read the same cache rows at the same time.
-// combine_q8_kernel (attention_q8.hpp) merges the rows that several waves have and writes those without a
-// key. Where sequences have many 16-bit rows prompt_q8.hip takes over.
+// its own have been used. The waves of neighbouring key/value heads have the same share and so read the same
+// cache rows at the same time.
+// combine_q8_kernel or merge_q8_kernel (attention_q8.hpp) merges the rows that several waves have and writes those
+// without a key; a decode from short tables is one launch, decode_q8_short_kernel. Where sequences have many 16-bit
+// rows prompt_q8.hip takes over.
+// Bound by HBM: bf16 over int8, 4 sequences of up to 131072 keys, 32 heads over 8, head_dim 128, 169 us (6.4 TB/s; a
+// 1 GiB copy reaches 5.1), fp16, 64 sequences of up to 8192 keys 91 (6.0), 16 x 5 tokens of 8196 keys 53 (5.2).
 
 #include "attention_q8.hpp"
 
@@ -628,55 +632,59 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
     using Work = AttentionQ8<T, D, C, NR, kPage>;
     __shared__ __attribute__((aligned(16))) float s_acc[kQ8Waves][R][Work::kPitch];
     __shared__ float2 s_ml[kQ8Waves][R];
-    const int tiles = (a.plan.group + R - 1) / R;
-    const int unit = blockIdx.x / tiles;
-    const int tile = blockIdx.x - unit * tiles;
-    const int b = unit / a.Hkv;
-    const int hk = unit - b * a.Hkv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    const Work work{
-        a,
-        Q,
-        K + static_cast<size_t>(hk) * D,
-        V + static_cast<size_t>(hk) * D,
-        Kx + static_cast<size_t>(hk) * a.page_size,
-        Vx + static_cast<size_t>(hk) * a.page_size,
-        O,
-        L,
-        hk};
-    Q8Segment s;
-    s.seq = q8_seq(a.plan, b);
-    s.b = b;
-    s.rows = a.plan.group;
-    s.r0 = tile * R;
-    s.slot = 0;
-    const int blocks = (s.seq.keys + 31) / 32;
-    const int each = (blocks + kQ8Waves - 1) / kQ8Waves * 32;
-    s.kbeg = wave * each;
-    s.kend = min(s.kbeg + each, s.seq.keys);
-    if (s.kbeg < s.kend) {
-        work.template segment<true>(
-            s, a.block_table + static_cast<size_t>(b) * a.max_pages, s_acc[wave][0],
-            [&](int r) { return s_acc[wave][r]; }, [&](int r) { return &s_ml[wave][r]; });
-    } else if (lane < R) {
-        s_ml[wave][lane] = make_float2(-INFINITY, 0.0f);
-    }
-    __syncthreads();
-    constexpr int LPR = D / 4;
-    const int part = threadIdx.x % LPR;
-    for (int r = threadIdx.x / LPR; r < min(R, s.rows - s.r0); r += 64 * kQ8Waves / LPR) {
-        float2 v[kQ8Waves];
-        f32x4 x[kQ8Waves];
-#pragma unroll
-        for (int w = 0; w < kQ8Waves; ++w) {
-            v[w] = s_ml[w][r];
-            x[w] = __builtin_bit_cast(f32x4, ld16(&s_acc[w][r][4 * part]));
+    const int tiles = (a.plan.group + R - 1) / R;
+    const uint32_t items = static_cast<uint32_t>(a.plan.B) * a.Hkv * tiles;  // at most B H, below 2^31
+    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int unit = item / tiles;
+        const int tile = item - unit * tiles;
+        const int b = unit / a.Hkv;
+        const int hk = unit - b * a.Hkv;
+        const Work work{
+            a,
+            Q,
+            K + static_cast<size_t>(hk) * D,
+            V + static_cast<size_t>(hk) * D,
+            Kx + static_cast<size_t>(hk) * a.page_size,
+            Vx + static_cast<size_t>(hk) * a.page_size,
+            O,
+            L,
+            hk};
+        Q8Segment s;
+        s.seq = q8_seq(a.plan, b);
+        s.b = b;
+        s.rows = a.plan.group;
+        s.r0 = tile * R;
+        s.slot = 0;
+        const int blocks = (s.seq.keys + 31) / 32;
+        const int each = (blocks + kQ8Waves - 1) / kQ8Waves * 32;
+        s.kbeg = wave * each;
+        s.kend = min(s.kbeg + each, s.seq.keys);
+        if (s.kbeg < s.kend) {
+            work.template segment<true>(
+                s, a.block_table + static_cast<size_t>(b) * a.max_pages, s_acc[wave][0],
+                [&](int r) { return s_acc[wave][r]; }, [&](int r) { return &s_ml[wave][r]; });
+        } else if (lane < R) {
+            s_ml[wave][lane] = make_float2(-INFINITY, 0.0f);
         }
-        Q8Merge sum;
-        sum.add(v, x);
-        const size_t row = static_cast<size_t>(b) * a.H + hk * a.plan.group + s.r0 + r;
-        sum.store<T>(O + row * D + 4 * part, L + row, part == 0);
+        __syncthreads();
+        constexpr int LPR = D / 4;
+        const int part = threadIdx.x % LPR;
+        for (int r = threadIdx.x / LPR; r < min(R, s.rows - s.r0); r += 64 * kQ8Waves / LPR) {
+            float2 v[kQ8Waves];
+            f32x4 x[kQ8Waves];
+#pragma unroll
+            for (int w = 0; w < kQ8Waves; ++w) {
+                v[w] = s_ml[w][r];
+                x[w] = __builtin_bit_cast(f32x4, ld16(&s_acc[w][r][4 * part]));
+            }
+            Q8Merge sum;
+            sum.add(v, x);
+            const size_t row = static_cast<size_t>(b) * a.H + hk * a.plan.group + s.r0 + r;
+            sum.store<T>(O + row * D + 4 * part, L + row, part == 0);
+        }
+        __syncthreads();  // before the next item's parts
     }
 }
 
@@ -739,8 +747,10 @@ FlashAttentionError run_attention(const PagedQ8Call& q8, hipStream_t stream) {
     if (short_tables(c)) {
         auto run = [&](auto nr) {
             constexpr int NR = decltype(nr)::value;
-            const long long groups = static_cast<long long>(c.batch_size) * c.num_kv_heads *
-                                     ((c.num_heads / c.num_kv_heads + 16 * NR - 1) / (16 * NR));
+            // A launch has at most 2^32 - 1 threads in x; workgroups take several items beyond.
+            const long long groups = std::min<long long>(
+                1 << 22, static_cast<long long>(c.batch_size) * c.num_kv_heads *
+                             ((c.num_heads / c.num_kv_heads + 16 * NR - 1) / (16 * NR)));
             auto go = [&](auto kernel) {
                 launch_kernel(profile_kernel<T, D>("decode_q8_short"), kernel,
                               dim3(static_cast<unsigned>(groups)), dim3(64 * dev::kQ8Waves), 0,

@@ -70,10 +70,17 @@ enum class QuantCode : int { INT8 = 0, E4M3 = 1 };
 // same meaning of every argument, masks, empty rows and outputs. Where keys are cut into parts these
 // leave partial results in a workspace, as described in cuflash/paged_cache.h: null takes the library's, a
 // captured call needs the caller's, of the size that the *_workspace_* functions return, and is refused
-// without one (OUT_OF_MEMORY).
-// float queries take part as three bf16 numbers each, and so do the softmax's weights before they meet
-// V: what is lost is below float's own rounding, at more than the rate of the float matrix products (184 to 227
-// TFLOP/s in prompts of 4096 tokens, where a large product of float matrices runs at 151).
+// without one (OUT_OF_MEMORY). Only a decode from tables of at most 1024 keys (page_size * max_pages_per_seq) takes
+// none.
+// Every wave has as many keys as any other, so a token with a long cache costs no more beside prompts than alone.
+// In 16 bits the softmax's weights are rounded to that type before they meet V. float queries take part as three
+// bf16 numbers each, and so do their weights: what is lost is below float's own rounding, at more than the rate of
+// the float matrix products (184 to 227 TFLOP/s in prompts of 4096 tokens, where a large product of float matrices
+// runs at 151).
+// Cache rows from seq_lens[b] on may hold anything; table entries past a sequence's pages are not read. Keys that
+// a query does not see do not reach it. Of the values that `causal` hides from it it may take 0 times those of up to
+// 94 positions past its own (the 32 rows that share a wave end up to 31 positions later, in steps of 64 keys): a NaN
+// there makes its output NaN. A query that sees no key has O = 0 whatever the cache holds.
 #define CUFLASH_Q8_DECODE(T)                                                                      \
     CUFLASH_EXPORT FlashAttentionError flash_attention_decode_paged_q8(                           \
         const T* Q, const void* K_cache, const void* V_cache, const uint8_t* K_exp,               \

@@ -185,6 +185,54 @@ def test_a_poisoned_row_reaches_those_that_see_it(torch_gpu, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,heads,kv_heads,new", [
+    (64, 4, 2, 300), (128, 8, 1, 300), (32, 2, 2, 150), (128, 8, 8, 20), (64, 8, 2, 5)])
+@pytest.mark.parametrize("at", [140, 200, 298])
+def test_the_reach_of_a_hidden_value(torch_gpu, dtype, d, heads, kv_heads, new, at):
+    """A NaN value at a position changes no bit of queries that stand 95 or more before it, nor of another
+    sequence, and makes those from it on NaN. The keys' rows there are NaN too in a second run: no query before
+    sees them."""
+    torch = torch_gpu
+    c = Q8Case(dtype, "int8", d, heads, kv_heads, 16, [300, 300])
+    pg, row = c.places[1]
+    x, q = queries(c, 2 * new)
+    starts = c.ints([0, new, 2 * new])
+    clean = forward(c, q, starts, causal=True)
+    c.exps[1][pg[at], row[at]] = 255
+    c.upload()
+    o, lse = forward(c, q, starts, causal=True)
+    far = new + max(0, at - 94 - (300 - new))  # tokens of both sequences before the reach
+    seen = new + max(0, at - (300 - new))
+    assert torch.equal(o[:far], clean[0][:far]) and torch.equal(lse, clean[1])
+    assert bool(torch.isnan(o[seen:]).all())
+    c.exps[1][pg[at], row[at]] = 127
+    c.exps[0][pg[at], row[at]] = 255
+    c.upload()
+    o, lse = forward(c, q, starts, causal=True)
+    assert torch.equal(lse[:seen], clean[1][:seen])
+    assert bool(torch.isnan(lse[seen:]).all() and torch.isnan(o[seen:]).all())
+
+
+@pytest.mark.gpu
+def test_decode_of_more_sequences_than_a_launch_has_workgroups(torch_gpu):
+    """A million sequences of one key, or none, in one launch: O is the key's value."""
+    torch = torch_gpu
+    c = Q8Case("float16", "int8", 32, 8, 8, 16, [16])
+    B = (1 << 20) + 1
+    q = torch.ones(B, 8, 1, 32, dtype=torch.float16, device="cuda")
+    lens = torch.ones(B, dtype=torch.int32, device="cuda")
+    lens[::3] = 0
+    table = c.t_table[0, :1].expand(B, 1).contiguous()
+    o, lse = cuflash_attn.flash_attention_decode_paged_q8(q, *c.cache, table, lens)
+    _, v = cuflash_attn.flash_attention_read_paged_q8(*c.cache, c.t_table, c.t_lens,
+                                                      c.ints([0, 16]), 16, dtype=torch.float16)
+    some = lens == 1
+    assert bool((o[some] == v[0].view(1, 8, 1, 32)).all())
+    assert bool((o[~some] == 0).all()) and bool(torch.isneginf(lse[~some]).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 def test_infinite_and_nan_queries(torch_gpu, dtype):
     """Of one head: NaN where scores are; the others as without."""
