@@ -72,7 +72,8 @@ enum class QuantCode : int { INT8 = 0, E4M3 = 1 };
 // captured call needs the caller's, of the size that the *_workspace_* functions return, and is refused
 // without one (OUT_OF_MEMORY). Only a decode from tables of at most 1024 keys (page_size * max_pages_per_seq) takes
 // none.
-// Every wave has as many keys as any other, so a token with a long cache costs no more beside prompts than alone.
+// All keys are cut into equal shares, whatever the lengths: a long cache beside prompts delays nothing but its own
+// keys' work.
 // In 16 bits the softmax's weights are rounded to that type before they meet V. float queries take part as three
 // bf16 numbers each, and so do their weights: what is lost is below float's own rounding, at more than the rate of
 // the float matrix products (184 to 227 TFLOP/s in prompts of 4096 tokens, where a large product of float matrices
