@@ -20,9 +20,9 @@
 // combine_q8_kernel or merge_q8_kernel (attention_q8.hpp) merges the rows that several waves have and writes those
 // without a key; a decode from short tables is one launch, decode_q8_short_kernel. Where sequences have many 16-bit
 // rows prompt_q8.hip takes over.
-// Bound by HBM: bf16 over e4m3, 4 sequences of up to 131072 keys, 32 heads over 8, head_dim 128, 169 us (6.4 TB/s; a
-// 1 GiB copy reaches 5.1), fp16 over
-// int8, 64 sequences of up to 8192 keys 91 (6.0), over e4m3, 16 x 5 tokens of 8196 keys 53 (5.2).
+// Bound by HBM (32 heads over 8, head_dim 128; a 1 GiB copy reaches 5.1 TB/s): 4 sequences of up to 131072 keys, bf16
+// over e4m3, 169 us, 6.4 TB/s; 64 of up to 8192 keys, fp16 over int8, 91 us, 6.0; 16 x 5 tokens of 8196 keys, fp16
+// over e4m3, 53 us, 5.2.
 
 #include "attention_q8.hpp"
 
