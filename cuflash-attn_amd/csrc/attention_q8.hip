@@ -18,7 +18,7 @@
 // its own have been used. The waves of neighbouring key/value heads have the same share and so read the same
 // cache rows at the same time.
 // combine_q8_kernel or merge_q8_kernel (attention_q8.hpp) merges the rows that several waves have and writes those
-// without a key; a decode from short tables is one launch, decode_q8_short_kernel. Where sequences have many 16-bit
+// without a key; from short tables all is one launch, attention_q8_short_kernel. Where sequences have many 16-bit
 // rows prompt_q8.hip takes over.
 // Bound by HBM (32 heads over 8, head_dim 128; a 1 GiB copy reaches 5.1 TB/s): 4 sequences of up to 131072 keys, bf16
 // over e4m3, 169 us, 6.4 TB/s; 64 of up to 8192 keys, fp16 over int8, 91 us, 6.0; 16 x 5 tokens of 8196 keys, fp16
@@ -620,28 +620,26 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
     }
 }
 
-// A decode from short tables in one launch: a workgroup has a tile of one sequence, each wave a piece of its keys,
-// and their parts are merged through LDS.
+// Attention from short tables in one launch: a workgroup has a tile, each wave a piece of its keys, and their parts
+// are merged through LDS.
 template <typename T, int D, QuantCode C, int NR, int kPage>
 __global__ void __launch_bounds__((64 * kQ8Waves), 2)
-    decode_q8_short_kernel(const typename Mma<T>::elem* __restrict__ Q,
-                           const uint8_t* __restrict__ K, const uint8_t* __restrict__ V,
-                           const uint8_t* __restrict__ Kx, const uint8_t* __restrict__ Vx,
-                           typename Mma<T>::elem* __restrict__ O, float* __restrict__ L,
-                           AttentionQ8Args a) {
+    attention_q8_short_kernel(const typename Mma<T>::elem* __restrict__ Q,
+                              const uint8_t* __restrict__ K, const uint8_t* __restrict__ V,
+                              const uint8_t* __restrict__ Kx, const uint8_t* __restrict__ Vx,
+                              typename Mma<T>::elem* __restrict__ O, float* __restrict__ L,
+                              AttentionQ8Args a, uint32_t items) {
     constexpr int R = 16 * NR;
     using Work = AttentionQ8<T, D, C, NR, kPage>;
     __shared__ __attribute__((aligned(16))) float s_acc[kQ8Waves][R][Work::kPitch];
     __shared__ float2 s_ml[kQ8Waves][R];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    const int tiles = (a.plan.group + R - 1) / R;
-    const uint32_t items = static_cast<uint32_t>(a.plan.B) * a.Hkv * tiles;  // at most B H, below 2^31
     for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int unit = item / tiles;
-        const int tile = item - unit * tiles;
-        const int b = unit / a.Hkv;
-        const int hk = unit - b * a.Hkv;
+        const int x = item / a.Hkv;
+        const int hk = item - x * a.Hkv;
+        int b, tile;
+        if (!q8_tile_at<R, GpuWave>(a.plan, x, b, tile)) return;
         const Work work{
             a,
             Q,
@@ -655,13 +653,15 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
         Q8Segment s;
         s.seq = q8_seq(a.plan, b);
         s.b = b;
-        s.rows = a.plan.group;
+        const Q8Line<R> line(a.plan, s.seq);
+        const int keys = line.keys(a.plan, s.seq, tile);
+        s.rows = line.rows;
         s.r0 = tile * R;
         s.slot = 0;
-        const int blocks = (s.seq.keys + 31) / 32;
+        const int blocks = (keys + 31) / 32;
         const int each = (blocks + kQ8Waves - 1) / kQ8Waves * 32;
         s.kbeg = wave * each;
-        s.kend = min(s.kbeg + each, s.seq.keys);
+        s.kend = min(s.kbeg + each, keys);
         if (s.kbeg < s.kend) {
             work.template segment<true>(
                 s, a.block_table + static_cast<size_t>(b) * a.max_pages, s_acc[wave][0],
@@ -682,7 +682,9 @@ __global__ void __launch_bounds__((64 * kQ8Waves), 2)
             }
             Q8Merge sum;
             sum.add(v, x);
-            const size_t row = static_cast<size_t>(b) * a.H + hk * a.plan.group + s.r0 + r;
+            const int token = a.plan.group_div(s.r0 + r);
+            const size_t row = static_cast<size_t>(s.seq.t0 + token) * a.H + hk * a.plan.group +
+                               (s.r0 + r - token * a.plan.group);
             sum.store<T>(O + row * D + 4 * part, L + row, part == 0);
         }
         __syncthreads();  // before the next item's parts
@@ -720,22 +722,47 @@ Q8Grid waves_grid(const PagedCall& c) {
                   1);
 }
 
-// Decodes from tables of at most so many keys are one launch (bf16 over e4m3, 32 heads over 8, head_dim 128, us of
-// kernels in one and in two: one sequence of 500 keys 6.7 and 11.5, of 1000 9.8 and 12.1, of 2000 15.9 and 12.0; 64
-// of up to 500 13.5 and 17.4, of up to 1000 23.2 and 24.1, of up to 2000 37.7 and 33.0).
-constexpr long long kShortKeys = 1024;
-bool short_tables(const PagedCall& c) {
-    return !c.query_starts && static_cast<long long>(c.page_size) * c.max_pages <= kShortKeys;
+// Whether a call is one launch, a workgroup a tile of rows. Decodes are, from tables of at most 1024 keys (bf16 over
+// e4m3, 32 heads over 8, head_dim 128, us of kernels in one and in two: one sequence of 500 keys 6.7 and 11.5, of 1000
+// 9.8 and 12.1, of 2000 15.9 and 12.0; 64 of up to 500 13.5 and 17.4, of up to 1000 23.2 and 24.1, of up to 2000 37.7
+// and 33.0). Of several tokens, where the workgroups' rounds are few for their keys and the rest of the chip would not
+// be of much use: the same heads, 4 tokens of 200 keys 6.5 and 13.2, 250 of 1000 13.1 and 40.9, 500 of 1000 23 and 44,
+// 250 of 2000 20 and 44, 500 of 2000 35 and 52, 128 of 4000 32 and 39; against that 2000 of 2000 101 and 66, 32 of 4000
+// 32 and 23, 128 of 8000 57 and 47, 256 sequences with 2 tokens of 60 keys 40 and 22; fp32, 8 heads over 4, head_dim 64,
+// 1000 of 1000 14.5 and 31.7, 2000 of 2000 35 and 43, 32 of 2000 23 and 18, 250 of 4000 38 and 31.
+bool one_launch(const PagedCall& c, const Q8Grid& grid) {
+    const long long keys = static_cast<long long>(c.page_size) * c.max_pages;
+    if (!c.query_starts) return keys <= 1024;
+    const long long items = dev::q8_most_tiles(grid.args(c).plan, grid.rows) * c.num_kv_heads;
+    const long long rounds = (items + compute_units() - 1) / compute_units();
+    return rounds * (keys + 700) <= 5500 && (keys <= 1024 || items * 32 >= keys);
+}
+
+template <typename T>
+long long workspace_of(const PagedCall& c) {
+    auto grid = [&] {
+        if constexpr (!std::is_same<T, float>::value) {
+            if (many_rows<T>(c)) return prompt_q8_grid<T>(c);
+        }
+        return waves_grid<T>(c);
+    }();
+    return static_cast<long long>(grid.bytes());
 }
 
 template <typename T, int D, QuantCode C>
 FlashAttentionError run_attention(const PagedQ8Call& q8, hipStream_t stream) {
     using E = typename dev::Mma<T>::elem;
     const PagedCall& c = q8.call;
-    if (many_rows<T>(c)) {
+    const Q8Grid grid = waves_grid<T>(c);
+    const bool one = one_launch(c, grid);
+    // A forward's workspace is asked for by its sizes, whether keys are cut or not.
+    if (one && c.query_starts) {
+        const FlashAttentionError err = workspace_refusal(c, workspace_of<T>(c), stream);
+        if (err != FlashAttentionError::SUCCESS) return err;
+    }
+    if (!one && many_rows<T>(c)) {
         if constexpr (!std::is_same<T, float>::value) return launch_prompt_q8<T>(q8, stream);
     }
-    const Q8Grid grid = waves_grid<T>(c);
     // go(n) with n rows that lie on one page.
     auto by_page = [&](auto go) {
         if (c.page_size % 16 == 0)
@@ -745,23 +772,24 @@ FlashAttentionError run_attention(const PagedQ8Call& q8, hipStream_t stream) {
         else
             go(std::integral_constant<int, 1>{});
     };
-    if (short_tables(c)) {
+    if (one) {
         auto run = [&](auto nr) {
             constexpr int NR = decltype(nr)::value;
-            // A launch has at most 2^32 - 1 threads in x; workgroups take several items beyond.
-            const long long groups = std::min<long long>(
-                1 << 22, static_cast<long long>(c.batch_size) * c.num_kv_heads *
-                             ((c.num_heads / c.num_kv_heads + 16 * NR - 1) / (16 * NR)));
+            const dev::AttentionQ8Args a = grid.args(c);
+            // At most B H of them, below 2^31. A launch has at most 2^32 - 1 threads in x; workgroups take several
+            // items beyond.
+            const long long items = dev::q8_most_tiles(a.plan, grid.rows) * c.num_kv_heads;
+            const long long groups = std::min<long long>(1 << 22, items);
             auto go = [&](auto kernel) {
-                launch_kernel(profile_kernel<T, D>("decode_q8_short"), kernel,
+                launch_kernel(profile_kernel<T, D>("attention_q8_short"), kernel,
                               dim3(static_cast<unsigned>(groups)), dim3(64 * dev::kQ8Waves), 0,
                               stream, static_cast<const E*>(c.Q),
                               static_cast<const uint8_t*>(c.K_cache),
                               static_cast<const uint8_t*>(c.V_cache), q8.K_exp, q8.V_exp,
-                              static_cast<E*>(c.O), c.L, grid.args(c));
+                              static_cast<E*>(c.O), c.L, a, static_cast<uint32_t>(items));
             };
             by_page([&](auto page) {
-                go(dev::decode_q8_short_kernel<T, D, C, NR, decltype(page)::value>);
+                go(dev::attention_q8_short_kernel<T, D, C, NR, decltype(page)::value>);
             });
             return from_hip(hipGetLastError());
         };
@@ -812,13 +840,7 @@ FlashAttentionError run_dim(const PagedQ8Call& c, hipStream_t stream) {
 
 template <typename T>
 long long paged_q8_workspace(const PagedCall& c) {
-    auto grid = [&] {
-        if constexpr (!std::is_same<T, float>::value) {
-            if (many_rows<T>(c)) return prompt_q8_grid<T>(c);
-        }
-        return waves_grid<T>(c);
-    }();
-    return static_cast<long long>(grid.bytes());
+    return workspace_of<T>(c);
 }
 
 template <typename T>

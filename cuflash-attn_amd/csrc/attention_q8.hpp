@@ -275,21 +275,26 @@ struct Q8Grid {
     }
 };
 
+// A given workspace that is too small, or a captured call without one: a graph's replays need memory that is theirs.
+inline FlashAttentionError workspace_refusal(const PagedCall& c, size_t bytes, hipStream_t stream) {
+    return (c.workspace ? c.workspace_bytes < bytes : stream_capturing(stream))
+               ? FlashAttentionError::OUT_OF_MEMORY
+               : FlashAttentionError::SUCCESS;
+}
+
 // Launches attend(args) and then the merge of R-row tiles, with the partial results in the caller's
 // workspace or the library's.
 template <typename T, int D, int R, class Attend>
 FlashAttentionError run_q8(const PagedCall& c, const Q8Grid& grid, hipStream_t stream, Attend attend) {
     using E = typename dev::Mma<T>::elem;
     StreamWorkspace ws(stream, true);
+    const FlashAttentionError refused = workspace_refusal(c, grid.bytes(), stream);
+    if (refused != FlashAttentionError::SUCCESS) return refused;
     void* base = c.workspace;
     if (base == nullptr) {
-        // A graph's replays need memory that is theirs: the caller's.
-        if (stream_capturing(stream)) return FlashAttentionError::OUT_OF_MEMORY;
         const FlashAttentionError err = ws.alloc(grid.bytes());
         if (err != FlashAttentionError::SUCCESS) return err;
         base = ws.get();
-    } else if (c.workspace_bytes < grid.bytes()) {
-        return FlashAttentionError::OUT_OF_MEMORY;
     }
     dev::AttentionQ8Args a = grid.args(c);
     a.acc = static_cast<float*>(base);

@@ -65,7 +65,7 @@ struct Q8Line {
     int size;   // in all
     __host__ __device__ __forceinline__ Q8Line(const Q8PlanArgs& a, const Q8Seq& s) {
         rows = s.n * a.group;
-        tiles = static_cast<int>((static_cast<uint32_t>(rows) + (R - 1)) / R);
+        tiles = tiles_of(a, s);
         const int last = tiles > 0 ? grains(a, keys(a, s, tiles - 1)) : 0;
         if (!a.causal || tiles <= 1) {
             pairs = tiles;
@@ -77,6 +77,9 @@ struct Q8Line {
             size = pairs * pair;
             if (tiles % 2) size += grains(a, keys(a, s, pairs++));
         }
+    }
+    __host__ __device__ __forceinline__ static int tiles_of(const Q8PlanArgs& a, const Q8Seq& s) {
+        return static_cast<int>((static_cast<uint32_t>(s.n * a.group) + (R - 1)) / R);
     }
     // Keys that the rows of a tile see, and their grains.
     __host__ __device__ __forceinline__ int keys(const Q8PlanArgs& a, const Q8Seq& s, int tile) const {
@@ -156,6 +159,36 @@ __host__ __device__ __forceinline__ int q8_begin_of(const Q8PlanArgs& a, int b) 
         begin += W::lane(incl, b - b0 < 64 ? b - b0 - 1 : 63);
     }
     return begin;
+}
+
+// Where one launch does everything, a workgroup has a tile: tile x of all sequences', in their order; false: there
+// are fewer.
+template <int R, class W>
+__host__ __device__ __forceinline__ bool q8_tile_at(const Q8PlanArgs& a, int x, int& b, int& tile) {
+    if (!a.starts) {
+        const int each = static_cast<int>((static_cast<uint32_t>(a.group) + (R - 1)) / R);
+        b = x / each;
+        tile = x - b * each;
+        return b < a.B;
+    }
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const auto incl = W::scan(W::each([&](int lane) {
+            return b0 + lane < a.B ? Q8Line<R>::tiles_of(a, q8_seq(a, b0 + lane)) : 0;
+        }));
+        const int i = W::first(incl, [&](int n) { return n > x; });
+        if (i >= 0) {
+            b = b0 + i;
+            tile = x - (i > 0 ? W::lane(incl, i - 1) : 0);
+            return true;
+        }
+        x -= W::lane(incl, 63);
+    }
+    return false;
+}
+// No launch has more of them.
+inline long long q8_most_tiles(const Q8PlanArgs& a, int rows_per_tile) {
+    if (!a.starts) return static_cast<long long>(a.B) * ((a.group + rows_per_tile - 1) / rows_per_tile);
+    return static_cast<long long>(a.T) * a.group / rows_per_tile + a.B;
 }
 
 // The part of a wave: tile by tile, rows from r0 on of sequence b over its keys [kbeg, kend).

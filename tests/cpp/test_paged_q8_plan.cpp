@@ -120,9 +120,15 @@ bool launch(std::mt19937& rng) {  // whether a tile was cut
         }
         CHECK(grains <= total.share);
     }
+    int tiles = 0;
     for (int b = 0; b < a.B; ++b) {
         const Q8Seq q = q8_seq(a, b);
         const Q8Line<R> line(a, q);
+        // A workgroup a tile: the tiles in their order, and none behind them.
+        for (int tile = 0; tile < line.tiles; ++tile, ++tiles) {
+            int at_b = -1, at = -1;
+            CHECK((q8_tile_at<R, HostWave>(a, tiles, at_b, at)) && at_b == b && at == tile);
+        }
         CHECK(line.tiles == (q.n * a.group + R - 1) / R);
         const int without = q8_rows_without_keys<R>(a, q);
         for (int tile = 0; tile < line.tiles; ++tile) {
@@ -155,6 +161,8 @@ bool launch(std::mt19937& rng) {  // whether a tile was cut
             }
         }
     }
+    int none_b, none;
+    CHECK(!(q8_tile_at<R, HostWave>(a, tiles, none_b, none)) && tiles <= q8_most_tiles(a, R));
     return cut;
 }
 
@@ -179,6 +187,14 @@ void disorder(std::mt19937& rng) {
     a.seq_lens = lens.data();
     a.starts = starts.data();
     q8_set_grains(a, R, R == 256 ? 1 : 0);
+    for (int x = 0; x < q8_most_tiles(a, R); ++x) {
+        int b, tile;
+        if (!q8_tile_at<R, HostWave>(a, x, b, tile)) break;
+        const Q8Seq s = q8_seq(a, b);
+        const Q8Line<R> line(a, s);
+        CHECK(b >= 0 && b < a.B && tile >= 0 && tile < line.tiles && s.t0 + s.n <= a.T);
+        CHECK(line.keys(a, s, tile) >= 0 && line.keys(a, s, tile) <= a.cap);
+    }
     const Q8Total total = q8_total<R, HostWave>(a);
     for (int p = 0; p < a.shares; ++p) {
         Q8Walk<R, HostWave> walk(a, p);

@@ -50,6 +50,22 @@ def _check_decode(c, scale, only):
 
 
 def check_forward(c, new, causal, extra=0, scale=None, only=None):
+    """Twice, too: no table of 4900 keys is short for any number of rows."""
+    table = c.t_table
+    if int(c.t_lens.max()) <= c.max_pages * c.page < 4900:
+        c.t_table = longer(c, 4900)
+        _check_forward(c, new, causal, extra, scale, only)
+        c.t_table = table
+    _check_forward(c, new, causal, extra, scale, only)
+
+
+def longer(c, keys):
+    """The block table with unused pages behind, for that many keys."""
+    more = -(-keys // c.page) - c.max_pages
+    return c.ints(np.concatenate((c.table, np.repeat(c.table[:, :1] * 0 + c.unused, more, 1)), 1))
+
+
+def _check_forward(c, new, causal, extra, scale, only):
     import torch
 
     T = sum(new) + extra
@@ -189,18 +205,23 @@ def test_a_poisoned_row_reaches_those_that_see_it(torch_gpu, dtype):
 @pytest.mark.parametrize("d,heads,kv_heads,new", [
     (64, 4, 2, 300), (128, 8, 1, 300), (32, 2, 2, 150), (128, 8, 8, 20), (64, 8, 2, 5)])
 @pytest.mark.parametrize("at", [140, 200, 298])
-def test_the_reach_of_a_hidden_value(torch_gpu, dtype, d, heads, kv_heads, new, at):
+@pytest.mark.parametrize("table", ["short", "long"])
+def test_the_reach_of_a_hidden_value(torch_gpu, dtype, d, heads, kv_heads, new, at, table):
     """A NaN value at a position changes no bit of queries that stand 95 or more before it, nor of another
     sequence, and makes those from it on NaN. The keys' rows there are NaN too in a second run: no query before
     sees them."""
     torch = torch_gpu
     c = Q8Case(dtype, "int8", d, heads, kv_heads, 16, [300, 300])
     pg, row = c.places[1]
+    if table == "long":
+        c.t_table = longer(c, 4900)
+    t_table = c.t_table
     x, q = queries(c, 2 * new)
     starts = c.ints([0, new, 2 * new])
     clean = forward(c, q, starts, causal=True)
     c.exps[1][pg[at], row[at]] = 255
     c.upload()
+    c.t_table = t_table
     o, lse = forward(c, q, starts, causal=True)
     far = new + max(0, at - 94 - (300 - new))  # tokens of both sequences before the reach
     seen = new + max(0, at - (300 - new))
@@ -209,6 +230,7 @@ def test_the_reach_of_a_hidden_value(torch_gpu, dtype, d, heads, kv_heads, new, 
     c.exps[1][pg[at], row[at]] = 127
     c.exps[0][pg[at], row[at]] = 255
     c.upload()
+    c.t_table = t_table
     o, lse = forward(c, q, starts, causal=True)
     assert torch.equal(lse[:seen], clean[1][:seen])
     assert bool(torch.isnan(lse[seen:]).all() and torch.isnan(o[seen:]).all())
