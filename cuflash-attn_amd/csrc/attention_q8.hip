@@ -278,6 +278,31 @@ struct AttentionQ8 {
     static __device__ __forceinline__ float factor(const uint32_t (&x)[XW], int e) {
         return Q8<C>::factor(kFours ? (x[e >> 2] >> (8 * (e & 3))) & 0xffu : x[e]);
     }
+    // Of int8 keys, whether one of the lane's has an exponent that leads beyond fp16's numbers: 137 or more (127 *
+    // 2^10 is infinite there) or less than 103 (2^-25 is none of them). Such a block's codes become fp16 numbers
+    // before the product, as in prompt_q8.hip and the read: which kernel a call takes does not show. (The look costs
+    // up to 2%: 64 sequences of 4000 keys, head_dim 64, 34.0 -> 34.8 us, head_dim 128 94.1 -> 94.3.)
+    static __device__ __forceinline__ bool beyond_half(const uint32_t (&x)[XW]) {
+        uint32_t high = 0u, low = ~0u;  // in a byte's top bit: one is 137 or more, all are 103 or more
+#pragma unroll
+        for (int i = 0; i < XW; ++i) {
+            const uint32_t w7 = x[i] & 0x7f7f7f7fu;
+            high |= (w7 + 0x77777777u) & x[i];
+            low &= (w7 + 0x19191919u) | x[i];
+        }
+        return ((high | ~low) & (kFours ? 0x80808080u : 0x80u)) != 0u;
+    }
+    // Of key l % 16 of half t: lanes 16 (key / 4) .. + 15 have it as one of their four.
+    static __device__ __forceinline__ float key_factor(const uint32_t (&x)[XW], int t) {
+        const int key = threadIdx.x & 15;
+        float f = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float of = __shfl(factor(x, 4 * t + r), key >> 2 << 4, 64);
+            f = (key & 3) == r ? of : f;
+        }
+        return f;
+    }
 
     // The outputs of a segment's rows, or (slot >= 0) their partial results, those of row r of the tile D floats
     // at acc_of(r) and (m, l) at ml_of(r). `stage`: 16 rows of the wave's in LDS; kKeep: R rows, and the partial
@@ -354,31 +379,47 @@ struct AttentionQ8 {
         const float cs = fmaxf(a.c, kFltMin);  // scale 0: -inf * 0 would make the masked scores NaN
 
         f32x4 sc[NR][2];
-        auto scores = [&](const Codes& x) {
+        // Half t's scores, its codes scaled by `by` on their way or (kScaled false) as they are.
+        auto half = [&](const Codes& x, int t, auto scaled, float by) {
+            constexpr bool kScaled = decltype(scaled)::value;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int nr = 0; nr < NR; ++nr) sc[nr][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int nr = 0; nr < NR; ++nr) sc[nr][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                const float by = kScaleK ? Q8<C>::factor(x.kx[t]) : 1.0f;
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint32_t* w = &x.k[t][ks / (KB / 8)][ks % (KB / 8) * 2];
+                const u32x2 lo = Q8<C>::template four<M, kScaled>(w[0], by);
+                const u32x2 hi = Q8<C>::template four<M, kScaled>(w[1], by);
+                const Frag k = as_frag<M>(u32x4{lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const uint32_t* w = &x.k[t][ks / (KB / 8)][ks % (KB / 8) * 2];
-                    const u32x2 lo = Q8<C>::template four<M, kScaleK>(w[0], by);
-                    const u32x2 hi = Q8<C>::template four<M, kScaleK>(w[1], by);
-                    const Frag k = as_frag<M>(u32x4{lo[0], lo[1], hi[0], hi[1]});
+                for (int part = kParts - 1; part >= 0; --part) {
 #pragma unroll
-                    for (int part = kParts - 1; part >= 0; --part) {
-#pragma unroll
-                        for (int nr = 0; nr < NR; ++nr)
-                            sc[nr][t] = mma16<M>(k, f[nr][part][ks], sc[nr][t]);
-                    }
+                    for (int nr = 0; nr < NR; ++nr)
+                        sc[nr][t] = mma16<M>(k, f[nr][part][ks], sc[nr][t]);
                 }
-                if constexpr (!kScaleK) {
+            }
+        };
+        auto scores = [&](const Codes& x) {
+            if constexpr (kScaleK) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float k_by = factor(x.kx, 4 * t + r);
+                for (int t = 0; t < 2; ++t)
+                    half(x, t, std::integral_constant<bool, true>{}, Q8<C>::factor(x.kx[t]));
+            } else {
+                bool beyond = false;
+                if constexpr (std::is_same<M, __half>::value) beyond = __ballot(beyond_half(x.kx)) != 0;
+                if (__builtin_expect(beyond, false)) {
 #pragma unroll
-                        for (int nr = 0; nr < NR; ++nr) sc[nr][t][r] *= k_by;
+                    for (int t = 0; t < 2; ++t)
+                        half(x, t, std::integral_constant<bool, true>{}, key_factor(x.kx, t));
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        half(x, t, std::integral_constant<bool, false>{}, 1.0f);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float by = factor(x.kx, 4 * t + r);
+#pragma unroll
+                            for (int nr = 0; nr < NR; ++nr) sc[nr][t][r] *= by;
+                        }
                     }
                 }
             }

@@ -16,7 +16,8 @@
 //    A power of two because such a product is exact in float and bf16, and in fp16 where that has the
 //    number: the attentions take it as it is, without a rounding, and gfx950 scales as it converts.
 //  * In calls with fp16 queries an element beyond fp16's range is its nearest fp16 number, or infinite.
-//    The fp16 append writes none that is infinite.
+//    The fp16 append writes none that is infinite. x above 248 (e4m3: 246), which no append writes, leads beyond
+//    float's range: the attentions take such an element as infinite or as the number that it is.
 // Pages, tables, packed tokens, positions, padding, lengths, head_dim, head groups, alignment (of
 // the exponents' pointers too) and errors are as in cuflash/paged_cache.h; a QuantCode that is none is
 // UNSUPPORTED_DTYPE, found after null pointers, and a page of 2^31 bytes or more in an attention INVALID_DIMENSION.
