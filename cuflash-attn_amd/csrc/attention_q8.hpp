@@ -248,7 +248,8 @@ struct Q8Grid {
     // Many rows, of which few are cut: the merge goes by shares, else by tokens and heads.
     bool by_share() const { return static_cast<long long>(tokens) * heads >= kByShare; }
     static constexpr long long kByShare = 1 << 13;
-    dev::AttentionQ8Args args(const PagedCall& c) const {
+    // fits: whether all tiles find their place in one line (paged_q8_plan.hpp).
+    dev::AttentionQ8Args args(const PagedCall& c, bool* fits = nullptr) const {
         dev::AttentionQ8Args a{};
         a.plan.seq_lens = c.seq_lens;
         a.plan.starts = c.query_starts;
@@ -259,7 +260,8 @@ struct Q8Grid {
         a.plan.shares = shares;
         a.plan.causal = c.causal;
         a.plan.group_div = dev::fast_div(a.plan.group);
-        dev::q8_set_grains(a.plan, rows, least_shift);
+        const bool fit = dev::q8_set_grains(a.plan, rows, least_shift);
+        if (fits) *fits = fit;
         a.plan.least = least;
         a.block_table = c.block_table;
         a.H = c.num_heads;
@@ -287,6 +289,9 @@ inline FlashAttentionError workspace_refusal(const PagedCall& c, size_t bytes, h
 template <typename T, int D, int R, class Attend>
 FlashAttentionError run_q8(const PagedCall& c, const Q8Grid& grid, hipStream_t stream, Attend attend) {
     using E = typename dev::Mma<T>::elem;
+    bool fits;
+    dev::AttentionQ8Args a = grid.args(c, &fits);
+    if (!fits) return FlashAttentionError::INVALID_DIMENSION;
     StreamWorkspace ws(stream, true);
     const FlashAttentionError refused = workspace_refusal(c, grid.bytes(), stream);
     if (refused != FlashAttentionError::SUCCESS) return refused;
@@ -296,7 +301,6 @@ FlashAttentionError run_q8(const PagedCall& c, const Q8Grid& grid, hipStream_t s
         if (err != FlashAttentionError::SUCCESS) return err;
         base = ws.get();
     }
-    dev::AttentionQ8Args a = grid.args(c);
     a.acc = static_cast<float*>(base);
     a.ml = reinterpret_cast<float2*>(a.acc + grid.slots() * D);
     attend(a);

@@ -129,7 +129,7 @@ template <int R, class W>
 __host__ __device__ __forceinline__ Q8Total q8_total(const Q8PlanArgs& a) {
     int sum = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) sum += W::lane(W::scan(q8_sizes<R, W>(a, b0)), 63);
-    // Only starts that decrease lead past what q8_shift() leaves room for; they are undefined, not unsafe.
+    // Only starts that decrease lead past what q8_set_grains() leaves room for.
     if (sum < 0 || sum > kQ8Line) sum = 0;
     const int share = (sum + (a.shares - 1)) / a.shares;
     return {sum, share > a.least ? share : a.least};
@@ -264,13 +264,20 @@ __host__ __device__ __forceinline__ Q8Parts q8_parts(const Q8PlanArgs& a, const 
     return {from, to, begin > from * total.share ? 1 : 0};
 }
 
-// The grains of a launch, of 32 << least keys or more: what the host knows keeps the line below 2^30 of them.
-inline void q8_set_grains(Q8PlanArgs& a, int rows_per_tile, int least) {
-    const long long tiles = static_cast<long long>(a.T) * a.group / rows_per_tile + 2LL * a.B;
+// The grains of a launch, of 32 << least keys or more, so that by what the host knows the line has less than 2^30 of
+// them. With the largest, of 2^31 keys, a tile is one grain, and between pairs of tiles, of which a sequence of r rows
+// has at most r / R, stand `slack` more. false: more than 2^30 even so, or so many sequences that their number, 64 at
+// a time, passes 32 bits.
+inline bool q8_set_grains(Q8PlanArgs& a, int rows_per_tile, int least) {
+    const long long full = static_cast<long long>(a.T) * a.group / rows_per_tile;
+    if (a.B > 0x7fffffff - 63) return false;
     for (a.shift = least;; ++a.shift) {
         a.slack = 2 + static_cast<int>(rows_per_tile / (static_cast<long long>(a.group) << (5 + a.shift)));
-        if (a.shift >= 26 || tiles * (((a.cap + 31LL) / 32 >> a.shift) + 1 + a.slack) < kQ8Line) return;
+        if ((full + 2LL * a.B) * (((a.cap + 31LL) / 32 >> a.shift) + 1 + a.slack) < kQ8Line) return true;
+        if (a.shift >= 26) break;
     }
+    if (!a.starts) return q8_most_tiles(a, rows_per_tile) <= kQ8Line;
+    return full * (1 + (a.causal ? a.slack : 0)) + (a.B < a.T ? a.B : a.T) <= kQ8Line;
 }
 
 }  // namespace dev

@@ -73,7 +73,9 @@ enum class QuantCode : int { INT8 = 0, E4M3 = 1 };
 // captured call needs the caller's, of the size that the *_workspace_* functions return, and is refused
 // without one (OUT_OF_MEMORY). Only a decode from tables of at most 1024 keys (page_size * max_pages_per_seq) never
 // takes one. Short tables (page_size * max_pages_per_seq) are faster than long ones that hold the same lengths: such a
-// call may be one launch.
+// call may be one launch. A call of several launches that may have more than 2^30 tiles of rows, which takes some 900
+// million sequences with tokens, or 2^31 - 63 sequences and more is refused (INVALID_DIMENSION; the *_workspace_*
+// functions do not look at this).
 // All keys are cut into equal shares, whatever the lengths: a long cache beside prompts delays nothing but its own
 // keys' work.
 // In 16 bits the softmax's weights are rounded to that type before they meet V. float queries take part as three
