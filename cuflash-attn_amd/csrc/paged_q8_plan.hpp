@@ -112,12 +112,12 @@ struct Q8Line {
     }
 };
 
-// Sums over the sequences, W: the 64 lanes of a wave.
+// Sums over the sequences, W: the 64 lanes of a wave. Of sequences b0 + lane, in units of 1 << shift.
 template <int R, class W>
-__host__ __device__ __forceinline__ typename W::Int q8_sizes(const Q8PlanArgs& a, int b0) {
+__host__ __device__ __forceinline__ typename W::Int q8_sizes(const Q8PlanArgs& a, int b0, int shift = 0) {
     return W::each([&](int lane) {
         if (b0 + lane >= a.B) return 0;
-        return Q8Line<R>(a, q8_seq(a, b0 + lane)).size;
+        return Q8Line<R>(a, q8_seq(a, b0 + lane)).size >> shift;
     });
 }
 
@@ -128,9 +128,18 @@ struct Q8Total {
 template <int R, class W>
 __host__ __device__ __forceinline__ Q8Total q8_total(const Q8PlanArgs& a) {
     int sum = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) sum += W::lane(W::scan(q8_sizes<R, W>(a, b0)), 63);
-    // Only starts that decrease lead past what q8_set_grains() leaves room for.
-    if (sum < 0 || sum > kQ8Line) sum = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const auto sizes = q8_sizes<R, W>(a, b0);
+        // Only starts that decrease lead past what q8_set_grains() leaves room for. What comes out then is undefined,
+        // but the shares of a sum that wrapped would reach beyond the rows and the workspace. A size is at most the
+        // line; where 64 of them may pass 32 bits, they are first summed in units of 64.
+        if (W::first(sizes, [](int n) { return n > kQ8Line / 64; }) >= 0 &&
+            W::lane(W::scan(q8_sizes<R, W>(a, b0, 6)), 63) > kQ8Line / 64)
+            return {0, a.least};
+        const int block = W::lane(W::scan(sizes), 63);
+        if (block > kQ8Line - sum) return {0, a.least};
+        sum += block;
+    }
     const int share = (sum + (a.shares - 1)) / a.shares;
     return {sum, share > a.least ? share : a.least};
 }

@@ -26,3 +26,8 @@ def test_too_many_tiles_are_refused(lib, sfx, code, d):
 
 def test_tiles_that_fit_and_those_that_do_not(tmp_path):
     run_program("test_paged_q8_limits", tmp_path)
+
+
+def test_starts_that_decrease_stay_in_bounds(tmp_path):
+    """Also where the sum over all sequences passes 32 bits."""
+    run_program("test_paged_q8_disorder", tmp_path, 300, 1)
