@@ -18,7 +18,6 @@ namespace cuflash {
 namespace dev {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // The 16-bit type in which the matrix products take the cache's numbers: the queries' own, bf16 for float.
@@ -50,10 +49,11 @@ struct Q8<QuantCode::E4M3> {
             return __builtin_bit_cast(uint32_t,
                                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, f, i != 0));
     }
-    // All four, scaled or as they are.
+    // All four; the conversion scales anyway.
     template <typename M, bool kScaled>
     static __device__ __forceinline__ u32x2 four(uint32_t codes, float f) {
-        return u32x2{expand<M, 0>(codes, kScaled ? f : 1.0f), expand<M, 1>(codes, kScaled ? f : 1.0f)};
+        static_assert(kScaled, "e4m3 codes are scaled as they are converted");
+        return u32x2{expand<M, 0>(codes, f), expand<M, 1>(codes, f)};
     }
     // Codes 2 i and 2 i + 1 of two rows, scaled: the first ones as one pair, the second ones as another.
     template <typename M, int i>
@@ -102,6 +102,7 @@ struct Q8<QuantCode::INT8> {
     static __device__ __forceinline__ uint32_t expand(uint32_t codes, float f) {
         return pair<M>(one<2 * i>(codes, f), one<2 * i + 1>(codes, f));
     }
+    // All four, scaled or as they are.
     template <typename M, bool kScaled>
     static __device__ __forceinline__ u32x2 four(uint32_t codes, float f) {
         if constexpr (!kScaled && std::is_same<M, __half>::value) {
