@@ -21,8 +21,11 @@
 // without a key; from short tables all is one launch, attention_q8_short_kernel. Where sequences have many 16-bit
 // rows prompt_q8.hip takes over.
 // Bound by HBM (32 heads over 8, head_dim 128; a 1 GiB copy reaches 5.1 TB/s): 4 sequences of up to 131072 keys, bf16
-// over e4m3, 169 us, 6.4 TB/s; 64 of up to 8192 keys, fp16 over int8, 91 us, 6.0; 16 x 5 tokens of 8196 keys, fp16
-// over e4m3, 53 us, 5.2.
+// over e4m3, 167 us, 6.5 TB/s; 64 of up to 8192 keys, fp16 over int8, 94 us, 5.9, float over int8 102 us, 5.4; 16 x 5
+// tokens of 8196 keys, fp16 over e4m3, 54 us, 5.0. float prompts by the conversions and three bf16 products for one:
+// 4096 tokens over int8 712 us, 193 TFLOP/s.
+// Every wave sums the sequences' sizes to find its share, 64 in a step: 1024 sequences of 1100 keys 384 us where 64 of
+// 17600 take 374, 16384 sequences of one 8-head group, head_dim 64, 591 where 256 with as many keys take 432.
 
 #include "attention_q8.hpp"
 
@@ -126,8 +129,9 @@ struct AttentionQ8 {
                                : *reinterpret_cast<const uint32_t*>(from);
         }
     }
-    // The same for lines that one load reads whole and nothing reads again (64 sequences of up to 8192 keys,
-    // int8: 111 -> 99 us; K, half a line a load, so 100 -> 123).
+    // The same for lines that one load reads whole and, where a sequence has one tile of rows, nothing reads again (64
+    // sequences of up to 8192 keys, int8: 111 -> 99 us; K, half a line a load, so 100 -> 123). Measured in decodes: what
+    // the hint does where several tiles of rows read the same values is not known.
     template <int N>
     static __device__ __forceinline__ void copy_once(uint32_t (&to)[N], const uint8_t* from, int bytes) {
         if constexpr (N == 2) {
@@ -281,7 +285,8 @@ struct AttentionQ8 {
     // Of int8 keys, whether one of the lane's has an exponent that leads beyond fp16's numbers: 137 or more (127 *
     // 2^10 is infinite there) or less than 103 (2^-25 is none of them). Such a block's codes become fp16 numbers
     // before the product, as in prompt_q8.hip and the read: which kernel a call takes does not show. (The look costs
-    // up to 2%: 64 sequences of 4000 keys, head_dim 64, 34.0 -> 34.8 us, head_dim 128 94.1 -> 94.3.)
+    // up to 4%: 16 x 5 tokens of 8196 keys, head_dim 64, 30.4 -> 31.6 us; 64 sequences of 4000 keys, head_dim 64, 34.0
+    // -> 34.8, head_dim 128 93.3 -> 94.1.)
     static __device__ __forceinline__ bool beyond_half(const uint32_t (&x)[XW]) {
         uint32_t high = 0u, low = ~0u;  // in a byte's top bit: one is 137 or more, all are 103 or more
 #pragma unroll

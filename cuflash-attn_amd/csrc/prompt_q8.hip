@@ -18,9 +18,11 @@
 // took 3% longer), puts it into LDS and asks for the next.
 // K_{j+2} takes the place of K_j, last read in half 2 j, and V_{j+2} that of V_{j-1}, too: two buffers for K and
 // three for V.
-// Measured: one prompt of 16384 tokens, bf16 over e4m3, 32 heads over 8, head_dim 128: 2080 us, 1055 TFLOP/s (a large
-// matrix product 1307); the products alone take 1603, the softmax alone 917. Seven prompts of 285 to 2001 tokens, over
-// int8, head_dim 64: 129 to 150 us, vector unit busy 54% of the time, MFMA 23%.
+// Measured: one prompt of 16384 tokens, bf16 over e4m3, 32 heads over 8, head_dim 128: 2133 us with its merge in a
+// long loop, 1031 TFLOP/s (a large matrix product 1307), 2074 to 2186 by itself in a trace of 20 launches; the
+// products alone take 1603, the softmax alone 917. Seven prompts of 285 to 2001 tokens, over int8, head_dim 64: 137 us
+// with their merge in a loop, 153 by themselves in the trace, whose clock is lower; vector unit busy 54% of the time,
+// MFMA 23%.
 
 #include "attention_q8.hpp"
 #include "tile_groups.hpp"

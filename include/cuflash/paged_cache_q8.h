@@ -76,12 +76,19 @@ enum class QuantCode : int { INT8 = 0, E4M3 = 1 };
 // call may be one launch. A call of several launches that may have more than 2^30 tiles of rows, which takes some 900
 // million sequences with tokens, or 2^31 - 63 sequences and more is refused (INVALID_DIMENSION; the *_workspace_*
 // functions do not look at this).
-// All keys are cut into equal shares, whatever the lengths: a long cache beside prompts delays nothing but its own
-// keys' work.
-// In 16 bits the softmax's weights are rounded to that type before they meet V. float queries take part as three
-// bf16 numbers each, and so do their weights: what is lost is below float's own rounding, at more than the rate of
-// the float matrix products (184 to 227 TFLOP/s in prompts of 4096 tokens, where a large product of float matrices
-// runs at 151).
+// All keys are cut into equal shares, whatever the lengths, so no long cache leaves the rest of the chip without work.
+// But in 16 bits a call takes the tokens of all its sequences in tiles of one height, of 256 rows where their average
+// is more than 48 rows (head_dim 64 and 32: 96; a single sequence: 16): single tokens beside prompts then cost as much
+// for each of their keys as 256 rows do, and are faster in a call of their own (4 prompts of 2000 tokens and 32 tokens
+// behind 4000 keys 367 us, in two calls 255; 5000 tokens and one behind 100000 keys 430 and 348, behind 8000 keys 334
+// and 337; bf16, 32 heads over 8, head_dim 128).
+// In 16 bits the softmax's weights are rounded to that type before they meet V (also where a query head has a key/value
+// head for itself, where flash_attention_decode_paged keeps them in float). float queries take part as three bf16
+// numbers each, and so do their weights: what is lost is below float's own rounding, at more than the rate of the
+// float matrix products (193 TFLOP/s in a prompt of 4096 tokens over int8, head_dim 128, 219 over e4m3, head_dim 64,
+// where a large product of float matrices runs at 151).
+// Most calls scale the scores of int8 keys instead of their codes: queries of 2^113 and more, which bf16 and float
+// have, may there reach infinite scores whose scaled numbers would be finite.
 // Cache rows from seq_lens[b] on may hold anything; table entries past a sequence's pages are not read. Keys that
 // a query does not see do not reach it. Of the values that `causal` hides from it it may take 0 times those of up to
 // 94 positions past its own (the 32 rows that share a wave end up to 31 positions later, in steps of 64 keys): a NaN
